@@ -690,6 +690,101 @@ int ma_fused_sample(const void* logits, int dtype, int64_t rows, int64_t vocab, 
                     const float* uniform, int top_k, float inv_temperature, float top_p,
                     void* workspace, size_t ws_bytes, int64_t* out, void* stream);
 
+/*
+ * Decoding with a tree of drafted tokens per row: the next four operators.
+ * parents int32 [batch, nodes], nodes <= 64: node 0 is the row's last token
+ * (parents[b, 0] == -1; any other value there marks a row without a sequence),
+ * 0 <= parents[b, i] < i names node i's parent; a node with any other parent,
+ * or below such a node, is absent (padding).  Node i's K/V live at cache
+ * position seqlen[b] + i, its rotary position is seqlen[b] + its depth.  A node
+ * whose slot falls behind the cache (max_len) is neither stored nor attended;
+ * mapped rows are clamped to [0, cache_rows), seqlen to [0, max_len].  batch x
+ * nodes and batch x n_kv_heads at most 65535.
+ *
+ * QK RMSNorm + rotary positions + K/V store of the nodes: qkv bf16 [batch,
+ * nodes, (n_heads + 2 n_kv_heads) * head_dim] (strides ldb, ldt, 1); per head
+ * x * rsqrt(mean(x^2) + eps) * w (q_norm_w / k_norm_w [head_dim] of w_dtype,
+ * both NULL: no norm); rotary positions on the first rotary_dim dims (even, at
+ * most head_dim) in rope_mode 1 (half layout: dims d and d + rotary_dim / 2
+ * turn together, dim d with column d of the tables) or 2 (interleaved: dims 2i
+ * and 2i + 1, with columns i and i + rotary_dim / 2); 0: none.  cos / sin
+ * [n_pos, >= rotary_dim] of cs_dtype, row stride ld_cs, read at the node's
+ * position (the last row past the table), rounded to bf16 before use.  q_out
+ * bf16 [batch, nodes, n_heads, head_dim] (0 for absent nodes).  head_dim 64 or
+ * 128.  The one-token form of it is ma_qk_norm_rope_store.
+ */
+int ma_tree_qkv(const void* qkv, int64_t ldb, int64_t ldt, int64_t batch, int64_t nodes, int n_heads,
+                int n_kv_heads, int head_dim, const void* q_norm_w, const void* k_norm_w, int w_dtype,
+                const void* cos, const void* sin, int cs_dtype, int64_t ld_cs, int64_t n_pos,
+                int rotary_dim, int rope_mode, float eps, const int64_t* seqlen,
+                const int32_t* parents, const int64_t* row_map, void* k_cache, void* v_cache,
+                int64_t cache_rows, int64_t max_len, void* q_out, void* stream);
+
+/*
+ * Attention of a tree's nodes: out[b, i, h] = softmax(q[b, i, h] . K^T * scale)
+ * V over the positions [0, seqlen[b]) of cache row row_map[b] (b when NULL),
+ * the node's ancestors and itself (positions seqlen[b] + a); with window > 0
+ * only what is less than window steps above the node.  q / out bf16 [batch,
+ * nodes, n_heads, head_dim]; float32 statistics and sums, P rounded to bf16
+ * before P.V as in ma_decode_gqa_attn, whose results a tree of one node
+ * repeats up to rounding.  Absent nodes, and nodes that see nothing, give 0; a
+ * K or V that a node does not see does not reach it, finite or not.
+ * workspace: ma_tree_attn_workspace_bytes(...) bytes (may be 0), 16-byte
+ * aligned, its content of no matter before and after; calls that share one
+ * must not overlap.  head_dim 64 or 128.
+ */
+size_t ma_tree_attn_workspace_bytes(int64_t batch, int64_t nodes, int n_heads, int n_kv_heads,
+                                    int head_dim, int64_t max_len, int64_t window);
+int ma_tree_attn(const void* q, int64_t batch, int64_t nodes, int n_heads, int n_kv_heads,
+                 int head_dim, const void* k_cache, const void* v_cache, int64_t cache_rows,
+                 int64_t max_len, const int64_t* seqlen, const int32_t* parents,
+                 const int64_t* row_map, int64_t window, float scale, void* out, void* workspace,
+                 size_t workspace_bytes, void* stream);
+
+/*
+ * Verification of a tree's tokens (int64 [batch, nodes]; node 0's is not read)
+ * against the target's law, that of ma_fused_sample: the top_k largest of the
+ * node's logits (bf16, fp16 or float32 [batch, nodes, vocab], strides ldb, ldt,
+ * 1), softmax at the temperature, nucleus top_p.  From the root with P = its
+ * law, the current node's children in index order: child c with token t is
+ * accepted if uniform[b, c] * q(t) < P(t), and the walk goes on at c with P =
+ * c's law; else P = max(P - q, 0) normalised (unchanged where that is 0).  At
+ * the end one more token is drawn from P: the first whose inclusive prefix
+ * (most likely first) exceeds uniform[b, 0] * sum.  q: probs[b, c] (bf16, fp16
+ * or float32 [batch, nodes, vocab], strides probs_ldb, probs_ldt, 1), the law
+ * that node c's token was drawn from; NULL: q = 1 at t (a chosen token).
+ * out_tokens int64 [batch, nodes]: the accepted tokens, then the drawn one, then
+ * -1; accepted int32 [batch]: how many were accepted (-1 for a row without a
+ * sequence, whose outputs are all -1); path int32 [batch, nodes]: the nodes from
+ * the root to the last accepted one, then -1.  Laws and walk in 64 bits.  1 <=
+ * top_k <= min(64, vocab), inv_temperature finite > 0, 0 < top_p <= 1; top_k = 1
+ * is greedy.  workspace: ma_verify_tree_workspace_bytes(...) bytes, 8-byte
+ * aligned, its content of no matter; calls that share one must not overlap.
+ */
+size_t ma_verify_tree_workspace_bytes(int64_t batch, int64_t nodes, int64_t vocab, int top_k);
+int ma_verify_tree(const void* logits, int dtype, int64_t ldb, int64_t ldt, int64_t batch,
+                   int64_t nodes, int64_t vocab, const int64_t* tokens, const int32_t* parents,
+                   const float* uniform, const void* probs, int probs_dtype, int64_t probs_ldb,
+                   int64_t probs_ldt, int top_k, double inv_temperature, double top_p,
+                   void* workspace, size_t workspace_bytes, int64_t* out_tokens,
+                   int32_t* accepted, int32_t* path, void* stream);
+
+/*
+ * The accepted nodes' K/V moved together behind the sequence, in every layer:
+ * for 0 < j <= accepted[b], position seqlen[b] + path[b, j] of cache row
+ * row_map[b] (b when NULL) goes to seqlen[b] + j; new_seqlen[b] = seqlen[b] +
+ * accepted[b] + 1 (accepted and path as ma_verify_tree writes them: path
+ * ascending; new_seqlen is not seqlen).  k_caches / v_caches: host arrays of
+ * `layers` device pointers to bf16 caches [cache_rows, n_kv_heads, max_len,
+ * head_dim], distinct from one another; one launch per 64 layers.  head_dim 64
+ * or 128.
+ */
+int ma_tree_commit(void* const* k_caches, void* const* v_caches, int64_t layers, int64_t batch,
+                   int64_t nodes, int n_kv_heads, int head_dim, int64_t cache_rows,
+                   int64_t max_len, const int64_t* seqlen, const int32_t* path,
+                   const int32_t* accepted, const int64_t* row_map, int64_t* new_seqlen,
+                   void* stream);
+
 #ifdef __cplusplus
 }
 #endif

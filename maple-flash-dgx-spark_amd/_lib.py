@@ -24,6 +24,7 @@ _P = ctypes.c_void_p
 _I = ctypes.c_int
 _L = ctypes.c_int64
 _F = ctypes.c_float
+_D = ctypes.c_double
 _Z = ctypes.c_size_t
 _PL = ctypes.POINTER(ctypes.c_int64)
 
@@ -95,6 +96,14 @@ _SIGNATURES = {
                       _L, _P, _P, _P, _Z, _P],
     "ma_moe_grouped_noalloc": [_P, _L, _P, _P, _L, _L, _P, _P, _P, _P, _I, _L, _L, _L, _P, _P, _P, _P,
                                _P, _I, _P, _L, _P, _P],
+    "ma_tree_qkv": [_P, _L, _L, _L, _L, _I, _I, _I, _P, _P, _I, _P, _P, _I, _L, _L, _I, _I, _F, _P, _P, _P, _P,
+                    _P, _L, _L, _P, _P],
+    "ma_tree_attn_workspace_bytes": [_L, _L, _I, _I, _I, _L, _L],
+    "ma_tree_attn": [_P, _L, _L, _I, _I, _I, _P, _P, _L, _L, _P, _P, _P, _L, _F, _P, _P, _Z, _P],
+    "ma_verify_tree_workspace_bytes": [_L, _L, _L, _I],
+    "ma_verify_tree": [_P, _I, _L, _L, _L, _L, _L, _P, _P, _P, _P, _I, _L, _L, _I, _D, _D, _P, _Z, _P, _P, _P,
+                       _P],
+    "ma_tree_commit": [_P, _P, _L, _L, _L, _I, _I, _L, _L, _P, _P, _P, _P, _P, _P],
 }
 _RESTYPES = {"ma_last_error": ctypes.c_char_p, "ma_router_workspace_bytes": _Z,
              "ma_ternary_gemv_workspace_bytes": _Z,
@@ -102,7 +111,8 @@ _RESTYPES = {"ma_last_error": ctypes.c_char_p, "ma_router_workspace_bytes": _Z,
              "ma_moe_fused_workspace_bytes": _Z, "ma_moe_route_workspace_bytes": _Z,
              "ma_moe_grouped_noalloc_max_bytes": _Z, "ma_sampler_workspace_bytes": _Z,
              "ma_flash_head_workspace_bytes": _Z, "ma_rtn4_gemv_workspace_bytes": _Z,
-             "ma_rtn4_gemv_mx_workspace_bytes": _Z, "ma_ternary_gemv_call_workspace_bytes": _Z}
+             "ma_rtn4_gemv_mx_workspace_bytes": _Z, "ma_ternary_gemv_call_workspace_bytes": _Z,
+             "ma_tree_attn_workspace_bytes": _Z, "ma_verify_tree_workspace_bytes": _Z}
 
 _lib = None
 

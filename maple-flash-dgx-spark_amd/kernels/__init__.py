@@ -17,6 +17,7 @@ from .router import router_topk
 from .rtn4 import rtn4_embedding, rtn4_gemv, rtn4_indexed_gemv
 from .ternary_expert import ternary_expert_down_sum, ternary_expert_gemv, ternary_expert_swiglu
 from .ternary_gemv import ternary_gemv
+from .tree import apply_qkv_tree, commit_tree, tree_attention, verify_tree
 
 __all__ = [
     "ternary_gemv",
@@ -36,4 +37,8 @@ __all__ = [
     "decode_attention",
     "gqa_workspace",
     "greedy_argmax",
+    "apply_qkv_tree",
+    "tree_attention",
+    "verify_tree",
+    "commit_tree",
 ]
