@@ -20,19 +20,45 @@ stored nor attended.
 
 from __future__ import annotations
 
-import ctypes
+import array
+from operator import attrgetter
 from typing import NamedTuple
 
 import torch
 
 from .. import _lib
-from .decode_attn import _check_rows, _i64
 from .sampler import _check
 
 MAX_NODES = 64
 
+# Decoding calls these once per layer and step, so the checks below read each
+# property once and nothing goes through a context manager or a stream object
+# that a call does not need.
+_stream = torch._C._cuda_getCurrentRawStream
+_current = torch._C._cuda_getDevice
 
-def _check_tree(parents: torch.Tensor, bsz: int, nodes: int, device: torch.device, what: str) -> torch.Tensor:
+
+def _call(idx: int, name: str, *args) -> None:
+    """``name`` with the tensors' device current, on its current stream."""
+    if _current() == idx:
+        _lib.call(name, *args, _stream(idx))
+    else:
+        with torch.cuda.device(idx):
+            _lib.call(name, *args, _stream(idx))
+
+
+def _device(what: str, t: torch.Tensor, *others) -> int:
+    """The one device that all of the tensors are on."""
+    idx = t.get_device()
+    if idx < 0:
+        raise RuntimeError(f"{what} requires CUDA tensors.")
+    for o in others:
+        if o is not None and o.get_device() != idx:
+            raise ValueError(f"{what}: tensors on {o.device} and {t.device}.")
+    return idx
+
+
+def _tree(what: str, parents: torch.Tensor, bsz: int, nodes: int) -> torch.Tensor:
     if not 1 <= nodes <= MAX_NODES:
         raise ValueError(f"{what}: a tree has 1 to {MAX_NODES} nodes, got {nodes}.")
     if parents.shape != (bsz, nodes):
@@ -41,24 +67,32 @@ def _check_tree(parents: torch.Tensor, bsz: int, nodes: int, device: torch.devic
         if parents.dtype != torch.int64:
             raise TypeError(f"{what}: parents must be int32 or int64; got {parents.dtype}.")
         parents = parents.to(torch.int32)
-    _same_device(what, device, parents)
-    return parents.contiguous()
+    return parents if parents.is_contiguous() else parents.contiguous()
 
 
-def _same_device(what: str, device: torch.device, *tensors) -> None:
-    if device.type != "cuda":
-        raise RuntimeError(f"{what} requires CUDA tensors.")
-    for t in tensors:
-        if t is not None and t.device != device:
-            raise ValueError(f"{what}: tensors on {t.device} and {device}.")
+def _positions(name: str, t: torch.Tensor, bsz: int) -> torch.Tensor:
+    if t.numel() != bsz:
+        raise ValueError(f"{name} has {t.numel()} entries, expected {bsz}.")
+    if t.dtype != torch.int64:
+        if t.dtype.is_floating_point or t.dtype == torch.bool:
+            raise TypeError(f"{name} must hold whole numbers; got {t.dtype}.")
+        t = t.to(torch.int64)
+    return t if t.is_contiguous() else t.contiguous()
 
 
-def _check_cache(what: str, k_cache: torch.Tensor, v_cache: torch.Tensor, n_kv: int, head_dim: int) -> None:
-    if k_cache.ndim != 4 or k_cache.shape != v_cache.shape:
-        raise ValueError(f"{what}: K {tuple(k_cache.shape)} and V {tuple(v_cache.shape)} caches, "
+def _cache(what: str, k_cache: torch.Tensor, v_cache: torch.Tensor, bsz: int, row_map: torch.Tensor | None):
+    """The caches' shape ``[rows, n_kv, max_len, head_dim]``."""
+    shape = k_cache.shape
+    if len(shape) != 4 or v_cache.shape != shape:
+        raise ValueError(f"{what}: K {tuple(shape)} and V {tuple(v_cache.shape)} caches, "
                          "expected [rows, n_kv, max_len, head_dim] twice.")
-    if k_cache.shape[1] != n_kv or k_cache.shape[3] != head_dim:
-        raise ValueError(f"{what}: cache {tuple(k_cache.shape)} for {n_kv} KV heads of {head_dim}.")
+    if k_cache.dtype != torch.bfloat16 or v_cache.dtype != torch.bfloat16:
+        raise TypeError("the KV cache must be bf16.")
+    if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+        raise ValueError("the KV cache must be contiguous [rows, n_kv, max_len, head_dim].")
+    if row_map is None and shape[0] != bsz:
+        raise ValueError(f"KV cache batch {shape[0]} != {what} batch {bsz}.")
+    return shape
 
 
 def apply_qkv_tree(
@@ -93,42 +127,41 @@ def apply_qkv_tree(
     bsz, nodes, width = qkv.shape
     if width != (num_heads + 2 * num_kv_heads) * head_dim:
         raise ValueError(f"qkv rows of {width}, expected {(num_heads + 2 * num_kv_heads) * head_dim}.")
-    if width > 1 and qkv.stride(2) != 1:
+    ldb, ldt, one = qkv.stride()
+    if one != 1:
         raise ValueError("apply_qkv_tree needs a row-contiguous qkv.")
-    _check_rows("qkv", bsz, k_cache, v_cache, seqlen, row_map)
-    _check_cache("apply_qkv_tree", k_cache, v_cache, num_kv_heads, head_dim)
-    if (q_weight is None) != (k_weight is None):
-        raise ValueError("q_weight and k_weight go together.")
-    if q_weight is not None:
+    rows, n_kv, max_len, d = _cache("apply_qkv_tree", k_cache, v_cache, bsz, row_map)
+    if n_kv != num_kv_heads or d != head_dim:
+        raise ValueError(f"apply_qkv_tree: cache {tuple(k_cache.shape)} for {num_kv_heads} KV heads of {head_dim}.")
+    qw = kw = c = s = None
+    w_dt = dt = ld = n_pos = mode = 0
+    if q_weight is not None or k_weight is not None:
+        if q_weight is None or k_weight is None:
+            raise ValueError("q_weight and k_weight go together.")
         if q_weight.dtype != k_weight.dtype:
             raise TypeError("q_norm and k_norm weights must share a dtype.")
         if q_weight.numel() != head_dim or k_weight.numel() != head_dim:
             raise ValueError(f"norm weights need {head_dim} entries.")
-        q_weight, k_weight = q_weight.reshape(-1).contiguous(), k_weight.reshape(-1).contiguous()
-    c = s = None
-    dt = ld = n_pos = 0
-    if use_rope and rotary_dim > 0:
-        c, s = cos_table, sin_table
+        qw, kw, w_dt = q_weight.contiguous(), k_weight.contiguous(), _lib.dtype_code(q_weight, "q_weight")
+    if use_rope and rotary_dim != 0:
+        c, s, mode = cos_table, sin_table, 2 if interleaved else 1
         if c.ndim != 2 or s.shape != c.shape or s.dtype != c.dtype or s.stride() != c.stride() or c.stride(1) != 1:
             raise ValueError("cos and sin tables must share dtype and layout, rows contiguous.")
-        if c.shape[0] < 1 or c.shape[1] < rotary_dim:
+        n_pos, cols = c.shape
+        if n_pos < 1 or cols < rotary_dim:
             raise ValueError(f"tables {tuple(c.shape)} for a rotary_dim of {rotary_dim}.")
-        dt, ld, n_pos = _lib.dtype_code(c, "cos_table"), c.stride(0), int(c.shape[0])
-    dev = qkv.device
-    parents = _check_tree(parents, bsz, nodes, dev, "apply_qkv_tree")
-    sl, rm = _i64(seqlen), _i64(row_map)
-    _same_device("apply_qkv_tree", dev, k_cache, v_cache, sl, rm, q_weight, k_weight, c, s)
-    out = torch.empty(bsz, nodes, num_heads, head_dim, device=dev, dtype=torch.bfloat16)
-    with torch.cuda.device(dev):
-        _lib.call(
-            "ma_tree_qkv",
-            _lib.ptr(qkv), qkv.stride(0), qkv.stride(1), bsz, nodes, num_heads, num_kv_heads, head_dim,
-            _lib.ptr(q_weight), _lib.ptr(k_weight), 0 if q_weight is None else _lib.dtype_code(q_weight, "q_weight"),
-            _lib.ptr(c), _lib.ptr(s), dt, ld, n_pos, int(rotary_dim) if c is not None else 0,
-            0 if c is None else (2 if interleaved else 1), float(eps), _lib.ptr(sl), _lib.ptr(parents), _lib.ptr(rm),
-            _lib.ptr(k_cache), _lib.ptr(v_cache), int(k_cache.shape[0]), int(k_cache.shape[2]), _lib.ptr(out),
-            _lib.stream_of(qkv),
-        )
+        dt, ld = _lib.dtype_code(c, "cos_table"), c.stride(0)
+    parents = _tree("apply_qkv_tree", parents, bsz, nodes)
+    sl = _positions("seqlen", seqlen, bsz)
+    rm = None if row_map is None else _positions("row_map", row_map, bsz)
+    idx = _device("apply_qkv_tree", qkv, k_cache, v_cache, sl, parents, rm, qw, kw, c, s)
+    out = torch.empty((bsz, nodes, num_heads, head_dim), device=qkv.device, dtype=torch.bfloat16)
+    _call(
+        idx, "ma_tree_qkv",
+        qkv.data_ptr(), ldb, ldt, bsz, nodes, num_heads, num_kv_heads, head_dim, _lib.ptr(qw), _lib.ptr(kw), w_dt,
+        _lib.ptr(c), _lib.ptr(s), dt, ld, n_pos, rotary_dim if mode else 0, mode, eps, sl.data_ptr(),
+        parents.data_ptr(), _lib.ptr(rm), k_cache.data_ptr(), v_cache.data_ptr(), rows, max_len, out.data_ptr(),
+    )
     return out
 
 
@@ -150,31 +183,30 @@ def tree_attention(
     if q.ndim != 4 or q.dtype != torch.bfloat16:
         raise ValueError(f"tree_attention expects bf16 q [B, T, H, D], got {q.dtype} {tuple(q.shape)}.")
     bsz, nodes, n_q, head_dim = q.shape
-    _check_rows("q", bsz, k_cache, v_cache, seqlen, row_map)
-    n_kv, max_len = int(k_cache.shape[1]), int(k_cache.shape[2])
-    _check_cache("tree_attention", k_cache, v_cache, n_kv, head_dim)
-    if n_q % n_kv != 0:
+    rows, n_kv, max_len, d = _cache("tree_attention", k_cache, v_cache, bsz, row_map)
+    if d != head_dim:
+        raise ValueError(f"tree_attention: cache {tuple(k_cache.shape)} for heads of {head_dim}.")
+    if n_kv < 1 or n_q % n_kv != 0:
         raise ValueError(f"n_q={n_q} not divisible by n_kv={n_kv}.")
-    if window is not None and window < 1:
+    if window is None:
+        window = 0
+    elif window < 1:
         raise ValueError(f"window must be positive, got {window}.")
-    dev = q.device
-    parents = _check_tree(parents, bsz, nodes, dev, "tree_attention")
-    sl, rm = _i64(seqlen), _i64(row_map)
-    _same_device("tree_attention", dev, k_cache, v_cache, sl, rm)
+    parents = _tree("tree_attention", parents, bsz, nodes)
+    sl = _positions("seqlen", seqlen, bsz)
+    rm = None if row_map is None else _positions("row_map", row_map, bsz)
+    idx = _device("tree_attention", q, k_cache, v_cache, sl, parents, rm)
     q = q.contiguous()
     out = torch.empty_like(q)
-    win = int(window or 0)
-    nbytes = int(_lib.load().ma_tree_attn_workspace_bytes(bsz, nodes, n_q, n_kv, head_dim, max_len, win))
-    with torch.cuda.device(dev):
-        # scratch of this call alone: the allocator keeps it to this stream, a
-        # captured graph to its own pool
-        ws = torch.empty(nbytes, device=dev, dtype=torch.uint8) if nbytes else None
-        _lib.call(
-            "ma_tree_attn",
-            _lib.ptr(q), bsz, nodes, n_q, n_kv, head_dim, _lib.ptr(k_cache), _lib.ptr(v_cache),
-            int(k_cache.shape[0]), max_len, _lib.ptr(sl), _lib.ptr(parents), _lib.ptr(rm), win, float(scale),
-            _lib.ptr(out), _lib.ptr(ws), nbytes, _lib.stream_of(q),
-        )
+    nbytes = _lib.load().ma_tree_attn_workspace_bytes(bsz, nodes, n_q, n_kv, head_dim, max_len, window)
+    # scratch of this call alone: the allocator keeps it to this stream, a
+    # captured graph to its own pool
+    ws = torch.empty(nbytes, device=q.device, dtype=torch.uint8) if nbytes else None
+    _call(
+        idx, "ma_tree_attn",
+        q.data_ptr(), bsz, nodes, n_q, n_kv, head_dim, k_cache.data_ptr(), v_cache.data_ptr(), rows, max_len,
+        sl.data_ptr(), parents.data_ptr(), _lib.ptr(rm), window, scale, out.data_ptr(), _lib.ptr(ws), nbytes,
+    )
     return out
 
 
@@ -213,41 +245,48 @@ def verify_tree(
     ``tokens [B, T]`` int64, ``uniform [B, T]`` float32 in [0, 1)."""
     if logits.ndim != 3:
         raise ValueError(f"verify_tree expects logits [B, T, vocab], got {tuple(logits.shape)}.")
-    bsz, nodes, vocab = logits.shape
-    _check(top_k, temperature, int(vocab))
-    dev = logits.device
-    parents = _check_tree(parents, bsz, nodes, dev, "verify_tree")
-    if logits.stride(2) != 1 and vocab > 1:
+    shape = logits.shape
+    bsz, nodes, vocab = shape
+    _check(top_k, temperature, vocab)
+    parents = _tree("verify_tree", parents, bsz, nodes)
+    ldb, ldt, one = logits.stride()
+    if one != 1 and vocab > 1:
         raise ValueError("logits rows must be contiguous.")
     if tokens.shape != (bsz, nodes) or uniform.shape != (bsz, nodes):
         raise ValueError(f"tokens {tuple(tokens.shape)} and uniform {tuple(uniform.shape)}, expected {(bsz, nodes)}.")
-    if tokens.dtype not in (torch.int64, torch.int32):
-        raise TypeError(f"tokens must be int64 or int32; got {tokens.dtype}.")
+    if tokens.dtype != torch.int64:
+        if tokens.dtype != torch.int32:
+            raise TypeError(f"tokens must be int64 or int32; got {tokens.dtype}.")
+        tokens = tokens.to(torch.int64)
     if uniform.dtype != torch.float32:
         raise TypeError("uniform must be a float32 CUDA tensor.")
-    tokens, uniform = tokens.to(torch.int64).contiguous(), uniform.contiguous()
-    dt, p_dt, p_lb, p_lt = _lib.dtype_code(logits, "logits"), 0, 0, 0
+    tokens, uniform = tokens.contiguous(), uniform.contiguous()
+    p_dt = p_lb = p_lt = 0
     if draft_probs is not None:
-        if draft_probs.shape != logits.shape:
-            raise ValueError(f"draft_probs {tuple(draft_probs.shape)}, expected {tuple(logits.shape)}.")
-        if draft_probs.stride(2) != 1 and vocab > 1:
+        if draft_probs.shape != shape:
+            raise ValueError(f"draft_probs {tuple(draft_probs.shape)}, expected {tuple(shape)}.")
+        p_lb, p_lt, one = draft_probs.stride()
+        if one != 1 and vocab > 1:
             raise ValueError("draft_probs rows must be contiguous.")
-        p_dt, p_lb, p_lt = _lib.dtype_code(draft_probs, "draft_probs"), draft_probs.stride(0), draft_probs.stride(1)
-    _same_device("verify_tree", dev, tokens, uniform, draft_probs)
-    out = TreeVerdict(torch.empty(bsz, nodes, device=dev, dtype=torch.int64),
+        p_dt = _lib.dtype_code(draft_probs, "draft_probs")
+    idx = _device("verify_tree", logits, tokens, parents, uniform, draft_probs)
+    dev = logits.device
+    out = TreeVerdict(torch.empty((bsz, nodes), device=dev, dtype=torch.int64),
                       torch.empty(bsz, device=dev, dtype=torch.int32),
-                      torch.empty(bsz, nodes, device=dev, dtype=torch.int32))
-    nbytes = int(_lib.load().ma_verify_tree_workspace_bytes(bsz, nodes, vocab, int(top_k)))
-    with torch.cuda.device(dev):
-        ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
-        _lib.call(
-            "ma_verify_tree",
-            _lib.ptr(logits), dt, logits.stride(0), logits.stride(1), bsz, nodes, vocab, _lib.ptr(tokens),
-            _lib.ptr(parents), _lib.ptr(uniform), _lib.ptr(draft_probs), p_dt, p_lb, p_lt, int(top_k),
-            1.0 / float(temperature), float(top_p), _lib.ptr(ws), nbytes, _lib.ptr(out.tokens),
-            _lib.ptr(out.accepted), _lib.ptr(out.path), _lib.stream_of(logits),
-        )
+                      torch.empty((bsz, nodes), device=dev, dtype=torch.int32))
+    nbytes = _lib.load().ma_verify_tree_workspace_bytes(bsz, nodes, vocab, top_k)
+    ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)  # scratch of this call alone, as in tree_attention
+    _call(
+        idx, "ma_verify_tree",
+        logits.data_ptr(), _lib.dtype_code(logits, "logits"), ldb, ldt, bsz, nodes, vocab, tokens.data_ptr(),
+        parents.data_ptr(), uniform.data_ptr(), _lib.ptr(draft_probs), p_dt, p_lb, p_lt, top_k,
+        1.0 / float(temperature), top_p, ws.data_ptr(), nbytes, out[0].data_ptr(), out[1].data_ptr(),
+        out[2].data_ptr(),
+    )
     return out
+
+
+_shape, _dtype = attrgetter("shape"), attrgetter("dtype")
 
 
 def commit_tree(
@@ -263,8 +302,9 @@ def commit_tree(
     lists of caches) together behind each row's sequence; returns the new write
     positions ``seqlen + accepted + 1`` (int64 ``[B]``).  ``path`` / ``accepted``
     as ``verify_tree`` returns them."""
-    if len(k_caches) == 0 or len(k_caches) != len(v_caches):
-        raise ValueError(f"commit_tree expects as many K as V caches, got {len(k_caches)} and {len(v_caches)}.")
+    n = len(k_caches)
+    if n == 0 or n != len(v_caches):
+        raise ValueError(f"commit_tree expects as many K as V caches, got {n} and {len(v_caches)}.")
     if path.ndim != 2 or not 1 <= path.shape[1] <= MAX_NODES:
         raise ValueError(f"commit_tree expects path [B, T], T <= {MAX_NODES}, got {tuple(path.shape)}.")
     bsz, nodes = path.shape
@@ -272,23 +312,27 @@ def commit_tree(
         raise ValueError(f"accepted is {tuple(accepted.shape)}, expected {(bsz,)}.")
     if path.dtype != torch.int32 or accepted.dtype != torch.int32:
         raise TypeError("path and accepted must be int32.")
-    first = k_caches[0]
-    if first.ndim != 4:
-        raise ValueError(f"commit_tree expects caches [rows, n_kv, max_len, head_dim], got {tuple(first.shape)}.")
-    dev, shape = first.device, first.shape
-    for t in (*k_caches, *v_caches):
-        if t.shape != shape or t.dtype != torch.bfloat16 or not t.is_contiguous() or t.device != dev:
-            raise ValueError("commit_tree: the caches must be contiguous bf16 tensors of one shape and device.")
-    _check_rows("path", bsz, first, first, seqlen, row_map)
-    sl, rm = _i64(seqlen), _i64(row_map)
+    caches = [*k_caches, *v_caches]
+    first = caches[0]
+    shape = _cache("commit_tree", first, caches[n], bsz, row_map)
+    # every layer's cache like the first (a set each: one pass without bytecode)
+    if (set(map(_shape, caches)) != {shape} or set(map(_dtype, caches)) != {torch.bfloat16}
+            or not all(map(torch.Tensor.is_contiguous, caches))):
+        raise ValueError("commit_tree: the caches must be contiguous bf16 tensors of one shape.")
+    ptrs = array.array("Q", map(torch.Tensor.data_ptr, caches))
+    if len(set(ptrs)) != 2 * n:
+        raise ValueError("commit_tree: the same cache twice.")
+    sl = _positions("seqlen", seqlen, bsz)
+    rm = None if row_map is None else _positions("row_map", row_map, bsz)
     path, accepted = path.contiguous(), accepted.contiguous()
-    _same_device("commit_tree", dev, sl, rm, path, accepted)
-    out = torch.empty(bsz, device=dev, dtype=torch.int64)
-    n = len(k_caches)
-    kp = (ctypes.c_void_p * n)(*[t.data_ptr() for t in k_caches])
-    vp = (ctypes.c_void_p * n)(*[t.data_ptr() for t in v_caches])
-    with torch.cuda.device(dev):
-        _lib.call("ma_tree_commit", kp, vp, n, bsz, nodes, int(shape[1]), int(shape[3]), int(shape[0]), int(shape[2]),
-                  _lib.ptr(sl), _lib.ptr(path), _lib.ptr(accepted), _lib.ptr(rm), _lib.ptr(out),
-                  _lib.stream_of(first))
+    idx = _device("commit_tree", first, sl, rm, path, accepted)
+    if set(map(torch.Tensor.get_device, caches)) != {idx}:
+        raise ValueError("commit_tree: caches on several devices.")
+    out = torch.empty(bsz, device=first.device, dtype=torch.int64)
+    at = ptrs.buffer_info()[0]
+    _call(
+        idx, "ma_tree_commit",
+        at, at + 8 * n, n, bsz, nodes, shape[1], shape[3], shape[0], shape[2], sl.data_ptr(), path.data_ptr(),
+        accepted.data_ptr(), _lib.ptr(rm), out.data_ptr(),
+    )
     return out
