@@ -9,13 +9,8 @@
 namespace ma {
 
 typedef __bf16 bf16x8t_t __attribute__((ext_vector_type(8)));
-typedef float f32x4t_t __attribute__((ext_vector_type(4)));
+typedef float f32x16t_t __attribute__((ext_vector_type(16)));
 typedef short s16x4t_t __attribute__((ext_vector_type(4)));
-
-__device__ __forceinline__ f32x4t_t mfma_tree(uint4 a, uint4 b, f32x4t_t c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8t_t, a), __builtin_bit_cast(bf16x8t_t, b),
-                                                 c, 0, 0, 0);
-}
 
 __device__ __forceinline__ int64_t clamp_pos(int64_t v, int64_t lo, int64_t hi) { return v < lo ? lo : (v > hi ? hi : v); }
 
@@ -120,337 +115,429 @@ __global__ __launch_bounds__(64) void k_tree_qkv(
 // ---------------------------------------------------------------------------
 // Attention
 // ---------------------------------------------------------------------------
-constexpr int kTreeChunk = 128;  // positions a workgroup takes at a time, 32 per wave
-constexpr int kTreeWaves = 4;
+typedef __attribute__((address_space(3))) void* tree_lds_t;
 constexpr int kTreeTargetGroups = 1024;  // workgroups a launch aims for
 constexpr float kTreeGrow = 8.0f;        // a row's reference maximum is moved when a score passes it by 2^8
+constexpr int tree_vmcnt(int n) { return (n & 0xF) | (0x7 << 4) | ((n >> 4) << 14); }  // and lgkmcnt(0)
 
-// Workgroup (split sp, tile, pair): 16 RB query rows of (row b, KV head), row r
-// of the pair = (node r / group, query head r % group); a split's chunks of 128
-// positions, 32 per wave.  On v_mfma_f32_16x16x32_bf16 (A lane l: row l % 16,
-// k 8 (l / 16)..+8; B: col l % 16, the same k; C: col l % 16, rows 4 (l / 16)..+4):
-//   S^T = K Q^T: A = 16 cache positions read straight from memory, B = the
-//     query rows, so lane l holds the scores of query row l % 16 at positions
-//     4 (l / 16)..+4 of each block of 16;
+__device__ __forceinline__ f32x16t_t mfma_tree(uint4 a, uint4 b, f32x16t_t c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8t_t, a), __builtin_bit_cast(bf16x8t_t, b),
+                                                 c, 0, 0, 0);
+}
+
+// A tile's shape: 32 RW query rows, RW waves of 32 rows times 4 / RW waves of
+// NP positions each.
+template <int HD, int RW>
+struct TreeTile {
+  static constexpr int kRows = 32 * RW;
+  static constexpr int kPW = 4 / RW;                                  // position groups
+  static constexpr int kNP = HD == 64 && RW > 1 ? 64 : 32;            // positions of a group per step
+  static constexpr int kStep = kPW * kNP;                             // positions of a workgroup per step
+  static constexpr int kBufs = RW == 4 ? 3 : 2;
+  static constexpr int kRowBytes = HD * 2;
+  static constexpr int kRegion = kNP * kRowBytes;                     // K or V of a group
+  static constexpr int kStage = kPW * 2 * kRegion;
+  static constexpr int kCopies = kNP / RW * kRowBytes / 1024;         // 1 KB copies of a wave, K and V each
+};
+
+// The 16-byte piece c of LDS row r lies at piece c ^ tree_key(r) of that row:
+// the 8 rows that a K read takes the same piece of, and the 4 that a V read
+// takes 4 pieces of, then fall into different banks.
+__device__ __forceinline__ int tree_key(int r) { return ((r & 1) << 2) | ((r >> 1) & 3); }
+
+struct TreeRow {
+  uint64_t anc;  // the ancestors seen
+  int64_t from;  // first position of the sequence that is seen
+};
+
+// Workgroup: a tile of (row b, KV head), row r of the pair = (node r / group,
+// query head r % group), and a split of its positions.  K and V come through
+// LDS, copied there without registers kBufs - 1 steps ahead.  On
+// v_mfma_f32_32x32x16_bf16 (A lane l: row l % 32, k 8 (l / 32)..+8; B: col l % 32,
+// the same k; C: col l % 32, rows 8 (i / 4) + 4 (l / 32) + i % 4):
+//   S^T = K Q^T: lane l holds query row l % 32's scores, half of the 32 positions;
 //   P = 2^(S scale log2 e - m), m a reference per query row that is moved only
 //     when a score passes it by 8 (any m gives the same quotient; this one
-//     keeps P below 2^8 without a reduction over the lanes in every chunk), P
-//     rounded to bf16 as the matrix instruction takes it (2^-9 of each weight,
-//     below the output's own rounding), masked places exactly 0;
-//   O += P V, and the sum of P by a product with ones, from the same rounded
-//     P: a weight's rounding then enters the quotient on both sides.  A = the lane's
-//     own 8 P values (positions 4g..4g+3 of the two blocks), B = V in the same
-//     order, read from LDS rows with the transposing read.
-// A chunk in which some row sees only part (the tree's own slots, the edge of
-// the window) is masked element by element; there a V that is not finite must
-// not reach the rows that do not see it (0 x inf), so such values are taken
-// out of the product and added to the rows that see them.
-template <int HD, int RB>
+//     keeps P below 2^8 without an exchange between lanes in every step), P
+//     rounded to bf16 as the matrix instruction takes it (half a step, 2^-8 of
+//     each weight at most, as in k_decode_attn), masked places exactly 0;
+//   the sum of P from the same rounded values, so that a weight's rounding
+//     enters the quotient on both sides;
+//   O += P V: A = the lane's own P values in the order they are in, B = V in the
+//     same order, read from its rows with the transposing LDS read.
+// 32 positions of which some row sees only part (the tree's own slots, the edge
+// of the window) are masked by a word per query row; there a V that is not
+// finite must not reach the rows that do not see it (0 x inf), so such values
+// are taken out of the product and added to the rows that see them.
+template <int HD, int RW>
 __global__ __launch_bounds__(256) void k_tree_attn(
-    const uint16_t* __restrict__ q, int nodes, int nq, int nkv, const uint16_t* __restrict__ k_cache,
-    const uint16_t* __restrict__ v_cache, int64_t cache_rows, int64_t max_len, const int64_t* __restrict__ seqlen,
-    const int32_t* __restrict__ parents, const int64_t* __restrict__ row_map, int64_t window, float scale,
-    uint16_t* __restrict__ out, float* __restrict__ part_acc, float2* __restrict__ part_ml) {
-  constexpr int ROWS = 16 * RB;
-  constexpr int KS = HD / 32;  // k slices of a score
-  constexpr int NB = HD / 16;  // 16-dim blocks of the output
+    const uint16_t* __restrict__ q, int nodes, int nq, int nkv, int tiles, int S, int n_units,
+    const uint16_t* __restrict__ k_cache, const uint16_t* __restrict__ v_cache, int64_t cache_rows, int64_t max_len,
+    const int64_t* __restrict__ seqlen, const int32_t* __restrict__ parents, const int64_t* __restrict__ row_map,
+    int64_t window, float scale, uint16_t* __restrict__ out, float* __restrict__ part_acc,
+    float2* __restrict__ part_ml) {
+  using T = TreeTile<HD, RW>;
+  constexpr int KS = HD / 16;  // k slices of a score
+  constexpr int DB = HD / 32;  // 32-dim blocks of the output
   constexpr int CPR = HD / 8;  // 16-byte pieces of a cache row
-  constexpr int VL = CPR / 2;  // 16-byte loads of a lane per 32 positions of V
-  __shared__ __align__(16) uint16_t vs[kTreeWaves][32 * HD];
+  __shared__ __align__(16) char buf0[T::kStage];
+  __shared__ __align__(16) char buf1[T::kStage];
+  __shared__ __align__(16) char buf2[T::kBufs == 3 ? T::kStage : 16];
   __shared__ uint64_t t_anc[kTreeNodes];
   __shared__ int t_depth[kTreeNodes];
-  __shared__ float wm[kTreeWaves][ROWS], wl[kTreeWaves][ROWS];
-  static_assert(sizeof(vs) >= sizeof(float) * ROWS * HD, "the merge buffer lies over V");
+  __shared__ float wm[4][32], wl[4][32];
+  constexpr int kWave = DB * 16 * 64;  // floats of a wave's sums
+  static_assert((T::kPW - 1) * RW * kWave * 4 <= T::kStage, "the position groups' sums fit one buffer");
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int r16 = lane & 15, g = lane >> 4;
-  const int S = gridDim.x, sp = blockIdx.x, tile = blockIdx.y;
-  const int64_t b = blockIdx.z / nkv;
-  const int kvh = blockIdx.z % nkv;
+  const int rw = wv % RW, pw = wv / RW;
+  const int r32 = lane & 31, h = lane >> 5;
+  // tiles of the same positions follow each other on one XCD
+  const int xcd = blockIdx.x % kXcds, turn = blockIdx.x / kXcds;
+  const int tile = turn % tiles, unit = turn / tiles * kXcds + xcd;
+  if (unit >= n_units) return;
+  const int sp = unit % S;
+  const int64_t pair = unit / S;
+  const int64_t b = pair / nkv;
+  const int kvh = static_cast<int>(pair - b * nkv);
   const int group = nq / nkv, M = nodes * group;
 
   const TreeLane me = tree_lane(parents + b * nodes, nodes);
+  const int64_t n0 = clamp_pos(seqlen[b], 0, max_len);
+  const int64_t crow = row_map ? clamp_pos(row_map[b], 0, cache_rows - 1) : b;
   if (wv == 0) {
     t_anc[lane] = me.anc;
     t_depth[lane] = me.depth;
   }
   const uint64_t here = __ballot(me.depth >= 0);
-  const int64_t n0 = clamp_pos(seqlen[b], 0, max_len);
-  const int64_t crow = row_map ? clamp_pos(row_map[b], 0, cache_rows - 1) : b;
-  __syncthreads();
-
-  // the query rows of this lane's columns
-  uint64_t anc[RB];
-  int64_t from[RB];  // first position of the sequence that the row sees
-  uint4 qf[RB][KS];
-#pragma unroll
-  for (int rb = 0; rb < RB; ++rb) {
-    const int r = tile * ROWS + rb * 16 + r16;
-    const int node = r < M ? r / group : 0;
-    const int depth = r < M ? t_depth[node] : -1;
-    anc[rb] = depth >= 0 ? t_anc[node] : 0ull;
-    from[rb] = 0;
-    if (window > 0 && depth >= 0) {
-      from[rb] = n0 + depth + 1 - window;
-      for (int c = depth + 1; c > window; --c) anc[rb] &= anc[rb] - 1;  // the nearest `window` ancestors
-    }
-    if (depth < 0) from[rb] = INT64_MAX;
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks)
-      qf[rb][ks] = depth >= 0 ? *reinterpret_cast<const uint4*>(
-                                    q + ((b * nodes + node) * nq + kvh * group + r % group) * HD + 8 * g + 32 * ks)
-                              : make_uint4(0u, 0u, 0u, 0u);
-  }
-  const int last = here ? 63 - __builtin_clzll(here) : -1;
+  const int last = here ? 63 - static_cast<int>(__builtin_clzll(here)) : -1;
   int64_t end = n0 + last + 1;
   end = end < max_len ? end : max_len;
   const int64_t start = window > 0 && n0 + 1 > window ? n0 + 1 - window : 0;
-  const int n_chunks = last >= 0 && end > start ? static_cast<int>(cdiv(end - start, kTreeChunk)) : 0;
-  // a chunk at or past this position is masked; in a window also one before `whole`
+  const bool any_row = last >= 0 && tile * T::kRows < (last + 1) * group;
+  const int n_steps = any_row && end > start ? static_cast<int>(cdiv(end - start, T::kStep)) : 0;
+  const int sps = (n_steps + S - 1) / S;
+  const int s_beg = sp * sps < n_steps ? sp * sps : n_steps;
+  const int s_end = s_beg + sps < n_steps ? s_beg + sps : n_steps;
+  // 32 positions at or behind n0, or (with a window) before `whole`, are masked
   const int64_t whole = window > 0 ? n0 + nodes - window : 0;
-  const int cps = (n_chunks + S - 1) / S;
-  const int c_beg = sp * cps, c_end = c_beg + cps < n_chunks ? c_beg + cps : n_chunks;
-  const float scale2 = scale * kLog2e;
   const int64_t base = (crow * nkv + kvh) * max_len;
 
-  f32x4t_t o[RB][NB], ol[RB];
-  float mref[RB];
+  // copies of step s into a buffer: each wave its share of its group's rows
+  const int copy_row = rw * (T::kNP / RW) + lane / CPR;
+  auto copy = [&](int s, char* buf) {
+    const int64_t t0 = start + static_cast<int64_t>(s) * T::kStep + pw * T::kNP;
+    char* const dst = buf + pw * 2 * T::kRegion + rw * (T::kNP / RW) * T::kRowBytes;
 #pragma unroll
-  for (int rb = 0; rb < RB; ++rb) {
-    mref[rb] = -INFINITY;
-    ol[rb] = f32x4t_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb) o[rb][nb] = f32x4t_t{0.f, 0.f, 0.f, 0.f};
-  }
-  const uint32_t one2 = 0x3F803F80u;
-  const uint4 ones = make_uint4(one2, one2, one2, one2);
-  char* const vw = reinterpret_cast<char*>(vs[wv]);
-
-  for (int c = c_beg; c < c_end; ++c) {
-    const int64_t t0 = start + static_cast<int64_t>(c) * kTreeChunk + 32 * wv;
-    if (t0 >= end) break;
-    uint4 kf[2][KS], vr[VL];
-#pragma unroll
-    for (int pb = 0; pb < 2; ++pb) {
-      int64_t t = t0 + 16 * pb + r16;
+    for (int i = 0; i < T::kCopies; ++i) {
+      const int row = copy_row + i * (64 / CPR);
+      int64_t t = t0 + row;
       t = t < end ? t : end - 1;
+      const int64_t off = (base + t) * HD + 8 * ((lane % CPR) ^ tree_key(row));
+      __builtin_amdgcn_global_load_lds(k_cache + off, (tree_lds_t)(dst + i * 1024), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds(v_cache + off, (tree_lds_t)(dst + T::kRegion + i * 1024), 16, 0, 0);
+    }
+  };
+  if (s_beg < s_end) copy(s_beg, buf0);
+  if (T::kBufs == 3 && s_beg + 1 < s_end) copy(s_beg + 1, buf1);
+  // the tree's table for every wave (the copies stay in flight)
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+
+  // this lane's query row
+  const int r = tile * T::kRows + rw * 32 + r32;
+  const int node = r < M ? r / group : 0;
+  const int depth = r < M ? t_depth[node] : -1;
+  TreeRow row{0ull, INT64_MAX};
+  if (depth >= 0) {
+    row.anc = t_anc[node];
+    if (max_len - n0 < kTreeNodes) row.anc &= (1ull << (max_len - n0)) - 1;
+    row.from = 0;
+    if (window > 0) {
+      row.from = n0 + depth + 1 - window;
+      for (int c = depth + 1; c > window; --c) row.anc &= row.anc - 1;  // the nearest `window` ancestors stay
+    }
+  }
+  const bool busy = __any(depth >= 0);  // this wave has rows
+  // a negative scale is taken with -q, a zero one with q = 0 (both exact)
+  const float scale2 = scale == 0.f ? 1.f : fabsf(scale) * kLog2e;
+  uint4 qf[KS];
+  {
+    const uint16_t* const src = q + ((b * nodes + node) * nq + kvh * group + (r < M ? r % group : 0)) * HD + 8 * h;
+    const uint32_t flip = scale < 0.f ? 0x80008000u : 0u;
+    const uint32_t keep = depth >= 0 && scale != 0.f ? 0xffffffffu : 0u;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      const uint4 w = *reinterpret_cast<const uint4*>(src + 16 * ks);
+      qf[ks] = make_uint4((w.x ^ flip) & keep, (w.y ^ flip) & keep, (w.z ^ flip) & keep, (w.w ^ flip) & keep);
+    }
+  }
+
+  f32x16t_t o[DB];
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[db][i] = 0.f;
+  float mref = -INFINITY, lsum = 0.f;
+
+  auto attend = [&](int s, const char* buf) {
+    const int64_t tb = start + static_cast<int64_t>(s) * T::kStep + pw * T::kNP;
+    const char* const kb = buf + pw * 2 * T::kRegion;
+    const char* const vb = kb + T::kRegion;
+    const int g2 = (lane >> 4) & 1, i16 = lane & 15;
+#pragma unroll
+    for (int st = 0; st < T::kNP / 32; ++st) {
+      const int64_t t0 = tb + 32 * st;
+      if (t0 >= end) break;
+      f32x16t_t sc;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sc[i] = 0.f;
+      const int kr = 32 * st + r32, kk = tree_key(kr);
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks)
-        kf[pb][ks] = *reinterpret_cast<const uint4*>(k_cache + (base + t) * HD + 8 * g + 32 * ks);
-    }
+        sc = mfma_tree(*reinterpret_cast<const uint4*>(kb + kr * T::kRowBytes + (((2 * ks + h) ^ kk) << 4)), qf[ks], sc);
+      const bool masked = t0 + 32 > n0 || t0 < whole;
+      uint32_t sees = 0xffffffffu;  // bit p: the row sees position t0 + p
+      if (masked) {
+        const int64_t off = t0 - n0;  // node index of the first position
+        uint64_t w = off >= 64 ? 0ull : (off >= 0 ? row.anc >> off : (off > -32 ? row.anc << -off : 0ull));
+        if (off < 0) {  // and the sequence's part, from row.from on
+          const uint32_t seq = off <= -32 ? 0xffffffffu : (1u << -off) - 1u;
+          const int64_t lo = row.from - t0;
+          w |= lo >= 32 ? 0u : (lo > 0 ? seq & (0xffffffffu << lo) : seq);
+        }
+        sees = static_cast<uint32_t>(w);
+        const uint32_t mine = sees >> (4 * h);
 #pragma unroll
-    for (int i = 0; i < VL; ++i) {
-      int64_t t = t0 + (i * 64 + lane) / CPR;
-      t = t < end ? t : end - 1;
-      vr[i] = *reinterpret_cast<const uint4*>(v_cache + (base + t) * HD + 8 * (lane % CPR));
-    }
-    const bool masked = t0 + 32 > n0 || t0 < whole;
-    bool odd = false;  // some V of this masked chunk is not finite
-    if (masked) {
+        for (int i = 0; i < 16; ++i) sc[i] = (mine >> (8 * (i >> 2) + (i & 3))) & 1u ? sc[i] : -INFINITY;
+      }
+      float cm = sc[0];
+#pragma unroll
+      for (int i = 1; i < 16; ++i) cm = fmaxf(cm, sc[i]);
+      cm *= scale2;
+      if (__any(!(cm <= mref + kTreeGrow))) {
+        cm = fmaxf(cm, __shfl_xor(cm, 32, 64));
+        const float mn = fmaxf(mref, cm);
+        const float a = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mref - mn);
+        mref = mn;
+        lsum *= a;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float ai = __shfl(a, 8 * (i >> 2) + 4 * h + (i & 3), 64);
+#pragma unroll
+          for (int db = 0; db < DB; ++db) o[db][i] *= ai;
+        }
+      }
+      const float m = mref == -INFINITY ? 0.f : mref;
       uint32_t bad = 0;
 #pragma unroll
-      for (int i = 0; i < VL; ++i) {
-        uint32_t w[4] = {vr[i].x, vr[i].y, vr[i].z, vr[i].w};
+      for (int k2 = 0; k2 < 2; ++k2) {
+        uint32_t p[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t lo = (w[j] & 0x7F80u) == 0x7F80u ? 0xFFFFu : 0u;
-          const uint32_t hi = (w[j] & 0x7F800000u) == 0x7F800000u ? 0xFFFF0000u : 0u;
-          bad |= lo | hi;
-          w[j] &= ~(lo | hi);
+        for (int e = 0; e < 4; ++e) {
+          const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[8 * k2 + 2 * e], scale2, -m));
+          const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[8 * k2 + 2 * e + 1], scale2, -m));
+          p[e] = pack_bf16x2_rn(p0, p1);
+          lsum = dot2(p[e], kOneBf16x2, lsum);
         }
-        vr[i] = make_uint4(w[0], w[1], w[2], w[3]);
-      }
-      odd = __any(bad != 0);
-    }
+        const uint4 pa = make_uint4(p[0], p[1], p[2], p[3]);
 #pragma unroll
-    for (int i = 0; i < VL; ++i) {
-      const int row = (i * 64 + lane) / CPR, pc = lane % CPR;
-      *reinterpret_cast<uint4*>(vw + row * (HD * 2) + ((pc ^ (row & 7)) << 4)) = vr[i];
-    }
-    // scores
-    f32x4t_t s[2][RB];
+        for (int db = 0; db < DB; ++db) {
+          s16x4t_t v[2];
 #pragma unroll
-    for (int pb = 0; pb < 2; ++pb)
-#pragma unroll
-      for (int rb = 0; rb < RB; ++rb) {
-        s[pb][rb] = f32x4t_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) s[pb][rb] = mfma_tree(kf[pb][ks], qf[rb][ks], s[pb][rb]);
-      }
-    uint4 pa[RB];
-#pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-      float x[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = s[e >> 2][rb][e & 3] * scale2;
-      if (masked) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int64_t t = t0 + 16 * (e >> 2) + 4 * g + (e & 3);
-          const int64_t j = t - n0;
-          const bool sees = j < 0 ? t >= from[rb] : (j < kTreeNodes && t < end && ((anc[rb] >> j) & 1ull));
-          x[e] = sees ? x[e] : -INFINITY;
-        }
-      }
-      float cm = x[0];
-#pragma unroll
-      for (int e = 1; e < 8; ++e) cm = fmaxf(cm, x[e]);
-      if (__any(cm > mref[rb] + kTreeGrow)) {
-        cm = fmaxf(cm, __shfl_xor(cm, 16, 64));
-        cm = fmaxf(cm, __shfl_xor(cm, 32, 64));
-        const float mn = fmaxf(mref[rb], cm);
-        const float a = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mref[rb] - mn);
-        mref[rb] = mn;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float ai = __shfl(a, 4 * g + i, 64);
-          ol[rb][i] *= ai;
-#pragma unroll
-          for (int nb = 0; nb < NB; ++nb) o[rb][nb][i] *= ai;
-        }
-      }
-      const float m = mref[rb] == -INFINITY ? 0.f : mref[rb];
-      float p[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(x[e] - m);
-      pa[rb] = make_uint4(pack_bf16x2_rn(p[0], p[1]), pack_bf16x2_rn(p[2], p[3]), pack_bf16x2_rn(p[4], p[5]),
-                          pack_bf16x2_rn(p[6], p[7]));
-    }
-    // the wave's own LDS writes above, before its reads below
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-      s16x4t_t h[2];
-#pragma unroll
-      for (int pb = 0; pb < 2; ++pb) {
-        const int row = 16 * pb + 4 * g + (r16 >> 2), pc = nb * 2 + ((r16 & 3) >> 1);
-        h[pb] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4t_t*)(
-            vw + row * (HD * 2) + ((pc ^ (row & 7)) << 4) + (r16 & 1) * 8));
-      }
-      const uint2 h0 = __builtin_bit_cast(uint2, h[0]), h1 = __builtin_bit_cast(uint2, h[1]);
-      const uint4 vb = make_uint4(h0.x, h0.y, h1.x, h1.y);
-#pragma unroll
-      for (int rb = 0; rb < RB; ++rb) o[rb][nb] = mfma_tree(pa[rb], vb, o[rb][nb]);
-    }
-#pragma unroll
-    for (int rb = 0; rb < RB; ++rb) ol[rb] = mfma_tree(pa[rb], ones, ol[rb]);
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    if (odd) {
-      for (int j = 0; j < 32; ++j) {
-        const int64_t t = t0 + j;
-        if (t >= end) break;
-        float v[NB];
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-          v[nb] = bf16_to_f32(v_cache[(base + t) * HD + nb * 16 + r16]);
-          if ((__float_as_uint(v[nb]) & 0x7F800000u) != 0x7F800000u) v[nb] = 0.f;
-        }
-#pragma unroll
-        for (int rb = 0; rb < RB; ++rb)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint64_t ra = __shfl(anc[rb], 4 * g + i, 64);
-            const int64_t rf = __shfl(static_cast<long long>(from[rb]), 4 * g + i, 64);
-            const bool sees = t < n0 ? t >= rf : ((ra >> (t - n0)) & 1ull) != 0;
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb) o[rb][nb][i] += sees ? v[nb] : 0.f;
+          for (int e = 0; e < 2; ++e) {
+            const int vr = 32 * st + 16 * k2 + 8 * e + 4 * h + (i16 >> 2);
+            const int pc = 4 * db + 2 * g2 + ((i16 & 3) >> 1);
+            v[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4t_t*)(
+                vb + vr * T::kRowBytes + ((pc ^ tree_key(vr)) << 4) + (i16 & 1) * 8));
           }
+          const uint2 v0 = __builtin_bit_cast(uint2, v[0]), v1 = __builtin_bit_cast(uint2, v[1]);
+          uint32_t w[4] = {v0.x, v0.y, v1.x, v1.y};
+          if (masked) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const uint32_t odd = ((w[j] & 0x7F80u) == 0x7F80u ? 0xFFFFu : 0u) |
+                                   ((w[j] & 0x7F800000u) == 0x7F800000u ? 0xFFFF0000u : 0u);
+              bad |= odd;
+              w[j] &= ~odd;
+            }
+          }
+          o[db] = mfma_tree(pa, make_uint4(w[0], w[1], w[2], w[3]), o[db]);
+        }
       }
+      if (masked && __any(bad != 0)) {
+        for (int p = 0; p < 32; ++p) {
+          const int64_t t = t0 + p < end ? t0 + p : end - 1;
+          float v[DB];
+#pragma unroll
+          for (int db = 0; db < DB; ++db) {
+            v[db] = bf16_to_f32(v_cache[(base + t) * HD + 32 * db + r32]);
+            if ((__float_as_uint(v[db]) & 0x7F800000u) != 0x7F800000u) v[db] = 0.f;
+          }
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const uint32_t w = __shfl(sees, 8 * (i >> 2) + 4 * h + (i & 3), 64);
+#pragma unroll
+            for (int db = 0; db < DB; ++db) o[db][i] += (w >> p) & 1u ? v[db] : 0.f;
+          }
+        }
+      }
+    }
+  };
+
+  // Wait for step s's copies (those of later steps may be in flight), meet the
+  // other waves, which also frees the buffer of step s - 1, send the copies of
+  // step s + kBufs - 1 there, and attend.
+  auto step = [&](int s, const char* cur, char* prev) {
+    if (T::kBufs == 3 && s + 1 < s_end) __builtin_amdgcn_s_waitcnt(tree_vmcnt(2 * T::kCopies));
+    else __builtin_amdgcn_s_waitcnt(tree_vmcnt(0));
+    asm volatile("" ::: "memory");
+    if (RW > 1) __builtin_amdgcn_s_barrier();  // (RW = 1: every wave reads its own copies only)
+    asm volatile("" ::: "memory");
+    if (s + T::kBufs - 1 < s_end) copy(s + T::kBufs - 1, prev);
+    if (busy) attend(s, cur);
+  };
+  for (int s = s_beg; s < s_end;) {
+    if (T::kBufs == 3) {
+      step(s++, buf0, buf2);
+      if (s >= s_end) break;
+      step(s++, buf1, buf0);
+      if (s >= s_end) break;
+      step(s++, buf2, buf1);
+    } else {
+      step(s++, buf0, buf1);
+      if (s >= s_end) break;
+      step(s++, buf1, buf0);
     }
   }
 
-  // the four waves' results, in wave order
-#pragma unroll
-  for (int rb = 0; rb < RB; ++rb) {
-    if (g == 0) wm[wv][rb * 16 + r16] = mref[rb];
-    if (r16 == 0)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) wl[wv][rb * 16 + 4 * g + i] = ol[rb][i];
-  }
-  __syncthreads();
-  float* const buf = reinterpret_cast<float*>(&vs[0][0]);
-  for (int w = 0; w < kTreeWaves; ++w) {
-    if (wv == w) {
-#pragma unroll
-      for (int rb = 0; rb < RB; ++rb)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int row = rb * 16 + 4 * g + i;
-          const float m = fmaxf(fmaxf(wm[0][row], wm[1][row]), fmaxf(wm[2][row], wm[3][row]));
-          const bool any = wl[w][row] != 0.f;  // (a sum that is not a number stays one)
-          const float f = __builtin_amdgcn_exp2f(wm[w][row] - m);
-#pragma unroll
-          for (int nb = 0; nb < NB; ++nb) {
-            float* const d = buf + row * HD + nb * 16 + r16;
-            const float v = any ? f * o[rb][nb][i] : 0.f;
-            *d = w == 0 ? v : *d + v;
-          }
-        }
+  lsum += __shfl_xor(lsum, 32, 64);
+  float m = mref, l = lsum;
+  if (T::kPW > 1) {  // the position groups' results, in order
+    if (h == 0) {
+      wm[wv][r32] = mref;
+      wl[wv][r32] = lsum;
     }
     __syncthreads();
-  }
-  const int64_t pt = (static_cast<int64_t>(blockIdx.z) * gridDim.y + tile) * S + sp;
-  for (int i = tid; i < ROWS * HD / 4; i += 256) {
-    const int row = i / (HD / 4), d4 = i % (HD / 4);
-    const int r = tile * ROWS + row;
-    const int node = r < M ? r / group : 0;
-    const bool present = r < M && t_depth[node] >= 0;
-    const float m = fmaxf(fmaxf(wm[0][row], wm[1][row]), fmaxf(wm[2][row], wm[3][row]));
-    float l = 0.f;
+    m = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < kTreeWaves; ++w)
-      l += wl[w][row] != 0.f ? __builtin_amdgcn_exp2f(wm[w][row] - m) * wl[w][row] : 0.f;
-    const bool seen = present && l != 0.f;
-    const float4 a = *reinterpret_cast<const float4*>(buf + row * HD + 4 * d4);
-    if (S > 1) {
-      if (c_beg < c_end) *reinterpret_cast<float4*>(part_acc + (pt * ROWS + row) * HD + 4 * d4) = a;
-      if (d4 == 0) part_ml[pt * ROWS + row] = seen ? make_float2(m, l) : make_float2(-INFINITY, 0.f);
-    } else if (r < M) {
-      const float inv = 1.0f / l;
-      const uint2 w = seen ? make_uint2(pack_bf16x2_rn(a.x * inv, a.y * inv), pack_bf16x2_rn(a.z * inv, a.w * inv))
-                           : make_uint2(0u, 0u);
-      *reinterpret_cast<uint2*>(out + ((b * nodes + node) * nq + kvh * group + r % group) * HD + 4 * d4) = w;
+    for (int g = 0; g < T::kPW; ++g) m = fmaxf(m, wm[g * RW + rw][r32]);
+    l = 0.f;
+#pragma unroll
+    for (int g = 0; g < T::kPW; ++g) {
+      const float lg = wl[g * RW + rw][r32];
+      l += lg != 0.f ? __builtin_amdgcn_exp2f(wm[g * RW + rw][r32] - m) * lg : 0.f;
+    }
+    // (a sum that is not a number stays one: only a row that saw nothing has 0)
+    const float f = lsum != 0.f ? __builtin_amdgcn_exp2f(mref - m) : 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float fi = __shfl(f, 8 * (i >> 2) + 4 * h + (i & 3), 64);
+#pragma unroll
+      for (int db = 0; db < DB; ++db) o[db][i] = fi != 0.f ? o[db][i] * fi : 0.f;
+    }
+    auto at = [&](int g) { return reinterpret_cast<float*>(buf0) + ((g - 1) * RW + rw) * kWave + lane; };
+    if (pw > 0) {
+      float* const d = at(pw);
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) d[(db * 16 + i) * 64] = o[db][i];
+    }
+    __syncthreads();
+    if (pw > 0) return;
+#pragma unroll
+    for (int g = 1; g < T::kPW; ++g) {
+      const float* const d = at(g);
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[db][i] += d[(db * 16 + i) * 64];
+    }
+  }
+  const bool seen = depth >= 0 && l != 0.f;
+  if (S > 1) {
+    const int64_t p0 = ((pair * tiles + tile) * S + sp) * T::kRows + rw * 32;
+    if (h == 0) part_ml[p0 + r32] = seen ? make_float2(m, l) : make_float2(-INFINITY, 0.f);
+    if (s_beg < s_end && busy)
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+          part_acc[(p0 + 8 * (i >> 2) + 4 * h + (i & 3)) * HD + 32 * db + r32] = o[db][i];
+    return;
+  }
+  const float inv = seen ? 1.0f / l : 0.f;
+  const int has = __shfl(seen ? 1 : 0, r32, 64);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int ri = 8 * (i >> 2) + 4 * h + (i & 3);
+    const float fi = __shfl(inv, ri, 64);
+    const int on = __shfl(has, ri, 64);
+    const int rr = tile * T::kRows + rw * 32 + ri;
+    if (rr < M) {
+      uint16_t* const dst = out + ((b * nodes + rr / group) * nq + kvh * group + rr % group) * HD + r32;
+#pragma unroll
+      for (int db = 0; db < DB; ++db) dst[32 * db] = on ? f32_to_bf16(o[db][i] * fi) : 0;
     }
   }
 }
 
-// The splits of a tile together: out = sum_s 2^(m_s - m) acc_s / sum_s 2^(m_s - m) l_s,
-// in split order.  A row that no split saw anything for is 0.
+// The splits of a query row together: out = sum_s 2^(m_s - m) acc_s / sum_s
+// 2^(m_s - m) l_s, in split order; a row that no split saw anything for is 0.
+// 16 (HD 64) or 32 lanes a row, 4 dims each; the lanes first take the splits'
+// weights, one each, then pass them round, so that the loads of the sums do not
+// wait for each other.
 template <int HD>
 __global__ __launch_bounds__(256) void k_tree_merge(const float* __restrict__ part_acc,
                                                     const float2* __restrict__ part_ml, int S, int rows_tile,
                                                     int tiles, int nodes, int nq, int nkv, int64_t total_rows,
                                                     uint16_t* __restrict__ out) {
+  constexpr int LPR = HD / 4;
   const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  const int d4 = static_cast<int>(i % (HD / 4));
-  const int64_t gr = i / (HD / 4);  // (pair, row of the pair)
-  if (gr >= total_rows) return;
+  const int d4 = static_cast<int>(threadIdx.x) % LPR;
+  const int lane0 = static_cast<int>(threadIdx.x & 63) - d4;  // the row's first lane
+  const int64_t gr0 = i / LPR;  // (pair, row of the pair)
+  const int64_t gr = gr0 < total_rows ? gr0 : total_rows - 1;
   const int group = nq / nkv, M = nodes * group;
   const int64_t pair = gr / M;
   const int r = static_cast<int>(gr % M);
   const int tile = r / rows_tile, row = r % rows_tile;
   const int64_t p0 = ((pair * tiles + tile) * S) * rows_tile + row;
   float m = -INFINITY;
-  for (int s = 0; s < S; ++s) m = fmaxf(m, part_ml[p0 + static_cast<int64_t>(s) * rows_tile].x);
+  for (int s = d4; s < S; s += LPR) m = fmaxf(m, part_ml[p0 + static_cast<int64_t>(s) * rows_tile].x);
+#pragma unroll
+  for (int off = 1; off < LPR; off <<= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
   float l = 0.f;
   float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int s = 0; s < S; ++s) {
-    const int64_t p = p0 + static_cast<int64_t>(s) * rows_tile;
-    const float2 ml = part_ml[p];
-    if (ml.y == 0.f) continue;  // nothing seen; its sums were not written
-    const float f = __builtin_amdgcn_exp2f(ml.x - m);
-    const float4 v = *reinterpret_cast<const float4*>(part_acc + p * HD + 4 * d4);
-    l += f * ml.y;
-    a.x += f * v.x;
-    a.y += f * v.y;
-    a.z += f * v.z;
-    a.w += f * v.w;
+  for (int s0 = 0; s0 < S; s0 += LPR) {
+    const int s = s0 + d4;
+    const float2 ml = s < S ? part_ml[p0 + static_cast<int64_t>(s) * rows_tile] : make_float2(-INFINITY, 0.f);
+    const float f = ml.y != 0.f ? __builtin_amdgcn_exp2f(ml.x - m) : 0.f;  // (0: nothing seen, sums not written)
+    const float fl = ml.y != 0.f ? f * ml.y : 0.f;
+    const int n = S - s0 < LPR ? S - s0 : LPR;
+    for (int j0 = 0; j0 < n; j0 += 8) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {  // (f is 0 past the last split)
+        const int j = j0 + e < n ? j0 + e : n - 1;
+        const float fj = j0 + e < LPR ? __shfl(f, lane0 + j0 + e, 64) : 0.f;
+        l += j0 + e < LPR ? __shfl(fl, lane0 + j0 + e, 64) : 0.f;
+        const float4 v =
+            *reinterpret_cast<const float4*>(part_acc + (p0 + static_cast<int64_t>(s0 + j) * rows_tile) * HD + 4 * d4);
+        a.x += fj != 0.f ? fj * v.x : 0.f;
+        a.y += fj != 0.f ? fj * v.y : 0.f;
+        a.z += fj != 0.f ? fj * v.z : 0.f;
+        a.w += fj != 0.f ? fj * v.w : 0.f;
+      }
+    }
   }
   if (l != 0.f) {
     const float inv = 1.0f / l;
     a = make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
   }
+  if (gr0 >= total_rows) return;
   const int64_t b = pair / nkv;
   const int kvh = static_cast<int>(pair % nkv);
   const uint2 w = {pack_bf16x2_rn(a.x, a.y), pack_bf16x2_rn(a.z, a.w)};
@@ -458,19 +545,20 @@ __global__ __launch_bounds__(256) void k_tree_merge(const float* __restrict__ pa
 }
 
 struct TreePlan {
-  int rb, tiles, splits;
+  int rw, tiles, splits;
   int64_t pairs;
 };
 
-static TreePlan tree_plan(int64_t batch, int64_t nodes, int nq, int nkv, int64_t max_len, int64_t window) {
+static TreePlan tree_plan(int64_t batch, int64_t nodes, int nq, int nkv, int head_dim, int64_t max_len,
+                          int64_t window) {
   TreePlan p;
   const int64_t M = nodes * (nq / nkv);
-  p.rb = M <= 16 ? 1 : (M <= 32 ? 2 : 4);
-  p.tiles = static_cast<int>(cdiv(M, 16 * p.rb));
+  p.rw = M <= 32 ? 1 : (M <= 64 ? 2 : 4);
+  p.tiles = static_cast<int>(cdiv(M, 32 * p.rw));
   p.pairs = batch * nkv;
   int64_t span = max_len;
   if (window > 0 && window + nodes < span) span = window + nodes;
-  const int64_t most = cdiv(span, kTreeChunk);
+  const int64_t most = cdiv(span, (head_dim == 64 && p.rw > 1 ? 64 : 32) * (4 / p.rw));
   int64_t s = kTreeTargetGroups / (p.pairs * p.tiles > 0 ? p.pairs * p.tiles : 1);
   s = s < 1 ? 1 : (s > most ? most : s);
   p.splits = static_cast<int>(s);
@@ -479,7 +567,7 @@ static TreePlan tree_plan(int64_t batch, int64_t nodes, int nq, int nkv, int64_t
 
 static size_t tree_ws_bytes(const TreePlan& p, int head_dim) {
   if (p.splits <= 1) return 0;
-  const size_t rows = static_cast<size_t>(p.pairs) * p.tiles * p.splits * 16 * p.rb;
+  const size_t rows = static_cast<size_t>(p.pairs) * p.tiles * p.splits * 32 * p.rw;
   return rows * (static_cast<size_t>(head_dim) * sizeof(float) + sizeof(float2));
 }
 
@@ -593,7 +681,7 @@ extern "C" size_t ma_tree_attn_workspace_bytes(int64_t batch, int64_t nodes, int
   if (batch < 1 || nodes < 1 || nodes > kTreeNodes || n_kv_heads < 1 || n_heads < n_kv_heads ||
       n_heads % n_kv_heads != 0 || (head_dim != 64 && head_dim != 128) || max_len < 1)
     return 0;
-  return tree_ws_bytes(tree_plan(batch, nodes, n_heads, n_kv_heads, max_len, window), head_dim);
+  return tree_ws_bytes(tree_plan(batch, nodes, n_heads, n_kv_heads, head_dim, max_len, window), head_dim);
 }
 
 extern "C" int ma_tree_attn(const void* q, int64_t batch, int64_t nodes, int n_heads, int n_kv_heads, int head_dim,
@@ -607,28 +695,29 @@ extern "C" int ma_tree_attn(const void* q, int64_t batch, int64_t nodes, int n_h
   if (!q || !k_cache || !v_cache || !seqlen || !parents || !out) return fail(MA_EVALUE, "tree_attn: null pointer");
   if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(out) || !aligned16(workspace))
     return fail(MA_EVALUE, "tree_attn: q, the cache, out and the workspace must be 16-byte aligned");
-  const TreePlan p = tree_plan(batch, nodes, n_heads, n_kv_heads, max_len, window);
+  const TreePlan p = tree_plan(batch, nodes, n_heads, n_kv_heads, head_dim, max_len, window);
   const size_t need = tree_ws_bytes(p, head_dim);
   if (need && (!workspace || workspace_bytes < need))
     return fail(MA_EVALUE, "tree_attn: workspace of %zu bytes, need %zu", workspace ? workspace_bytes : 0, need);
-  const int64_t part_rows = p.pairs * p.tiles * p.splits * 16 * p.rb;
+  const int64_t part_rows = p.pairs * p.tiles * p.splits * 32 * p.rw;
   float* const acc = static_cast<float*>(workspace);
   float2* const ml = need ? reinterpret_cast<float2*>(acc + part_rows * head_dim) : nullptr;
-  const dim3 grid(static_cast<unsigned>(p.splits), static_cast<unsigned>(p.tiles), static_cast<unsigned>(p.pairs));
+  const int64_t units = p.pairs * p.splits;
+  const dim3 grid(static_cast<unsigned>(cdiv(units, kXcds) * kXcds * p.tiles));
   hipStream_t s = static_cast<hipStream_t>(stream);
   auto go = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, static_cast<const uint16_t*>(q), static_cast<int>(nodes),
-                       n_heads, n_kv_heads, static_cast<const uint16_t*>(k_cache),
-                       static_cast<const uint16_t*>(v_cache), cache_rows, max_len, seqlen, parents, row_map, window,
-                       scale, static_cast<uint16_t*>(out), acc, ml);
+                       n_heads, n_kv_heads, p.tiles, p.splits, static_cast<int>(units),
+                       static_cast<const uint16_t*>(k_cache), static_cast<const uint16_t*>(v_cache), cache_rows,
+                       max_len, seqlen, parents, row_map, window, scale, static_cast<uint16_t*>(out), acc, ml);
   };
   if (head_dim == 64) {
-    if (p.rb == 1) go(k_tree_attn<64, 1>);
-    else if (p.rb == 2) go(k_tree_attn<64, 2>);
+    if (p.rw == 1) go(k_tree_attn<64, 1>);
+    else if (p.rw == 2) go(k_tree_attn<64, 2>);
     else go(k_tree_attn<64, 4>);
   } else {
-    if (p.rb == 1) go(k_tree_attn<128, 1>);
-    else if (p.rb == 2) go(k_tree_attn<128, 2>);
+    if (p.rw == 1) go(k_tree_attn<128, 1>);
+    else if (p.rw == 2) go(k_tree_attn<128, 2>);
     else go(k_tree_attn<128, 4>);
   }
   rc = check_launch("tree_attn");
@@ -636,7 +725,7 @@ extern "C" int ma_tree_attn(const void* q, int64_t batch, int64_t nodes, int n_h
   const int64_t rows = p.pairs * nodes * (n_heads / n_kv_heads);
   const dim3 mg(static_cast<unsigned>(cdiv(rows * (head_dim / 4), 256)));
   auto merge = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, mg, dim3(256), 0, s, acc, ml, p.splits, 16 * p.rb, p.tiles, static_cast<int>(nodes),
+    hipLaunchKernelGGL(kernel, mg, dim3(256), 0, s, acc, ml, p.splits, 32 * p.rw, p.tiles, static_cast<int>(nodes),
                        n_heads, n_kv_heads, rows, static_cast<uint16_t*>(out));
   };
   if (head_dim == 64) merge(k_tree_merge<64>);
