@@ -4,6 +4,8 @@
 // (ma_tree_commit).  Positions are clamped to the cache: a node whose slot
 // falls behind its end is neither stored nor attended, a mapped row outside
 // it is clamped, so nothing is read or written outside the cache.
+#include <type_traits>
+
 #include "tree.h"
 
 namespace ma {
@@ -138,6 +140,7 @@ struct TreeTile {
   static constexpr int kRegion = kNP * kRowBytes;                     // K or V of a group
   static constexpr int kStage = kPW * 2 * kRegion;
   static constexpr int kCopies = kNP / RW * kRowBytes / 1024;         // 1 KB copies of a wave, K and V each
+  static constexpr int kWaves = RW == 4 && HD == 64 ? 3 : (HD == 128 && RW == 1 ? 1 : 2);  // waves per SIMD (LDS, registers)
 };
 
 // The 16-byte piece c of LDS row r lies at piece c ^ tree_key(r) of that row:
@@ -170,7 +173,7 @@ struct TreeRow {
 // finite must not reach the rows that do not see it (0 x inf), so such values
 // are taken out of the product and added to the rows that see them.
 template <int HD, int RW>
-__global__ __launch_bounds__(256) void k_tree_attn(
+__global__ __launch_bounds__(256, (TreeTile<HD, RW>::kWaves)) void k_tree_attn(
     const uint16_t* __restrict__ q, int nodes, int nq, int nkv, int tiles, int S, int n_units,
     const uint16_t* __restrict__ k_cache, const uint16_t* __restrict__ v_cache, int64_t cache_rows, int64_t max_len,
     const int64_t* __restrict__ seqlen, const int32_t* __restrict__ parents, const int64_t* __restrict__ row_map,
@@ -282,92 +285,96 @@ __global__ __launch_bounds__(256) void k_tree_attn(
     for (int i = 0; i < 16; ++i) o[db][i] = 0.f;
   float mref = -INFINITY, lsum = 0.f;
 
-  auto attend = [&](int s, const char* buf) {
-    const int64_t tb = start + static_cast<int64_t>(s) * T::kStep + pw * T::kNP;
-    const char* const kb = buf + pw * 2 * T::kRegion;
-    const char* const vb = kb + T::kRegion;
-    const int g2 = (lane >> 4) & 1, i16 = lane & 15;
+  // Byte offsets into a group's K and V rows: piece 2 ks + h of row r32 (ks of
+  // one half; 128 bytes on for the other), and the lane's 8 bytes of the
+  // transposing read for even and odd 32-dim blocks (128 bytes on for each two).
+  // Rows 8 further have the same key.
+  const int g2 = (lane >> 4) & 1, i16 = lane & 15;
+  int koff[4], voff[2];
 #pragma unroll
-    for (int st = 0; st < T::kNP / 32; ++st) {
-      const int64_t t0 = tb + 32 * st;
-      if (t0 >= end) break;
-      f32x16t_t sc;
+  for (int i = 0; i < 4; ++i) koff[i] = r32 * T::kRowBytes + (((2 * i + h) ^ tree_key(r32)) << 4);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) sc[i] = 0.f;
-      const int kr = 32 * st + r32, kk = tree_key(kr);
+  for (int i = 0; i < 2; ++i) {
+    const int vr = 4 * h + (i16 >> 2);
+    voff[i] = vr * T::kRowBytes + (((4 * i + 2 * g2 + ((i16 & 3) >> 1)) ^ tree_key(vr)) << 4) + (i16 & 1) * 8;
+  }
+
+  // 32 positions from t0, their K rows at kb and V rows at vb.
+  auto attend32 = [&](auto masked_c, int64_t t0, const char* kb, const char* vb) {
+    constexpr bool MASKED = decltype(masked_c)::value;
+    f32x16t_t sc;
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
-        sc = mfma_tree(*reinterpret_cast<const uint4*>(kb + kr * T::kRowBytes + (((2 * ks + h) ^ kk) << 4)), qf[ks], sc);
-      const bool masked = t0 + 32 > n0 || t0 < whole;
-      uint32_t sees = 0xffffffffu;  // bit p: the row sees position t0 + p
-      if (masked) {
-        const int64_t off = t0 - n0;  // node index of the first position
-        uint64_t w = off >= 64 ? 0ull : (off >= 0 ? row.anc >> off : (off > -32 ? row.anc << -off : 0ull));
-        if (off < 0) {  // and the sequence's part, from row.from on
-          const uint32_t seq = off <= -32 ? 0xffffffffu : (1u << -off) - 1u;
-          const int64_t lo = row.from - t0;
-          w |= lo >= 32 ? 0u : (lo > 0 ? seq & (0xffffffffu << lo) : seq);
-        }
-        sees = static_cast<uint32_t>(w);
-        const uint32_t mine = sees >> (4 * h);
+    for (int i = 0; i < 16; ++i) sc[i] = 0.f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) sc[i] = (mine >> (8 * (i >> 2) + (i & 3))) & 1u ? sc[i] : -INFINITY;
+    for (int ks = 0; ks < KS; ++ks)
+      sc = mfma_tree(*reinterpret_cast<const uint4*>(kb + koff[ks & 3] + 128 * (ks >> 2)), qf[ks], sc);
+    uint32_t sees = 0xffffffffu;  // bit p: the row sees position t0 + p
+    if constexpr (MASKED) {
+      const int64_t off = t0 - n0;  // node index of the first position
+      uint64_t w = off >= 64 ? 0ull : (off >= 0 ? row.anc >> off : (off > -32 ? row.anc << -off : 0ull));
+      if (off < 0) {  // and the sequence's part, from row.from on
+        const uint32_t seq = off <= -32 ? 0xffffffffu : (1u << -off) - 1u;
+        const int64_t lo = row.from - t0;
+        w |= lo >= 32 ? 0u : (lo > 0 ? seq & (0xffffffffu << lo) : seq);
       }
-      float cm = sc[0];
+      sees = static_cast<uint32_t>(w);
+      const uint32_t mine = sees >> (4 * h);
 #pragma unroll
-      for (int i = 1; i < 16; ++i) cm = fmaxf(cm, sc[i]);
-      cm *= scale2;
-      if (__any(!(cm <= mref + kTreeGrow))) {
-        cm = fmaxf(cm, __shfl_xor(cm, 32, 64));
-        const float mn = fmaxf(mref, cm);
-        const float a = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mref - mn);
-        mref = mn;
-        lsum *= a;
+      for (int i = 0; i < 16; ++i) sc[i] = (mine >> (8 * (i >> 2) + (i & 3))) & 1u ? sc[i] : -INFINITY;
+    }
+    float cm = sc[0];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float ai = __shfl(a, 8 * (i >> 2) + 4 * h + (i & 3), 64);
+    for (int i = 1; i < 16; ++i) cm = fmaxf(cm, sc[i]);
+    cm *= scale2;
+    if (__any(!(cm <= mref + kTreeGrow))) {
+      cm = fmaxf(cm, __shfl_xor(cm, 32, 64));
+      const float mn = fmaxf(mref, cm);
+      const float a = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mref - mn);
+      mref = mn;
+      lsum *= a;
 #pragma unroll
-          for (int db = 0; db < DB; ++db) o[db][i] *= ai;
-        }
+      for (int i = 0; i < 16; ++i) {
+        const float ai = __shfl(a, 8 * (i >> 2) + 4 * h + (i & 3), 64);
+#pragma unroll
+        for (int db = 0; db < DB; ++db) o[db][i] *= ai;
       }
-      const float m = mref == -INFINITY ? 0.f : mref;
-      uint32_t bad = 0;
+    }
+    const float m = mref == -INFINITY ? 0.f : mref;
+    uint32_t bad = 0;
 #pragma unroll
-      for (int k2 = 0; k2 < 2; ++k2) {
-        uint32_t p[4];
+    for (int k2 = 0; k2 < 2; ++k2) {
+      uint32_t p[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[8 * k2 + 2 * e], scale2, -m));
-          const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[8 * k2 + 2 * e + 1], scale2, -m));
-          p[e] = pack_bf16x2_rn(p0, p1);
-          lsum = dot2(p[e], kOneBf16x2, lsum);
-        }
-        const uint4 pa = make_uint4(p[0], p[1], p[2], p[3]);
+      for (int e = 0; e < 4; ++e) {
+        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[8 * k2 + 2 * e], scale2, -m));
+        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[8 * k2 + 2 * e + 1], scale2, -m));
+        p[e] = pack_bf16x2_rn(p0, p1);
+        lsum = dot2(p[e], kOneBf16x2, lsum);
+      }
+      const uint4 pa = make_uint4(p[0], p[1], p[2], p[3]);
 #pragma unroll
-        for (int db = 0; db < DB; ++db) {
-          s16x4t_t v[2];
+      for (int db = 0; db < DB; ++db) {
+        s16x4t_t v[2];
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int vr = 32 * st + 16 * k2 + 8 * e + 4 * h + (i16 >> 2);
-            const int pc = 4 * db + 2 * g2 + ((i16 & 3) >> 1);
-            v[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4t_t*)(
-                vb + vr * T::kRowBytes + ((pc ^ tree_key(vr)) << 4) + (i16 & 1) * 8));
+        for (int e = 0; e < 2; ++e)
+          v[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4t_t*)(
+              vb + voff[db & 1] + (16 * k2 + 8 * e) * T::kRowBytes + 128 * (db >> 1)));
+        const uint2 v0 = __builtin_bit_cast(uint2, v[0]), v1 = __builtin_bit_cast(uint2, v[1]);
+        uint32_t w[4] = {v0.x, v0.y, v1.x, v1.y};
+        if constexpr (MASKED) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t odd = ((w[j] & 0x7F80u) == 0x7F80u ? 0xFFFFu : 0u) |
+                                 ((w[j] & 0x7F800000u) == 0x7F800000u ? 0xFFFF0000u : 0u);
+            bad |= odd;
+            w[j] &= ~odd;
           }
-          const uint2 v0 = __builtin_bit_cast(uint2, v[0]), v1 = __builtin_bit_cast(uint2, v[1]);
-          uint32_t w[4] = {v0.x, v0.y, v1.x, v1.y};
-          if (masked) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const uint32_t odd = ((w[j] & 0x7F80u) == 0x7F80u ? 0xFFFFu : 0u) |
-                                   ((w[j] & 0x7F800000u) == 0x7F800000u ? 0xFFFF0000u : 0u);
-              bad |= odd;
-              w[j] &= ~odd;
-            }
-          }
-          o[db] = mfma_tree(pa, make_uint4(w[0], w[1], w[2], w[3]), o[db]);
         }
+        o[db] = mfma_tree(pa, make_uint4(w[0], w[1], w[2], w[3]), o[db]);
       }
-      if (masked && __any(bad != 0)) {
+    }
+    if constexpr (MASKED) {
+      if (__any(bad != 0)) {
         for (int p = 0; p < 32; ++p) {
           const int64_t t = t0 + p < end ? t0 + p : end - 1;
           float v[DB];
@@ -384,6 +391,18 @@ __global__ __launch_bounds__(256) void k_tree_attn(
           }
         }
       }
+    }
+  };
+  auto attend = [&](int s, const char* buf) {
+    const int64_t tb = start + static_cast<int64_t>(s) * T::kStep + pw * T::kNP;
+    const char* const kb = buf + pw * 2 * T::kRegion;
+#pragma unroll
+    for (int st = 0; st < T::kNP / 32; ++st) {
+      const int64_t t0 = tb + 32 * st;
+      if (t0 >= end) break;
+      const char* const k = kb + 32 * st * T::kRowBytes;
+      if (t0 + 32 > n0 || t0 < whole) attend32(std::true_type{}, t0, k, k + T::kRegion);
+      else attend32(std::false_type{}, t0, k, k + T::kRegion);
     }
   };
 
@@ -486,60 +505,85 @@ __global__ __launch_bounds__(256) void k_tree_attn(
 }
 
 // The splits of a query row together: out = sum_s 2^(m_s - m) acc_s / sum_s
-// 2^(m_s - m) l_s, in split order; a row that no split saw anything for is 0.
-// 16 (HD 64) or 32 lanes a row, 4 dims each; the lanes first take the splits'
-// weights, one each, then pass them round, so that the loads of the sums do not
-// wait for each other.
+// 2^(m_s - m) l_s; a row that no split saw anything for is 0.  HD / 4 lanes of 4
+// dims times G groups of splits a row: a thread takes the splits g, g + G, ..,
+// all loads of four at once and relative to its own maximum, then the groups
+// meet in LDS, in order.
 template <int HD>
 __global__ __launch_bounds__(256) void k_tree_merge(const float* __restrict__ part_acc,
-                                                    const float2* __restrict__ part_ml, int S, int rows_tile,
+                                                    const float2* __restrict__ part_ml, int S, int G, int rows_tile,
                                                     int tiles, int nodes, int nq, int nkv, int64_t total_rows,
                                                     uint16_t* __restrict__ out) {
   constexpr int LPR = HD / 4;
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  const int d4 = static_cast<int>(threadIdx.x) % LPR;
-  const int lane0 = static_cast<int>(threadIdx.x & 63) - d4;  // the row's first lane
-  const int64_t gr0 = i / LPR;  // (pair, row of the pair)
+  __shared__ float4 sa[256];
+  __shared__ float2 sml[256];
+  const int tid = threadIdx.x, d4 = tid % LPR, g = tid / LPR % G;
+  const int64_t gr0 = static_cast<int64_t>(blockIdx.x) * (256 / (LPR * G)) + tid / (LPR * G);  // (pair, its row)
   const int64_t gr = gr0 < total_rows ? gr0 : total_rows - 1;
   const int group = nq / nkv, M = nodes * group;
   const int64_t pair = gr / M;
-  const int r = static_cast<int>(gr % M);
-  const int tile = r / rows_tile, row = r % rows_tile;
+  const int r = static_cast<int>(gr - pair * M);
+  const int tile = r / rows_tile, row = r - tile * rows_tile;
   const int64_t p0 = ((pair * tiles + tile) * S) * rows_tile + row;
-  float m = -INFINITY;
-  for (int s = d4; s < S; s += LPR) m = fmaxf(m, part_ml[p0 + static_cast<int64_t>(s) * rows_tile].x);
-#pragma unroll
-  for (int off = 1; off < LPR; off <<= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
-  float l = 0.f;
+  float m = -INFINITY, l = 0.f;
   float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int s0 = 0; s0 < S; s0 += LPR) {
-    const int s = s0 + d4;
-    const float2 ml = s < S ? part_ml[p0 + static_cast<int64_t>(s) * rows_tile] : make_float2(-INFINITY, 0.f);
-    const float f = ml.y != 0.f ? __builtin_amdgcn_exp2f(ml.x - m) : 0.f;  // (0: nothing seen, sums not written)
-    const float fl = ml.y != 0.f ? f * ml.y : 0.f;
-    const int n = S - s0 < LPR ? S - s0 : LPR;
-    for (int j0 = 0; j0 < n; j0 += 8) {
+  for (int s0 = g; s0 < S; s0 += 4 * G) {
+    float2 ml[4];
+    float4 v[4];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {  // (f is 0 past the last split)
-        const int j = j0 + e < n ? j0 + e : n - 1;
-        const float fj = j0 + e < LPR ? __shfl(f, lane0 + j0 + e, 64) : 0.f;
-        l += j0 + e < LPR ? __shfl(fl, lane0 + j0 + e, 64) : 0.f;
-        const float4 v =
-            *reinterpret_cast<const float4*>(part_acc + (p0 + static_cast<int64_t>(s0 + j) * rows_tile) * HD + 4 * d4);
-        a.x += fj != 0.f ? fj * v.x : 0.f;
-        a.y += fj != 0.f ? fj * v.y : 0.f;
-        a.z += fj != 0.f ? fj * v.z : 0.f;
-        a.w += fj != 0.f ? fj * v.w : 0.f;
+    for (int e = 0; e < 4; ++e) {
+      const int s = s0 + e * G < S ? s0 + e * G : g;
+      const int64_t p = p0 + static_cast<int64_t>(s) * rows_tile;
+      ml[e] = part_ml[p];
+      v[e] = *reinterpret_cast<const float4*>(part_acc + p * HD + 4 * d4);
+      if (s0 + e * G >= S) ml[e] = make_float2(-INFINITY, 0.f);
+    }
+    float mn = m;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) mn = fmaxf(mn, ml[e].x);
+    const float f = l != 0.f ? __builtin_amdgcn_exp2f(m - mn) : 0.f;
+    m = mn;
+    l *= f;
+    a = make_float4(a.x * f, a.y * f, a.z * f, a.w * f);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (ml[e].y != 0.f) {  // (0: nothing seen, sums not written)
+        const float fe = __builtin_amdgcn_exp2f(ml[e].x - m);
+        l += fe * ml[e].y;
+        a.x += fe * v[e].x;
+        a.y += fe * v[e].y;
+        a.z += fe * v[e].z;
+        a.w += fe * v[e].w;
       }
+  }
+  if (G > 1) {
+    sa[tid] = a;
+    sml[tid] = make_float2(m, l);
+    __syncthreads();
+    if (g > 0) return;
+    for (int e = 1; e < G; ++e) m = fmaxf(m, sml[tid + e * LPR].x);
+    const float f = l != 0.f ? __builtin_amdgcn_exp2f(sml[tid].x - m) : 0.f;
+    l *= f;
+    a = l != 0.f ? make_float4(a.x * f, a.y * f, a.z * f, a.w * f) : make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int e = 1; e < G; ++e) {
+      const float2 ml = sml[tid + e * LPR];
+      if (ml.y == 0.f) continue;
+      const float fe = __builtin_amdgcn_exp2f(ml.x - m);
+      const float4 v = sa[tid + e * LPR];
+      l += fe * ml.y;
+      a.x += fe * v.x;
+      a.y += fe * v.y;
+      a.z += fe * v.z;
+      a.w += fe * v.w;
     }
   }
+  if (gr0 >= total_rows) return;
   if (l != 0.f) {
     const float inv = 1.0f / l;
     a = make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
   }
-  if (gr0 >= total_rows) return;
   const int64_t b = pair / nkv;
-  const int kvh = static_cast<int>(pair % nkv);
+  const int kvh = static_cast<int>(pair - b * nkv);
   const uint2 w = {pack_bf16x2_rn(a.x, a.y), pack_bf16x2_rn(a.z, a.w)};
   *reinterpret_cast<uint2*>(out + ((b * nodes + r / group) * nq + kvh * group + r % group) * HD + 4 * d4) = w;
 }
@@ -723,9 +767,11 @@ extern "C" int ma_tree_attn(const void* q, int64_t batch, int64_t nodes, int n_h
   rc = check_launch("tree_attn");
   if (rc != MA_OK || p.splits == 1) return rc;
   const int64_t rows = p.pairs * nodes * (n_heads / n_kv_heads);
-  const dim3 mg(static_cast<unsigned>(cdiv(rows * (head_dim / 4), 256)));
+  int G = 1;  // split groups of the merge: one for each four splits
+  while (G < 1024 / head_dim && 4 * G < p.splits) G *= 2;
+  const dim3 mg(static_cast<unsigned>(cdiv(rows * (head_dim / 4) * G, 256)));
   auto merge = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, mg, dim3(256), 0, s, acc, ml, p.splits, 32 * p.rw, p.tiles, static_cast<int>(nodes),
+    hipLaunchKernelGGL(kernel, mg, dim3(256), 0, s, acc, ml, p.splits, G, 32 * p.rw, p.tiles, static_cast<int>(nodes),
                        n_heads, n_kv_heads, rows, static_cast<uint16_t*>(out));
   };
   if (head_dim == 64) merge(k_tree_merge<64>);
