@@ -23,9 +23,15 @@ struct TreeLane {
 // nodes on the last 2^n steps of its way up and the node those end at, and
 // doubles both by what that node holds (six rounds for 64 nodes), so that no
 // lane walks up node by node.
-__device__ __forceinline__ TreeLane tree_lane(const int32_t* __restrict__ parents, int nodes) {
+//
+// tree_parent: the lane's entry of parents; tree_lane: its node (par: all lanes'
+// entries).
+__device__ __forceinline__ int tree_parent(const int32_t* __restrict__ parents, int nodes) {
   const int lane = static_cast<int>(threadIdx.x & 63);
-  const int par = lane < nodes ? parents[lane] : -1;
+  return lane < nodes ? parents[lane] : -1;
+}
+__device__ __forceinline__ TreeLane tree_lane(int par, int nodes) {
+  const int lane = static_cast<int>(threadIdx.x & 63);
   int up = lane > 0 && par >= 0 && par < lane ? par : -1;
   uint64_t anc = 1ull << lane;
   const bool root = __builtin_amdgcn_readfirstlane(par) == -1;
@@ -39,6 +45,9 @@ __device__ __forceinline__ TreeLane tree_lane(const int32_t* __restrict__ parent
   }
   const bool present = root && lane < nodes && (anc & 1ull);
   return {present ? anc : 0ull, present ? static_cast<int>(__popcll(anc)) - 1 : -1};
+}
+__device__ __forceinline__ TreeLane tree_lane(const int32_t* __restrict__ parents, int nodes) {
+  return tree_lane(tree_parent(parents, nodes), nodes);
 }
 
 }  // namespace ma

@@ -4,7 +4,8 @@
 // (ma_tree_commit).  Positions are clamped to the cache: a node whose slot
 // falls behind its end is neither stored nor attended, a mapped row outside
 // it is clamped, so nothing is read or written outside the cache.
-#include <type_traits>
+
+#include <math.h>
 
 #include "tree.h"
 
@@ -118,7 +119,6 @@ __global__ __launch_bounds__(64) void k_tree_qkv(
 // Attention
 // ---------------------------------------------------------------------------
 typedef __attribute__((address_space(3))) void* tree_lds_t;
-constexpr int kTreeTargetGroups = 1024;  // workgroups a launch aims for
 constexpr float kTreeGrow = 8.0f;        // a row's reference maximum is moved when a score passes it by 2^8
 constexpr int tree_vmcnt(int n) { return (n & 0xF) | (0x7 << 4) | ((n >> 4) << 14); }  // and lgkmcnt(0)
 
@@ -147,6 +147,14 @@ struct TreeTile {
 // the 8 rows that a K read takes the same piece of, and the 4 that a V read
 // takes 4 pieces of, then fall into different banks.
 __device__ __forceinline__ int tree_key(int r) { return ((r & 1) << 2) | ((r >> 1) & 3); }
+
+// Two bf16 values without those that are not finite; what was taken out.
+__device__ __forceinline__ uint32_t take_odd(uint32_t& w) {
+  const uint32_t odd =
+      ((w & 0x7F80u) == 0x7F80u ? 0xFFFFu : 0u) | ((w & 0x7F800000u) == 0x7F800000u ? 0xFFFF0000u : 0u);
+  w &= ~odd;
+  return odd;
+}
 
 struct TreeRow {
   uint64_t anc;  // the ancestors seen
@@ -183,6 +191,7 @@ __global__ __launch_bounds__(256, (TreeTile<HD, RW>::kWaves)) void k_tree_attn(
   constexpr int KS = HD / 16;  // k slices of a score
   constexpr int DB = HD / 32;  // 32-dim blocks of the output
   constexpr int CPR = HD / 8;  // 16-byte pieces of a cache row
+  constexpr int NT = T::kNP / 32;
   __shared__ __align__(16) char buf0[T::kStage];
   __shared__ __align__(16) char buf1[T::kStage];
   __shared__ __align__(16) char buf2[T::kBufs == 3 ? T::kStage : 16];
@@ -194,7 +203,7 @@ __global__ __launch_bounds__(256, (TreeTile<HD, RW>::kWaves)) void k_tree_attn(
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int rw = wv % RW, pw = wv / RW;
+  const int rw = RW == 4 ? wv : wv % RW, pw = RW == 4 ? 0 : wv / RW;
   const int r32 = lane & 31, h = lane >> 5;
   // tiles of the same positions follow each other on one XCD
   const int xcd = blockIdx.x % kXcds, turn = blockIdx.x / kXcds;
@@ -206,52 +215,69 @@ __global__ __launch_bounds__(256, (TreeTile<HD, RW>::kWaves)) void k_tree_attn(
   const int kvh = static_cast<int>(pair - b * nkv);
   const int group = nq / nkv, M = nodes * group;
 
-  const TreeLane me = tree_lane(parents + b * nodes, nodes);
+  // The first copies wait for the row's length alone; its tree is found while
+  // they are in flight.
   const int64_t n0 = clamp_pos(seqlen[b], 0, max_len);
   const int64_t crow = row_map ? clamp_pos(row_map[b], 0, cache_rows - 1) : b;
+  const int64_t end = n0 + nodes < max_len ? n0 + nodes : max_len;
+  const int64_t start = window > 0 && n0 + 1 > window ? n0 + 1 - window : 0;
+  const int n_steps = static_cast<int>(cdiv(end - start, T::kStep));
+  const int sps = (n_steps + S - 1) / S;
+  const int s_beg = sp * sps < n_steps ? sp * sps : n_steps;
+  int s_end = s_beg + sps < n_steps ? s_beg + sps : n_steps;
+  // positions at or behind n0, or (with a window) before `whole`, are not seen by every row
+  const int64_t whole = window > 0 ? n0 + nodes - window : 0;
+  const int64_t base = (crow * nkv + kvh) * max_len;
+
+  // copies of step s into a buffer: each wave its share of its group's rows,
+  // rows past the end read again from the last one
+  const int copy_row = rw * (T::kNP / RW) + lane / CPR;
+  auto copy = [&](int s, char* buf) {
+    const int64_t t0 = start + static_cast<int64_t>(s) * T::kStep + pw * T::kNP;
+    char* const dst = buf + pw * 2 * T::kRegion + rw * (T::kNP / RW) * T::kRowBytes;
+    const int64_t left = end - 1 - t0;  // (negative: the group has none; its copies all take the last row)
+    const int64_t at = left < 0 ? end - 1 : t0;
+    const int most = left < 0 ? 0 : (left < T::kNP ? static_cast<int>(left) : T::kNP - 1);
+    const char* const ks = reinterpret_cast<const char*>(k_cache + (base + at) * HD);
+    const char* const vs = reinterpret_cast<const char*>(v_cache + (base + at) * HD);
+#pragma unroll
+    for (int i = 0; i < T::kCopies; ++i) {
+      const int row = copy_row + i * (64 / CPR);
+      const uint32_t off = (row < most ? row : most) * T::kRowBytes + 16 * ((lane % CPR) ^ tree_key(row));
+      __builtin_amdgcn_global_load_lds(ks + off, (tree_lds_t)(dst + i * 1024), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds(vs + off, (tree_lds_t)(dst + T::kRegion + i * 1024), 16, 0, 0);
+    }
+  };
+  // this lane's query row, as it is in memory
+  const int r = tile * T::kRows + rw * 32 + r32;
+  const int node = r < M ? r / group : 0;
+  uint4 qf[KS];
+  {
+    const uint16_t* const src = q + ((b * nodes + node) * nq + kvh * group + (r < M ? r % group : 0)) * HD + 8 * h;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) qf[ks] = *reinterpret_cast<const uint4*>(src + 16 * ks);
+  }
+  const int par = tree_parent(parents + b * nodes, nodes);
+  MA_ISSUE_FENCE();
+  if (s_beg < s_end) copy(s_beg, buf0);
+  if (T::kBufs == 3 && s_beg + 1 < s_end) copy(s_beg + 1, buf1);
+  MA_ISSUE_FENCE();
+  const TreeLane me = tree_lane(par, nodes);
   if (wv == 0) {
     t_anc[lane] = me.anc;
     t_depth[lane] = me.depth;
   }
   const uint64_t here = __ballot(me.depth >= 0);
-  const int last = here ? 63 - static_cast<int>(__builtin_clzll(here)) : -1;
-  int64_t end = n0 + last + 1;
-  end = end < max_len ? end : max_len;
-  const int64_t start = window > 0 && n0 + 1 > window ? n0 + 1 - window : 0;
-  const bool any_row = last >= 0 && tile * T::kRows < (last + 1) * group;
-  const int n_steps = any_row && end > start ? static_cast<int>(cdiv(end - start, T::kStep)) : 0;
-  const int sps = (n_steps + S - 1) / S;
-  const int s_beg = sp * sps < n_steps ? sp * sps : n_steps;
-  const int s_end = s_beg + sps < n_steps ? s_beg + sps : n_steps;
-  // 32 positions at or behind n0, or (with a window) before `whole`, are masked
-  const int64_t whole = window > 0 ? n0 + nodes - window : 0;
-  const int64_t base = (crow * nkv + kvh) * max_len;
-
-  // copies of step s into a buffer: each wave its share of its group's rows
-  const int copy_row = rw * (T::kNP / RW) + lane / CPR;
-  auto copy = [&](int s, char* buf) {
-    const int64_t t0 = start + static_cast<int64_t>(s) * T::kStep + pw * T::kNP;
-    char* const dst = buf + pw * 2 * T::kRegion + rw * (T::kNP / RW) * T::kRowBytes;
-#pragma unroll
-    for (int i = 0; i < T::kCopies; ++i) {
-      const int row = copy_row + i * (64 / CPR);
-      int64_t t = t0 + row;
-      t = t < end ? t : end - 1;
-      const int64_t off = (base + t) * HD + 8 * ((lane % CPR) ^ tree_key(row));
-      __builtin_amdgcn_global_load_lds(k_cache + off, (tree_lds_t)(dst + i * 1024), 16, 0, 0);
-      __builtin_amdgcn_global_load_lds(v_cache + off, (tree_lds_t)(dst + T::kRegion + i * 1024), 16, 0, 0);
-    }
-  };
-  if (s_beg < s_end) copy(s_beg, buf0);
-  if (T::kBufs == 3 && s_beg + 1 < s_end) copy(s_beg + 1, buf1);
+  const int rows_here = here ? (64 - static_cast<int>(__builtin_clzll(here))) * group : 0;
+  if (tile * T::kRows >= rows_here) {  // a tile of padding
+    __builtin_amdgcn_s_waitcnt(tree_vmcnt(0));
+    s_end = s_beg;
+  }
   // the tree's table for every wave (the copies stay in flight)
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 
-  // this lane's query row
-  const int r = tile * T::kRows + rw * 32 + r32;
-  const int node = r < M ? r / group : 0;
   const int depth = r < M ? t_depth[node] : -1;
   TreeRow row{0ull, INT64_MAX};
   if (depth >= 0) {
@@ -266,16 +292,13 @@ __global__ __launch_bounds__(256, (TreeTile<HD, RW>::kWaves)) void k_tree_attn(
   const bool busy = __any(depth >= 0);  // this wave has rows
   // a negative scale is taken with -q, a zero one with q = 0 (both exact)
   const float scale2 = scale == 0.f ? 1.f : fabsf(scale) * kLog2e;
-  uint4 qf[KS];
   {
-    const uint16_t* const src = q + ((b * nodes + node) * nq + kvh * group + (r < M ? r % group : 0)) * HD + 8 * h;
     const uint32_t flip = scale < 0.f ? 0x80008000u : 0u;
     const uint32_t keep = depth >= 0 && scale != 0.f ? 0xffffffffu : 0u;
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      const uint4 w = *reinterpret_cast<const uint4*>(src + 16 * ks);
-      qf[ks] = make_uint4((w.x ^ flip) & keep, (w.y ^ flip) & keep, (w.z ^ flip) & keep, (w.w ^ flip) & keep);
-    }
+    for (int ks = 0; ks < KS; ++ks)
+      qf[ks] = make_uint4((qf[ks].x ^ flip) & keep, (qf[ks].y ^ flip) & keep, (qf[ks].z ^ flip) & keep,
+                          (qf[ks].w ^ flip) & keep);
   }
 
   f32x16t_t o[DB];
@@ -299,137 +322,201 @@ __global__ __launch_bounds__(256, (TreeTile<HD, RW>::kWaves)) void k_tree_attn(
     voff[i] = vr * T::kRowBytes + (((4 * i + 2 * g2 + ((i16 & 3) >> 1)) ^ tree_key(vr)) << 4) + (i16 & 1) * 8;
   }
 
-  // 32 positions from t0, their K rows at kb and V rows at vb.
-  auto attend32 = [&](auto masked_c, int64_t t0, const char* kb, const char* vb) {
-    constexpr bool MASKED = decltype(masked_c)::value;
+  // Lane address (bytes) of output row i's query row: 4 (8 (i / 4) + 4 h + i % 4).
+  // (Made anew where it is used: held in registers, the 16 of them cost the
+  // main loop its third wave.)
+  auto row_lane = [&](int i) {
+    int a = 16 * h;
+    asm volatile("" : "+v"(a));
+    return a + 4 * (8 * (i >> 2) + (i & 3));
+  };
+  auto of_row = [&](float v, int i) {
+    return __int_as_float(__builtin_amdgcn_ds_bpermute(row_lane(i), __float_as_int(v)));
+  };
+  auto rescale = [&](float cm) {
+    cm = fmaxf(cm, __shfl_xor(cm, 32, 64));
+    const float mn = fmaxf(mref, cm);
+    const float a = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mref - mn);
+    mref = mn;
+    lsum *= a;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float ai = of_row(a, i);
+#pragma unroll
+      for (int db = 0; db < DB; ++db) o[db][i] *= ai;
+    }
+  };
+  auto v_read = [&](const char* vb, int t, int k2, int db) {
+    uint2 v[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      v[e] = __builtin_bit_cast(uint2,
+                                __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4t_t*)(
+                                    vb + voff[db & 1] + (32 * t + 16 * k2 + 8 * e) * T::kRowBytes + 128 * (db >> 1))));
+    return make_uint4(v[0].x, v[0].y, v[1].x, v[1].y);
+  };
+  // The weights of scores 8 k2 .. +7, as the A operand of their product.
+  auto weights = [&](const f32x16t_t& sc, int k2, float m) {
+    uint32_t p[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[8 * k2 + 2 * e], scale2, -m));
+      const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[8 * k2 + 2 * e + 1], scale2, -m));
+      p[e] = pack_bf16x2_rn(p0, p1);
+      lsum = dot2(p[e], kOneBf16x2, lsum);
+    }
+    return make_uint4(p[0], p[1], p[2], p[3]);
+  };
+
+  // The NT x 32 positions of a group that all rows see: all K reads ahead of the
+  // first product, the V reads ahead of the softmax.
+  auto attend = [&](const char* buf) {
+    const char* const kb = buf + pw * 2 * T::kRegion;
+    const char* const vb = kb + T::kRegion;
+    f32x16t_t sc[NT];
+    {
+      uint4 kf[NT][KS];
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+          kf[t][ks] = *reinterpret_cast<const uint4*>(kb + 32 * t * T::kRowBytes + koff[ks & 3] + 128 * (ks >> 2));
+      MA_ISSUE_FENCE();
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sc[t][i] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) sc[t] = mfma_tree(kf[t][ks], qf[ks], sc[t]);
+    }
+    uint4 vf[NT][2][DB];
+    auto v_tile = [&](int t) {
+#pragma unroll
+      for (int k2 = 0; k2 < 2; ++k2)
+#pragma unroll
+        for (int db = 0; db < DB; ++db) vf[t][k2][db] = v_read(vb, t, k2, db);
+    };
+    v_tile(0);
+    MA_ISSUE_FENCE();
+    float cm = sc[0][0];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) cm = fmaxf(cm, sc[t][i]);
+    cm *= scale2;
+    if (__any(!(cm <= mref + kTreeGrow))) rescale(cm);
+    const float m = mref == -INFINITY ? 0.f : mref;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const uint4 pa0 = weights(sc[t], 0, m);
+      if (t + 1 < NT) v_tile(t + 1);
+#pragma unroll
+      for (int db = 0; db < DB; ++db) o[db] = mfma_tree(pa0, vf[t][0][db], o[db]);
+      const uint4 pa1 = weights(sc[t], 1, m);
+#pragma unroll
+      for (int db = 0; db < DB; ++db) o[db] = mfma_tree(pa1, vf[t][1][db], o[db]);
+    }
+  };
+
+  // 32 positions from t0 of which some row may see only part.
+  auto attend_edge = [&](int64_t t0, const char* kb, const char* vb) {
     f32x16t_t sc;
 #pragma unroll
     for (int i = 0; i < 16; ++i) sc[i] = 0.f;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks)
       sc = mfma_tree(*reinterpret_cast<const uint4*>(kb + koff[ks & 3] + 128 * (ks >> 2)), qf[ks], sc);
-    uint32_t sees = 0xffffffffu;  // bit p: the row sees position t0 + p
-    if constexpr (MASKED) {
-      const int64_t off = t0 - n0;  // node index of the first position
-      uint64_t w = off >= 64 ? 0ull : (off >= 0 ? row.anc >> off : (off > -32 ? row.anc << -off : 0ull));
-      if (off < 0) {  // and the sequence's part, from row.from on
-        const uint32_t seq = off <= -32 ? 0xffffffffu : (1u << -off) - 1u;
-        const int64_t lo = row.from - t0;
-        w |= lo >= 32 ? 0u : (lo > 0 ? seq & (0xffffffffu << lo) : seq);
-      }
-      sees = static_cast<uint32_t>(w);
-      const uint32_t mine = sees >> (4 * h);
-#pragma unroll
-      for (int i = 0; i < 16; ++i) sc[i] = (mine >> (8 * (i >> 2) + (i & 3))) & 1u ? sc[i] : -INFINITY;
+    const int64_t off = t0 - n0;  // node index of the first position
+    uint64_t w = off >= 64 ? 0ull : (off >= 0 ? row.anc >> off : (off > -32 ? row.anc << -off : 0ull));
+    if (off < 0) {  // and the sequence's part, from row.from on
+      const uint32_t seq = off <= -32 ? 0xffffffffu : (1u << -off) - 1u;
+      const int64_t lo = row.from - t0;
+      w |= lo >= 32 ? 0u : (lo > 0 ? seq & (0xffffffffu << lo) : seq);
     }
+    const uint32_t sees = static_cast<uint32_t>(w);  // bit p: the row sees position t0 + p
+    const uint32_t mine = sees >> (4 * h);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sc[i] = (mine >> (8 * (i >> 2) + (i & 3))) & 1u ? sc[i] : -INFINITY;
     float cm = sc[0];
 #pragma unroll
     for (int i = 1; i < 16; ++i) cm = fmaxf(cm, sc[i]);
     cm *= scale2;
-    if (__any(!(cm <= mref + kTreeGrow))) {
-      cm = fmaxf(cm, __shfl_xor(cm, 32, 64));
-      const float mn = fmaxf(mref, cm);
-      const float a = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mref - mn);
-      mref = mn;
-      lsum *= a;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float ai = __shfl(a, 8 * (i >> 2) + 4 * h + (i & 3), 64);
-#pragma unroll
-        for (int db = 0; db < DB; ++db) o[db][i] *= ai;
-      }
-    }
+    if (__any(!(cm <= mref + kTreeGrow))) rescale(cm);
     const float m = mref == -INFINITY ? 0.f : mref;
     uint32_t bad = 0;
 #pragma unroll
     for (int k2 = 0; k2 < 2; ++k2) {
-      uint32_t p[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[8 * k2 + 2 * e], scale2, -m));
-        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[8 * k2 + 2 * e + 1], scale2, -m));
-        p[e] = pack_bf16x2_rn(p0, p1);
-        lsum = dot2(p[e], kOneBf16x2, lsum);
-      }
-      const uint4 pa = make_uint4(p[0], p[1], p[2], p[3]);
+      const uint4 pa = weights(sc, k2, m);
 #pragma unroll
       for (int db = 0; db < DB; ++db) {
-        s16x4t_t v[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-          v[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4t_t*)(
-              vb + voff[db & 1] + (16 * k2 + 8 * e) * T::kRowBytes + 128 * (db >> 1)));
-        const uint2 v0 = __builtin_bit_cast(uint2, v[0]), v1 = __builtin_bit_cast(uint2, v[1]);
-        uint32_t w[4] = {v0.x, v0.y, v1.x, v1.y};
-        if constexpr (MASKED) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint32_t odd = ((w[j] & 0x7F80u) == 0x7F80u ? 0xFFFFu : 0u) |
-                                 ((w[j] & 0x7F800000u) == 0x7F800000u ? 0xFFFF0000u : 0u);
-            bad |= odd;
-            w[j] &= ~odd;
-          }
-        }
-        o[db] = mfma_tree(pa, make_uint4(w[0], w[1], w[2], w[3]), o[db]);
+        uint4 v = v_read(vb, 0, k2, db);
+        bad |= take_odd(v.x) | take_odd(v.y) | take_odd(v.z) | take_odd(v.w);
+        o[db] = mfma_tree(pa, v, o[db]);
       }
     }
-    if constexpr (MASKED) {
-      if (__any(bad != 0)) {
-        for (int p = 0; p < 32; ++p) {
-          const int64_t t = t0 + p < end ? t0 + p : end - 1;
-          float v[DB];
+    if (__any(bad != 0)) {
+      for (int p = 0; p < 32; ++p) {
+        const int64_t at = t0 + p < end ? t0 + p : end - 1;
+        float v[DB];
 #pragma unroll
-          for (int db = 0; db < DB; ++db) {
-            v[db] = bf16_to_f32(v_cache[(base + t) * HD + 32 * db + r32]);
-            if ((__float_as_uint(v[db]) & 0x7F800000u) != 0x7F800000u) v[db] = 0.f;
-          }
+        for (int db = 0; db < DB; ++db) {
+          v[db] = bf16_to_f32(v_cache[(base + at) * HD + 32 * db + r32]);
+          if ((__float_as_uint(v[db]) & 0x7F800000u) != 0x7F800000u) v[db] = 0.f;
+        }
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const uint32_t w = __shfl(sees, 8 * (i >> 2) + 4 * h + (i & 3), 64);
+        for (int i = 0; i < 16; ++i) {
+          const uint32_t ws = __builtin_amdgcn_ds_bpermute(row_lane(i), static_cast<int>(sees));
 #pragma unroll
-            for (int db = 0; db < DB; ++db) o[db][i] += (w >> p) & 1u ? v[db] : 0.f;
-          }
+          for (int db = 0; db < DB; ++db) o[db][i] += (ws >> p) & 1u ? v[db] : 0.f;
         }
       }
-    }
-  };
-  auto attend = [&](int s, const char* buf) {
-    const int64_t tb = start + static_cast<int64_t>(s) * T::kStep + pw * T::kNP;
-    const char* const kb = buf + pw * 2 * T::kRegion;
-#pragma unroll
-    for (int st = 0; st < T::kNP / 32; ++st) {
-      const int64_t t0 = tb + 32 * st;
-      if (t0 >= end) break;
-      const char* const k = kb + 32 * st * T::kRowBytes;
-      if (t0 + 32 > n0 || t0 < whole) attend32(std::true_type{}, t0, k, k + T::kRegion);
-      else attend32(std::false_type{}, t0, k, k + T::kRegion);
     }
   };
 
-  // Wait for step s's copies (those of later steps may be in flight), meet the
-  // other waves, which also frees the buffer of step s - 1, send the copies of
-  // step s + kBufs - 1 there, and attend.
-  auto step = [&](int s, const char* cur, char* prev) {
+  // Step s's copies are in (those of later steps may be in flight), the other
+  // waves' too, which have also left step s - 1 (RW = 1: every wave reads its
+  // own copies only); the copies of step s + kBufs - 1 go to its buffer.
+  auto arrive = [&](int s, char* prev) {
     if (T::kBufs == 3 && s + 1 < s_end) __builtin_amdgcn_s_waitcnt(tree_vmcnt(2 * T::kCopies));
     else __builtin_amdgcn_s_waitcnt(tree_vmcnt(0));
     asm volatile("" ::: "memory");
-    if (RW > 1) __builtin_amdgcn_s_barrier();  // (RW = 1: every wave reads its own copies only)
+    if (RW > 1) __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     if (s + T::kBufs - 1 < s_end) copy(s + T::kBufs - 1, prev);
-    if (busy) attend(s, cur);
   };
-  for (int s = s_beg; s < s_end;) {
-    if (T::kBufs == 3) {
-      step(s++, buf0, buf2);
-      if (s >= s_end) break;
-      step(s++, buf1, buf0);
-      if (s >= s_end) break;
-      step(s++, buf2, buf1);
-    } else {
-      step(s++, buf0, buf1);
-      if (s >= s_end) break;
-      step(s++, buf1, buf0);
+  // Steps [p_beg, p_end) are seen whole; the buffers turn with s - s_beg.
+  const int64_t p0 = whole > start ? cdiv(whole - start, T::kStep) : 0, p1 = n0 > start ? (n0 - start) / T::kStep : 0;
+  const int p_beg = p0 < s_beg ? s_beg : (p0 < s_end ? static_cast<int>(p0) : s_end);
+  const int p_end = p1 < s_end ? static_cast<int>(p1) : s_end;
+  for (int s = s_beg, turn = 0; s < s_end;) {
+    if (turn == 0 && s >= p_beg && s + T::kBufs <= p_end) {
+      do {
+        arrive(s, T::kBufs == 3 ? buf2 : buf1);
+        if (busy) attend(buf0);
+        arrive(s + 1, buf0);
+        if (busy) attend(buf1);
+        if (T::kBufs == 3) {
+          arrive(s + 2, buf1);
+          if (busy) attend(buf2);
+        }
+        s += T::kBufs;
+      } while (s + T::kBufs <= p_end);
+      continue;
     }
+    char* const cur = turn == 0 ? buf0 : (turn == 1 ? buf1 : buf2);
+    char* const prev = T::kBufs == 2 ? (turn == 0 ? buf1 : buf0) : (turn == 0 ? buf2 : (turn == 1 ? buf0 : buf1));
+    arrive(s, prev);
+    if (busy) {
+      const int64_t tb = start + static_cast<int64_t>(s) * T::kStep + pw * T::kNP;
+      for (int t = 0; t < NT; ++t) {
+        const char* const kb = cur + pw * 2 * T::kRegion + 32 * t * T::kRowBytes;
+        if (tb + 32 * t < end) attend_edge(tb + 32 * t, kb, kb + T::kRegion);
+      }
+    }
+    ++s;
+    turn = turn + 1 == T::kBufs ? 0 : turn + 1;
   }
 
   lsum += __shfl_xor(lsum, 32, 64);
@@ -453,7 +540,7 @@ __global__ __launch_bounds__(256, (TreeTile<HD, RW>::kWaves)) void k_tree_attn(
     const float f = lsum != 0.f ? __builtin_amdgcn_exp2f(mref - m) : 0.f;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      const float fi = __shfl(f, 8 * (i >> 2) + 4 * h + (i & 3), 64);
+      const float fi = of_row(f, i);
 #pragma unroll
       for (int db = 0; db < DB; ++db) o[db][i] = fi != 0.f ? o[db][i] * fi : 0.f;
     }
@@ -478,14 +565,14 @@ __global__ __launch_bounds__(256, (TreeTile<HD, RW>::kWaves)) void k_tree_attn(
   }
   const bool seen = depth >= 0 && l != 0.f;
   if (S > 1) {
-    const int64_t p0 = ((pair * tiles + tile) * S + sp) * T::kRows + rw * 32;
-    if (h == 0) part_ml[p0 + r32] = seen ? make_float2(m, l) : make_float2(-INFINITY, 0.f);
+    const int64_t pr = ((pair * tiles + tile) * S + sp) * T::kRows + rw * 32;
+    if (h == 0) part_ml[pr + r32] = seen ? make_float2(m, l) : make_float2(-INFINITY, 0.f);
     if (s_beg < s_end && busy)
 #pragma unroll
       for (int i = 0; i < 16; ++i)
 #pragma unroll
         for (int db = 0; db < DB; ++db)
-          part_acc[(p0 + 8 * (i >> 2) + 4 * h + (i & 3)) * HD + 32 * db + r32] = o[db][i];
+          part_acc[(pr + 8 * (i >> 2) + 4 * h + (i & 3)) * HD + 32 * db + r32] = o[db][i];
     return;
   }
   const float inv = seen ? 1.0f / l : 0.f;
@@ -602,9 +689,20 @@ static TreePlan tree_plan(int64_t batch, int64_t nodes, int nq, int nkv, int hea
   p.pairs = batch * nkv;
   int64_t span = max_len;
   if (window > 0 && window + nodes < span) span = window + nodes;
-  const int64_t most = cdiv(span, (head_dim == 64 && p.rw > 1 ? 64 : 32) * (4 / p.rw));
-  int64_t s = kTreeTargetGroups / (p.pairs * p.tiles > 0 ? p.pairs * p.tiles : 1);
-  s = s < 1 ? 1 : (s > most ? most : s);
+  // Splits: as many as keep every workgroup resident (2 or 3 to a compute unit:
+  // TreeTile::kWaves), but no more than pay.  With N steps in all a split costs
+  // its N / S steps, about 1.2 us each while the card is not full, and S adds to
+  // the merge: 0.05 us and its sums, written and read at 5 TB/s.  Measured (attention + merge,
+  // us): 32 x 32 nodes over 4096 of 64: 64 in one split, 60 in two, 57 in three
+  // (all resident), 68 in four; 7 x 23 over a window of 512 of 128: 19 in two, 17
+  // in four to six, 23 in 17; 1 x 8 over 4096 of 64: 16 in 8, 13 in 33.
+  const int64_t n = cdiv(span, (head_dim == 64 && p.rw > 1 ? 64 : 32) * (4 / p.rw));
+  const int64_t per_cu = p.rw == 4 && head_dim == 64 ? 3 : (head_dim == 128 && p.rw == 1 ? 1 : 2);
+  const double sums = static_cast<double>(p.pairs) * p.tiles * 32 * p.rw * head_dim * 8.0 / 5e6;
+  const int64_t pays = static_cast<int64_t>(sqrt(1.2 * static_cast<double>(n) / (0.05 + sums)));
+  int64_t s = per_cu * 256 / (p.pairs * p.tiles > 0 ? p.pairs * p.tiles : 1);
+  s = s < pays ? s : pays;
+  s = s < 1 ? 1 : (s > n ? n : s);
   p.splits = static_cast<int>(s);
   return p;
 }
