@@ -50,4 +50,19 @@ __device__ __forceinline__ TreeLane tree_lane(const int32_t* __restrict__ parent
   return tree_lane(tree_parent(parents, nodes), nodes);
 }
 
+
+// The depth alone (-1 for an absent node): every lane holds the node 2^n steps
+// up, or where its way ends, and the steps to it, in one word.
+__device__ __forceinline__ int tree_depth(int par, int nodes) {
+  const int lane = static_cast<int>(threadIdx.x & 63);
+  const bool root = __builtin_amdgcn_readfirstlane(par) == -1;
+  int at = lane > 0 && par >= 0 && par < lane ? (par | 1 << 8) : lane;
+#pragma unroll
+  for (int r = 0; r < 6; ++r) {
+    const int up = __shfl(at, at & 63, 64);
+    at = (up & 63) | ((at & ~63) + (up & ~63));
+  }
+  return root && lane < nodes && (at & 63) == 0 ? at >> 8 : -1;
+}
+
 }  // namespace ma

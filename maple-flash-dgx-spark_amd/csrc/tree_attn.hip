@@ -30,89 +30,201 @@ struct TreeRope {
   int mode;  // 0 none, 1 half layout, 2 interleaved
 };
 
-// One wave per (head slot, node): q heads, then k heads, then v heads; lane l
-// owns dims l + 64 e.  Per head y = x rsqrt(mean(x^2) + eps) w, then over the
-// first rot dims, h = rot / 2 and (c, s) the table's row at seqlen + depth:
+// Eight consecutive elements of a float32, bf16 or f16 array from element i, as
+// loads without a dtype branch around them (a branch would put the wait for a
+// load right behind it) and their conversion.  VEC: i's bytes are 16-byte
+// aligned; else element by element.
+struct Eight {
+  uint4 lo, hi;  // VEC: the bytes (hi: the upper four float32)
+  AnyWord w[8];  // else
+};
+template <bool VEC>
+__device__ __forceinline__ void ld_eight(Eight& r, const void* p, int dt, int64_t i) {
+  if constexpr (VEC) {
+    const uint4* const a = reinterpret_cast<const uint4*>(static_cast<const char*>(p) + i * (dt == MA_F32 ? 4 : 2));
+    r.lo = a[0];
+    if (dt == MA_F32) r.hi = a[1];
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) r.w[e] = ld_any_word(p, dt, i + e);
+  }
+}
+template <bool VEC>
+__device__ __forceinline__ void of_eight(float (&f)[8], const Eight& r, int dt) {
+  if constexpr (VEC) {
+    const uint32_t u[8] = {r.lo.x, r.lo.y, r.lo.z, r.lo.w, r.hi.x, r.hi.y, r.hi.z, r.hi.w};
+    if (dt == MA_F32) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(u[e]);
+    } else if (dt == MA_BF16) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(e & 1 ? u[e / 2] & 0xffff0000u : u[e / 2] << 16);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] = from_raw<MA_F16>((u[e / 2] >> (16 * (e & 1))) & 0xffffu);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = any_word_f(r.w[e], dt);
+  }
+}
+// The table columns that dims d0 .. +7 turn by, d0 < rot counted (others read
+// column 0 and are not used): half layout columns d0 .. +7; interleaved columns
+// d0 / 2 .. +3, then the same + rot / 2.
+template <bool VEC>
+__device__ __forceinline__ void ld_turns(Eight& r, const void* p, int dt, int64_t row, int d0, int rot, int mode) {
+  const int half = rot / 2;
+  if constexpr (VEC) {  // (rot is a multiple of 8: a lane's dims all turn or none does)
+    const int d = d0 < rot ? d0 : 0;
+    if (mode == 1) {
+      ld_eight<true>(r, p, dt, row + d);
+      return;
+    }
+    const int es = dt == MA_F32 ? 4 : 2;
+    const char* const a = static_cast<const char*>(p) + (row + d / 2) * es;
+    const char* const b = a + half * es;
+    if (dt == MA_F32) {
+      r.lo = *reinterpret_cast<const uint4*>(a);
+      r.hi = *reinterpret_cast<const uint4*>(b);
+    } else {
+      const uint2 a0 = *reinterpret_cast<const uint2*>(a), b0 = *reinterpret_cast<const uint2*>(b);
+      r.lo = make_uint4(a0.x, a0.y, b0.x, b0.y);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int pair = d0 / 2 + (e & 3);
+      const int col = mode == 1 ? (d0 + e < rot ? d0 + e : 0) : (pair < half ? pair + (e < 4 ? 0 : half) : 0);
+      r.w[e] = ld_any_word(p, dt, row + col);
+    }
+  }
+}
+
+constexpr int kQkvThreads = 256;
+
+// A thread per 8 dims of a (node, head): q heads, then k heads, then v heads of
+// a node, HD / 8 lanes each.  Per head y = x rsqrt(mean(x^2) + eps) w, then over
+// the first rot dims, h = rot / 2 and (c, s) the table's row at seqlen + depth:
 //   half         y_d      -> y_d c_d - y_{d+h} s_d,  y_{d+h} -> y_{d+h} c_{d+h} + y_d s_{d+h}
 //   interleaved  y_2i     -> y_2i c_i - y_{2i+1} s_i, y_{2i+1} -> y_{2i+1} c_{i+h} + y_2i s_{i+h}
-// float32 inside; c and s are rounded to bf16 first and y to bf16 at the end,
-// as the one-token path does, so a token's K is the same whichever wrote it.
-template <int HD>
-__global__ __launch_bounds__(64) void k_tree_qkv(
+// (the half layout's partners meet in LDS, whatever h is).  float32 inside; c
+// and s are rounded to bf16 first and y to bf16 at the end, as the one-token
+// path does, so a token's K is the same whichever wrote it.  Latency: two rounds
+// of loads (x, weights, tree and length; then the table's row).  A wave a head
+// with a tree of its own took 15.2 us for 1024 nodes of 32 + 8 heads of 64.
+// VEC: all rows are 16-byte aligned.
+template <int HD, bool VEC>
+__global__ __launch_bounds__(kQkvThreads) void k_tree_qkv(
     const uint16_t* __restrict__ qkv, int64_t ldb, int64_t ldt, int nodes, const void* __restrict__ q_w,
     const void* __restrict__ k_w, int w_dt, TreeRope rope, float eps, const int64_t* __restrict__ seqlen,
     const int32_t* __restrict__ parents, const int64_t* __restrict__ row_map, uint16_t* __restrict__ k_cache,
     uint16_t* __restrict__ v_cache, int64_t cache_rows, int64_t max_len, int nq, int nkv,
     uint16_t* __restrict__ q_out) {
-  constexpr int E = HD / 64;
-  const int lane = threadIdx.x;
-  const int hs = blockIdx.x;
-  const int64_t b = blockIdx.y / nodes;
-  const int node = static_cast<int>(blockIdx.y - b * nodes);
-  const int depth = __builtin_amdgcn_readlane(tree_lane(parents + b * nodes, nodes).depth, node);
-  const bool is_q = hs < nq;
-  uint16_t* const q_row = q_out + ((b * nodes + node) * nq + hs) * HD;
-  if (depth < 0) {
-    if (is_q)
+  constexpr int LPH = HD / 8;  // lanes per head
+  __shared__ __align__(16) float ys[kQkvThreads * 8];
+  const int tid = threadIdx.x;
+  const int64_t b = blockIdx.y;
+  const int heads = nq + 2 * nkv;
+  const int item = static_cast<int>(blockIdx.x) * kQkvThreads + tid;
+  const bool on = item < nodes * heads * LPH;
+  const int l = item % LPH, hd = on ? item / LPH : 0;
+  const int node = hd / heads, hs = hd - node * heads;
+  const bool is_q = hs < nq, is_v = hs >= nq + nkv;
+  const int d0 = 8 * l;
+  // every load that needs neither the length nor the tree
+  const uint16_t* const x_row = qkv + b * ldb + node * ldt + static_cast<int64_t>(hs) * HD + d0;
+  uint4 xv = make_uint4(0u, 0u, 0u, 0u);
+  uint16_t xs[8];
+  if constexpr (VEC) {
+    xv = *reinterpret_cast<const uint4*>(x_row);
+  } else {
 #pragma unroll
-      for (int e = 0; e < E; ++e) q_row[lane + 64 * e] = 0;
-    return;
+    for (int e = 0; e < 8; ++e) xs[e] = x_row[e];
   }
+  Eight wr{};
+  if (q_w) ld_eight<VEC>(wr, is_q ? q_w : k_w, w_dt, d0);
+  const int par = tree_parent(parents + b * nodes, nodes);
   const int64_t n0 = clamp_pos(seqlen[b], 0, max_len);
-  const int64_t slot = n0 + node;
-  if (!is_q && slot >= max_len) return;
   const int64_t crow = row_map ? clamp_pos(row_map[b], 0, cache_rows - 1) : b;
-  const uint16_t* const x_row = qkv + b * ldb + node * ldt + static_cast<int64_t>(hs) * HD;
-  if (hs >= nq + nkv) {
-    uint16_t* const dst = v_cache + ((crow * nkv + (hs - nq - nkv)) * max_len + slot) * HD;
-#pragma unroll
-    for (int e = 0; e < E; ++e) dst[lane + 64 * e] = x_row[lane + 64 * e];
-    return;
-  }
-  const void* const w = is_q ? q_w : k_w;
-  float y[E], sq = 0.f;
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    y[e] = bf16_to_f32(x_row[lane + 64 * e]);
-    sq += y[e] * y[e];
-  }
-  if (w) {
-    const float inv = rsqrtf(group_sum<64>(sq) / HD + eps);
-#pragma unroll
-    for (int e = 0; e < E; ++e) y[e] = y[e] * inv * ld_f(w, w_dt, lane + 64 * e);
-  }
-  if (rope.mode && rope.rot > 0) {
-    const int64_t pos = n0 + depth;
+  MA_ISSUE_FENCE();
+  const int depth = __shfl(tree_depth(par, nodes), node, 64);
+  // the table's row
+  const bool turn = rope.mode && rope.rot > 0;
+  const int half = rope.rot / 2;
+  Eight cr{}, sr{};
+  if (turn) {
+    const int64_t pos = n0 + (depth > 0 ? depth : 0);
     const int64_t row = (pos < rope.n_pos ? pos : rope.n_pos - 1) * rope.ld;
-    const int half = rope.rot / 2;
-    float other[E];
+    ld_turns<VEC>(cr, rope.cos, rope.dt, row, d0, rope.rot, rope.mode);
+    ld_turns<VEC>(sr, rope.sin, rope.dt, row, d0, rope.rot, rope.mode);
+  }
+  float y[8];
+  {
+    const uint32_t u[4] = {xv.x, xv.y, xv.z, xv.w};
+    float sq = 0.f;
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int d = lane + 64 * e;
-      const int pd = rope.mode == 2 ? d ^ 1 : (d < half ? d + half : d - half);
-      float o = 0.f;
-#pragma unroll
-      for (int f = 0; f < E; ++f) {
-        const float v = __shfl(y[f], pd & 63, 64);
-        o = (pd >> 6) == f ? v : o;
-      }
-      other[e] = o;
+    for (int e = 0; e < 8; ++e) {
+      y[e] = VEC ? __uint_as_float(e & 1 ? u[e / 2] & 0xffff0000u : u[e / 2] << 16) : bf16_to_f32(xs[e]);
+      sq += y[e] * y[e];
     }
+    if (q_w) {
+      const float inv = rsqrtf(group_sum<LPH>(sq) / HD + eps);
+      float w[8];
+      of_eight<VEC>(w, wr, w_dt);
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int d = lane + 64 * e;
-      if (d < rope.rot) {
-        const bool lo = rope.mode == 2 ? !(d & 1) : d < half;
-        const int col = rope.mode == 2 ? d / 2 + (lo ? 0 : half) : d;
-        const float c = bf16_to_f32(f32_to_bf16(ld_f(rope.cos, rope.dt, row + col)));
-        const float s = bf16_to_f32(f32_to_bf16(ld_f(rope.sin, rope.dt, row + col)));
-        y[e] = lo ? y[e] * c - other[e] * s : y[e] * c + other[e] * s;
-      }
+      for (int e = 0; e < 8; ++e) y[e] = is_v ? y[e] : y[e] * inv * w[e];
     }
   }
-  uint16_t* const dst = is_q ? q_row : k_cache + ((crow * nkv + (hs - nq)) * max_len + slot) * HD;
+  if (turn) {
+    float other[8];
+    if (rope.mode == 1) {
 #pragma unroll
-  for (int e = 0; e < E; ++e) dst[lane + 64 * e] = f32_to_bf16(y[e]);
+      for (int e = 0; e < 8; ++e) ys[tid * 8 + e] = y[e];
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int d = d0 + e;
+        const int pd = d < half ? d + half : d - half;
+        other[e] = ys[(tid - l) * 8 + (d < rope.rot ? pd : d)];
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) other[e] = y[e ^ 1];
+    }
+    float c[8], s[8];
+    of_eight<VEC>(c, cr, rope.dt);
+    of_eight<VEC>(s, sr, rope.dt);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int d = d0 + e;
+      const bool lo = rope.mode == 2 ? !(e & 1) : d < half;
+      const float ce = bf16_to_f32(f32_to_bf16(rope.mode == 2 ? c[(e >> 1) + 4 * (e & 1)] : c[e]));
+      const float se = bf16_to_f32(f32_to_bf16(rope.mode == 2 ? s[(e >> 1) + 4 * (e & 1)] : s[e]));
+      const float r = lo ? y[e] * ce - other[e] * se : y[e] * ce + other[e] * se;
+      other[e] = d < rope.rot && !is_v ? r : y[e];
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = other[e];
+  }
+  if (!on) return;
+  const int64_t slot = n0 + node;
+  if (!is_q && (depth < 0 || slot >= max_len)) return;
+  uint4 r = make_uint4(pack_bf16x2_rn(y[0], y[1]), pack_bf16x2_rn(y[2], y[3]), pack_bf16x2_rn(y[4], y[5]),
+                       pack_bf16x2_rn(y[6], y[7]));
+  uint16_t* dst;
+  if (is_q) {
+    dst = q_out + ((b * nodes + node) * nq + hs) * HD;
+    if (depth < 0) r = make_uint4(0u, 0u, 0u, 0u);
+  } else {
+    const int64_t at = (crow * nkv + (hs - nq) % nkv) * max_len + slot;
+    dst = (is_v ? v_cache : k_cache) + at * HD;
+    if (is_v && VEC) r = xv;  // (the bits as they are)
+    if (is_v && !VEC) {
+      r = make_uint4(xs[0] | static_cast<uint32_t>(xs[1]) << 16, xs[2] | static_cast<uint32_t>(xs[3]) << 16,
+                     xs[4] | static_cast<uint32_t>(xs[5]) << 16, xs[6] | static_cast<uint32_t>(xs[7]) << 16);
+    }
+  }
+  *reinterpret_cast<uint4*>(dst + d0) = r;
 }
 
 // ---------------------------------------------------------------------------
@@ -718,6 +830,8 @@ static size_t tree_ws_bytes(const TreePlan& p, int head_dim) {
 // ---------------------------------------------------------------------------
 constexpr int kCommitLayers = 64;  // layers per launch: their pointers travel as kernel arguments
 
+typedef uint32_t commit_u4 __attribute__((ext_vector_type(4)));
+
 struct CommitPtrs {
   uint16_t* p[2 * kCommitLayers];  // K then V of each layer
 };
@@ -726,41 +840,47 @@ struct CommitPtrs {
 // slots 1..n behind the sequence.  path ascends with path[j] >= j, so a row's
 // source may be another's destination: all of a round's rows are read before
 // any is written, and rounds go up the path (a later round's sources lie above
-// every slot written so far).
+// every slot written so far).  Latency: the row's numbers at once, then its
+// data.
 template <int HD>
-__global__ __launch_bounds__(64) void k_tree_commit(CommitPtrs ptrs, int n_caches, int nodes, int nkv,
-                                                    int64_t cache_rows, int64_t max_len,
-                                                    const int64_t* __restrict__ seqlen,
-                                                    const int32_t* __restrict__ path,
-                                                    const int32_t* __restrict__ accepted,
-                                                    const int64_t* __restrict__ row_map,
-                                                    int64_t* __restrict__ new_seqlen) {
-  constexpr int LPR = HD / 8;     // lanes per row
-  constexpr int RPI = 64 / LPR;   // rows per step
-  constexpr int ROUND = 4;        // steps read before they are written
-  const int lane = threadIdx.x;
-  const int64_t b = blockIdx.z;
+__global__ __launch_bounds__(256) void k_tree_commit(CommitPtrs ptrs, int items, int nodes, int nkv,
+                                                     int64_t cache_rows, int64_t max_len,
+                                                     const int64_t* __restrict__ seqlen,
+                                                     const int32_t* __restrict__ path,
+                                                     const int32_t* __restrict__ accepted,
+                                                     const int64_t* __restrict__ row_map,
+                                                     int64_t* __restrict__ new_seqlen) {
+  constexpr int LPR = HD / 8;    // lanes per row
+  constexpr int RPI = 64 / LPR;  // rows per step
+  constexpr int ROUND = 4;       // steps read before they are written
+  const int lane = static_cast<int>(threadIdx.x & 63);
+  const int item = __builtin_amdgcn_readfirstlane(static_cast<int>(blockIdx.x) * 4 + static_cast<int>(threadIdx.x >> 6));
+  if (item >= items) return;
+  const int64_t b = blockIdx.y;
+  const int cache = item / nkv, head = item - cache * nkv;
+  const int mine = lane < nodes ? path[b * nodes + lane] : -1;
+  const int64_t sl = seqlen[b], rm = row_map ? row_map[b] : b;
   int n = accepted[b];
   n = n < -1 ? -1 : (n > nodes - 1 ? nodes - 1 : n);
-  const int64_t n0 = clamp_pos(seqlen[b], 0, max_len);
-  if (new_seqlen && blockIdx.x == 0 && blockIdx.y == 0 && lane == 0) new_seqlen[b] = seqlen[b] + n + 1;
-  const int64_t crow = row_map ? clamp_pos(row_map[b], 0, cache_rows - 1) : b;
-  uint16_t* const base = ptrs.p[blockIdx.x] + (crow * nkv + blockIdx.y) * max_len * HD + (lane % LPR) * 8;
+  if (new_seqlen && item == 0 && lane == 0) new_seqlen[b] = sl + n + 1;
+  const int64_t n0 = clamp_pos(sl, 0, max_len);
+  const int64_t crow = row_map ? clamp_pos(rm, 0, cache_rows - 1) : b;
+  uint16_t* const base = ptrs.p[cache] + (crow * nkv + head) * max_len * HD + (lane % LPR) * 8;
   for (int j0 = 1; j0 <= n; j0 += RPI * ROUND) {
-    uint4 v[ROUND];
-    bool on[ROUND];
+    commit_u4 v[ROUND];
+    int src[ROUND];
 #pragma unroll
     for (int i = 0; i < ROUND; ++i) {
       const int j = j0 + i * RPI + lane / LPR;
-      const int src = j <= n ? path[b * nodes + j] : -1;
-      on[i] = src > j && src < nodes && n0 + src < max_len;
-      if (on[i]) v[i] = *reinterpret_cast<const uint4*>(base + (n0 + src) * HD);
+      const int s = __shfl(mine, j & 63, 64);
+      src[i] = j <= n && s > j && s < nodes && n0 + s < max_len ? s : -1;  // -1: nothing to move
+      v[i] = *reinterpret_cast<const commit_u4*>(base + (src[i] < 0 ? 0 : n0 + src[i]) * HD);
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 #pragma unroll
     for (int i = 0; i < ROUND; ++i) {
       const int j = j0 + i * RPI + lane / LPR;
-      if (on[i]) *reinterpret_cast<uint4*>(base + (n0 + j) * HD) = v[i];
+      if (src[i] >= 0) *reinterpret_cast<commit_u4*>(base + (n0 + j) * HD) = v[i];
     }
   }
 }
@@ -804,17 +924,25 @@ extern "C" int ma_tree_qkv(const void* qkv, int64_t ldb, int64_t ldt, int64_t ba
   if ((q_norm_w == nullptr) != (k_norm_w == nullptr)) return fail(MA_EVALUE, "tree_qkv: one norm weight without the other");
   if (batch == 0) return MA_OK;
   if (!qkv || !seqlen || !parents || !k_cache || !v_cache || !q_out) return fail(MA_EVALUE, "tree_qkv: null pointer");
+  if (!aligned16(k_cache) || !aligned16(v_cache) || !aligned16(q_out))
+    return fail(MA_EVALUE, "tree_qkv: the cache and q_out must be 16-byte aligned");
   const TreeRope rope{cos, sin, cs_dtype, ld_cs, n_pos, rotary_dim, rope_mode};
-  const dim3 grid(static_cast<unsigned>(n_heads + 2 * n_kv_heads), static_cast<unsigned>(batch * nodes));
+  // 16-byte loads throughout: rows aligned, and the rotary part ends with a lane's dims
+  const int es = cs_dtype == MA_F32 ? 4 : 2;
+  const bool rope_vec = !rope_mode || rotary_dim == 0 ||
+                        (aligned16(cos) && aligned16(sin) && ld_cs * es % 16 == 0 && rotary_dim % 8 == 0);
+  const bool vec = aligned16(qkv) && ldb % 8 == 0 && ldt % 8 == 0 && rope_vec && aligned16(q_norm_w) && aligned16(k_norm_w);
+  const int64_t items = nodes * (n_heads + 2 * n_kv_heads) * (head_dim / 8);
+  const dim3 grid(static_cast<unsigned>(cdiv(items, kQkvThreads)), static_cast<unsigned>(batch));
   hipStream_t s = static_cast<hipStream_t>(stream);
   auto go = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, grid, dim3(64), 0, s, static_cast<const uint16_t*>(qkv), ldb, ldt,
+    hipLaunchKernelGGL(kernel, grid, dim3(kQkvThreads), 0, s, static_cast<const uint16_t*>(qkv), ldb, ldt,
                        static_cast<int>(nodes), q_norm_w, k_norm_w, w_dtype, rope, eps, seqlen, parents, row_map,
                        static_cast<uint16_t*>(k_cache), static_cast<uint16_t*>(v_cache), cache_rows, max_len, n_heads,
                        n_kv_heads, static_cast<uint16_t*>(q_out));
   };
-  if (head_dim == 64) go(k_tree_qkv<64>);
-  else go(k_tree_qkv<128>);
+  if (head_dim == 64) vec ? go(k_tree_qkv<64, true>) : go(k_tree_qkv<64, false>);
+  else vec ? go(k_tree_qkv<128, true>) : go(k_tree_qkv<128, false>);
   return check_launch("tree_qkv");
 }
 
@@ -898,9 +1026,10 @@ extern "C" int ma_tree_commit(void* const* k_caches, void* const* v_caches, int6
       ptrs.p[2 * i] = static_cast<uint16_t*>(k_caches[l0 + i]);
       ptrs.p[2 * i + 1] = static_cast<uint16_t*>(v_caches[l0 + i]);
     }
-    const dim3 grid(static_cast<unsigned>(2 * n), static_cast<unsigned>(n_kv_heads), static_cast<unsigned>(batch));
+    const int items = 2 * n * n_kv_heads;
+    const dim3 grid(static_cast<unsigned>(cdiv(items, 4)), static_cast<unsigned>(batch));
     auto go = [&](auto kernel) {
-      hipLaunchKernelGGL(kernel, grid, dim3(64), 0, s, ptrs, 2 * n, static_cast<int>(nodes), n_kv_heads, cache_rows,
+      hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, ptrs, items, static_cast<int>(nodes), n_kv_heads, cache_rows,
                          max_len, seqlen, path, accepted, row_map, l0 == 0 ? new_seqlen : nullptr);
     };
     if (head_dim == 64) go(k_tree_commit<64>);
