@@ -35,13 +35,14 @@ build a FlashHead for batch-1 decode (``model.py:750-770``,
 
 from __future__ import annotations
 
+import dataclasses
 import json
 from pathlib import Path
 
 import torch
 
 from . import synthetic
-from .model import DecoderConfig, DecoderLayerWeights, SyntheticDecoder
+from .model import DecoderConfig, DecoderLayerWeights, RopeScaling, SyntheticDecoder
 
 FORMAT = "packed-ternary-v1"
 HEAD_GROUP_SIZE = 64  # RTN group of the head when the config names none (pack.py:14)
@@ -133,6 +134,7 @@ def decoder_config(config: dict) -> DecoderConfig:
         layer_types=layer_types,
         sliding_window=int(config.get("sliding_window", 512)),
         nope_on_global=bool(config.get("nope_on_global_attention", True)) and bool(layer_types),
+        rope_scaling=RopeScaling(**meta["rope_scaling"]) if meta.get("rope_scaling") else None,
     )
 
 
@@ -237,6 +239,7 @@ def save_decoder(model, model_dir) -> None:
             "expert_template": "model.layers.{layer}.mlp.switch_mlp.{proj}.weight",
             "ternary": {"bits": 2, "pack": "uint32_lsb_first", "scale": "row_alpha"},
             "rtn_4bit": {"bits": 4, "group_size": c.rtn_group, "mode": "affine", "pack": "uint32_lsb_first"},
+            **({"rope_scaling": dataclasses.asdict(c.rope_scaling)} if c.rope_scaling else {}),
         },
     }
     (model_dir / "config.json").write_text(json.dumps(config, indent=2, sort_keys=True))

@@ -22,6 +22,10 @@ Mirrors the decode drivers of reference ``src/maple_run/generate.py``:
   ``check_every`` steps when stop ids are given), and the persistent kernels'
   timeout words checked there.
 
+* ``tree_step``: one step over a tree of drafted tokens per row (no reference
+  counterpart): the model over all nodes, the verification under the same
+  sampling settings, the accepted branch kept in the cache.
+
 Sampling randomness stays with the caller's generator: each step draws one
 uniform per row with ``torch.rand(rows, generator=...)`` on the device, eager
 and replay alike, so a seeded run is reproducible and the equality gate
@@ -40,6 +44,7 @@ import torch
 from . import workspace
 from .kernels.greedy import greedy_argmax
 from .kernels.sampler import MAX_TOP_K, batched_sampler_workspace, fused_sample_batched
+from .kernels.tree import TreeVerdict, verify_tree
 
 GRAPH_WARMUP = 3
 GRAPH_CHECK_TOKENS = 8
@@ -296,6 +301,35 @@ class BucketedDecodeGraphs:
         """Step ``tokens [live]``; returns the logits ``[live, vocab]``."""
         g, live = self._run(tokens, None)
         return g.logits[:live]
+
+
+def tree_step(model, cache, tokens: torch.Tensor, parents: torch.Tensor, sampling: Sampling | None = None, *,
+              uniform: torch.Tensor | None = None, draft_probs: torch.Tensor | None = None) -> TreeVerdict:
+    """One step over drafted trees: ``tokens [w, T]`` (node 0 each row's last
+    token, its K/V not yet cached) hung together by ``parents [w, T]`` over cache
+    slots ``[0, w)``, each with room for ``T`` more positions.  Scores every node,
+    accepts tokens under ``sampling`` (greedy: where they are the argmax; else as
+    ``verify_tree``, with ``draft_probs`` if the tokens were drawn), draws one
+    more and keeps the accepted branch in the cache.  Every row gets 1 to T
+    tokens that follow the law of as many ordinary steps; the last of them is
+    the next step's node 0.  ``uniform [w, T]`` float32 replaces the draw from
+    ``sampling.generator``.  No host synchronisation; capturable with
+    ``uniform`` given (or greedy)."""
+    sampling = sampling or Sampling()
+    sampling.check()
+    w, t = tokens.shape
+    logits = model.forward_tree(tokens, parents, cache)
+    if sampling.greedy:
+        # the law is one token: every uniform below 1 decides alike
+        zero = torch.zeros(w, t, device=logits.device, dtype=torch.float32)
+        out = verify_tree(logits, tokens, parents, zero, temperature=1.0, top_p=1.0, top_k=1)
+    else:
+        if uniform is None:
+            uniform = torch.rand(w, t, device=logits.device, generator=sampling.generator)
+        out = verify_tree(logits, tokens, parents, uniform, temperature=sampling.temperature, top_p=sampling.top_p,
+                          top_k=sampling.top_k, draft_probs=draft_probs)
+    cache.commit(out.path, out.accepted)
+    return out
 
 
 @dataclass

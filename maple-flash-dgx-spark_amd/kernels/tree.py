@@ -3,8 +3,8 @@
 A draft proposes, behind a row's last token, a tree of tokens; one pass of the
 model scores them all and the branch that the target's law accepts is kept.  Per
 layer ``apply_qkv_tree`` then ``tree_attention``, on the logits ``verify_tree``,
-and ``commit_tree`` on the cache (``model.SyntheticDecoder.tree_step`` runs
-them).  No reference counterpart: its decode step takes one token per row
+and ``commit_tree`` on the cache (``decode_graph.tree_step`` runs them).  No
+reference counterpart: its decode step takes one token per row
 (``src/maple_run/kernels/decode_attn.py:362-592``, whose QK-norm, RoPE, K/V
 store and GQA these are for several, and ``src/maple_run/kernels/sampler.py``,
 whose law the verification keeps).
@@ -47,14 +47,14 @@ def _call(idx: int, name: str, *args) -> None:
             _lib.call(name, *args, _stream(idx))
 
 
-def _device(what: str, t: torch.Tensor, *others) -> int:
-    """The one device that all of the tensors are on."""
-    idx = t.get_device()
+def _device(what: str, tensors: tuple) -> int:
+    """The one device that all of the tensors (or None) are on."""
+    idx = tensors[0].get_device()
     if idx < 0:
         raise RuntimeError(f"{what} requires CUDA tensors.")
-    for o in others:
+    for o in tensors:
         if o is not None and o.get_device() != idx:
-            raise ValueError(f"{what}: tensors on {o.device} and {t.device}.")
+            raise ValueError(f"{what}: tensors on {o.device} and {tensors[0].device}.")
     return idx
 
 
@@ -66,7 +66,7 @@ def _tree(what: str, parents: torch.Tensor, bsz: int, nodes: int) -> torch.Tenso
     if parents.dtype != torch.int32:
         if parents.dtype != torch.int64:
             raise TypeError(f"{what}: parents must be int32 or int64; got {parents.dtype}.")
-        parents = parents.to(torch.int32)
+        parents = parents.clamp(-2, MAX_NODES).to(torch.int32)  # (no large value may wrap to a node)
     return parents if parents.is_contiguous() else parents.contiguous()
 
 
@@ -154,8 +154,8 @@ def apply_qkv_tree(
     parents = _tree("apply_qkv_tree", parents, bsz, nodes)
     sl = _positions("seqlen", seqlen, bsz)
     rm = None if row_map is None else _positions("row_map", row_map, bsz)
-    idx = _device("apply_qkv_tree", qkv, k_cache, v_cache, sl, parents, rm, qw, kw, c, s)
-    out = torch.empty((bsz, nodes, num_heads, head_dim), device=qkv.device, dtype=torch.bfloat16)
+    idx = _device("apply_qkv_tree", (qkv, k_cache, v_cache, sl, parents, rm, qw, kw, c, s))
+    out = qkv.new_empty((bsz, nodes, num_heads, head_dim))
     _call(
         idx, "ma_tree_qkv",
         qkv.data_ptr(), ldb, ldt, bsz, nodes, num_heads, num_kv_heads, head_dim, _lib.ptr(qw), _lib.ptr(kw), w_dt,
@@ -195,13 +195,13 @@ def tree_attention(
     parents = _tree("tree_attention", parents, bsz, nodes)
     sl = _positions("seqlen", seqlen, bsz)
     rm = None if row_map is None else _positions("row_map", row_map, bsz)
-    idx = _device("tree_attention", q, k_cache, v_cache, sl, parents, rm)
+    idx = _device("tree_attention", (q, k_cache, v_cache, sl, parents, rm))
     q = q.contiguous()
     out = torch.empty_like(q)
     nbytes = _lib.load().ma_tree_attn_workspace_bytes(bsz, nodes, n_q, n_kv, head_dim, max_len, window)
     # scratch of this call alone: the allocator keeps it to this stream, a
     # captured graph to its own pool
-    ws = torch.empty(nbytes, device=q.device, dtype=torch.uint8) if nbytes else None
+    ws = q.new_empty(nbytes // 2) if nbytes else None
     _call(
         idx, "ma_tree_attn",
         q.data_ptr(), bsz, nodes, n_q, n_kv, head_dim, k_cache.data_ptr(), v_cache.data_ptr(), rows, max_len,
@@ -248,6 +248,7 @@ def verify_tree(
     shape = logits.shape
     bsz, nodes, vocab = shape
     _check(top_k, temperature, vocab)
+    l_dt = _lib.dtype_code(logits, "logits")
     parents = _tree("verify_tree", parents, bsz, nodes)
     ldb, ldt, one = logits.stride()
     if one != 1 and vocab > 1:
@@ -269,16 +270,13 @@ def verify_tree(
         if one != 1 and vocab > 1:
             raise ValueError("draft_probs rows must be contiguous.")
         p_dt = _lib.dtype_code(draft_probs, "draft_probs")
-    idx = _device("verify_tree", logits, tokens, parents, uniform, draft_probs)
-    dev = logits.device
-    out = TreeVerdict(torch.empty((bsz, nodes), device=dev, dtype=torch.int64),
-                      torch.empty(bsz, device=dev, dtype=torch.int32),
-                      torch.empty((bsz, nodes), device=dev, dtype=torch.int32))
+    idx = _device("verify_tree", (logits, tokens, parents, uniform, draft_probs))
+    out = TreeVerdict(torch.empty_like(tokens), parents.new_empty(bsz), torch.empty_like(parents))
     nbytes = _lib.load().ma_verify_tree_workspace_bytes(bsz, nodes, vocab, top_k)
-    ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)  # scratch of this call alone, as in tree_attention
+    ws = tokens.new_empty(nbytes // 8)  # scratch of this call alone, as in tree_attention
     _call(
         idx, "ma_verify_tree",
-        logits.data_ptr(), _lib.dtype_code(logits, "logits"), ldb, ldt, bsz, nodes, vocab, tokens.data_ptr(),
+        logits.data_ptr(), l_dt, ldb, ldt, bsz, nodes, vocab, tokens.data_ptr(),
         parents.data_ptr(), uniform.data_ptr(), _lib.ptr(draft_probs), p_dt, p_lb, p_lt, top_k,
         1.0 / float(temperature), top_p, ws.data_ptr(), nbytes, out[0].data_ptr(), out[1].data_ptr(),
         out[2].data_ptr(),
@@ -325,10 +323,10 @@ def commit_tree(
     sl = _positions("seqlen", seqlen, bsz)
     rm = None if row_map is None else _positions("row_map", row_map, bsz)
     path, accepted = path.contiguous(), accepted.contiguous()
-    idx = _device("commit_tree", first, sl, rm, path, accepted)
+    idx = _device("commit_tree", (first, sl, rm, path, accepted))
     if set(map(torch.Tensor.get_device, caches)) != {idx}:
         raise ValueError("commit_tree: caches on several devices.")
-    out = torch.empty(bsz, device=first.device, dtype=torch.int64)
+    out = sl.new_empty(bsz)
     at = ptrs.buffer_info()[0]
     _call(
         idx, "ma_tree_commit",

@@ -18,6 +18,11 @@ One decode step, per layer:
   which builds hidden from the slot outputs in its operand launch)
 then seqlen += 1, final rms_norm, RTN4 lm_head, greedy argmax.
 
+A step over a tree of drafted tokens per row (``forward_tree``) runs the same
+layers over all nodes at once, with ``apply_qkv_tree`` and ``tree_attention`` in
+the place of ``decode_attention``; ``KVCache.commit`` then keeps an accepted
+branch.
+
 Weights are random with the synthetic distributions (``synthetic.py``): every
 projection packed ternary, norm weights 1, the lm_head and embedding 4-bit RTN
 with group 128 and zero-centred dequantised values, RoPE on every layer over
@@ -27,6 +32,7 @@ half the head (rotary_dim 32, theta 1e4), full attention (no window).
 from __future__ import annotations
 
 import dataclasses
+import math
 from dataclasses import dataclass, field
 
 import torch
@@ -37,7 +43,51 @@ from .kernels.fused_norm import rms_norm
 from .kernels.greedy import greedy_argmax
 from .kernels.rtn4 import rtn4_embedding, rtn4_gemv
 from .kernels.ternary_gemv import combine_gemv_supported, ternary_gemv, ternary_gemv_combine
+from .kernels.tree import apply_qkv_tree, commit_tree, tree_attention
 from .moe import PendingCombine, fused_form, fused_supported, moe_fused, moe_layer
+
+
+@dataclass(frozen=True)
+class RopeScaling:
+    """Rotary positions past the trained context, by a ``factor`` over
+    ``original_len`` positions (published methods, angles in 64 bits):
+
+    * ``"linear"``: positions divided by ``factor``;
+    * ``"ntk"``: the base raised to ``theta * factor^(rot / (rot - 2))``, so that
+      the slowest frequency is divided by ``factor`` and the fastest kept;
+    * ``"yarn"``: a frequency that turns fewer than ``slow`` times in
+      ``original_len`` positions is divided by ``factor``, one that turns more than
+      ``fast`` times kept, those between blended linearly; cos and sin are multiplied by
+      ``0.1 ln(factor) + 1``."""
+
+    kind: str
+    factor: float
+    original_len: int = 4096
+    slow: float = 1.0
+    fast: float = 32.0
+
+    def __post_init__(self):
+        if self.kind not in ("linear", "ntk", "yarn"):
+            raise ValueError(f"rope scaling {self.kind!r}: linear, ntk or yarn")
+        if not (self.factor >= 1.0 and math.isfinite(self.factor)) or self.original_len < 1 or not (
+                0.0 < self.slow < self.fast):
+            raise ValueError(f"rope scaling needs factor >= 1, original_len >= 1 and 0 < slow < fast: {self}")
+
+    def frequencies(self, rotary_dim: int, theta: float, device) -> tuple:
+        """``(inv_freq [rotary_dim / 2] float64, factor of cos and sin)``."""
+        i = torch.arange(0, rotary_dim, 2, device=device, dtype=torch.float64)
+        if self.kind == "ntk":
+            if rotary_dim <= 2:
+                raise ValueError("ntk scaling needs a rotary_dim above 2")
+            theta = theta * self.factor ** (rotary_dim / (rotary_dim - 2))
+        inv = theta ** (-i / rotary_dim)
+        if self.kind == "ntk":
+            return inv, 1.0
+        if self.kind == "linear":
+            return inv / self.factor, 1.0
+        turns = self.original_len * inv / (2.0 * math.pi)
+        keep = ((turns - self.slow) / (self.fast - self.slow)).clamp(0.0, 1.0)
+        return inv * keep + inv / self.factor * (1.0 - keep), 0.1 * math.log(self.factor) + 1.0
 
 
 @dataclass
@@ -62,6 +112,7 @@ class DecoderConfig:
     layer_types: tuple = ()
     sliding_window: int = 512
     nope_on_global: bool = False
+    rope_scaling: RopeScaling | None = None
 
     def layer_attention(self, i: int) -> tuple:
         """``(window or None, use_rope)`` of layer ``i``."""
@@ -91,9 +142,16 @@ class DecoderLayerWeights:
     moe: synthetic.MoELayer
 
 
-def rope_tables(max_len: int, rotary_dim: int, theta: float, device):
+def rope_tables(max_len: int, rotary_dim: int, theta: float, device, scaling: RopeScaling | None = None):
     """float32 cos/sin ``[max_len, rotary_dim]`` built like ``model.py:66-92``
-    (``inv_freq = theta^(-2i/rot)``, ``emb = cat(freqs, freqs)``)."""
+    (``inv_freq = theta^(-2i/rot)``, ``emb = cat(freqs, freqs)``); with
+    ``scaling``, its frequencies, and angles in 64 bits (a float32 angle at
+    position 2^20 is off by 2^-5)."""
+    if scaling is not None:
+        inv, mult = scaling.frequencies(rotary_dim, theta, device)
+        a = torch.outer(torch.arange(max_len, device=device, dtype=torch.float64), inv)
+        a = torch.cat((a, a), dim=-1)
+        return (a.cos() * mult).float().contiguous(), (a.sin() * mult).float().contiguous()
     inv_freq = 1.0 / (theta ** (torch.arange(0, rotary_dim, 2, device=device, dtype=torch.float32) / rotary_dim))
     t = torch.arange(max_len, device=device, dtype=torch.float32)
     freqs = torch.outer(t, inv_freq)
@@ -154,6 +212,14 @@ class KVCache:
         """Forget a slot's history so a new sequence can take it."""
         self.seqlen[slot] = 0
 
+    def commit(self, path: torch.Tensor, accepted: torch.Tensor) -> None:
+        """Keep an accepted branch of the nodes that ``forward_tree`` wrote behind
+        slots ``[0, len(accepted))`` (``path`` / ``accepted`` as ``verify_tree``
+        returns them): their K/V move together, in every layer, and the write
+        positions advance past them.  Graph-safe; no host synchronisation."""
+        seqlen, row_map = self.slot_rows(int(accepted.shape[0]))
+        seqlen.copy_(commit_tree(self.k, self.v, seqlen, path, accepted, row_map=row_map))
+
     def snapshot(self, steps: int | None = None) -> dict:
         """Write positions, slot map and a copy of the K/V that the next
         ``steps`` decode steps can overwrite (all of it when ``steps`` is
@@ -203,7 +269,8 @@ class SyntheticDecoder:
         self.lm_head = synthetic.rtn4_table(c.vocab, c.hidden, c.rtn_group, s + 901, dev, lo, hi)
         self.embed = synthetic.rtn4_table(c.vocab, c.hidden, c.rtn_group, s + 902, dev, lo, hi)
         self.final_norm = ones(c.hidden)
-        self.cos, self.sin = rope_tables(max_len, c.rotary_dim, c.rope_theta, dev)
+        self.cos, self.sin = rope_tables(max_len, c.rotary_dim, c.rope_theta, dev, c.rope_scaling)
+        self.cos_sin16 = self.cos.bfloat16(), self.sin.bfloat16()
         self.flash_head = None
         self._pack_read_ahead()
 
@@ -223,7 +290,8 @@ class SyntheticDecoder:
         self.max_len = max_len
         self.layers = list(layers)
         self.embed, self.lm_head, self.final_norm = embed, lm_head, final_norm
-        self.cos, self.sin = rope_tables(max_len, cfg.rotary_dim, cfg.rope_theta, self.device)
+        self.cos, self.sin = rope_tables(max_len, cfg.rotary_dim, cfg.rope_theta, self.device, cfg.rope_scaling)
+        self.cos_sin16 = self.cos.bfloat16(), self.sin.bfloat16()
         self.flash_head = None
         self._pack_read_ahead()
         return self
@@ -353,6 +421,33 @@ class SyntheticDecoder:
             hidden, qkv = self._layer(i, hidden, cache, routing, qkv)
         cache.seqlen[:width].add_(1)
         return self.head(hidden)
+
+    def forward_tree(self, tokens: torch.Tensor, parents: torch.Tensor, cache: KVCache,
+                     routing: list | None = None) -> torch.Tensor:
+        """The model over a tree of drafted tokens per row: ``tokens [w, T]``, node
+        0 each row's last token, ``parents [w, T]`` (``kernels.tree``) over cache
+        slots ``[0, w)``.  Writes the nodes' K/V at ``seqlen .. seqlen + T - 1``
+        without advancing ``seqlen`` (``KVCache.commit`` does) and returns bf16
+        logits ``[w, T, vocab]``; a chain's are those of as many decode steps up to
+        rounding.  Padding's logits say nothing."""
+        c = self.cfg
+        w, t = tokens.shape
+        seqlen, row_map = cache.slot_rows(w)
+        hidden = self.embed_tokens(tokens.reshape(-1))  # (padding's ids are clamped to the table)
+        for i, L in enumerate(self.layers):
+            window, use_rope = c.layer_attention(i)
+            qkv = ternary_gemv(hidden, L.qkv, L.qkv_alpha, rms_weight=L.input_ln, rms_eps=c.eps)
+            # (decode_attention rounds the tables to bf16 as it reads them)
+            q = apply_qkv_tree(qkv.view(w, t, -1), L.q_norm, L.k_norm, *self.cos_sin16, cache.k[i], cache.v[i], seqlen,
+                               parents, row_map=row_map, num_heads=c.heads, num_kv_heads=c.kv_heads,
+                               head_dim=c.head_dim, rotary_dim=c.rotary_dim, use_rope=use_rope, eps=c.eps)
+            attn = tree_attention(q, cache.k[i], cache.v[i], seqlen, parents, row_map=row_map,
+                                  scale=c.head_dim ** -0.5, window=window)
+            o = ternary_gemv(attn.view(w * t, -1), L.o, L.o_alpha)
+            hidden, ids = moe_layer(hidden, L.moe, c.top_k, L.post_ln, c.eps, add=o.reshape(hidden.shape))
+            if routing is not None:
+                routing.append(ids)
+        return self.head(hidden).view(w, t, -1)
 
     def embed_tokens(self, input_ids: torch.Tensor) -> torch.Tensor:
         w, sc, bs = self.embed
