@@ -21,8 +21,8 @@ struct TreeLane {
 
 // Node `lane` of a row's tree, found by the whole wave: every lane holds the
 // nodes on the last 2^n steps of its way up and the node those end at, and
-// doubles both by what that node holds (six rounds for 64 nodes), so that no
-// lane walks up node by node.
+// doubles both by what that node holds until every way has ended (six rounds at
+// most), so that no lane walks up node by node.
 //
 // tree_parent: the lane's entry of parents; tree_lane: its node (par: all lanes'
 // entries).
@@ -35,8 +35,7 @@ __device__ __forceinline__ TreeLane tree_lane(int par, int nodes) {
   int up = lane > 0 && par >= 0 && par < lane ? par : -1;
   uint64_t anc = 1ull << lane;
   const bool root = __builtin_amdgcn_readfirstlane(par) == -1;
-#pragma unroll
-  for (int r = 0; r < 6; ++r) {
+  for (int r = 0; r < 6 && __any(up >= 0); ++r) {
     const int src = up < 0 ? lane : up;
     const uint64_t a = __shfl(anc, src, 64);
     const int u = __shfl(up, src, 64);
@@ -57,9 +56,9 @@ __device__ __forceinline__ int tree_depth(int par, int nodes) {
   const int lane = static_cast<int>(threadIdx.x & 63);
   const bool root = __builtin_amdgcn_readfirstlane(par) == -1;
   int at = lane > 0 && par >= 0 && par < lane ? (par | 1 << 8) : lane;
-#pragma unroll
   for (int r = 0; r < 6; ++r) {
     const int up = __shfl(at, at & 63, 64);
+    if (!__any(up > 63)) break;  // every way has ended
     at = (up & 63) | ((at & ~63) + (up & ~63));
   }
   return root && lane < nodes && (at & 63) == 0 ? at >> 8 : -1;

@@ -231,7 +231,8 @@ __global__ __launch_bounds__(kQkvThreads) void k_tree_qkv(
 // Attention
 // ---------------------------------------------------------------------------
 typedef __attribute__((address_space(3))) void* tree_lds_t;
-constexpr float kTreeGrow = 8.0f;        // a row's reference maximum is moved when a score passes it by 2^8
+constexpr float kTreeGrow = 8.0f;    // a row's reference is moved when a score in a masked tile passes it by 2^8,
+constexpr float kTreeSum = 65536.f;  // or, where all rows see all positions, when a lane's sum passes this
 constexpr int tree_vmcnt(int n) { return (n & 0xF) | (0x7 << 4) | ((n >> 4) << 14); }  // and lgkmcnt(0)
 
 __device__ __forceinline__ f32x16t_t mfma_tree(uint4 a, uint4 b, f32x16t_t c) {
@@ -280,10 +281,13 @@ struct TreeRow {
 // the same k; C: col l % 32, rows 8 (i / 4) + 4 (l / 32) + i % 4):
 //   S^T = K Q^T: lane l holds query row l % 32's scores, half of the 32 positions;
 //   P = 2^(S scale log2 e - m), m a reference per query row that is moved only
-//     when a score passes it by 8 (any m gives the same quotient; this one
-//     keeps P below 2^8 without an exchange between lanes in every step), P
-//     rounded to bf16 as the matrix instruction takes it (half a step, 2^-8 of
-//     each weight at most, as in k_decode_attn), masked places exactly 0;
+//     when the weights' sum shows that it has become too low (any m that keeps
+//     them in range gives the same quotient, and bf16 and float32 share one
+//     range; a running maximum costs 9 of 100 cycles of a tile and a wait for
+//     it: 54.5 us without, 57.9 with, at 32 rows of 32 nodes over 4096
+//     positions of 32 / 4 heads of 64), P rounded to bf16 as the matrix
+//     instruction takes it (half a step, 2^-8 of each weight at most),
+//     masked places exactly 0;
 //   the sum of P from the same rounded values, so that a weight's rounding
 //     enters the quotient on both sides;
 //   O += P V: A = the lane's own P values in the order they are in, B = V in the
@@ -341,6 +345,11 @@ __global__ __launch_bounds__(256, (TreeTile<HD, RW>::kWaves)) void k_tree_attn(
   const int64_t whole = window > 0 ? n0 + nodes - window : 0;
   const int64_t base = (crow * nkv + kvh) * max_len;
 
+  // Steps [p_beg, p_end) are seen whole and start with the first buffer.
+  const int64_t p0 = whole > start ? cdiv(whole - start, T::kStep) : 0, p1 = n0 > start ? (n0 - start) / T::kStep : 0;
+  const int p_beg = p0 < s_beg ? s_beg : (p0 < s_end ? static_cast<int>(p0) : s_end);
+  const int turn0 = (p_beg - s_beg) % T::kBufs == 0 ? 0 : T::kBufs - (p_beg - s_beg) % T::kBufs;
+
   // copies of step s into a buffer: each wave its share of its group's rows,
   // rows past the end read again from the last one
   const int copy_row = rw * (T::kNP / RW) + lane / CPR;
@@ -371,8 +380,8 @@ __global__ __launch_bounds__(256, (TreeTile<HD, RW>::kWaves)) void k_tree_attn(
   }
   const int par = tree_parent(parents + b * nodes, nodes);
   MA_ISSUE_FENCE();
-  if (s_beg < s_end) copy(s_beg, buf0);
-  if (T::kBufs == 3 && s_beg + 1 < s_end) copy(s_beg + 1, buf1);
+  if (s_beg < s_end) copy(s_beg, turn0 == 0 ? buf0 : (turn0 == 1 ? buf1 : buf2));
+  if (T::kBufs == 3 && s_beg + 1 < s_end) copy(s_beg + 1, turn0 == 0 ? buf1 : (turn0 == 1 ? buf2 : buf0));
   MA_ISSUE_FENCE();
   const TreeLane me = tree_lane(par, nodes);
   if (wv == 0) {
@@ -449,7 +458,9 @@ __global__ __launch_bounds__(256, (TreeTile<HD, RW>::kWaves)) void k_tree_attn(
     cm = fmaxf(cm, __shfl_xor(cm, 32, 64));
     const float mn = fmaxf(mref, cm);
     const float a = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mref - mn);
+    const bool first = !__any(mref != -INFINITY);
     mref = mn;
+    if (first) return;  // (nothing summed yet)
     lsum *= a;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
@@ -499,9 +510,9 @@ __global__ __launch_bounds__(256, (TreeTile<HD, RW>::kWaves)) void k_tree_attn(
 #pragma unroll
         for (int i = 0; i < 16; ++i) sc[t][i] = 0.f;
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
+      for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int t = 0; t < NT; ++t) sc[t] = mfma_tree(kf[t][ks], qf[ks], sc[t]);
+        for (int ks = 0; ks < KS; ++ks) sc[t] = mfma_tree(kf[t][ks], qf[ks], sc[t]);
     }
     uint4 vf[NT][2][DB];
     auto v_tile = [&](int t) {
@@ -512,21 +523,26 @@ __global__ __launch_bounds__(256, (TreeTile<HD, RW>::kWaves)) void k_tree_attn(
     };
     v_tile(0);
     MA_ISSUE_FENCE();
-    float cm = sc[0][0];
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) cm = fmaxf(cm, sc[t][i]);
-    cm *= scale2;
-    if (__any(!(cm <= mref + kTreeGrow))) rescale(cm);
-    const float m = mref == -INFINITY ? 0.f : mref;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      const uint4 pa0 = weights(sc[t], 0, m);
+      uint4 pa0, pa1;
+      const float before = lsum;  // (a weight out of range, or the first scores: once more, from a new reference)
+      float m = mref;
+      for (bool again = false;;) {
+        pa0 = weights(sc[t], 0, m);
+        pa1 = weights(sc[t], 1, m);
+        if (again || !__any(!(lsum <= kTreeSum))) break;
+        again = true;
+        lsum = before;
+        float cm = sc[t][0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) cm = fmaxf(cm, sc[t][i]);
+        rescale(fmaxf(cm * scale2, before > 1.0f ? mref + __builtin_amdgcn_logf(before) : -INFINITY));
+        m = mref == -INFINITY ? 0.f : mref;
+      }
       if (t + 1 < NT) v_tile(t + 1);
 #pragma unroll
       for (int db = 0; db < DB; ++db) o[db] = mfma_tree(pa0, vf[t][0][db], o[db]);
-      const uint4 pa1 = weights(sc[t], 1, m);
 #pragma unroll
       for (int db = 0; db < DB; ++db) o[db] = mfma_tree(pa1, vf[t][1][db], o[db]);
     }
@@ -540,6 +556,12 @@ __global__ __launch_bounds__(256, (TreeTile<HD, RW>::kWaves)) void k_tree_attn(
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks)
       sc = mfma_tree(*reinterpret_cast<const uint4*>(kb + koff[ks & 3] + 128 * (ks >> 2)), qf[ks], sc);
+    uint4 vf[2][DB];
+#pragma unroll
+    for (int k2 = 0; k2 < 2; ++k2)
+#pragma unroll
+      for (int db = 0; db < DB; ++db) vf[k2][db] = v_read(vb, 0, k2, db);
+    MA_ISSUE_FENCE();
     const int64_t off = t0 - n0;  // node index of the first position
     uint64_t w = off >= 64 ? 0ull : (off >= 0 ? row.anc >> off : (off > -32 ? row.anc << -off : 0ull));
     if (off < 0) {  // and the sequence's part, from row.from on
@@ -560,13 +582,12 @@ __global__ __launch_bounds__(256, (TreeTile<HD, RW>::kWaves)) void k_tree_attn(
     uint32_t bad = 0;
 #pragma unroll
     for (int k2 = 0; k2 < 2; ++k2) {
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+        bad |= take_odd(vf[k2][db].x) | take_odd(vf[k2][db].y) | take_odd(vf[k2][db].z) | take_odd(vf[k2][db].w);
       const uint4 pa = weights(sc, k2, m);
 #pragma unroll
-      for (int db = 0; db < DB; ++db) {
-        uint4 v = v_read(vb, 0, k2, db);
-        bad |= take_odd(v.x) | take_odd(v.y) | take_odd(v.z) | take_odd(v.w);
-        o[db] = mfma_tree(pa, v, o[db]);
-      }
+      for (int db = 0; db < DB; ++db) o[db] = mfma_tree(pa, vf[k2][db], o[db]);
     }
     if (__any(bad != 0)) {
       for (int p = 0; p < 32; ++p) {
@@ -598,23 +619,29 @@ __global__ __launch_bounds__(256, (TreeTile<HD, RW>::kWaves)) void k_tree_attn(
     asm volatile("" ::: "memory");
     if (s + T::kBufs - 1 < s_end) copy(s + T::kBufs - 1, prev);
   };
-  // Steps [p_beg, p_end) are seen whole; the buffers turn with s - s_beg.
-  const int64_t p0 = whole > start ? cdiv(whole - start, T::kStep) : 0, p1 = n0 > start ? (n0 - start) / T::kStep : 0;
-  const int p_beg = p0 < s_beg ? s_beg : (p0 < s_end ? static_cast<int>(p0) : s_end);
   const int p_end = p1 < s_end ? static_cast<int>(p1) : s_end;
-  for (int s = s_beg, turn = 0; s < s_end;) {
-    if (turn == 0 && s >= p_beg && s + T::kBufs <= p_end) {
+  for (int s = s_beg, turn = turn0; s < s_end;) {
+    if (turn == 0 && s >= p_beg && s < p_end) {
       do {
         arrive(s, T::kBufs == 3 ? buf2 : buf1);
         if (busy) attend(buf0);
-        arrive(s + 1, buf0);
-        if (busy) attend(buf1);
-        if (T::kBufs == 3) {
-          arrive(s + 2, buf1);
-          if (busy) attend(buf2);
+        if (++s == p_end) {
+          turn = 1;
+          break;
         }
-        s += T::kBufs;
-      } while (s + T::kBufs <= p_end);
+        arrive(s, buf0);
+        if (busy) attend(buf1);
+        ++s;
+        if (T::kBufs == 3) {
+          if (s == p_end) {
+            turn = 2;
+            break;
+          }
+          arrive(s, buf1);
+          if (busy) attend(buf2);
+          ++s;
+        }
+      } while (s < p_end);
       continue;
     }
     char* const cur = turn == 0 ? buf0 : (turn == 1 ? buf1 : buf2);

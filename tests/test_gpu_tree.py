@@ -293,6 +293,29 @@ def test_attention_scores_of_any_size(dev):
         compare_attention(out, q, k, v, parents, [n], 0.25)
 
 
+@pytest.mark.parametrize("heads", [(32, 1, 64), (16, 1, 128), (4, 4, 64)])
+def test_attention_references_that_stay_too_low(dev, heads):
+    """Scores that stay above the first ones for the rest of the sequence: just
+    below what moves the reference, one jump and level, level after a spike, rising
+    slowly; in nats over a scale of 1, exact in bf16."""
+    from maple_amd.kernels import tree_attention
+
+    nq, nkv, d = heads
+    n, t = 6000, 5
+    parents = [[-1, 0, 1, 1, 3]]
+    q = torch.zeros(1, t, nq, d, device=dev, dtype=torch.bfloat16)
+    q[..., 0] = 1
+    v = bf16(dev, 1, nkv, n + t, d, seed=2)
+    at = torch.arange(n + t, device=dev)
+    for rise in (torch.where(at < 40, 0.0, 10.5), torch.where(at < 64, -60.0, 0.0), torch.where(at == 200, 11.0, 0.0),
+                 torch.where(at < 100, -200.0, torch.where(at == 3000, 11.0, 0.0)), (at // 500) * 4.0,
+                 torch.where(at % 700 == 699, 60.0, -20.0), torch.where(at < n, -150.0, -160.0)):
+        k = bf16(dev, 1, nkv, n + t, d, seed=3)
+        k[..., 0] = rise.to(torch.bfloat16)
+        out = tree_attention(q, k, v, torch.tensor([n], device=dev), as_parents(parents, dev), scale=1.0)
+        compare_attention(out, q, k, v, parents, [n], 1.0)
+
+
 def test_one_node_is_decode_gqa_attn(dev):
     from maple_amd.kernels import decode_gqa_attn, tree_attention
 
