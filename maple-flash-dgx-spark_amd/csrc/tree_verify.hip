@@ -15,7 +15,8 @@
 //
 //   k_verify_topk   the logits, once: per (node, segment of the vocabulary) its
 //                   top_k keys
-//   k_verify_merge  per node the top_k of its segments (with several segments)
+//   k_verify_merge  per node the top_k of its segments (with several segments;
+//                   greedy decoding takes their maximum in the walk)
 //   k_verify_walk   one wave per row: laws and walk, in 64 bits (a lane per
 //                   token of a law; a value at a border decides a token)
 //
@@ -465,11 +466,33 @@ __device__ __forceinline__ double wave_scan_d(double v) {
 }
 __device__ __forceinline__ double wave_sum_d(double v) { return lane_d(wave_scan_d(v), 63); }
 
+// The largest of the lanes' keys, in lane 0 (0 in the others).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_max_u(uint32_t v) {
+  const uint32_t o = __builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROWS, 0xF, false);
+  return o > v ? o : v;
+}
+__device__ __forceinline__ uint32_t wave_max_u(uint32_t v) {
+  v = dpp_max_u<0x111, 0xF>(v);
+  v = dpp_max_u<0x112, 0xF>(v);
+  v = dpp_max_u<0x114, 0xF>(v);
+  v = dpp_max_u<0x118, 0xF>(v);
+  v = dpp_max_u<0x142, 0xA>(v);
+  v = dpp_max_u<0x143, 0xC>(v);
+  return __builtin_amdgcn_readlane(static_cast<int>(v), 63);
+}
+__device__ __forceinline__ uint64_t wave_max_key(uint64_t key) {
+  const uint32_t hi = wave_max_u(static_cast<uint32_t>(key >> 32));
+  const uint32_t lo = wave_max_u(static_cast<uint32_t>(key >> 32) == hi ? static_cast<uint32_t>(key) : 0u);
+  return threadIdx.x == 0 ? static_cast<uint64_t>(hi) << 32 | lo : 0ull;
+}
+
 // One wave per row: a lane per token of the current law (and per node of the
-// tree).  Latency: a step waits for one round of loads, the child's law and the
+// tree).  `each` keys a node: its law's k, or (k = 1) its segments' maxima.
+// Latency: a step waits for one round of loads, the child's law and the
 // draft's probabilities together, asked for while the child before it is judged.
 __global__ __launch_bounds__(64) void k_verify_walk(
-    const uint64_t* __restrict__ top, int k, int nodes, int64_t vocab, const int64_t* __restrict__ tokens,
+    const uint64_t* __restrict__ top, int k, int each, int nodes, int64_t vocab, const int64_t* __restrict__ tokens,
     const int32_t* __restrict__ parents, const float* __restrict__ uniform, const void* __restrict__ probs,
     int probs_dt, int64_t probs_ldb, int64_t probs_ldt, double inv_t, double top_p, int64_t* __restrict__ out_tokens,
     int32_t* __restrict__ accepted, int32_t* __restrict__ path) {
@@ -480,7 +503,7 @@ __global__ __launch_bounds__(64) void k_verify_walk(
   const int par0 = tree_parent(parents + bn, nodes);
   const int64_t tok = mine ? tokens[bn + lane] : -1;
   const float uni = mine ? uniform[bn + lane] : 0.f;
-  uint64_t key = lane < k ? top[bn * k + lane] : 0;  // (the root's; not read if there is none)
+  uint64_t key = lane < each ? top[bn * each + lane] : 0;  // (the root's; not read if there is none)
   const TreeLane me = tree_lane(par0, nodes);
   const int par = me.depth > 0 ? par0 : -1;
   int64_t o_tok = -1;  // lane j's output: token j, node j of the path
@@ -489,6 +512,7 @@ __global__ __launch_bounds__(64) void k_verify_walk(
     int64_t id = -1;
     double p = 0.0;
     auto law = [&]() {
+      if (each > k) key = wave_max_key(key);
       const double z = static_cast<double>(verify_value(key));
       const double z0 = lane_d(z, 0);
       id = key ? static_cast<int64_t>(0xffffffffu - static_cast<uint32_t>(key)) : -1;
@@ -503,7 +527,7 @@ __global__ __launch_bounds__(64) void k_verify_walk(
       double q, qt;
     };
     auto ask = [&](int i) {
-      Child c{lane < k ? top[(bn + i) * k + lane] : 0, 0.0, 1.0};
+      Child c{lane < each ? top[(bn + i) * each + lane] : 0, 0.0, 1.0};
       if (probs) {
         const int64_t t = lane_l(tok, i), pr = b * probs_ldb + i * probs_ldt;
         c.q = id >= 0 ? static_cast<double>(ld_f(probs, probs_dt, pr + id)) : 0.0;
@@ -615,14 +639,18 @@ extern "C" int ma_verify_tree(const void* logits, int dtype, int64_t ldb, int64_
   else go(k_verify_topk<MA_F32>);
   int rc = check_launch("verify_tree top-k");
   if (rc != MA_OK) return rc;
-  if (S > 1) {
+  // (greedy: the walk takes a node's segments itself, one launch less: 16 us a call at 8 nodes, 19 with it)
+  int each = top_k;
+  if (top_k == 1 && S <= 64) {
+    each = S;
+  } else if (S > 1) {
     top = cand + rows * S * top_k;
     hipLaunchKernelGGL(k_verify_merge, dim3(static_cast<unsigned>(rows)), dim3(kVerifyThreads), 0, s, cand, S, top_k,
                        static_cast<int>(nodes), parents, top);
     rc = check_launch("verify_tree merge");
     if (rc != MA_OK) return rc;
   }
-  hipLaunchKernelGGL(k_verify_walk, dim3(static_cast<unsigned>(batch)), dim3(64), 0, s, top, top_k,
+  hipLaunchKernelGGL(k_verify_walk, dim3(static_cast<unsigned>(batch)), dim3(64), 0, s, top, top_k, each,
                      static_cast<int>(nodes), vocab, tokens, parents, uniform, probs, probs_dtype, probs_ldb,
                      probs_ldt, inv_temperature, top_p, out_tokens, accepted, path);
   return check_launch("verify_tree walk");

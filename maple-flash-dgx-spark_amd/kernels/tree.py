@@ -47,14 +47,16 @@ def _call(idx: int, name: str, *args) -> None:
             _lib.call(name, *args, _stream(idx))
 
 
-def _device(what: str, tensors: tuple) -> int:
-    """The one device that all of the tensors (or None) are on."""
+_index = torch.Tensor.get_device
+
+
+def _device(what: str, *tensors: torch.Tensor) -> int:
+    """The one device that all of the tensors are on."""
     idx = tensors[0].get_device()
     if idx < 0:
         raise RuntimeError(f"{what} requires CUDA tensors.")
-    for o in tensors:
-        if o is not None and o.get_device() != idx:
-            raise ValueError(f"{what}: tensors on {o.device} and {tensors[0].device}.")
+    if set(map(_index, tensors)) != {idx}:
+        raise ValueError(f"{what}: tensors on several devices: {[str(t.device) for t in tensors]}.")
     return idx
 
 
@@ -133,7 +135,7 @@ def apply_qkv_tree(
     rows, n_kv, max_len, d = _cache("apply_qkv_tree", k_cache, v_cache, bsz, row_map)
     if n_kv != num_kv_heads or d != head_dim:
         raise ValueError(f"apply_qkv_tree: cache {tuple(k_cache.shape)} for {num_kv_heads} KV heads of {head_dim}.")
-    qw = kw = c = s = None
+    more, qw, kw, c, s = [], None, None, None, None
     w_dt = dt = ld = n_pos = mode = 0
     if q_weight is not None or k_weight is not None:
         if q_weight is None or k_weight is None:
@@ -142,25 +144,33 @@ def apply_qkv_tree(
             raise TypeError("q_norm and k_norm weights must share a dtype.")
         if q_weight.numel() != head_dim or k_weight.numel() != head_dim:
             raise ValueError(f"norm weights need {head_dim} entries.")
-        qw, kw, w_dt = q_weight.contiguous(), k_weight.contiguous(), _lib.dtype_code(q_weight, "q_weight")
+        w_dt = _lib.dtype_code(q_weight, "q_weight")
+        more = [q_weight.contiguous(), k_weight.contiguous()]
+        qw, kw = more[0].data_ptr(), more[1].data_ptr()
     if use_rope and rotary_dim != 0:
-        c, s, mode = cos_table, sin_table, 2 if interleaved else 1
-        if c.ndim != 2 or s.shape != c.shape or s.dtype != c.dtype or s.stride() != c.stride() or c.stride(1) != 1:
+        mode, shape, strides = 2 if interleaved else 1, cos_table.shape, cos_table.stride()
+        if (len(shape) != 2 or sin_table.shape != shape or sin_table.stride() != strides or strides[1] != 1
+                or sin_table.dtype != cos_table.dtype):
             raise ValueError("cos and sin tables must share dtype and layout, rows contiguous.")
-        n_pos, cols = c.shape
-        if n_pos < 1 or cols < rotary_dim:
-            raise ValueError(f"tables {tuple(c.shape)} for a rotary_dim of {rotary_dim}.")
-        dt, ld = _lib.dtype_code(c, "cos_table"), c.stride(0)
+        n_pos, ld = shape[0], strides[0]
+        if n_pos < 1 or shape[1] < rotary_dim:
+            raise ValueError(f"tables {tuple(shape)} for a rotary_dim of {rotary_dim}.")
+        dt = _lib.dtype_code(cos_table, "cos_table")
+        more += [cos_table, sin_table]
+        c, s = cos_table.data_ptr(), sin_table.data_ptr()
     parents = _tree("apply_qkv_tree", parents, bsz, nodes)
     sl = _positions("seqlen", seqlen, bsz)
-    rm = None if row_map is None else _positions("row_map", row_map, bsz)
-    idx = _device("apply_qkv_tree", (qkv, k_cache, v_cache, sl, parents, rm, qw, kw, c, s))
+    rm = None
+    if row_map is not None:
+        more.append(_positions("row_map", row_map, bsz))
+        rm = more[-1].data_ptr()
+    idx = _device("apply_qkv_tree", qkv, k_cache, v_cache, sl, parents, *more)
     out = qkv.new_empty((bsz, nodes, num_heads, head_dim))
     _call(
         idx, "ma_tree_qkv",
-        qkv.data_ptr(), ldb, ldt, bsz, nodes, num_heads, num_kv_heads, head_dim, _lib.ptr(qw), _lib.ptr(kw), w_dt,
-        _lib.ptr(c), _lib.ptr(s), dt, ld, n_pos, rotary_dim if mode else 0, mode, eps, sl.data_ptr(),
-        parents.data_ptr(), _lib.ptr(rm), k_cache.data_ptr(), v_cache.data_ptr(), rows, max_len, out.data_ptr(),
+        qkv.data_ptr(), ldb, ldt, bsz, nodes, num_heads, num_kv_heads, head_dim, qw, kw, w_dt,
+        c, s, dt, ld, n_pos, rotary_dim if mode else 0, mode, eps, sl.data_ptr(),
+        parents.data_ptr(), rm, k_cache.data_ptr(), v_cache.data_ptr(), rows, max_len, out.data_ptr(),
     )
     return out
 
@@ -195,7 +205,7 @@ def tree_attention(
     parents = _tree("tree_attention", parents, bsz, nodes)
     sl = _positions("seqlen", seqlen, bsz)
     rm = None if row_map is None else _positions("row_map", row_map, bsz)
-    idx = _device("tree_attention", (q, k_cache, v_cache, sl, parents, rm))
+    idx = _device("tree_attention", q, k_cache, v_cache, sl, parents, *(() if rm is None else (rm,)))
     q = q.contiguous()
     out = torch.empty_like(q)
     nbytes = _lib.load().ma_tree_attn_workspace_bytes(bsz, nodes, n_q, n_kv, head_dim, max_len, window)
@@ -270,7 +280,7 @@ def verify_tree(
         if one != 1 and vocab > 1:
             raise ValueError("draft_probs rows must be contiguous.")
         p_dt = _lib.dtype_code(draft_probs, "draft_probs")
-    idx = _device("verify_tree", (logits, tokens, parents, uniform, draft_probs))
+    idx = _device("verify_tree", logits, tokens, parents, uniform, *(() if draft_probs is None else (draft_probs,)))
     out = TreeVerdict(torch.empty_like(tokens), parents.new_empty(bsz), torch.empty_like(parents))
     nbytes = _lib.load().ma_verify_tree_workspace_bytes(bsz, nodes, vocab, top_k)
     ws = tokens.new_empty(nbytes // 8)  # scratch of this call alone, as in tree_attention
@@ -323,9 +333,7 @@ def commit_tree(
     sl = _positions("seqlen", seqlen, bsz)
     rm = None if row_map is None else _positions("row_map", row_map, bsz)
     path, accepted = path.contiguous(), accepted.contiguous()
-    idx = _device("commit_tree", (first, sl, rm, path, accepted))
-    if set(map(torch.Tensor.get_device, caches)) != {idx}:
-        raise ValueError("commit_tree: caches on several devices.")
+    idx = _device("commit_tree", *caches, sl, path, accepted, *(() if rm is None else (rm,)))
     out = sl.new_empty(bsz)
     at = ptrs.buffer_info()[0]
     _call(
