@@ -710,8 +710,9 @@ int ma_fused_sample(const void* logits, int dtype, int64_t rows, int64_t vocab, 
  * and 2i + 1, with columns i and i + rotary_dim / 2); 0: none.  cos / sin
  * [n_pos, >= rotary_dim] of cs_dtype, row stride ld_cs, read at the node's
  * position (the last row past the table), rounded to bf16 before use.  q_out
- * bf16 [batch, nodes, n_heads, head_dim] (0 for absent nodes).  head_dim 64 or
- * 128.  The one-token form of it is ma_qk_norm_rope_store.
+ * bf16 [batch, nodes, n_heads, head_dim] (0 for absent nodes).  q_out and the
+ * cache 16-byte aligned; head_dim 64 or 128.  The one-token form of it is
+ * ma_qk_norm_rope_store.
  */
 int ma_tree_qkv(const void* qkv, int64_t ldb, int64_t ldt, int64_t batch, int64_t nodes, int n_heads,
                 int n_kv_heads, int head_dim, const void* q_norm_w, const void* k_norm_w, int w_dtype,
@@ -731,7 +732,8 @@ int ma_tree_qkv(const void* qkv, int64_t ldb, int64_t ldt, int64_t batch, int64_
  * K or V that a node does not see does not reach it, finite or not.
  * workspace: ma_tree_attn_workspace_bytes(...) bytes (may be 0), 16-byte
  * aligned, its content of no matter before and after; calls that share one
- * must not overlap.  head_dim 64 or 128.
+ * must not overlap.  scale finite; q, out and the cache 16-byte aligned; head_dim
+ * 64 or 128.
  */
 size_t ma_tree_attn_workspace_bytes(int64_t batch, int64_t nodes, int n_heads, int n_kv_heads,
                                     int head_dim, int64_t max_len, int64_t window);
@@ -755,7 +757,8 @@ int ma_tree_attn(const void* q, int64_t batch, int64_t nodes, int n_heads, int n
  * that node c's token was drawn from; NULL: q = 1 at t (a chosen token).
  * out_tokens int64 [batch, nodes]: the accepted tokens, then the drawn one, then
  * -1; accepted int32 [batch]: how many were accepted (-1 for a row without a
- * sequence, whose outputs are all -1); path int32 [batch, nodes]: the nodes from
+ * sequence, whose outputs are all -1); a NaN logit is never chosen, a row of
+ * them draws token 0; path int32 [batch, nodes]: the nodes from
  * the root to the last accepted one, then -1.  Laws and walk in 64 bits.  1 <=
  * top_k <= min(64, vocab), inv_temperature finite > 0, 0 < top_p <= 1; top_k = 1
  * is greedy.  workspace: ma_verify_tree_workspace_bytes(...) bytes, 8-byte
@@ -776,8 +779,8 @@ int ma_verify_tree(const void* logits, int dtype, int64_t ldb, int64_t ldt, int6
  * accepted[b] + 1 (accepted and path as ma_verify_tree writes them: path
  * ascending; new_seqlen is not seqlen).  k_caches / v_caches: host arrays of
  * `layers` device pointers to bf16 caches [cache_rows, n_kv_heads, max_len,
- * head_dim], distinct from one another; one launch per 64 layers.  head_dim 64
- * or 128.
+ * head_dim], 16-byte aligned, distinct from one another; one launch per 64
+ * layers.  head_dim 64 or 128.
  */
 int ma_tree_commit(void* const* k_caches, void* const* v_caches, int64_t layers, int64_t batch,
                    int64_t nodes, int n_kv_heads, int head_dim, int64_t cache_rows,

@@ -110,8 +110,9 @@ constexpr int kQkvThreads = 256;
 // (the half layout's partners meet in LDS, whatever h is).  float32 inside; c
 // and s are rounded to bf16 first and y to bf16 at the end, as the one-token
 // path does, so a token's K is the same whichever wrote it.  Latency: two rounds
-// of loads (x, weights, tree and length; then the table's row).  A wave a head
-// with a tree of its own took 15.2 us for 1024 nodes of 32 + 8 heads of 64.
+// of loads (x, weights, tree and length; then the table's row): 4.3 us for 8
+// nodes of 32 + 8 heads of 64, 7.3 for 1024 (a wave a head with a tree of its
+// own: 15.2), 5.6 for 488 of 16 + 8 heads of 128.
 // VEC: all rows are 16-byte aligned.
 template <int HD, bool VEC>
 __global__ __launch_bounds__(kQkvThreads) void k_tree_qkv(
@@ -240,20 +241,19 @@ __device__ __forceinline__ f32x16t_t mfma_tree(uint4 a, uint4 b, f32x16t_t c) {
                                                  c, 0, 0, 0);
 }
 
-// A tile's shape: 32 RW query rows, RW waves of 32 rows times 4 / RW waves of
-// NP positions each.
-template <int HD, int RW>
+// A workgroup: four waves of 32 query rows, which share its K and V.  (64 or 32
+// rows and the waves left over on positions of their own, for trees of few rows:
+// 26 against 27 us at 32 x 8 nodes over 4096 of 64, 28 against 27 at 16 x 8 of 128,
+// 9.8 against 9.3 at 1 x 16 of 128; no better on the whole, and gone.)
+template <int HD>
 struct TreeTile {
-  static constexpr int kRows = 32 * RW;
-  static constexpr int kPW = 4 / RW;                                  // position groups
-  static constexpr int kNP = HD == 64 && RW > 1 ? 64 : 32;            // positions of a group per step
-  static constexpr int kStep = kPW * kNP;                             // positions of a workgroup per step
-  static constexpr int kBufs = RW == 4 ? 3 : 2;
+  static constexpr int kRows = 128;
+  static constexpr int kStep = HD == 64 ? 64 : 32;                  // positions per step
+  static constexpr int kBufs = 3;
   static constexpr int kRowBytes = HD * 2;
-  static constexpr int kRegion = kNP * kRowBytes;                     // K or V of a group
-  static constexpr int kStage = kPW * 2 * kRegion;
-  static constexpr int kCopies = kNP / RW * kRowBytes / 1024;         // 1 KB copies of a wave, K and V each
-  static constexpr int kWaves = RW == 4 && HD == 64 ? 3 : (HD == 128 && RW == 1 ? 1 : 2);  // waves per SIMD (LDS, registers)
+  static constexpr int kRegion = kStep * kRowBytes;                 // K or V of a step
+  static constexpr int kCopies = kStep / 4 * kRowBytes / 1024;      // 1 KB copies of a wave, K and V each
+  static constexpr int kWaves = HD == 64 ? 3 : 2;                   // waves per SIMD, so workgroups per compute unit (registers)
 };
 
 // The 16-byte piece c of LDS row r lies at piece c ^ tree_key(r) of that row:
@@ -296,30 +296,37 @@ struct TreeRow {
 // of the window) are masked by a word per query row; there a V that is not
 // finite must not reach the rows that do not see it (0 x inf), so such values
 // are taken out of the product and added to the rows that see them.
-template <int HD, int RW>
-__global__ __launch_bounds__(256, (TreeTile<HD, RW>::kWaves)) void k_tree_attn(
+//
+// What bounds it.  32 query rows and 32 positions of 64 dims take about 300 cycles
+// of the matrix unit, 260 of the vector unit and, four such waves to a compute
+// unit's LDS, 400 of its reads; they overlap in part.  From 4096 positions on each
+// further 4096 take 35 us at 32 x 32 nodes of 32 / 4 heads of 64 (970 TFLOP/s; a
+// large matrix product reaches 1210), a further 16384 take 18 us at 2 x 64 nodes
+// of 16 / 4 heads of 128 (930).  The rest of a launch is
+// fixed: 3 us to the first tile (a row's length, then its K and V, cold), the
+// tree's own masked tiles (about 1 us each), the splits' sums, all written at
+// the end: 50 us in all at 32 x 32 nodes over 4096, 45 where the rows hold half to
+// all of that.
+template <int HD>
+__global__ __launch_bounds__(256, (TreeTile<HD>::kWaves)) void k_tree_attn(
     const uint16_t* __restrict__ q, int nodes, int nq, int nkv, int tiles, int S, int n_units,
     const uint16_t* __restrict__ k_cache, const uint16_t* __restrict__ v_cache, int64_t cache_rows, int64_t max_len,
     const int64_t* __restrict__ seqlen, const int32_t* __restrict__ parents, const int64_t* __restrict__ row_map,
     int64_t window, float scale, uint16_t* __restrict__ out, float* __restrict__ part_acc,
     float2* __restrict__ part_ml) {
-  using T = TreeTile<HD, RW>;
+  using T = TreeTile<HD>;
   constexpr int KS = HD / 16;  // k slices of a score
   constexpr int DB = HD / 32;  // 32-dim blocks of the output
   constexpr int CPR = HD / 8;  // 16-byte pieces of a cache row
-  constexpr int NT = T::kNP / 32;
-  __shared__ __align__(16) char buf0[T::kStage];
-  __shared__ __align__(16) char buf1[T::kStage];
-  __shared__ __align__(16) char buf2[T::kBufs == 3 ? T::kStage : 16];
+  constexpr int NT = T::kStep / 32;
+  __shared__ __align__(16) char buf0[2 * T::kRegion];  // K, then V
+  __shared__ __align__(16) char buf1[2 * T::kRegion];
+  __shared__ __align__(16) char buf2[2 * T::kRegion];
   __shared__ uint64_t t_anc[kTreeNodes];
   __shared__ int t_depth[kTreeNodes];
-  __shared__ float wm[4][32], wl[4][32];
-  constexpr int kWave = DB * 16 * 64;  // floats of a wave's sums
-  static_assert((T::kPW - 1) * RW * kWave * 4 <= T::kStage, "the position groups' sums fit one buffer");
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int rw = RW == 4 ? wv : wv % RW, pw = RW == 4 ? 0 : wv / RW;
   const int r32 = lane & 31, h = lane >> 5;
   // tiles of the same positions follow each other on one XCD
   const int xcd = blockIdx.x % kXcds, turn = blockIdx.x / kXcds;
@@ -350,15 +357,13 @@ __global__ __launch_bounds__(256, (TreeTile<HD, RW>::kWaves)) void k_tree_attn(
   const int p_beg = p0 < s_beg ? s_beg : (p0 < s_end ? static_cast<int>(p0) : s_end);
   const int turn0 = (p_beg - s_beg) % T::kBufs == 0 ? 0 : T::kBufs - (p_beg - s_beg) % T::kBufs;
 
-  // copies of step s into a buffer: each wave its share of its group's rows,
-  // rows past the end read again from the last one
-  const int copy_row = rw * (T::kNP / RW) + lane / CPR;
+  // copies of step s into a buffer: each wave its share of the rows, rows past
+  // the end read again from the last one
+  const int copy_row = wv * (T::kStep / 4) + lane / CPR;
   auto copy = [&](int s, char* buf) {
-    const int64_t t0 = start + static_cast<int64_t>(s) * T::kStep + pw * T::kNP;
-    char* const dst = buf + pw * 2 * T::kRegion + rw * (T::kNP / RW) * T::kRowBytes;
-    const int64_t left = end - 1 - t0;  // (negative: the group has none; its copies all take the last row)
-    const int64_t at = left < 0 ? end - 1 : t0;
-    const int most = left < 0 ? 0 : (left < T::kNP ? static_cast<int>(left) : T::kNP - 1);
+    const int64_t at = start + static_cast<int64_t>(s) * T::kStep, left = end - 1 - at;
+    const int most = left < T::kStep ? static_cast<int>(left) : T::kStep - 1;
+    char* const dst = buf + wv * (T::kStep / 4) * T::kRowBytes;
     const char* const ks = reinterpret_cast<const char*>(k_cache + (base + at) * HD);
     const char* const vs = reinterpret_cast<const char*>(v_cache + (base + at) * HD);
 #pragma unroll
@@ -370,7 +375,7 @@ __global__ __launch_bounds__(256, (TreeTile<HD, RW>::kWaves)) void k_tree_attn(
     }
   };
   // this lane's query row, as it is in memory
-  const int r = tile * T::kRows + rw * 32 + r32;
+  const int r = tile * T::kRows + wv * 32 + r32;
   const int node = r < M ? r / group : 0;
   uint4 qf[KS];
   {
@@ -381,7 +386,7 @@ __global__ __launch_bounds__(256, (TreeTile<HD, RW>::kWaves)) void k_tree_attn(
   const int par = tree_parent(parents + b * nodes, nodes);
   MA_ISSUE_FENCE();
   if (s_beg < s_end) copy(s_beg, turn0 == 0 ? buf0 : (turn0 == 1 ? buf1 : buf2));
-  if (T::kBufs == 3 && s_beg + 1 < s_end) copy(s_beg + 1, turn0 == 0 ? buf1 : (turn0 == 1 ? buf2 : buf0));
+  if (s_beg + 1 < s_end) copy(s_beg + 1, turn0 == 0 ? buf1 : (turn0 == 1 ? buf2 : buf0));
   MA_ISSUE_FENCE();
   const TreeLane me = tree_lane(par, nodes);
   if (wv == 0) {
@@ -429,7 +434,7 @@ __global__ __launch_bounds__(256, (TreeTile<HD, RW>::kWaves)) void k_tree_attn(
     for (int i = 0; i < 16; ++i) o[db][i] = 0.f;
   float mref = -INFINITY, lsum = 0.f;
 
-  // Byte offsets into a group's K and V rows: piece 2 ks + h of row r32 (ks of
+  // Byte offsets into the K and V rows: piece 2 ks + h of row r32 (ks of
   // one half; 128 bytes on for the other), and the lane's 8 bytes of the
   // transposing read for even and odd 32-dim blocks (128 bytes on for each two).
   // Rows 8 further have the same key.
@@ -494,7 +499,7 @@ __global__ __launch_bounds__(256, (TreeTile<HD, RW>::kWaves)) void k_tree_attn(
   // The NT x 32 positions of a group that all rows see: all K reads ahead of the
   // first product, the V reads ahead of the softmax.
   auto attend = [&](const char* buf) {
-    const char* const kb = buf + pw * 2 * T::kRegion;
+    const char* const kb = buf;
     const char* const vb = kb + T::kRegion;
     f32x16t_t sc[NT];
     {
@@ -608,22 +613,21 @@ __global__ __launch_bounds__(256, (TreeTile<HD, RW>::kWaves)) void k_tree_attn(
     }
   };
 
-  // Step s's copies are in (those of later steps may be in flight), the other
-  // waves' too, which have also left step s - 1 (RW = 1: every wave reads its
-  // own copies only); the copies of step s + kBufs - 1 go to its buffer.
+  // Step s's copies are in (those of s + 1 may be in flight), the other waves'
+  // too, which have also left step s - 1; the copies of step s + 2 go to its buffer.
   auto arrive = [&](int s, char* prev) {
-    if (T::kBufs == 3 && s + 1 < s_end) __builtin_amdgcn_s_waitcnt(tree_vmcnt(2 * T::kCopies));
+    if (s + 1 < s_end) __builtin_amdgcn_s_waitcnt(tree_vmcnt(2 * T::kCopies));
     else __builtin_amdgcn_s_waitcnt(tree_vmcnt(0));
     asm volatile("" ::: "memory");
-    if (RW > 1) __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    if (s + T::kBufs - 1 < s_end) copy(s + T::kBufs - 1, prev);
+    if (s + 2 < s_end) copy(s + 2, prev);
   };
   const int p_end = p1 < s_end ? static_cast<int>(p1) : s_end;
   for (int s = s_beg, turn = turn0; s < s_end;) {
     if (turn == 0 && s >= p_beg && s < p_end) {
       do {
-        arrive(s, T::kBufs == 3 ? buf2 : buf1);
+        arrive(s, buf2);
         if (busy) attend(buf0);
         if (++s == p_end) {
           turn = 1;
@@ -631,26 +635,22 @@ __global__ __launch_bounds__(256, (TreeTile<HD, RW>::kWaves)) void k_tree_attn(
         }
         arrive(s, buf0);
         if (busy) attend(buf1);
-        ++s;
-        if (T::kBufs == 3) {
-          if (s == p_end) {
-            turn = 2;
-            break;
-          }
-          arrive(s, buf1);
-          if (busy) attend(buf2);
-          ++s;
+        if (++s == p_end) {
+          turn = 2;
+          break;
         }
+        arrive(s, buf1);
+        if (busy) attend(buf2);
+        ++s;
       } while (s < p_end);
       continue;
     }
     char* const cur = turn == 0 ? buf0 : (turn == 1 ? buf1 : buf2);
-    char* const prev = T::kBufs == 2 ? (turn == 0 ? buf1 : buf0) : (turn == 0 ? buf2 : (turn == 1 ? buf0 : buf1));
-    arrive(s, prev);
+    arrive(s, turn == 0 ? buf2 : (turn == 1 ? buf0 : buf1));
     if (busy) {
-      const int64_t tb = start + static_cast<int64_t>(s) * T::kStep + pw * T::kNP;
+      const int64_t tb = start + static_cast<int64_t>(s) * T::kStep;
       for (int t = 0; t < NT; ++t) {
-        const char* const kb = cur + pw * 2 * T::kRegion + 32 * t * T::kRowBytes;
+        const char* const kb = cur + 32 * t * T::kRowBytes;
         if (tb + 32 * t < end) attend_edge(tb + 32 * t, kb, kb + T::kRegion);
       }
     }
@@ -658,54 +658,11 @@ __global__ __launch_bounds__(256, (TreeTile<HD, RW>::kWaves)) void k_tree_attn(
     turn = turn + 1 == T::kBufs ? 0 : turn + 1;
   }
 
-  lsum += __shfl_xor(lsum, 32, 64);
-  float m = mref, l = lsum;
-  if (T::kPW > 1) {  // the position groups' results, in order
-    if (h == 0) {
-      wm[wv][r32] = mref;
-      wl[wv][r32] = lsum;
-    }
-    __syncthreads();
-    m = -INFINITY;
-#pragma unroll
-    for (int g = 0; g < T::kPW; ++g) m = fmaxf(m, wm[g * RW + rw][r32]);
-    l = 0.f;
-#pragma unroll
-    for (int g = 0; g < T::kPW; ++g) {
-      const float lg = wl[g * RW + rw][r32];
-      l += lg != 0.f ? __builtin_amdgcn_exp2f(wm[g * RW + rw][r32] - m) * lg : 0.f;
-    }
-    // (a sum that is not a number stays one: only a row that saw nothing has 0)
-    const float f = lsum != 0.f ? __builtin_amdgcn_exp2f(mref - m) : 0.f;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const float fi = of_row(f, i);
-#pragma unroll
-      for (int db = 0; db < DB; ++db) o[db][i] = fi != 0.f ? o[db][i] * fi : 0.f;
-    }
-    auto at = [&](int g) { return reinterpret_cast<float*>(buf0) + ((g - 1) * RW + rw) * kWave + lane; };
-    if (pw > 0) {
-      float* const d = at(pw);
-#pragma unroll
-      for (int db = 0; db < DB; ++db)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) d[(db * 16 + i) * 64] = o[db][i];
-    }
-    __syncthreads();
-    if (pw > 0) return;
-#pragma unroll
-    for (int g = 1; g < T::kPW; ++g) {
-      const float* const d = at(g);
-#pragma unroll
-      for (int db = 0; db < DB; ++db)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) o[db][i] += d[(db * 16 + i) * 64];
-    }
-  }
+  const float l = lsum + __shfl_xor(lsum, 32, 64);
   const bool seen = depth >= 0 && l != 0.f;
   if (S > 1) {
-    const int64_t pr = ((pair * tiles + tile) * S + sp) * T::kRows + rw * 32;
-    if (h == 0) part_ml[pr + r32] = seen ? make_float2(m, l) : make_float2(-INFINITY, 0.f);
+    const int64_t pr = ((pair * tiles + tile) * S + sp) * T::kRows + wv * 32;
+    if (h == 0) part_ml[pr + r32] = seen ? make_float2(mref, l) : make_float2(-INFINITY, 0.f);
     if (s_beg < s_end && busy)
 #pragma unroll
       for (int i = 0; i < 16; ++i)
@@ -721,7 +678,7 @@ __global__ __launch_bounds__(256, (TreeTile<HD, RW>::kWaves)) void k_tree_attn(
     const int ri = 8 * (i >> 2) + 4 * h + (i & 3);
     const float fi = __shfl(inv, ri, 64);
     const int on = __shfl(has, ri, 64);
-    const int rr = tile * T::kRows + rw * 32 + ri;
+    const int rr = tile * T::kRows + wv * 32 + ri;
     if (rr < M) {
       uint16_t* const dst = out + ((b * nodes + rr / group) * nq + kvh * group + rr % group) * HD + r32;
 #pragma unroll
@@ -734,7 +691,8 @@ __global__ __launch_bounds__(256, (TreeTile<HD, RW>::kWaves)) void k_tree_attn(
 // 2^(m_s - m) l_s; a row that no split saw anything for is 0.  HD / 4 lanes of 4
 // dims times G groups of splits a row: a thread takes the splits g, g + G, ..,
 // all loads of four at once and relative to its own maximum, then the groups
-// meet in LDS, in order.
+// meet in LDS, in order.  Its bytes: 25 MB of sums in 6.7 us, 34 MB in 9.0; 2.7 us
+// where there are few (a launch and two rounds of loads).
 template <int HD>
 __global__ __launch_bounds__(256) void k_tree_merge(const float* __restrict__ part_acc,
                                                     const float2* __restrict__ part_ml, int S, int G, int rows_tile,
@@ -815,7 +773,7 @@ __global__ __launch_bounds__(256) void k_tree_merge(const float* __restrict__ pa
 }
 
 struct TreePlan {
-  int rw, tiles, splits;
+  int tiles, splits;
   int64_t pairs;
 };
 
@@ -823,8 +781,7 @@ static TreePlan tree_plan(int64_t batch, int64_t nodes, int nq, int nkv, int hea
                           int64_t window) {
   TreePlan p;
   const int64_t M = nodes * (nq / nkv);
-  p.rw = M <= 32 ? 1 : (M <= 64 ? 2 : 4);
-  p.tiles = static_cast<int>(cdiv(M, 32 * p.rw));
+  p.tiles = static_cast<int>(cdiv(M, TreeTile<64>::kRows));
   p.pairs = batch * nkv;
   int64_t span = max_len;
   if (window > 0 && window + nodes < span) span = window + nodes;
@@ -832,12 +789,14 @@ static TreePlan tree_plan(int64_t batch, int64_t nodes, int nq, int nkv, int hea
   // TreeTile::kWaves), but no more than pay.  With N steps in all a split costs
   // its N / S steps, about 1.2 us each while the card is not full, and S adds to
   // the merge: 0.05 us and its sums, written and read at 5 TB/s.  Measured (attention + merge,
-  // us): 32 x 32 nodes over 4096 of 64: 64 in one split, 60 in two, 57 in three
-  // (all resident), 68 in four; 7 x 23 over a window of 512 of 128: 19 in two, 17
-  // in four to six, 23 in 17; 1 x 8 over 4096 of 64: 16 in 8, 13 in 33.
-  const int64_t n = cdiv(span, (head_dim == 64 && p.rw > 1 ? 64 : 32) * (4 / p.rw));
-  const int64_t per_cu = p.rw == 4 && head_dim == 64 ? 3 : (head_dim == 128 && p.rw == 1 ? 1 : 2);
-  const double sums = static_cast<double>(p.pairs) * p.tiles * 32 * p.rw * head_dim * 8.0 / 5e6;
+  // us): 32 x 32 nodes over 4096 of 64: 62 in one split, 49 + 6 in two, 45 + 7 in
+  // three (all resident), 48 + 8 in four; 2 x 64 over 32768 of 128: 54 + 6 in 16,
+  // 39 + 9 in 32 (all resident), 48 + 12 in 43; 7 x 23 over a window of 512 of 128: 21
+  // in one, 13 + 4 in two, 11 + 4 in four, 12 + 5 in eight; 1 x 8 over 4096 of 64:
+  // 13 + 4 in 4, 10 + 4 in 8, 8 + 4 in 12, 7 + 5 in 24 to 32.
+  const int64_t n = cdiv(span, head_dim == 64 ? TreeTile<64>::kStep : TreeTile<128>::kStep);
+  const int64_t per_cu = head_dim == 64 ? TreeTile<64>::kWaves : TreeTile<128>::kWaves;
+  const double sums = static_cast<double>(p.pairs) * p.tiles * TreeTile<64>::kRows * head_dim * 8.0 / 5e6;
   const int64_t pays = static_cast<int64_t>(sqrt(1.2 * static_cast<double>(n) / (0.05 + sums)));
   int64_t s = per_cu * 256 / (p.pairs * p.tiles > 0 ? p.pairs * p.tiles : 1);
   s = s < pays ? s : pays;
@@ -848,7 +807,7 @@ static TreePlan tree_plan(int64_t batch, int64_t nodes, int nq, int nkv, int hea
 
 static size_t tree_ws_bytes(const TreePlan& p, int head_dim) {
   if (p.splits <= 1) return 0;
-  const size_t rows = static_cast<size_t>(p.pairs) * p.tiles * p.splits * 32 * p.rw;
+  const size_t rows = static_cast<size_t>(p.pairs) * p.tiles * p.splits * TreeTile<64>::kRows;
   return rows * (static_cast<size_t>(head_dim) * sizeof(float) + sizeof(float2));
 }
 
@@ -868,7 +827,7 @@ struct CommitPtrs {
 // source may be another's destination: all of a round's rows are read before
 // any is written, and rounds go up the path (a later round's sources lie above
 // every slot written so far).  Latency: the row's numbers at once, then its
-// data.
+// data: 3.1 us for one row of 8 nodes in 24 layers, 4.4 for 32 of 32.
 template <int HD>
 __global__ __launch_bounds__(256) void k_tree_commit(CommitPtrs ptrs, int items, int nodes, int nkv,
                                                      int64_t cache_rows, int64_t max_len,
@@ -997,7 +956,7 @@ extern "C" int ma_tree_attn(const void* q, int64_t batch, int64_t nodes, int n_h
   const size_t need = tree_ws_bytes(p, head_dim);
   if (need && (!workspace || workspace_bytes < need))
     return fail(MA_EVALUE, "tree_attn: workspace of %zu bytes, need %zu", workspace ? workspace_bytes : 0, need);
-  const int64_t part_rows = p.pairs * p.tiles * p.splits * 32 * p.rw;
+  const int64_t part_rows = p.pairs * p.tiles * p.splits * TreeTile<64>::kRows;
   float* const acc = static_cast<float*>(workspace);
   float2* const ml = need ? reinterpret_cast<float2*>(acc + part_rows * head_dim) : nullptr;
   const int64_t units = p.pairs * p.splits;
@@ -1009,15 +968,8 @@ extern "C" int ma_tree_attn(const void* q, int64_t batch, int64_t nodes, int n_h
                        static_cast<const uint16_t*>(k_cache), static_cast<const uint16_t*>(v_cache), cache_rows,
                        max_len, seqlen, parents, row_map, window, scale, static_cast<uint16_t*>(out), acc, ml);
   };
-  if (head_dim == 64) {
-    if (p.rw == 1) go(k_tree_attn<64, 1>);
-    else if (p.rw == 2) go(k_tree_attn<64, 2>);
-    else go(k_tree_attn<64, 4>);
-  } else {
-    if (p.rw == 1) go(k_tree_attn<128, 1>);
-    else if (p.rw == 2) go(k_tree_attn<128, 2>);
-    else go(k_tree_attn<128, 4>);
-  }
+  if (head_dim == 64) go(k_tree_attn<64>);
+  else go(k_tree_attn<128>);
   rc = check_launch("tree_attn");
   if (rc != MA_OK || p.splits == 1) return rc;
   const int64_t rows = p.pairs * nodes * (n_heads / n_kv_heads);
@@ -1025,7 +977,7 @@ extern "C" int ma_tree_attn(const void* q, int64_t batch, int64_t nodes, int n_h
   while (G < 1024 / head_dim && 4 * G < p.splits) G *= 2;
   const dim3 mg(static_cast<unsigned>(cdiv(rows * (head_dim / 4) * G, 256)));
   auto merge = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, mg, dim3(256), 0, s, acc, ml, p.splits, G, 32 * p.rw, p.tiles, static_cast<int>(nodes),
+    hipLaunchKernelGGL(kernel, mg, dim3(256), 0, s, acc, ml, p.splits, G, TreeTile<64>::kRows, p.tiles, static_cast<int>(nodes),
                        n_heads, n_kv_heads, rows, static_cast<uint16_t*>(out));
   };
   if (head_dim == 64) merge(k_tree_merge<64>);

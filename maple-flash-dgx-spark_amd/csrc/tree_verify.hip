@@ -46,8 +46,8 @@ constexpr int kVerifyCap = kVerifyMaxK * (kVerifyPer + 1);  // candidates held
 constexpr int kVerifyPick = 512;                            // candidates whose places are counted
 // Workgroups that a launch aims for: segments of rows up to that many, since they
 // cost a merge (us, vocabulary 151936: 1024 rows whole 58, in two 61 + 6, in four
-// 59 + 7; 104 rows in 5 17 + 6, in 10 15 + 5, in 20 15 + 5; 8 rows in 10 8.5 + 5,
-// in 38 5.5 + 4).
+// 59 + 7; 104 rows in 5 17 + 6, in 10 15 + 5, in 20 15 + 5; 8 rows in 10 8.5, in 38
+// 5.5, and 4 to 5 for the merge).
 constexpr int kVerifyTargetGroups = 1024;
 
 __device__ __forceinline__ uint32_t verify_order(float v) {
@@ -390,6 +390,7 @@ __global__ __launch_bounds__(kVerifyThreads) void k_verify_topk(const void* __re
   if (tid < k) out[tid] = tid < st.have ? L.cand[tid] : 0;
 }
 
+// Latency: 104 nodes of 10 segments x 50 keys in 5 us.
 __global__ __launch_bounds__(kVerifyThreads) void k_verify_merge(const uint64_t* __restrict__ cand, int S, int k,
                                                                  int nodes, const int32_t* __restrict__ parents,
                                                                  uint64_t* __restrict__ out) {
@@ -490,7 +491,9 @@ __device__ __forceinline__ uint64_t wave_max_key(uint64_t key) {
 // One wave per row: a lane per token of the current law (and per node of the
 // tree).  `each` keys a node: its law's k, or (k = 1) its segments' maxima.
 // Latency: a step waits for one round of loads, the child's law and the
-// draft's probabilities together, asked for while the child before it is judged.
+// draft's probabilities together, asked for while the child before it is judged:
+// 3.2 us for one greedy row of 8 nodes, 7.0 for 8 rows of 13 with draft laws, 6.0
+// for 32 rows of 32.
 __global__ __launch_bounds__(64) void k_verify_walk(
     const uint64_t* __restrict__ top, int k, int each, int nodes, int64_t vocab, const int64_t* __restrict__ tokens,
     const int32_t* __restrict__ parents, const float* __restrict__ uniform, const void* __restrict__ probs,

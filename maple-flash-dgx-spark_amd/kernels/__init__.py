@@ -1,5 +1,6 @@
 """HIP kernels of the hot path, exported under the reference's names
-(``src/maple_run/kernels/__init__.py:5-39``), plus ``moe_dispatch``.
+(``src/maple_run/kernels/__init__.py:5-39``), plus ``moe_dispatch`` and the four
+of decoding with drafted token trees (``tree``).
 
 Importing this package does not load the HIP library; the first kernel call
 does (and raises if it has not been built).  The functions are bound eagerly

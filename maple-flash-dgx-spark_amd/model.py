@@ -270,7 +270,6 @@ class SyntheticDecoder:
         self.embed = synthetic.rtn4_table(c.vocab, c.hidden, c.rtn_group, s + 902, dev, lo, hi)
         self.final_norm = ones(c.hidden)
         self.cos, self.sin = rope_tables(max_len, c.rotary_dim, c.rope_theta, dev, c.rope_scaling)
-        self.cos_sin16 = self.cos.bfloat16(), self.sin.bfloat16()
         self.flash_head = None
         self._pack_read_ahead()
 
@@ -291,7 +290,6 @@ class SyntheticDecoder:
         self.layers = list(layers)
         self.embed, self.lm_head, self.final_norm = embed, lm_head, final_norm
         self.cos, self.sin = rope_tables(max_len, cfg.rotary_dim, cfg.rope_theta, self.device, cfg.rope_scaling)
-        self.cos_sin16 = self.cos.bfloat16(), self.sin.bfloat16()
         self.flash_head = None
         self._pack_read_ahead()
         return self
@@ -437,9 +435,8 @@ class SyntheticDecoder:
         for i, L in enumerate(self.layers):
             window, use_rope = c.layer_attention(i)
             qkv = ternary_gemv(hidden, L.qkv, L.qkv_alpha, rms_weight=L.input_ln, rms_eps=c.eps)
-            # (decode_attention rounds the tables to bf16 as it reads them)
-            q = apply_qkv_tree(qkv.view(w, t, -1), L.q_norm, L.k_norm, *self.cos_sin16, cache.k[i], cache.v[i], seqlen,
-                               parents, row_map=row_map, num_heads=c.heads, num_kv_heads=c.kv_heads,
+            q = apply_qkv_tree(qkv.view(w, t, -1), L.q_norm, L.k_norm, self.cos, self.sin, cache.k[i], cache.v[i],
+                               seqlen, parents, row_map=row_map, num_heads=c.heads, num_kv_heads=c.kv_heads,
                                head_dim=c.head_dim, rotary_dim=c.rotary_dim, use_rope=use_rope, eps=c.eps)
             attn = tree_attention(q, cache.k[i], cache.v[i], seqlen, parents, row_map=row_map,
                                   scale=c.head_dim ** -0.5, window=window)

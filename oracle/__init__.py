@@ -16,6 +16,9 @@ Modules
                MoE combine, RTN4 GEMV / embedding, RMSNorm, dispatch.
 ``decoder``  -- the synthetic decoder step (RoPE, decode GQA attention,
                decoder layer, lm_head) used for the full-model parity check.
+``tree``     -- trees of drafted tokens: branches, rotary positions in both
+               layouts, attention, the sampler's law and the walk over it, one
+               node at a time in float64 (no reference counterpart).
 
 How each function is pinned (against what fails if it is wrong) is listed in
 the docstring of each function and tested in ``tests/test_oracle_*.py``.
