@@ -671,18 +671,17 @@ __global__ __launch_bounds__(256, (TreeTile<HD>::kWaves)) void k_tree_attn(
           part_acc[(pr + 8 * (i >> 2) + 4 * h + (i & 3)) * HD + 32 * db + r32] = o[db][i];
     return;
   }
+  // (an output row's place and factor come from the lane that holds its query row)
   const float inv = seen ? 1.0f / l : 0.f;
-  const int has = __shfl(seen ? 1 : 0, r32, 64);
+  const int place = r < M ? ((node * nq + kvh * group + r % group) * HD << 1) | (seen ? 1 : 0) : -1;
+  uint16_t* const to = out + b * nodes * nq * HD + r32;
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
-    const int ri = 8 * (i >> 2) + 4 * h + (i & 3);
-    const float fi = __shfl(inv, ri, 64);
-    const int on = __shfl(has, ri, 64);
-    const int rr = tile * T::kRows + wv * 32 + ri;
-    if (rr < M) {
-      uint16_t* const dst = out + ((b * nodes + rr / group) * nq + kvh * group + rr % group) * HD + r32;
+    const float fi = of_row(inv, i);
+    const int pl = __builtin_amdgcn_ds_bpermute(row_lane(i), place);
+    if (pl >= 0) {
 #pragma unroll
-      for (int db = 0; db < DB; ++db) dst[32 * db] = on ? f32_to_bf16(o[db][i] * fi) : 0;
+      for (int db = 0; db < DB; ++db) to[(pl >> 1) + 32 * db] = pl & 1 ? f32_to_bf16(o[db][i] * fi) : 0;
     }
   }
 }
@@ -785,22 +784,33 @@ static TreePlan tree_plan(int64_t batch, int64_t nodes, int nq, int nkv, int hea
   p.pairs = batch * nkv;
   int64_t span = max_len;
   if (window > 0 && window + nodes < span) span = window + nodes;
-  // Splits: as many as keep every workgroup resident (2 or 3 to a compute unit:
-  // TreeTile::kWaves), but no more than pay.  With N steps in all a split costs
-  // its N / S steps, about 1.2 us each while the card is not full, and S adds to
-  // the merge: 0.05 us and its sums, written and read at 5 TB/s.  Measured (attention + merge,
-  // us): 32 x 32 nodes over 4096 of 64: 62 in one split, 49 + 6 in two, 45 + 7 in
-  // three (all resident), 48 + 8 in four; 2 x 64 over 32768 of 128: 54 + 6 in 16,
-  // 39 + 9 in 32 (all resident), 48 + 12 in 43; 7 x 23 over a window of 512 of 128: 21
-  // in one, 13 + 4 in two, 11 + 4 in four, 12 + 5 in eight; 1 x 8 over 4096 of 64:
-  // 13 + 4 in 4, 10 + 4 in 8, 8 + 4 in 12, 7 + 5 in 24 to 32.
+  // Splits.  With N steps in all a split costs its N / S steps, up to 1.2 us each
+  // while there is a workgroup at most to a compute unit, and S adds to the merge:
+  // 0.05 us and its sums, written and read at 5 TB/s.  The merge is a launch of
+  // about 4 us: none that saves fewer than 6 steps.  More workgroups than compute
+  // units, as many as are resident (2 or 3 to one: TreeTile::kWaves), hide each
+  // other's waits and take more of each other's time, and more sums: from 40 steps
+  // a workgroup on.  Measured (attention + merge, us):
+  //   32 x 32 nodes of 64 over 1024: 23 in one split, 22 + 6 in two, 23 + 6 in three;
+  //     over 2048 35, 31 + 6, 31 + 7; over 2752 44, 38 + 6, 37 + 7; over 4096 62, 49 + 6,
+  //     45 + 7 and 48 + 8 in four (not all resident)
+  //   8 x 32 of 64 over 4096: 31 + 4 in two, 21 + 4 in four, 23 + 5 in six, 23 + 7 in nine;
+  //     over 16384 60 + 5 in four, 52 + 6 in eight, 48 + 8 in twelve
+  //   2 x 64 of 128 over 20000: 38 + 6 in 16, 33 + 9 in 32; over 32768 54 + 6, 39 + 9, and
+  //     48 + 12 in 43
+  //   4 x 16 of 64 over 2048: 18 + 4 in two, 12 + 4 in four, 9 + 4 in eight, 11 + 5 in 16
+  //   1 x 8 of 64 over 370: 11 in one, 6 + 4 in six; over 4096 13 + 4 in 4, 10 + 4 in 8,
+  //     8 + 4 in 12, 7 + 5 in 24 to 32
   const int64_t n = cdiv(span, head_dim == 64 ? TreeTile<64>::kStep : TreeTile<128>::kStep);
   const int64_t per_cu = head_dim == 64 ? TreeTile<64>::kWaves : TreeTile<128>::kWaves;
-  const double sums = static_cast<double>(p.pairs) * p.tiles * TreeTile<64>::kRows * head_dim * 8.0 / 5e6;
+  const int64_t at_once = p.pairs * p.tiles > 0 ? p.pairs * p.tiles : 1;
+  const double sums = static_cast<double>(at_once) * TreeTile<64>::kRows * head_dim * 8.0 / 5e6;
   const int64_t pays = static_cast<int64_t>(sqrt(1.2 * static_cast<double>(n) / (0.05 + sums)));
-  int64_t s = per_cu * 256 / (p.pairs * p.tiles > 0 ? p.pairs * p.tiles : 1);
+  int64_t s = 256 / at_once > 1 ? 256 / at_once : 1;
+  if (n >= 40 * s) s = per_cu * 256 / at_once;
   s = s < pays ? s : pays;
   s = s < 1 ? 1 : (s > n ? n : s);
+  if (n - n / s < 6) s = 1;
   p.splits = static_cast<int>(s);
   return p;
 }
