@@ -699,7 +699,7 @@ int ma_fused_sample(const void* logits, int dtype, int64_t rows, int64_t vocab, 
  * position seqlen[b] + i, its rotary position is seqlen[b] + its depth.  A node
  * whose slot falls behind the cache (max_len) is neither stored nor attended;
  * mapped rows are clamped to [0, cache_rows), seqlen to [0, max_len].  batch x
- * nodes and batch x n_kv_heads at most 65535.
+ * nodes, batch x n_kv_heads and n_heads at most 65535.
  *
  * QK RMSNorm + rotary positions + K/V store of the nodes: qkv bf16 [batch,
  * nodes, (n_heads + 2 n_kv_heads) * head_dim] (strides ldb, ldt, 1); per head

@@ -894,9 +894,9 @@ int check_tree(const char* what, int64_t batch, int64_t nodes, int n_heads, int 
   if (batch < 0 || nodes < 1 || nodes > kTreeNodes)
     return fail(MA_EVALUE, "%s: a tree has 1 to %d nodes, got %lld", what, kTreeNodes, static_cast<long long>(nodes));
   if (head_dim != 64 && head_dim != 128) return fail(MA_EVALUE, "%s: head_dim %d unsupported (64 or 128)", what, head_dim);
-  if (n_kv_heads < 1 || n_heads < n_kv_heads || n_heads % n_kv_heads != 0)
+  if (n_kv_heads < 1 || n_heads < n_kv_heads || n_heads % n_kv_heads != 0 || n_heads > 65535)
     return fail(MA_EVALUE, "%s: %d query heads over %d KV heads", what, n_heads, n_kv_heads);
-  if (max_len < 1 || cache_rows < 1 || (!row_map && batch > cache_rows))
+  if (batch > 0 && (max_len < 1 || cache_rows < 1 || (!row_map && batch > cache_rows)))
     return fail(MA_EVALUE, "%s: bad cache sizes", what);
   if (batch * n_kv_heads > 65535 || batch * nodes > 65535)
     return fail(MA_EVALUE, "%s: batch %lld too large for one launch", what, static_cast<long long>(batch));
@@ -1001,7 +1001,7 @@ extern "C" int ma_tree_commit(void* const* k_caches, void* const* v_caches, int6
                               const int64_t* row_map, int64_t* new_seqlen, void* stream) {
   int rc = check_tree("tree_commit", batch, nodes, n_kv_heads, n_kv_heads, head_dim, cache_rows, max_len, row_map);
   if (rc != MA_OK) return rc;
-  if (layers < 1 || n_kv_heads > 65535) return fail(MA_EVALUE, "tree_commit: bad sizes");
+  if (layers < 1) return fail(MA_EVALUE, "tree_commit: bad sizes");
   if (batch == 0) return MA_OK;
   if (!k_caches || !v_caches || !seqlen || !path || !accepted || !new_seqlen || new_seqlen == seqlen)
     return fail(MA_EVALUE, "tree_commit: null pointer, or new_seqlen is seqlen");

@@ -316,6 +316,37 @@ def test_attention_references_that_stay_too_low(dev, heads):
         compare_attention(out, q, k, v, parents, [n], 1.0)
 
 
+@pytest.mark.parametrize("heads", [(8, 1, 64), (8, 2, 128)])
+def test_attention_of_what_is_not_finite_stays_in_its_rows(dev, heads):
+    """A NaN in one node's query, NaN or infinite keys that nodes do see: those rows
+    as in 64 bits, every other row untouched."""
+    from maple_amd.kernels import tree_attention
+
+    nq, nkv, d = heads
+    parents, seqlen = [[-1, 0, 1, 1, 0, 4], [-1, 0, 1, 2, 3, 4], [-1] * 6], [300, 290, 130]
+    q = bf16(dev, 3, 6, nq, d)
+    k, v = bf16(dev, 3, nkv, 320, d, seed=1), bf16(dev, 3, nkv, 320, d, seed=2)
+    q[0, 3, :, 5] = float("nan")
+    q[1, 2, 0, 0] = float("inf")
+    k[1, 0, 40, 7] = float("nan")  # one KV head of the second row: all its nodes see it
+    k[0, :, 304, 3] = float("inf")  # node 4 of the first: seen by itself and by node 5
+    sl = torch.tensor(seqlen, device=dev)
+    for window in (None, 280):  # (280: position 40 is seen by the second row's first nodes alone)
+        out = tree_attention(q, k, v, sl, as_parents(parents, dev), scale=d ** -0.5, window=window)
+        compare_attention(out, q, k, v, parents, seqlen, d ** -0.5, window)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.125, 1e-30, 3.0])
+def test_attention_scales(dev, scale):
+    from maple_amd.kernels import tree_attention
+
+    rng = np.random.default_rng(3)
+    parents = random_parents(rng, 2, 9)
+    q, k, v = bf16(dev, 2, 9, 8, 64), bf16(dev, 2, 2, 500, 64, seed=1), bf16(dev, 2, 2, 500, 64, seed=2)
+    out = tree_attention(q, k, v, torch.tensor([480, 77], device=dev), as_parents(parents, dev), scale=scale)
+    compare_attention(out, q, k, v, parents, [480, 77], scale)
+
+
 def test_one_node_is_decode_gqa_attn(dev):
     from maple_amd.kernels import decode_gqa_attn, tree_attention
 

@@ -135,23 +135,24 @@ def test_tree_step_keeps_the_accepted_branch(dev, sampling):
     _step_with_device_routing(model, m, ids, cache, "after the commit", MIXED.top_k)
 
 
-def test_tree_steps_generate_along_the_sequential_choices(dev):
+@pytest.mark.parametrize("rows", [1, 2])
+def test_tree_steps_without_a_draft(dev, rows):
     """Greedy steps over a one-node tree (no draft) are ordinary greedy decoding:
     each step's logits meet the oracle's, and the token is their argmax."""
-    model, cache = _setup(dev, SMALL, 2)
+    model, cache = _setup(dev, SMALL, rows)
     m = _to_np(model)
-    tok = torch.tensor([[7], [900]], device=dev)
-    parents = torch.full((2, 1), -1, device=dev, dtype=torch.int32)
+    tok = torch.tensor([[7], [900]], device=dev)[:rows]
+    parents = torch.full((rows, 1), -1, device=dev, dtype=torch.int32)
     for step in range(3):
         cnp, routing = _cache_np(cache), []
         logits = model.forward_tree(tok, parents, cache, routing=routing)
         ref, _ = od.decoder_step(m, cnp, tok.cpu().numpy(), router_ids=[r.cpu().numpy() for r in routing])
         _check_logits(logits[:, 0], ref, f"step {step}")
         out = tree_step(model, cache, tok, parents)
-        assert out.accepted.tolist() == [0, 0]
+        assert out.accepted.tolist() == [0] * rows
         assert torch.equal(out.tokens[:, 0], logits[:, 0].argmax(-1))
         tok = out.tokens.clone()
-    assert cache.seqlen.tolist() == [40, 40]
+    assert cache.seqlen.tolist() == [40] * rows
 
 
 @pytest.mark.parametrize("w,t,top_k", [(1, 8, 1), (3, 9, 20), (4, 64, 20)])

@@ -23,7 +23,7 @@ def qkv_args(**kw):
 
 @pytest.mark.parametrize("kw,match", [
     (dict(nodes=0), "1 to 64 nodes"), (dict(nodes=65), "1 to 64 nodes"), (dict(d=96), "head_dim"),
-    (dict(h=5), "query heads"), (dict(hkv=0), "query heads"), (dict(batch=2), "cache sizes"),
+    (dict(h=5), "query heads"), (dict(hkv=0), "query heads"), (dict(h=65536, hkv=1), "query heads"), (dict(batch=2), "cache sizes"),
     (dict(batch=70000, rows=70000), "too large"), (dict(rot=31), "rotary_dim"), (dict(rot=66), "rotary_dim"),
     (dict(mode=3), "rotary_dim"), (dict(cos=None), "tables"), (dict(n_pos=0), "tables"), (dict(ld_cs=16), "tables"),
     (dict(qw=None), "norm weight"), (dict(qkv=None), "null"), (dict(parents=None), "null"),
@@ -92,6 +92,12 @@ def test_tree_commit_refuses():
                       (dict(path=None), "null"), (dict(new=FAKE), "new_seqlen")):
         with pytest.raises(ValueError, match=match):
             call(**kw)
+
+
+def test_empty_batches_are_no_work():
+    for name, args in (("ma_tree_qkv", qkv_args(batch=0, rows=0)), ("ma_tree_attn", attn_args(batch=0, rows=0)),
+                       ("ma_verify_tree", verify_args(batch=0, ws=None, ws_bytes=0))):
+        _lib.call(name, *args)
 
 
 def test_workspace_queries():
