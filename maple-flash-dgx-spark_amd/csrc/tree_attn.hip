@@ -302,11 +302,10 @@ struct TreeRow {
 // unit's LDS, 400 of its reads; they overlap in part.  From 4096 positions on each
 // further 4096 take 35 us at 32 x 32 nodes of 32 / 4 heads of 64 (970 TFLOP/s; a
 // large matrix product reaches 1210), a further 16384 take 18 us at 2 x 64 nodes
-// of 16 / 4 heads of 128 (930).  The rest of a launch is
-// fixed: 3 us to the first tile (a row's length, then its K and V, cold), the
-// tree's own masked tiles (about 1 us each), the splits' sums, all written at
-// the end: 50 us in all at 32 x 32 nodes over 4096, 45 where the rows hold half to
-// all of that.
+// of 16 / 4 heads of 128 (930).  The rest of a launch is fixed: 3 us to the first
+// tile (a row's length, then its K and V, cold), the tree's own masked tiles
+// (about 1 us each), the splits' sums, all written at the end: 50 us in all at 32 x
+// 32 nodes over 4096, 44 where the rows hold half to all of that.
 template <int HD>
 __global__ __launch_bounds__(256, (TreeTile<HD>::kWaves)) void k_tree_attn(
     const uint16_t* __restrict__ q, int nodes, int nq, int nkv, int tiles, int S, int n_units,
@@ -771,6 +770,9 @@ __global__ __launch_bounds__(256) void k_tree_merge(const float* __restrict__ pa
   *reinterpret_cast<uint2*>(out + ((b * nodes + r / group) * nq + kvh * group + r % group) * HD + 4 * d4) = w;
 }
 
+// A window past every distance is none (and cannot overflow a position).
+static int64_t tree_window(int64_t window, int64_t max_len) { return window - kTreeNodes > max_len ? 0 : window; }
+
 struct TreePlan {
   int tiles, splits;
   int64_t pairs;
@@ -947,6 +949,7 @@ extern "C" size_t ma_tree_attn_workspace_bytes(int64_t batch, int64_t nodes, int
   if (batch < 1 || nodes < 1 || nodes > kTreeNodes || n_kv_heads < 1 || n_heads < n_kv_heads ||
       n_heads % n_kv_heads != 0 || (head_dim != 64 && head_dim != 128) || max_len < 1)
     return 0;
+  window = tree_window(window, max_len);
   return tree_ws_bytes(tree_plan(batch, nodes, n_heads, n_kv_heads, head_dim, max_len, window), head_dim);
 }
 
@@ -962,6 +965,7 @@ extern "C" int ma_tree_attn(const void* q, int64_t batch, int64_t nodes, int n_h
   if (!q || !k_cache || !v_cache || !seqlen || !parents || !out) return fail(MA_EVALUE, "tree_attn: null pointer");
   if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(out) || !aligned16(workspace))
     return fail(MA_EVALUE, "tree_attn: q, the cache, out and the workspace must be 16-byte aligned");
+  window = tree_window(window, max_len);
   const TreePlan p = tree_plan(batch, nodes, n_heads, n_kv_heads, head_dim, max_len, window);
   const size_t need = tree_ws_bytes(p, head_dim);
   if (need && (!workspace || workspace_bytes < need))

@@ -336,6 +336,23 @@ def test_attention_of_what_is_not_finite_stays_in_its_rows(dev, heads):
         compare_attention(out, q, k, v, parents, seqlen, d ** -0.5, window)
 
 
+def test_attention_windows_past_every_distance(dev):
+    """As without a window, up to the largest one."""
+    from maple_amd.kernels import tree_attention
+
+    rng = np.random.default_rng(5)
+    parents = as_parents(random_parents(rng, 2, 64, ragged=False), dev)
+    q, k, v = bf16(dev, 2, 64, 8, 64), bf16(dev, 2, 2, 640, 64, seed=1), bf16(dev, 2, 2, 640, 64, seed=2)
+    sl = torch.tensor([576, 0], device=dev)
+    want = tree_attention(q, k, v, sl, parents, scale=0.125)
+    for window in (640, 641, 703, 705, 2 ** 31, 2 ** 62, 2 ** 63 - 1):
+        out = tree_attention(q, k, v, sl, parents, scale=0.125, window=window)
+        if window > 704:
+            assert torch.equal(out, want)
+        else:  # (other splits: their sums' order)
+            compare_attention(out, q, k, v, parents.cpu().numpy(), [576, 0], 0.125, window)
+
+
 @pytest.mark.parametrize("scale", [0.0, -0.125, 1e-30, 3.0])
 def test_attention_scales(dev, scale):
     from maple_amd.kernels import tree_attention
