@@ -337,13 +337,15 @@ class SyntheticDecoder:
         return KVCache(ks, vs, seqlen, self.max_len, ws)
 
     def _layer(self, i: int, hidden: torch.Tensor, cache: KVCache, routing=None,
-               qkv: torch.Tensor | None = None, fuse_next: bool = True):
+               qkv: torch.Tensor | None = None, fuse_next: bool = True, tree: torch.Tensor | None = None):
         """Layer ``i``; returns ``(y, next_qkv)``.  ``qkv``: this layer's input
         projection if an earlier launch already computed it.  ``next_qkv`` is
         layer ``i + 1``'s projection when the one-launch MoE kernel computed it
         from ``y`` (batch 1, ``fuse_next``), else None.  ``y`` is a
         ``PendingCombine`` where layer ``i + 1``'s QKV launch runs the MoE
-        combine (``combine_next``, 17+ tokens); ``hidden`` may be one."""
+        combine (``combine_next``, 17+ tokens); ``hidden`` may be one.
+        ``tree [w, T]``: the parents of the ``w * T`` nodes that ``hidden``
+        holds, instead of one token per slot."""
         c, L = self.cfg, self.layers[i]
         if isinstance(hidden, PendingCombine):  # the previous layer's MoE combine runs here
             hidden, qkv = ternary_gemv_combine(hidden, L.qkv, L.qkv_alpha, rms_weight=L.input_ln,
@@ -355,9 +357,9 @@ class SyntheticDecoder:
         akw = dict(num_heads=c.heads, num_kv_heads=c.kv_heads, head_dim=c.head_dim,
                    rotary_dim=c.rotary_dim, eps=c.eps, scale=c.head_dim ** -0.5, window=window,
                    use_rope=use_rope)
-        seqlen, row_map = cache.slot_rows(bsz)
+        seqlen, row_map = cache.slot_rows(bsz if tree is None else tree.shape[0])
         akw["row_map"] = row_map
-        if bsz == 1 and self.fused_o and o_projection_supported(1, c.heads, c.kv_heads, c.head_dim,
+        if bsz == 1 and tree is None and self.fused_o and o_projection_supported(1, c.heads, c.kv_heads, c.head_dim,
                                                                 cache.max_len, window, c.hidden):
             # attention and its output projection in one launch (measured: no
             # faster than two launches at 4096 positions -- the grid barrier
@@ -365,8 +367,15 @@ class SyntheticDecoder:
             _, o = decode_attention(qkv, L.q_norm, L.k_norm, self.cos, self.sin, cache.k[i], cache.v[i],
                                     seqlen, cache.attn_ws, o_linear=(L.o, L.o_alpha), **akw)
         else:
-            attn = decode_attention(qkv, L.q_norm, L.k_norm, self.cos, self.sin, cache.k[i], cache.v[i],
-                                    seqlen, cache.attn_ws, **akw)
+            if tree is None:
+                attn = decode_attention(qkv, L.q_norm, L.k_norm, self.cos, self.sin, cache.k[i], cache.v[i],
+                                        seqlen, cache.attn_ws, **akw)
+            else:
+                scale, window = akw.pop("scale"), akw.pop("window")
+                q = apply_qkv_tree(qkv.view(*tree.shape, -1), L.q_norm, L.k_norm, self.cos, self.sin, cache.k[i],
+                                   cache.v[i], seqlen, tree, **akw)
+                attn = tree_attention(q, cache.k[i], cache.v[i], seqlen, tree, row_map=row_map, scale=scale,
+                                      window=window)
             # o_in_moe: at batch 1 the XCD-split MoE launch computes the output
             # projection itself (same bits; measured 1,294 against 1,306 tok/s
             # with the separate launch, so off by default)
@@ -428,22 +437,12 @@ class SyntheticDecoder:
         without advancing ``seqlen`` (``KVCache.commit`` does) and returns bf16
         logits ``[w, T, vocab]``; a chain's are those of as many decode steps up to
         rounding.  Padding's logits say nothing."""
-        c = self.cfg
         w, t = tokens.shape
-        seqlen, row_map = cache.slot_rows(w)
+        cache.slot_rows(w)
         hidden = self.embed_tokens(tokens.reshape(-1))  # (padding's ids are clamped to the table)
-        for i, L in enumerate(self.layers):
-            window, use_rope = c.layer_attention(i)
-            qkv = ternary_gemv(hidden, L.qkv, L.qkv_alpha, rms_weight=L.input_ln, rms_eps=c.eps)
-            q = apply_qkv_tree(qkv.view(w, t, -1), L.q_norm, L.k_norm, self.cos, self.sin, cache.k[i], cache.v[i],
-                               seqlen, parents, row_map=row_map, num_heads=c.heads, num_kv_heads=c.kv_heads,
-                               head_dim=c.head_dim, rotary_dim=c.rotary_dim, use_rope=use_rope, eps=c.eps)
-            attn = tree_attention(q, cache.k[i], cache.v[i], seqlen, parents, row_map=row_map,
-                                  scale=c.head_dim ** -0.5, window=window)
-            o = ternary_gemv(attn.view(w * t, -1), L.o, L.o_alpha)
-            hidden, ids = moe_layer(hidden, L.moe, c.top_k, L.post_ln, c.eps, add=o.reshape(hidden.shape))
-            if routing is not None:
-                routing.append(ids)
+        qkv = None
+        for i in range(self.cfg.layers):
+            hidden, qkv = self._layer(i, hidden, cache, routing, qkv, tree=parents)
         return self.head(hidden).view(w, t, -1)
 
     def embed_tokens(self, input_ids: torch.Tensor) -> torch.Tensor:
