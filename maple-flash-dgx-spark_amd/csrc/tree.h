@@ -45,10 +45,6 @@ __device__ __forceinline__ TreeLane tree_lane(int par, int nodes) {
   const bool present = root && lane < nodes && (anc & 1ull);
   return {present ? anc : 0ull, present ? static_cast<int>(__popcll(anc)) - 1 : -1};
 }
-__device__ __forceinline__ TreeLane tree_lane(const int32_t* __restrict__ parents, int nodes) {
-  return tree_lane(tree_parent(parents, nodes), nodes);
-}
-
 
 // The depth alone (-1 for an absent node): every lane holds the node 2^n steps
 // up, or where its way ends, and the steps to it, in one word.

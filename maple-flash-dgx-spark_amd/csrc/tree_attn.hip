@@ -244,7 +244,7 @@ __device__ __forceinline__ f32x16t_t mfma_tree(uint4 a, uint4 b, f32x16t_t c) {
 // A workgroup: four waves of 32 query rows, which share its K and V.  (64 or 32
 // rows and the waves left over on positions of their own, for trees of few rows:
 // 26 against 27 us at 32 x 8 nodes over 4096 of 64, 28 against 27 at 16 x 8 of 128,
-// 9.8 against 9.3 at 1 x 16 of 128; no better on the whole, and gone.)
+// 9.8 against 9.3 at 1 x 16 of 128: one shape does for all.)
 template <int HD>
 struct TreeTile {
   static constexpr int kRows = 128;
