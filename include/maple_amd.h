@@ -697,7 +697,9 @@ int ma_fused_sample(const void* logits, int dtype, int64_t rows, int64_t vocab, 
  * 0 <= parents[b, i] < i names node i's parent; a node with any other parent,
  * or below such a node, is absent (padding).  Node i's K/V live at cache
  * position seqlen[b] + i, its rotary position is seqlen[b] + its depth.  A node
- * whose slot falls behind the cache (max_len) is neither stored nor attended;
+ * whose slot falls behind the cache (max_len) is neither stored nor attended, so
+ * the parents given to ma_verify_tree, which does not see the cache, have to mark
+ * it as absent (seqlen[b] + i >= max_len: parents[b, i] = -2);
  * mapped rows are clamped to [0, cache_rows), seqlen to [0, max_len].  batch x
  * nodes, batch x n_kv_heads and n_heads at most 65535.
  *
@@ -777,7 +779,8 @@ int ma_verify_tree(const void* logits, int dtype, int64_t ldb, int64_t ldt, int6
  * for 0 < j <= accepted[b], position seqlen[b] + path[b, j] of cache row
  * row_map[b] (b when NULL) goes to seqlen[b] + j; new_seqlen[b] = seqlen[b] +
  * accepted[b] + 1 (accepted and path as ma_verify_tree writes them: path
- * ascending; new_seqlen is not seqlen).  k_caches / v_caches: host arrays of
+ * ascending, of nodes that were stored; one that was not, its slot behind max_len,
+ * moves nothing and is counted all the same; new_seqlen is not seqlen).  k_caches / v_caches: host arrays of
  * `layers` device pointers to bf16 caches [cache_rows, n_kv_heads, max_len,
  * head_dim], 16-byte aligned, distinct from one another; one launch per 64
  * layers.  head_dim 64 or 128.

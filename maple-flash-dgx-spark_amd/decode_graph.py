@@ -44,7 +44,7 @@ import torch
 from . import workspace
 from .kernels.greedy import greedy_argmax
 from .kernels.sampler import MAX_TOP_K, batched_sampler_workspace, fused_sample_batched
-from .kernels.tree import TreeVerdict, verify_tree
+from .kernels.tree import TreeVerdict, fit_tree, verify_tree
 
 GRAPH_WARMUP = 3
 GRAPH_CHECK_TOKENS = 8
@@ -307,17 +307,20 @@ def tree_step(model, cache, tokens: torch.Tensor, parents: torch.Tensor, samplin
               uniform: torch.Tensor | None = None, draft_probs: torch.Tensor | None = None) -> TreeVerdict:
     """One step over drafted trees: ``tokens [w, T]`` (node 0 each row's last
     token, its K/V not yet cached) hung together by ``parents [w, T]`` over cache
-    slots ``[0, w)``, each with room for ``T`` more positions.  Scores every node,
-    accepts tokens under ``sampling`` (greedy: where they are the argmax; else as
-    ``verify_tree``, with ``draft_probs`` if the tokens were drawn), draws one
-    more and keeps the accepted branch in the cache.  Every row gets 1 to T
-    tokens that follow the law of as many ordinary steps; the last of them is
-    the next step's node 0.  ``uniform [w, T]`` float32 replaces the draw from
+    slots ``[0, w)``.  Scores every node, accepts tokens under ``sampling``
+    (greedy: where they are the argmax; else as ``verify_tree``, with
+    ``draft_probs`` if the tokens were drawn), draws one more and keeps the
+    accepted branch in the cache.  Every row gets 1 to T tokens that follow the
+    law of as many ordinary steps; the last of them is the next step's node 0.
+    A row with fewer than ``T`` free positions steps over the nodes that fit, and
+    one with none takes no step (accepted -1, tokens -1), as a row without a
+    sequence.  ``uniform [w, T]`` float32 replaces the draw from
     ``sampling.generator``.  No host synchronisation; capturable with
     ``uniform`` given (or greedy)."""
     sampling = sampling or Sampling()
     sampling.check()
     w, t = tokens.shape
+    parents = fit_tree(parents, cache.slot_rows(w)[0], cache.max_len)
     logits = model.forward_tree(tokens, parents, cache)
     if sampling.greedy:
         # the law is one token: every uniform below 1 decides alike

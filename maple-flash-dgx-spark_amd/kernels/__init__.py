@@ -1,5 +1,5 @@
 """HIP kernels of the hot path, exported under the reference's names
-(``src/maple_run/kernels/__init__.py:5-39``), plus ``moe_dispatch`` and the four
+(``src/maple_run/kernels/__init__.py:5-39``), plus ``moe_dispatch`` and those
 of decoding with drafted token trees (``tree``).
 
 Importing this package does not load the HIP library; the first kernel call
@@ -18,7 +18,7 @@ from .router import router_topk
 from .rtn4 import rtn4_embedding, rtn4_gemv, rtn4_indexed_gemv
 from .ternary_expert import ternary_expert_down_sum, ternary_expert_gemv, ternary_expert_swiglu
 from .ternary_gemv import ternary_gemv
-from .tree import apply_qkv_tree, commit_tree, tree_attention, verify_tree
+from .tree import apply_qkv_tree, commit_tree, fit_tree, tree_attention, verify_tree
 
 __all__ = [
     "ternary_gemv",
@@ -42,4 +42,5 @@ __all__ = [
     "tree_attention",
     "verify_tree",
     "commit_tree",
+    "fit_tree",
 ]

@@ -13,9 +13,10 @@ The tree is ``parents [B, T]``, ``T <= 64``, on the device: node 0 is the row's
 last token (its K/V not yet cached) with parent -1, any other node's parent comes
 before it (``0 <= parents[b, i] < i``).  A node with any other parent, and all
 below it, is padding; a row whose entry 0 is not -1 has no sequence.  Node ``i``
-is cached at ``seqlen[b] + i`` and stands at position ``seqlen[b] + depth``.  Row
-``b`` needs ``seqlen[b] + T <= max_len``; nodes past the cache's end are neither
-stored nor attended.
+is cached at ``seqlen[b] + i`` and stands at position ``seqlen[b] + depth``.
+Nodes past the cache's end are neither stored nor attended, so they must not be
+accepted either: where ``seqlen[b] + T`` may exceed ``max_len``, all four get the
+tree from ``fit_tree``, in which such nodes are padding.
 """
 
 from __future__ import annotations
@@ -80,6 +81,20 @@ def _positions(name: str, t: torch.Tensor, bsz: int) -> torch.Tensor:
             raise TypeError(f"{name} must hold whole numbers; got {t.dtype}.")
         t = t.to(torch.int64)
     return t if t.is_contiguous() else t.contiguous()
+
+
+def fit_tree(parents: torch.Tensor, seqlen: torch.Tensor, max_len: int) -> torch.Tensor:
+    """``parents`` (int32) without the nodes that a cache of ``max_len`` positions
+    has no place for: node ``i`` of row ``b`` is padding where ``seqlen[b] + i >=
+    max_len``, and a full row has no sequence.  A node's slot lies behind its
+    parent's, so whatever is kept is kept with its branch, and an accepted branch
+    ends within the cache.  Capturable."""
+    if parents.ndim != 2:
+        raise ValueError(f"fit_tree expects parents [B, T], got {tuple(parents.shape)}.")
+    bsz, nodes = parents.shape
+    parents = _tree("fit_tree", parents, bsz, nodes)
+    slot = _positions("seqlen", seqlen, bsz).view(bsz, 1) + torch.arange(nodes, device=seqlen.device)
+    return parents.masked_fill(slot >= max_len, -2)
 
 
 def _cache(what: str, k_cache: torch.Tensor, v_cache: torch.Tensor, bsz: int, row_map: torch.Tensor | None):
@@ -309,7 +324,8 @@ def commit_tree(
     """Move the accepted nodes' K/V of every layer (``k_caches`` / ``v_caches``:
     lists of caches) together behind each row's sequence; returns the new write
     positions ``seqlen + accepted + 1`` (int64 ``[B]``).  ``path`` / ``accepted``
-    as ``verify_tree`` returns them."""
+    as ``verify_tree`` returns them for a tree that fits the cache (``fit_tree``):
+    a node that was never stored has no K/V to move."""
     n = len(k_caches)
     if n == 0 or n != len(v_caches):
         raise ValueError(f"commit_tree expects as many K as V caches, got {n} and {len(v_caches)}.")

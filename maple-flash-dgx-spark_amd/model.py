@@ -215,8 +215,9 @@ class KVCache:
     def commit(self, path: torch.Tensor, accepted: torch.Tensor) -> None:
         """Keep an accepted branch of the nodes that ``forward_tree`` wrote behind
         slots ``[0, len(accepted))`` (``path`` / ``accepted`` as ``verify_tree``
-        returns them): their K/V move together, in every layer, and the write
-        positions advance past them.  Graph-safe; no host synchronisation."""
+        returns them for a tree that fits the cache, ``kernels.tree.fit_tree``):
+        their K/V move together, in every layer, and the write positions advance
+        past them.  Graph-safe; no host synchronisation."""
         seqlen, row_map = self.slot_rows(int(accepted.shape[0]))
         seqlen.copy_(commit_tree(self.k, self.v, seqlen, path, accepted, row_map=row_map))
 

@@ -218,3 +218,56 @@ def test_captured_tree_step_replays_as_eager(dev, w, t, top_k):
                 for x, y in zip((cache.seqlen, *cache.k, *cache.v), state):
                     assert torch.equal(x, y)
                 torch.zeros(1, device=dev).add_(1)
+
+
+@pytest.mark.parametrize("sampling", [Sampling(), Sampling(temperature=0.9, top_p=0.95, top_k=20)],
+                         ids=["greedy", "sampled"])
+def test_tree_step_near_the_caches_end(dev, sampling):
+    """Rows with room for some nodes, for one and for none: a node whose K/V could
+    not be stored is never accepted, whatever its token; a full row takes no step;
+    no write position passes the cache's end."""
+    model, cache = _setup(dev, SMALL, 4)
+    room = [3, 0, 1, 60]
+    cache.seqlen.copy_(128 - torch.tensor(room, device=dev))
+    # nodes 1 .. 5 are unlikely; node 6 is the root's best token, node 7 the best behind it, node 8 behind that
+    tree = np.array([[-1, 0, 0, 1, 1, 2, 0, 6, 7]] * 4)
+    parents = torch.tensor(tree, device=dev)
+    w, t = tree.shape
+    tokens = _tokens(dev, w, t)
+    full = cache.seqlen.clone()
+    cache.seqlen.fill_(60)  # (any place with room: the tokens only have to be drafted well)
+    for _ in range(4):
+        probe = model.forward_tree(tokens, parents.int(), cache).float()
+        for i in (6, 7, 8):
+            tokens[:, i] = probe[:, tree[0, i]].argmax(-1)
+        tokens[:, 1:3] = probe[:, :1].argmin(-1)
+    cache.seqlen.copy_(full)
+    fitted = np.where(full.cpu().numpy()[:, None] + np.arange(t) < 128, tree, -2)
+    for _ in range(4):  # the same where the rows are now
+        probe = model.forward_tree(tokens, torch.tensor(fitted, device=dev, dtype=torch.int32), cache).float()
+        for i in (6, 7, 8):
+            tokens[3, i] = probe[3, tree[0, i]].argmax(-1)
+        tokens[:3, 6] = probe[:3, 0].argmax(-1)
+        tokens[:, 1:3] = probe[:, :1].argmin(-1)
+    logits = model.forward_tree(tokens, torch.tensor(fitted, device=dev, dtype=torch.int32), cache)
+    before, seqlen = [x.clone() for x in cache.k + cache.v], cache.seqlen.tolist()
+    uniform = torch.zeros(w, t, device=dev)  # (every token that is possible is accepted)
+    out = tree_step(model, cache, tokens, parents, sampling, uniform=uniform)
+    kw = dict(temperature=1.0, top_p=1.0, top_k=1) if sampling.greedy else dict(
+        temperature=sampling.temperature, top_p=sampling.top_p, top_k=sampling.top_k)
+    for b in range(w):
+        emitted, path = ot.verify(logits[b].double().cpu().numpy(), tokens[b].cpu().numpy(), fitted[b],
+                                  uniform[b].cpu().numpy(), **kw)
+        n = len(emitted)
+        assert out.tokens[b].tolist() == emitted + [-1] * (t - n), b
+        assert out.path[b].tolist() == path + [-1] * (t - len(path)), b
+        assert int(out.accepted[b]) == n - 1 and int(cache.seqlen[b]) == seqlen[b] + n <= 128, b
+        for new, old in zip(cache.k + cache.v, before):
+            assert torch.equal(new[b, :, :seqlen[b]], old[b, :, :seqlen[b]])
+            for j, node in enumerate(path):
+                assert torch.equal(new[b, :, seqlen[b] + j], old[b, :, seqlen[b] + node])
+    assert out.accepted.tolist() == [0, -1, 0, 3]
+    for _ in range(9):  # on to the end: the rows fill up and stay there
+        out = tree_step(model, cache, tokens, parents, sampling, uniform=uniform)
+        assert int(cache.seqlen.max()) <= 128
+    assert cache.seqlen[:3].tolist() == [128] * 3 and out.accepted[:3].tolist() == [-1] * 3

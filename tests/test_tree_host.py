@@ -213,3 +213,23 @@ def test_tree_step_refuses_settings_the_sampler_does_not_cover():
     with pytest.raises(ValueError, match="sampling"):
         tree_step(None, None, torch.zeros(1, 1, dtype=torch.int64), torch.full((1, 1), -1, dtype=torch.int32),
                   Sampling(temperature=1.0, top_k=0))
+
+
+def test_fit_tree_leaves_out_nodes_past_the_caches_end():
+    from maple_amd.kernels.tree import fit_tree
+
+    parents = torch.tensor([[-1, 0, 0, 1]] * 5 + [[-2, 0, 0, 1]])
+    seqlen = torch.tensor([0, 4, 6, 7, 8, 5])
+    want = [[-1, 0, 0, 1], [-1, 0, 0, 1], [-1, 0, -2, -2], [-1, -2, -2, -2], [-2] * 4, [-2, 0, 0, -2]]
+    for dtype in (torch.int32, torch.int64):
+        got = fit_tree(parents.to(dtype), seqlen, 8)
+        assert got.dtype == torch.int32 and got.is_contiguous() and got.tolist() == want
+    assert fit_tree(parents.int(), seqlen, 1 << 40).tolist() == parents.tolist()
+    far = torch.tensor([[-1, 1 << 32, (1 << 32) + 1, -(1 << 32)]])  # no large value becomes a node
+    assert fit_tree(far, seqlen[:1], 8).tolist() == [[-1, 64, 64, -2]]
+    with pytest.raises(ValueError):
+        fit_tree(parents, seqlen[:3], 8)
+    with pytest.raises(TypeError):
+        fit_tree(parents.float(), seqlen, 8)
+    with pytest.raises(ValueError):
+        fit_tree(torch.zeros(1, 65, dtype=torch.int32), seqlen[:1], 8)
