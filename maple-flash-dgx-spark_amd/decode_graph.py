@@ -311,7 +311,8 @@ def tree_step(model, cache, tokens: torch.Tensor, parents: torch.Tensor, samplin
     (greedy: where they are the argmax; else as ``verify_tree``, with
     ``draft_probs`` if the tokens were drawn), draws one more and keeps the
     accepted branch in the cache.  Every row gets 1 to T tokens that follow the
-    law of as many ordinary steps; the last of them is the next step's node 0.
+    law of as many ordinary steps (at one row the FlashHead's, where the model
+    has one); the last of them is the next step's node 0.
     A row with fewer than ``T`` free positions steps over the nodes that fit, and
     one with none takes no step (accepted -1, tokens -1), as a row without a
     sequence.  ``uniform [w, T]`` float32 replaces the draw from

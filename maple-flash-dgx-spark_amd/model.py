@@ -437,14 +437,23 @@ class SyntheticDecoder:
         slots ``[0, w)``.  Writes the nodes' K/V at ``seqlen .. seqlen + T - 1``
         without advancing ``seqlen`` (``KVCache.commit`` does) and returns bf16
         logits ``[w, T, vocab]``; a chain's are those of as many decode steps up to
-        rounding.  Padding's logits say nothing."""
+        rounding, from the head that such steps use: at one row the FlashHead, if
+        one is attached, node by node.  Padding's logits say nothing."""
         w, t = tokens.shape
         cache.slot_rows(w)
         hidden = self.embed_tokens(tokens.reshape(-1))  # (padding's ids are clamped to the table)
         qkv = None
         for i in range(self.cfg.layers):
             hidden, qkv = self._layer(i, hidden, cache, routing, qkv, tree=parents)
-        return self.head(hidden).view(w, t, -1)
+        if self.flash_head is None or w > 1:
+            return self.head(hidden).view(w, t, -1)
+        # (rows of their own, 16-byte aligned, which the next call leaves alone)
+        v = self.cfg.vocab
+        logits = torch.empty(t, -(-v // 8) * 8, device=hidden.device, dtype=torch.bfloat16)[:, :v]
+        hidden = rms_norm(hidden, self.final_norm, self.cfg.eps)
+        for i in range(t):
+            self.flash_head(hidden[i:i + 1], out=logits[i])
+        return logits.unsqueeze(0)
 
     def embed_tokens(self, input_ids: torch.Tensor) -> torch.Tensor:
         w, sc, bs = self.embed

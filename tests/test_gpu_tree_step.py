@@ -271,3 +271,105 @@ def test_tree_step_near_the_caches_end(dev, sampling):
         out = tree_step(model, cache, tokens, parents, sampling, uniform=uniform)
         assert int(cache.seqlen.max()) <= 128
     assert cache.seqlen[:3].tolist() == [128] * 3 and out.accepted[:3].tolist() == [-1] * 3
+
+
+def test_a_flash_head_scores_a_single_rows_tree(dev):
+    """With a FlashHead, ordinary steps of one row are scored by it and steps of
+    several rows by the exact head: so are trees, whatever their number of nodes."""
+    from test_gpu_flash_head import _flash
+
+    model, cache = _setup(dev, dataclasses.replace(SMALL, rtn_group=64), 1)
+    two = model.make_cache(2, prefill_len=37, seed=1)
+    flash = _flash(dev, model.lm_head, 32, 4, seed=4, force=(5,))[0]
+    calls = []
+
+    def spy(hidden, out=None):
+        calls.append(hidden.clone())
+        return flash(hidden, out=out)
+
+    def trees(w, t):
+        return _tokens(dev, w, t), torch.tensor(TREES[:w, :t], device=dev, dtype=torch.int32)
+
+    for t in (1, 2, 9):
+        tokens, parents = trees(1, t)
+        model.flash_head = None
+        exact = model.forward_tree(tokens, parents, cache)
+        model.flash_head = spy
+        calls.clear()
+        logits = model.forward_tree(tokens, parents, cache)
+        assert logits.shape == (1, t, SMALL.vocab) and len(calls) == t
+        kept = logits.clone()
+        for i, hidden in enumerate(calls):
+            assert torch.equal(flash(hidden).reshape(-1), kept[0, i])
+        assert torch.equal(logits, kept)  # (not the FlashHead's own row, which the next call overwrites)
+        on = torch.isfinite(kept.float())
+        assert (on.sum(-1) >= 4 * 32).all() and (on.sum(-1) <= 4 * 32 + 1).all() and on[..., 5].all()
+        assert torch.isneginf(kept[~on].float()).all()
+        got, ref = kept.float()[on], exact.float()[on]
+        assert (got - ref).abs().max() <= 1e-2 * ref.abs().max()
+        tokens, parents = trees(2, t)
+        model.flash_head = None
+        exact = model.forward_tree(tokens, parents, two)
+        model.flash_head = spy
+        calls.clear()
+        assert torch.equal(model.forward_tree(tokens, parents, two), exact) and not calls
+    # a whole step: the verdict is the law's on those logits
+    tokens, parents = trees(1, 9)
+    for sampling in (Sampling(), Sampling(temperature=0.9, top_p=0.95, top_k=20)):
+        cache.seqlen.fill_(37)
+        probe = model.forward_tree(tokens, parents, cache)
+        tokens[0, 1] = probe[0, 0].float().argmax()
+        logits = model.forward_tree(tokens, parents, cache)
+        uniform = torch.full((1, 9), 0.25, device=dev)
+        out = tree_step(model, cache, tokens, parents, sampling, uniform=uniform)
+        kw = dict(temperature=1.0, top_p=1.0, top_k=1) if sampling.greedy else dict(
+            temperature=sampling.temperature, top_p=sampling.top_p, top_k=sampling.top_k)
+        emitted, path = ot.verify(logits[0].double().cpu().numpy(), tokens[0].cpu().numpy(), TREES[0],
+                                  uniform[0].cpu().numpy(), **kw)
+        assert out.tokens[0].tolist() == emitted + [-1] * (9 - len(emitted))
+        assert out.path[0].tolist() == path + [-1] * (9 - len(path))
+        if sampling.greedy:
+            assert int(out.accepted[0]) >= 1
+
+
+def test_a_captured_tree_step_with_a_flash_head_replays_as_eager(dev):
+    from test_gpu_flash_head import _flash
+
+    model, cache = _setup(dev, dataclasses.replace(SMALL, rtn_group=64), 1)
+    model.flash_head = _flash(dev, model.lm_head, 32, 4, seed=4)[0]
+    bufs, parents = _tokens(dev, 1, 5), torch.tensor(TREES[:1, :5], device=dev, dtype=torch.int32)
+    run = lambda: tree_step(model, cache, bufs, parents)  # noqa: E731
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run()
+    side.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = run()
+    for seed in range(4):
+        tokens = _tokens(dev, 1, 5, seed=10 + seed)
+        cache.seqlen.fill_(37)
+        bufs.copy_(tokens)
+        want = [x.clone() for x in (*run(), cache.seqlen, *cache.k, *cache.v)]
+        cache.seqlen.fill_(37)
+        g.replay()
+        torch.cuda.synchronize()
+        for a, b in zip((*out, cache.seqlen, *cache.k, *cache.v), want):
+            assert torch.equal(a, b), seed
+
+
+def test_a_flash_heads_rows_of_any_vocabulary(dev):
+    """A vocabulary that is no multiple of 8: the nodes' rows start where the
+    FlashHead can write them."""
+    from test_gpu_flash_head import _flash
+
+    cfg = dataclasses.replace(SMALL, vocab=1028, rtn_group=64)
+    model, cache = _setup(dev, cfg, 1)
+    model.flash_head = _flash(dev, model.lm_head, 257, 40, seed=2)[0]
+    tokens, parents = _tokens(dev, 1, 3), torch.tensor([[-1, 0, 0]], device=dev, dtype=torch.int32)
+    logits = model.forward_tree(tokens, parents, cache)
+    assert logits.shape == (1, 3, 1028) and (torch.isfinite(logits.float()).sum(-1) == 160).all()
+    out = tree_step(model, cache, tokens, parents)
+    best = logits.float().argmax(-1)
+    assert int(out.tokens[0, 0]) == int(best[0, 0])
