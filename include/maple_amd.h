@@ -760,7 +760,8 @@ int ma_tree_attn(const void* q, int64_t batch, int64_t nodes, int n_heads, int n
  * out_tokens int64 [batch, nodes]: the accepted tokens, then the drawn one, then
  * -1; accepted int32 [batch]: how many were accepted (-1 for a row without a
  * sequence, whose outputs are all -1); a NaN logit is never chosen, a row of
- * them draws token 0; path int32 [batch, nodes]: the nodes from
+ * them draws token 0; equal logits weigh alike, infinite ones too (+inf, a forced
+ * token, takes the whole law); path int32 [batch, nodes]: the nodes from
  * the root to the last accepted one, then -1.  Laws and walk in 64 bits.  1 <=
  * top_k <= min(64, vocab), inv_temperature finite > 0, 0 < top_p <= 1; top_k = 1
  * is greedy.  workspace: ma_verify_tree_workspace_bytes(...) bytes, 8-byte

@@ -21,7 +21,9 @@
 //                   token of a law; a value at a border decides a token)
 //
 // Keys: (order-preserving bits of the float32 value) << 32 | ~id, distinct in a
-// row; 0 is no key.  A NaN logit has none: it is never chosen.
+// row; 0 is no key.  A NaN logit has none: it is never chosen.  Logits of +inf
+// (forced tokens) share the whole law, rows of nothing but -inf give their top_k
+// first tokens the same weight.
 //
 // Selection.  A thread keeps the maximum of the values it has seen.  The
 // ceil(k / 4)-th largest of a wave's 64 maxima (its share of k, where a short
@@ -519,7 +521,7 @@ __global__ __launch_bounds__(64) void k_verify_walk(
       const double z = static_cast<double>(verify_value(key));
       const double z0 = lane_d(z, 0);
       id = key ? static_cast<int64_t>(0xffffffffu - static_cast<uint32_t>(key)) : -1;
-      p = key ? exp((z - z0) * inv_t) : 0.0;
+      p = key ? (z == z0 ? 1.0 : exp((z - z0) * inv_t)) : 0.0;  // (inf - inf: equal logits weigh alike)
       p = p / wave_sum_d(p);
       const double before = wave_scan_d(p) - p;
       p = before <= top_p || top_p >= 1.0 ? p : 0.0;

@@ -89,7 +89,9 @@ def law(logits, *, temperature: float, top_p: float, top_k: int):
     """The sampler's law at a node: ids (most likely first) and probabilities."""
     z = np.asarray(logits, np.float64)
     ids = topk_desc(z, top_k)
-    p = np.exp((z[ids] - z[ids[0]]) / temperature)
+    low = np.zeros(ids.size)  # (equal logits weigh alike, infinite ones too)
+    np.subtract(z[ids], z[ids[0]], out=low, where=z[ids] != z[ids[0]])
+    p = np.exp(low / temperature)
     p /= p.sum()
     before = np.concatenate([[0.0], np.cumsum(p)[:-1]])
     p = np.where((before <= top_p) | (top_p >= 1.0), p, 0.0)

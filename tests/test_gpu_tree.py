@@ -538,6 +538,33 @@ def test_verify_padding_and_rows_without_a_sequence(dev):
         check_verify(dev, s, top_k=64, top_p=1.0)
 
 
+@pytest.mark.parametrize("top_k", [1, 2, 5, 64])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_verify_infinite_logits(dev, top_k, dtype):
+    """Logits of +inf (a forced token) carry all of the law, alike where there are
+    several; rows of nothing but -inf weigh their top_k first tokens alike."""
+    parents = [[-1, 0, 0, 1, 2], [-1, 0, 1, 2, 3], [-1, 0, 0, 0, 0], [-1, 0, 0, 0, 0]]
+    s = draft(dev, 4, 5, 900, parents=parents, seed=3, dtype=dtype)
+    x = s["logits"]
+    x[0, 0, 700] = x[0, 2, 3] = float("inf")  # forced: node 2's token, then node 4's
+    x[1, :, 899] = float("inf")  # along a chain
+    x[2, 0, [11, 12, 500]] = float("inf")  # three alike
+    x[3] = float("-inf")
+    s["tokens"] = torch.tensor([[0, 1, 700, 5, 3], [0, 899, 899, 899, 7], [0, 13, 12, 500, 11], [0, 800, 1, 0, 2]],
+                               device=dev)
+    drawn = torch.zeros(4, 5, 900, device=dev)
+    drawn.scatter_(2, s["tokens"].unsqueeze(-1), 0.5)
+    for u in (0.0, 0.3, 0.7, 0.999999):
+        s["uniform"].fill_(u)
+        for top_p in (1.0, 0.55):
+            s["draft_probs"] = None
+            got = check_verify(dev, s, top_k=top_k, top_p=top_p)
+            # a forced token that was drafted is always kept
+            assert got.path[0, :3].tolist() == [0, 2, 4] and got.accepted[1] == 3 and got.tokens[1, 3] == 899
+            s["draft_probs"] = drawn
+            check_verify(dev, s, top_k=top_k, top_p=top_p)
+
+
 def test_verify_without_a_draft_is_the_sampler(dev):
     from maple_amd.kernels.sampler import fused_sample_batched
 

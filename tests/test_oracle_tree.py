@@ -107,3 +107,22 @@ def test_greedy_keeps_the_branch_of_argmaxes(drafted):
     probs = None if drafted is None else np.full((5, 9), 1.0 / 9)
     out, path = ot.verify(logits, tokens, tree, [0.5] * 5, temperature=1.0, top_p=1.0, top_k=1, probs=probs)
     assert path == [0, 2, 3] and out == [best[0], best[2], best[3]]
+
+
+def test_the_law_of_infinite_logits():
+    """+inf (a forced token) takes all of the mass, alike where there are several;
+    rows of nothing but -inf weigh the first top_k tokens alike."""
+    kw = dict(temperature=0.7, top_p=1.0, top_k=4)
+    inf = np.inf
+    ids, p = ot.law(np.array([1.0, inf, 3.0, -inf, 2.0]), **kw)
+    assert ids.tolist() == [1, 2, 4, 0] and p.tolist() == [1.0, 0.0, 0.0, 0.0]
+    ids, p = ot.law(np.array([inf, 1.0, inf, -inf, 2.0]), **kw)
+    assert ids.tolist() == [0, 2, 4, 1] and p.tolist() == [0.5, 0.5, 0.0, 0.0]
+    ids, p = ot.law(np.full(6, -inf), **kw)
+    assert ids.tolist() == [0, 1, 2, 3] and p.tolist() == [0.25] * 4
+    ids, p = ot.law(np.array([-inf, 0.0, -inf, 0.0, -inf]), **kw)
+    assert ids.tolist() == [1, 3, 0, 2] and p.tolist() == [0.5, 0.5, 0.0, 0.0]
+    for top_k in (1, 3):  # a drafted token that is forced is kept, whatever the uniform
+        out, path = ot.verify(np.array([[0.0, 1.0, inf], [5.0, 1.0, 0.0]]), [0, 2], [-1, 0], [0.2, 0.999999],
+                              temperature=1.0, top_p=0.9, top_k=top_k)
+        assert path == [0, 1] and out == [2, 0]
