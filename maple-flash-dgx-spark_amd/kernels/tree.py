@@ -61,7 +61,8 @@ def _device(what: str, *tensors: torch.Tensor) -> int:
     return idx
 
 
-def _tree(what: str, parents: torch.Tensor, bsz: int, nodes: int) -> torch.Tensor:
+def check_tree(what: str, parents: torch.Tensor, bsz: int, nodes: int) -> torch.Tensor:
+    """``parents`` as the kernels take them: int32 ``[bsz, nodes]``, contiguous."""
     if not 1 <= nodes <= MAX_NODES:
         raise ValueError(f"{what}: a tree has 1 to {MAX_NODES} nodes, got {nodes}.")
     if parents.shape != (bsz, nodes):
@@ -92,7 +93,7 @@ def fit_tree(parents: torch.Tensor, seqlen: torch.Tensor, max_len: int) -> torch
     if parents.ndim != 2:
         raise ValueError(f"fit_tree expects parents [B, T], got {tuple(parents.shape)}.")
     bsz, nodes = parents.shape
-    parents = _tree("fit_tree", parents, bsz, nodes)
+    parents = check_tree("fit_tree", parents, bsz, nodes)
     slot = _positions("seqlen", seqlen, bsz).view(bsz, 1) + torch.arange(nodes, device=seqlen.device)
     return parents.masked_fill(slot >= max_len, -2)
 
@@ -173,7 +174,7 @@ def apply_qkv_tree(
         dt = _lib.dtype_code(cos_table, "cos_table")
         more += [cos_table, sin_table]
         c, s = cos_table.data_ptr(), sin_table.data_ptr()
-    parents = _tree("apply_qkv_tree", parents, bsz, nodes)
+    parents = check_tree("apply_qkv_tree", parents, bsz, nodes)
     sl = _positions("seqlen", seqlen, bsz)
     rm = None
     if row_map is not None:
@@ -217,7 +218,7 @@ def tree_attention(
         window = 0
     elif window < 1:
         raise ValueError(f"window must be positive, got {window}.")
-    parents = _tree("tree_attention", parents, bsz, nodes)
+    parents = check_tree("tree_attention", parents, bsz, nodes)
     sl = _positions("seqlen", seqlen, bsz)
     rm = None if row_map is None else _positions("row_map", row_map, bsz)
     idx = _device("tree_attention", q, k_cache, v_cache, sl, parents, *(() if rm is None else (rm,)))
@@ -274,7 +275,7 @@ def verify_tree(
     bsz, nodes, vocab = shape
     _check(top_k, temperature, vocab)
     l_dt = _lib.dtype_code(logits, "logits")
-    parents = _tree("verify_tree", parents, bsz, nodes)
+    parents = check_tree("verify_tree", parents, bsz, nodes)
     ldb, ldt, one = logits.stride()
     if one != 1 and vocab > 1:
         raise ValueError("logits rows must be contiguous.")

@@ -43,7 +43,7 @@ from .kernels.fused_norm import rms_norm
 from .kernels.greedy import greedy_argmax
 from .kernels.rtn4 import rtn4_embedding, rtn4_gemv
 from .kernels.ternary_gemv import combine_gemv_supported, ternary_gemv, ternary_gemv_combine
-from .kernels.tree import apply_qkv_tree, commit_tree, tree_attention
+from .kernels.tree import apply_qkv_tree, check_tree, commit_tree, tree_attention
 from .moe import PendingCombine, fused_form, fused_supported, moe_fused, moe_layer
 
 
@@ -441,6 +441,7 @@ class SyntheticDecoder:
         one is attached, node by node.  Padding's logits say nothing."""
         w, t = tokens.shape
         cache.slot_rows(w)
+        parents = check_tree("forward_tree", parents, w, t)  # (once, not in each layer)
         hidden = self.embed_tokens(tokens.reshape(-1))  # (padding's ids are clamped to the table)
         qkv = None
         for i in range(self.cfg.layers):

@@ -233,3 +233,47 @@ def test_fit_tree_leaves_out_nodes_past_the_caches_end():
         fit_tree(parents.float(), seqlen, 8)
     with pytest.raises(ValueError):
         fit_tree(torch.zeros(1, 65, dtype=torch.int32), seqlen[:1], 8)
+
+
+class _Stub:
+    """What ``forward_tree`` needs of a decoder and a cache; notes the trees that its layers get."""
+
+    def __init__(self, layers=3):
+        import types
+
+        self.cfg, self.flash_head, self.trees = types.SimpleNamespace(layers=layers), None, []
+
+    def slot_rows(self, width):
+        return torch.zeros(width, dtype=torch.int64), None
+
+    def embed_tokens(self, ids):
+        return torch.zeros(ids.numel(), 4)
+
+    def _layer(self, i, hidden, cache, routing, qkv, tree):
+        self.trees.append(tree)
+        return hidden, None
+
+    def head(self, hidden, *_):
+        return torch.zeros(hidden.shape[0], 7)
+
+
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
+def test_forward_tree_converts_its_tree_once(dtype):
+    from maple_amd.model import SyntheticDecoder
+
+    stub, parents = _Stub(), torch.tensor([[-1, 0, 0], [-1, 0, -1]], dtype=dtype)
+    out = SyntheticDecoder.forward_tree(stub, torch.zeros(2, 3, dtype=torch.int64), parents, stub)
+    assert out.shape == (2, 3, 7) and len(stub.trees) == 3
+    for tree_ in stub.trees:
+        assert tree_ is stub.trees[0] and tree_.dtype == torch.int32 and tree_.tolist() == parents.tolist()
+
+
+@pytest.mark.parametrize("shape", [(3, 2), (2, 4), (1, 6), (6,), (3, 3)])
+def test_forward_tree_refuses_parents_of_another_shape(shape):
+    from maple_amd.model import SyntheticDecoder
+
+    stub = _Stub()
+    with pytest.raises(ValueError):
+        SyntheticDecoder.forward_tree(stub, torch.zeros(2, 3, dtype=torch.int64),
+                                      torch.full(shape, -1, dtype=torch.int32), stub)
+    assert not stub.trees
