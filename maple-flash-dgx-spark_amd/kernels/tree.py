@@ -35,17 +35,16 @@ MAX_NODES = 64
 # Decoding calls these once per layer and step, so the checks below read each
 # property once and nothing goes through a context manager or a stream object
 # that a call does not need.
-_stream = torch._C._cuda_getCurrentRawStream
-_current = torch._C._cuda_getDevice
 
 
 def _call(idx: int, name: str, *args) -> None:
     """``name`` with the tensors' device current, on its current stream."""
-    if _current() == idx:
-        _lib.call(name, *args, _stream(idx))
+    # (looked up here: a torch built without GPU support does not have them)
+    if torch._C._cuda_getDevice() == idx:
+        _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(idx))
     else:
         with torch.cuda.device(idx):
-            _lib.call(name, *args, _stream(idx))
+            _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(idx))
 
 
 _index = torch.Tensor.get_device

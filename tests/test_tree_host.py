@@ -277,3 +277,27 @@ def test_forward_tree_refuses_parents_of_another_shape(shape):
         SyntheticDecoder.forward_tree(stub, torch.zeros(2, 3, dtype=torch.int64),
                                       torch.full(shape, -1, dtype=torch.int32), stub)
     assert not stub.trees
+
+
+def test_the_package_imports_with_a_torch_without_gpu_support():
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    code = ("import torch\n"
+            "for n in ('_cuda_getCurrentRawStream', '_cuda_getDevice'):\n"
+            "    if hasattr(torch._C, n): delattr(torch._C, n)\n"
+            "import __graft_entry__\n"
+            "__graft_entry__.load_package()\n"
+            "import maple_amd.kernels, maple_amd.model, maple_amd.decode_graph\n"
+            "a = dict(dtype=torch.bfloat16)\n"
+            "try:\n"
+            "    maple_amd.kernels.tree_attention(torch.zeros(1, 1, 1, 64, **a), torch.zeros(1, 1, 4, 64, **a),\n"
+            "        torch.zeros(1, 1, 4, 64, **a), torch.zeros(1, dtype=torch.int64),\n"
+            "        torch.full((1, 1), -1, dtype=torch.int32), scale=1.0)\n"
+            "except RuntimeError as e:\n"
+            "    print('refused:', e)\n")
+    done = subprocess.run([sys.executable, "-c", code], cwd=Path(__file__).resolve().parents[1], timeout=300,
+                          stdout=subprocess.PIPE, stderr=subprocess.PIPE, text=True)
+    assert done.returncode == 0, done.stderr
+    assert "refused: tree_attention requires CUDA tensors" in done.stdout
