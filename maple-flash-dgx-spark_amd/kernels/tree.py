@@ -31,6 +31,7 @@ from .. import _lib
 from .sampler import _check
 
 MAX_NODES = 64
+_FAR = 2 ** 62
 
 # Decoding calls these once per layer and step, so the checks below read each
 # property once and nothing goes through a context manager or a stream object
@@ -217,6 +218,8 @@ def tree_attention(
         window = 0
     elif window < 1:
         raise ValueError(f"window must be positive, got {window}.")
+    elif window > _FAR:
+        window = _FAR  # (past every position; more would wrap in 64 bits)
     parents = check_tree("tree_attention", parents, bsz, nodes)
     sl = _positions("seqlen", seqlen, bsz)
     rm = None if row_map is None else _positions("row_map", row_map, bsz)

@@ -301,3 +301,14 @@ def test_the_package_imports_with_a_torch_without_gpu_support():
                           stdout=subprocess.PIPE, stderr=subprocess.PIPE, text=True)
     assert done.returncode == 0, done.stderr
     assert "refused: tree_attention requires CUDA tensors" in done.stdout
+
+
+def test_windows_past_64_bits_are_none(monkeypatch):
+    """A window larger than any position sees everything; it does not wrap."""
+    a, windows = _cpu(), []
+    monkeypatch.setattr(tree, "_device", lambda what, *t: 0)
+    monkeypatch.setattr(tree, "_call", lambda idx, name, *args: windows.append(args[13]))
+    q = torch.zeros(2, 3, 4, 64, dtype=torch.bfloat16)
+    for window in (None, 1, 512, 2 ** 63 - 1, 2 ** 63, 2 ** 64, 2 ** 64 + 5, 2 ** 200):
+        tree.tree_attention(q, a["k"], a["k"], a["seqlen"], a["parents"], scale=0.125, window=window)
+    assert windows[:3] == [0, 1, 512] and all(w == 0 or 2 ** 62 <= w < 2 ** 63 for w in windows[3:])
