@@ -734,8 +734,8 @@ int ma_tree_qkv(const void* qkv, int64_t ldb, int64_t ldt, int64_t batch, int64_
  * K or V that a node does not see does not reach it, finite or not.
  * workspace: ma_tree_attn_workspace_bytes(...) bytes (may be 0), 16-byte
  * aligned, its content of no matter before and after; calls that share one
- * must not overlap.  scale finite; q, out and the cache 16-byte aligned; head_dim
- * 64 or 128.
+ * must not overlap.  scale x log2 e finite; q, out and the cache 16-byte aligned;
+ * head_dim 64 or 128.
  */
 size_t ma_tree_attn_workspace_bytes(int64_t batch, int64_t nodes, int n_heads, int n_kv_heads,
                                     int head_dim, int64_t max_len, int64_t window);

@@ -960,7 +960,7 @@ extern "C" int ma_tree_attn(const void* q, int64_t batch, int64_t nodes, int n_h
   int rc = check_tree("tree_attn", batch, nodes, n_heads, n_kv_heads, head_dim, cache_rows, max_len, row_map);
   if (rc != MA_OK) return rc;
   if (window < 0) return fail(MA_EVALUE, "tree_attn: window %lld", static_cast<long long>(window));
-  if (!isfinite(scale)) return fail(MA_EVALUE, "tree_attn: scale is not finite");
+  if (!isfinite(scale * kLog2e)) return fail(MA_EVALUE, "tree_attn: scale %g, or log2 e times it, is not finite", scale);
   if (batch == 0) return MA_OK;
   if (!q || !k_cache || !v_cache || !seqlen || !parents || !out) return fail(MA_EVALUE, "tree_attn: null pointer");
   if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(out) || !aligned16(workspace))

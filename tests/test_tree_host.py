@@ -312,3 +312,11 @@ def test_windows_past_64_bits_are_none(monkeypatch):
     for window in (None, 1, 512, 2 ** 63 - 1, 2 ** 63, 2 ** 64, 2 ** 64 + 5, 2 ** 200):
         tree.tree_attention(q, a["k"], a["k"], a["seqlen"], a["parents"], scale=0.125, window=window)
     assert windows[:3] == [0, 1, 512] and all(w == 0 or 2 ** 62 <= w < 2 ** 63 for w in windows[3:])
+
+
+@pytest.mark.parametrize("scale", [3e38, -3e38])
+def test_tree_attn_refuses_scales_that_overflow(scale):
+    """The scores are taken in powers of two: scale x log2 e has to be a float32 value."""
+    with pytest.raises(ValueError, match="scale"):
+        _lib.call("ma_tree_attn", *attn_args(scale=scale, batch=0, rows=0))
+    _lib.call("ma_tree_attn", *attn_args(scale=scale / 2, batch=0, rows=0))
