@@ -37,6 +37,7 @@ from __future__ import annotations
 
 import dataclasses
 import json
+import warnings
 from pathlib import Path
 
 import torch
@@ -117,6 +118,11 @@ def decoder_config(config: dict) -> DecoderConfig:
         raise NotImplementedError(f"head_dim {config['head_dim']}: the decode attention kernel is built "
                                   "for head_dim 64 and 128")
     meta = config.get("maple_run") or {}
+    entry = config.get("rope_scaling") or {}
+    if entry and not meta.get("rope_scaling") and entry.get("rope_type", entry.get("type")) != "default":
+        warnings.warn(f"the config's rope_scaling {entry} is not applied: positions past the trained context get the "
+                      "plain rotary tables (this loader reads maple_run.rope_scaling, as save_decoder writes it)",
+                      stacklevel=2)
     return DecoderConfig(
         hidden=int(config["hidden_size"]),
         layers=int(config["num_hidden_layers"]),

@@ -144,3 +144,29 @@ def test_maple_preview_config_maps_to_the_kernels(saved):
     assert (cfg.experts, cfg.inter, cfg.top_k, cfg.rtn_group, cfg.rotary_dim) == (256, 512, 8, 64, 64)
     assert [cfg.layer_attention(i) for i in range(4)] == [(512, True)] * 3 + [(None, False)]
     assert cfg.layer_attention(23) == (None, False) and cfg.layer_attention(22) == (512, True)
+
+
+def _config(**kw):
+    return {**dict(hidden_size=256, num_hidden_layers=1, num_attention_heads=4, num_key_value_heads=2, head_dim=64,
+                   num_experts=8, moe_intermediate_size=256, num_experts_per_tok=2, vocab_size=256), **kw}
+
+
+@pytest.mark.parametrize("entry", [{"type": "linear", "factor": 2.0}, {"rope_type": "yarn", "factor": 4.0},
+                                   {"factor": 2.0}])
+def test_a_rope_scaling_entry_that_is_not_applied_is_named(entry):
+    """A config's own rope_scaling entry is not read: the tables are the plain ones, and the user is told."""
+    with pytest.warns(UserWarning, match="rope_scaling"):
+        cfg = checkpoint.decoder_config(_config(rope_scaling=entry))
+    assert cfg.rope_scaling is None
+
+
+@pytest.mark.parametrize("kw", [{}, {"rope_scaling": None}, {"rope_scaling": {"rope_type": "default"}},
+                                {"rope_scaling": {"type": "linear", "factor": 2.0},
+                                 "maple_run": {"rope_scaling": {"kind": "linear", "factor": 2.0}}}])
+def test_configs_whose_rope_scaling_is_in_force_pass_without_a_word(kw):
+    import warnings
+
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        cfg = checkpoint.decoder_config(_config(**kw))
+    assert (cfg.rope_scaling is not None) == ("maple_run" in kw)
