@@ -691,7 +691,7 @@ int ma_fused_sample(const void* logits, int dtype, int64_t rows, int64_t vocab, 
                     void* workspace, size_t ws_bytes, int64_t* out, void* stream);
 
 /*
- * Decoding with a tree of drafted tokens per row: the next four operators.
+ * Decoding with a tree of drafted tokens per row: the next five entries.
  * parents int32 [batch, nodes], nodes <= 64: node 0 is the row's last token
  * (parents[b, 0] == -1; any other value there marks a row without a sequence),
  * 0 <= parents[b, i] < i names node i's parent; a node with any other parent,
@@ -699,7 +699,7 @@ int ma_fused_sample(const void* logits, int dtype, int64_t rows, int64_t vocab, 
  * position seqlen[b] + i, its rotary position is seqlen[b] + its depth.  A node
  * whose slot falls behind the cache (max_len) is neither stored nor attended, so
  * the parents given to ma_verify_tree, which does not see the cache, have to mark
- * it as absent (seqlen[b] + i >= max_len: parents[b, i] = -2);
+ * it as absent (ma_tree_fit);
  * mapped rows are clamped to [0, cache_rows), seqlen to [0, max_len].  batch x
  * nodes, batch x n_kv_heads and n_heads at most 65535.
  *
@@ -774,6 +774,16 @@ int ma_verify_tree(const void* logits, int dtype, int64_t ldb, int64_t ldt, int6
                    int64_t probs_ldt, int top_k, double inv_temperature, double top_p,
                    void* workspace, size_t workspace_bytes, int64_t* out_tokens,
                    int32_t* accepted, int32_t* path, void* stream);
+
+/*
+ * Trees that fit the cache: out int32 [batch, nodes] is parents (int32; int64
+ * where `wide` is not 0) with -2 for the nodes whose slot seqlen[b] + i lies
+ * behind max_len, so that an accepted branch ends within the cache.  A node's
+ * slot lies behind its parent's: what is kept is kept with its branch.  out may
+ * be parents (int32).
+ */
+int ma_tree_fit(const void* parents, int wide, int64_t batch, int64_t nodes, const int64_t* seqlen,
+                int64_t max_len, int32_t* out, void* stream);
 
 /*
  * The accepted nodes' K/V moved together behind the sequence, in every layer:

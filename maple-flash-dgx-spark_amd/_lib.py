@@ -103,6 +103,7 @@ _SIGNATURES = {
     "ma_verify_tree_workspace_bytes": [_L, _L, _L, _I],
     "ma_verify_tree": [_P, _I, _L, _L, _L, _L, _L, _P, _P, _P, _P, _I, _L, _L, _I, _D, _D, _P, _Z, _P, _P, _P,
                        _P],
+    "ma_tree_fit": [_P, _I, _L, _L, _P, _L, _P, _P],
     "ma_tree_commit": [_P, _P, _L, _L, _L, _I, _I, _L, _L, _P, _P, _P, _P, _P, _P],
 }
 _RESTYPES = {"ma_last_error": ctypes.c_char_p, "ma_router_workspace_bytes": _Z,

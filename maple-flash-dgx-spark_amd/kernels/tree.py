@@ -61,15 +61,19 @@ def _device(what: str, *tensors: torch.Tensor) -> int:
     return idx
 
 
-def check_tree(what: str, parents: torch.Tensor, bsz: int, nodes: int) -> torch.Tensor:
-    """``parents`` as the kernels take them: int32 ``[bsz, nodes]``, contiguous."""
+def _check_parents(what: str, parents: torch.Tensor, bsz: int, nodes: int) -> None:
     if not 1 <= nodes <= MAX_NODES:
         raise ValueError(f"{what}: a tree has 1 to {MAX_NODES} nodes, got {nodes}.")
     if parents.shape != (bsz, nodes):
         raise ValueError(f"{what}: parents is {tuple(parents.shape)}, expected {(bsz, nodes)}.")
+    if parents.dtype != torch.int32 and parents.dtype != torch.int64:
+        raise TypeError(f"{what}: parents must be int32 or int64; got {parents.dtype}.")
+
+
+def check_tree(what: str, parents: torch.Tensor, bsz: int, nodes: int) -> torch.Tensor:
+    """``parents`` as the kernels take them: int32 ``[bsz, nodes]``, contiguous."""
+    _check_parents(what, parents, bsz, nodes)
     if parents.dtype != torch.int32:
-        if parents.dtype != torch.int64:
-            raise TypeError(f"{what}: parents must be int32 or int64; got {parents.dtype}.")
         parents = parents.clamp(-2, MAX_NODES).to(torch.int32)  # (no large value may wrap to a node)
     return parents if parents.is_contiguous() else parents.contiguous()
 
@@ -93,9 +97,14 @@ def fit_tree(parents: torch.Tensor, seqlen: torch.Tensor, max_len: int) -> torch
     if parents.ndim != 2:
         raise ValueError(f"fit_tree expects parents [B, T], got {tuple(parents.shape)}.")
     bsz, nodes = parents.shape
-    parents = check_tree("fit_tree", parents, bsz, nodes)
-    slot = _positions("seqlen", seqlen, bsz).view(bsz, 1) + torch.arange(nodes, device=seqlen.device)
-    return parents.masked_fill(slot >= max_len, -2)
+    _check_parents("fit_tree", parents, bsz, nodes)
+    sl = _positions("seqlen", seqlen, bsz)
+    parents = parents.contiguous()
+    idx = _device("fit_tree", parents, sl)
+    out = torch.empty_like(parents, dtype=torch.int32)
+    _call(idx, "ma_tree_fit", parents.data_ptr(), int(parents.dtype == torch.int64), bsz, nodes, sl.data_ptr(),
+          max_len, out.data_ptr())
+    return out
 
 
 def _cache(what: str, k_cache: torch.Tensor, v_cache: torch.Tensor, bsz: int, row_map: torch.Tensor | None):

@@ -613,6 +613,37 @@ def test_commit_moves_the_accepted_rows(dev, layers, heads, nodes):
 
 
 # ---------------------------------------------------------------------------
+# Trees that fit the cache
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
+def test_fit_tree_leaves_out_nodes_past_the_caches_end(dev, dtype):
+    from maple_amd.kernels import fit_tree
+
+    parents = torch.tensor([[-1, 0, 0, 1]] * 5 + [[-2, 0, 0, 1]], dtype=dtype, device=dev)
+    seqlen = torch.tensor([0, 4, 6, 7, 8, 5], device=dev)
+    want = [[-1, 0, 0, 1], [-1, 0, 0, 1], [-1, 0, -2, -2], [-1, -2, -2, -2], [-2] * 4, [-2, 0, 0, -2]]
+    got = fit_tree(parents, seqlen, 8)
+    assert got.dtype == torch.int32 and got.is_contiguous() and got.tolist() == want
+    assert fit_tree(parents, seqlen, 1 << 40).tolist() == parents.tolist()
+    assert fit_tree(parents, seqlen, 0).tolist() == [[-2] * 4] * 6
+    wide = torch.full((6, 9), 5, dtype=dtype, device=dev)
+    wide[:, 3:7] = parents
+    assert fit_tree(wide[:, 3:7], seqlen.int(), 8).tolist() == want
+    assert fit_tree(parents[:0], seqlen[:0], 8).shape == (0, 4)
+    if dtype == torch.int64:  # no large value becomes a node
+        far = torch.tensor([[-1, 1 << 32, (1 << 32) + 1, -(1 << 32)]], device=dev)
+        assert fit_tree(far, seqlen[:1], 8).tolist() == [[-1, 64, 64, -2]]
+        far = torch.tensor([2 ** 63 - 1, -2 ** 63], device=dev)
+        assert fit_tree(parents[:2], far, 8).tolist() == [[-2] * 4, [-1, 0, 0, 1]]
+    rng = np.random.default_rng(1)
+    for b, t in ((1, 64), (1023, 64), (300, 7), (65535, 1)):
+        p = torch.tensor(random_parents(rng, min(b, 40), t), dtype=dtype, device=dev).repeat(-(-b // min(b, 40)), 1)[:b]
+        sl = torch.tensor(rng.integers(0, 200, b), device=dev)
+        fits = sl[:, None] + torch.arange(t, device=dev) < 130
+        assert torch.equal(fit_tree(p, sl, 130), torch.where(fits, p, -2).int())
+
+
+# ---------------------------------------------------------------------------
 # Streams and graphs
 # ---------------------------------------------------------------------------
 def _step(k, v, s, heads, cos, sin, qkv, rot, window=None):

@@ -215,24 +215,21 @@ def test_tree_step_refuses_settings_the_sampler_does_not_cover():
                   Sampling(temperature=1.0, top_k=0))
 
 
-def test_fit_tree_leaves_out_nodes_past_the_caches_end():
-    from maple_amd.kernels.tree import fit_tree
-
-    parents = torch.tensor([[-1, 0, 0, 1]] * 5 + [[-2, 0, 0, 1]])
-    seqlen = torch.tensor([0, 4, 6, 7, 8, 5])
-    want = [[-1, 0, 0, 1], [-1, 0, 0, 1], [-1, 0, -2, -2], [-1, -2, -2, -2], [-2] * 4, [-2, 0, 0, -2]]
-    for dtype in (torch.int32, torch.int64):
-        got = fit_tree(parents.to(dtype), seqlen, 8)
-        assert got.dtype == torch.int32 and got.is_contiguous() and got.tolist() == want
-    assert fit_tree(parents.int(), seqlen, 1 << 40).tolist() == parents.tolist()
-    far = torch.tensor([[-1, 1 << 32, (1 << 32) + 1, -(1 << 32)]])  # no large value becomes a node
-    assert fit_tree(far, seqlen[:1], 8).tolist() == [[-1, 64, 64, -2]]
-    with pytest.raises(ValueError):
-        fit_tree(parents, seqlen[:3], 8)
-    with pytest.raises(TypeError):
-        fit_tree(parents.float(), seqlen, 8)
-    with pytest.raises(ValueError):
-        fit_tree(torch.zeros(1, 65, dtype=torch.int32), seqlen[:1], 8)
+def test_fit_tree_checks_its_arguments():
+    parents, seqlen = torch.full((2, 3), -1), torch.zeros(2, dtype=torch.int64)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        kernels.fit_tree(parents, seqlen, 8)
+    for args, err in (((parents, seqlen[:1], 8), ValueError), ((parents.float(), seqlen, 8), TypeError),
+                      ((parents, seqlen.float(), 8), TypeError), ((parents[0], seqlen, 8), ValueError),
+                      ((torch.zeros(2, 65, dtype=torch.int32), seqlen, 8), ValueError)):
+        with pytest.raises(err):
+            kernels.fit_tree(*args)
+    for kw, match in ((dict(nodes=65), "1 to 64 nodes"), (dict(nodes=0), "1 to 64 nodes"), (dict(batch=40000), "too large"),
+                      (dict(max_len=-1), "cache sizes"), (dict(parents=None), "null"), (dict(out=None), "null")):
+        a = {**dict(parents=FAKE, wide=0, batch=1, nodes=2, seqlen=FAKE, max_len=8, out=FAKE, stream=None), **kw}
+        with pytest.raises(ValueError, match=match):
+            _lib.call("ma_tree_fit", *a.values())
+    _lib.call("ma_tree_fit", FAKE, 0, 0, 2, FAKE, 8, FAKE, None)  # an empty batch is no work
 
 
 class _Stub:
