@@ -35,17 +35,19 @@ _FAR = 2 ** 62
 
 # Decoding calls these once per layer and step, so the checks below read each
 # property once and nothing goes through a context manager or a stream object
-# that a call does not need.
+# that a call does not need.  (None in a torch built without GPU support, whose
+# tensors no call gets past _device with.)
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_current = getattr(torch._C, "_cuda_getDevice", None)
 
 
 def _call(idx: int, name: str, *args) -> None:
     """``name`` with the tensors' device current, on its current stream."""
-    # (looked up here: a torch built without GPU support does not have them)
-    if torch._C._cuda_getDevice() == idx:
-        _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(idx))
+    if _current() == idx:
+        _lib.call(name, *args, _stream(idx))
     else:
         with torch.cuda.device(idx):
-            _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(idx))
+            _lib.call(name, *args, _stream(idx))
 
 
 _index = torch.Tensor.get_device
