@@ -234,6 +234,9 @@ __global__ __launch_bounds__(kQkvThreads) void k_tree_qkv(
 typedef __attribute__((address_space(3))) void* tree_lds_t;
 constexpr float kTreeGrow = 8.0f;    // a row's reference is moved when a score in a masked tile passes it by 2^8,
 constexpr float kTreeSum = 65536.f;  // or, where all rows see all positions, when a lane's sum passes this
+// References of this size are no longer close to the unrounded products (half a
+// step is 2^3 here, 2^8 at scores of 2^32): from here on products are rounded too.
+constexpr float kTreeFar = 134217728.f;  // 2^27
 constexpr int tree_vmcnt(int n) { return (n & 0xF) | (0x7 << 4) | ((n >> 4) << 14); }  // and lgkmcnt(0)
 
 __device__ __forceinline__ f32x16t_t mfma_tree(uint4 a, uint4 b, f32x16t_t c) {
@@ -432,6 +435,7 @@ __global__ __launch_bounds__(256, (TreeTile<HD>::kWaves)) void k_tree_attn(
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[db][i] = 0.f;
   float mref = -INFINITY, lsum = 0.f;
+  bool far = false;  // a row of this wave has a reference past kTreeFar
 
   // Byte offsets into the K and V rows: piece 2 ks + h of row r32 (ks of
   // one half; 128 bytes on for the other), and the lane's 8 bytes of the
@@ -464,6 +468,7 @@ __global__ __launch_bounds__(256, (TreeTile<HD>::kWaves)) void k_tree_attn(
     const float a = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mref - mn);
     const bool first = !__any(mref != -INFINITY);
     mref = mn;
+    far = __any(fabsf(mn) >= kTreeFar && mn != -INFINITY);
     if (first) return;  // (nothing summed yet)
     lsum *= a;
 #pragma unroll
@@ -482,17 +487,27 @@ __global__ __launch_bounds__(256, (TreeTile<HD>::kWaves)) void k_tree_attn(
                                     vb + voff[db & 1] + (32 * t + 16 * k2 + 8 * e) * T::kRowBytes + 128 * (db >> 1))));
     return make_uint4(v[0].x, v[0].y, v[1].x, v[1].y);
   };
-  // The weights of scores 8 k2 .. +7, as the A operand of their product.
-  auto weights = [&](const f32x16t_t& sc, int k2, float m) {
+  // The weights 2^(s factor - m) of scores 8 k2 .. +7, as the A operand of their product.
+  auto weights = [&](const f32x16t_t& sc, int k2, float factor, float m) {
     uint32_t p[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[8 * k2 + 2 * e], scale2, -m));
-      const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[8 * k2 + 2 * e + 1], scale2, -m));
+      const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[8 * k2 + 2 * e], factor, -m));
+      const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[8 * k2 + 2 * e + 1], factor, -m));
       p[e] = pack_bf16x2_rn(p0, p1);
       lsum = dot2(p[e], kOneBf16x2, lsum);
     }
     return make_uint4(p[0], p[1], p[2], p[3]);
+  };
+  // Scores as exponents over a far reference: rounded products, as it is one, so that
+  // the largest is 0 at any score that float32 holds.
+  auto exponents = [&](f32x16t_t& sc, float m) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      float t = sc[i] * scale2;
+      asm volatile("" : "+v"(t));  // (no fused multiply-subtract)
+      sc[i] = t - m;
+    }
   };
 
   // The NT x 32 positions of a group that all rows see: all K reads ahead of the
@@ -531,11 +546,11 @@ __global__ __launch_bounds__(256, (TreeTile<HD>::kWaves)) void k_tree_attn(
     for (int t = 0; t < NT; ++t) {
       uint4 pa0, pa1;
       const float before = lsum;  // (a weight out of range, or the first scores: once more, from a new reference)
-      float m = mref;
+      float m = mref, factor = scale2;
       for (bool again = false;;) {
-        pa0 = weights(sc[t], 0, m);
-        pa1 = weights(sc[t], 1, m);
-        if (again || !__any(!(lsum <= kTreeSum))) break;
+        pa0 = weights(sc[t], 0, factor, m);
+        pa1 = weights(sc[t], 1, factor, m);
+        if (again || !(far || __any(!(lsum <= kTreeSum)))) break;
         again = true;
         lsum = before;
         float cm = sc[t][0];
@@ -543,6 +558,11 @@ __global__ __launch_bounds__(256, (TreeTile<HD>::kWaves)) void k_tree_attn(
         for (int i = 1; i < 16; ++i) cm = fmaxf(cm, sc[t][i]);
         rescale(fmaxf(cm * scale2, before > 1.0f ? mref + __builtin_amdgcn_logf(before) : -INFINITY));
         m = mref == -INFINITY ? 0.f : mref;
+        if (far) {
+          exponents(sc[t], m);
+          factor = 1.f;
+          m = 0.f;
+        }
       }
       if (t + 1 < NT) v_tile(t + 1);
 #pragma unroll
@@ -582,14 +602,19 @@ __global__ __launch_bounds__(256, (TreeTile<HD>::kWaves)) void k_tree_attn(
     for (int i = 1; i < 16; ++i) cm = fmaxf(cm, sc[i]);
     cm *= scale2;
     if (__any(!(cm <= mref + kTreeGrow))) rescale(cm);
-    const float m = mref == -INFINITY ? 0.f : mref;
+    float m = mref == -INFINITY ? 0.f : mref, factor = scale2;
+    if (far) {
+      exponents(sc, m);
+      factor = 1.f;
+      m = 0.f;
+    }
     uint32_t bad = 0;
 #pragma unroll
     for (int k2 = 0; k2 < 2; ++k2) {
 #pragma unroll
       for (int db = 0; db < DB; ++db)
         bad |= take_odd(vf[k2][db].x) | take_odd(vf[k2][db].y) | take_odd(vf[k2][db].z) | take_odd(vf[k2][db].w);
-      const uint4 pa = weights(sc, k2, m);
+      const uint4 pa = weights(sc, k2, factor, m);
 #pragma unroll
       for (int db = 0; db < DB; ++db) o[db] = mfma_tree(pa, vf[k2][db], o[db]);
     }

@@ -293,6 +293,35 @@ def test_attention_scores_of_any_size(dev):
         compare_attention(out, q, k, v, parents, [n], 0.25)
 
 
+@pytest.mark.parametrize("window", [None, 100])
+@pytest.mark.parametrize("heads,n", [((32, 1, 64), 1500), ((16, 1, 128), 1500), ((8, 2, 64), 9)])
+def test_attention_scores_past_float32s_whole_numbers(dev, heads, n, window):
+    """Finite scores up to 2^120, of either sign, where a step of float32 is more than
+    an exponent can hold: equal ones weigh alike, of others the largest takes all
+    (scores are powers of two times small numbers: exact in bf16 and in float32, so
+    equal where they are equal and far apart else)."""
+    from maple_amd.kernels import tree_attention
+
+    nq, nkv, d = heads
+    t = 5
+    parents = [[-1, 0, 1, 1, 3]]
+    q = torch.zeros(1, t, nq, d, device=dev, dtype=torch.bfloat16)
+    q[..., 0] = 1
+    v = bf16(dev, 1, nkv, n + t, d, seed=2)
+    at = torch.arange(n + t, device=dev, dtype=torch.float64)
+    shapes = (torch.ones_like(at), -torch.ones_like(at), 1 + (at * 7 % 100 < 1), -1 - (at * 7 % 100 > 1).double(),
+              (at // 16).clamp(max=100), -(at // 16).clamp(max=100), torch.where(at < n - 20, -1.0, 1.0),
+              torch.where(at < n - 20, 1.0, 0.0))
+    for power in (20, 27, 30, 32, 45, 113):
+        for shape in shapes:
+            k = bf16(dev, 1, nkv, n + t, d, seed=3)
+            k[..., 0] = (shape * 2.0 ** power).to(torch.bfloat16)
+            for scale in (1.0, -0.125):
+                out = tree_attention(q, k, v, torch.tensor([n], device=dev), as_parents(parents, dev), scale=scale,
+                                     window=window)
+                compare_attention(out, q, k, v, parents, [n], scale, window)
+
+
 @pytest.mark.parametrize("heads", [(32, 1, 64), (16, 1, 128), (4, 4, 64)])
 def test_attention_references_that_stay_too_low(dev, heads):
     """Scores that stay above the first ones for the rest of the sequence: just
@@ -334,6 +363,46 @@ def test_attention_of_what_is_not_finite_stays_in_its_rows(dev, heads):
     for window in (None, 280):  # (280: position 40 is seen by the second row's first nodes alone)
         out = tree_attention(q, k, v, sl, as_parents(parents, dev), scale=d ** -0.5, window=window)
         compare_attention(out, q, k, v, parents, seqlen, d ** -0.5, window)
+
+
+@pytest.mark.parametrize("heads", [(8, 1, 64), (8, 2, 128)])
+@pytest.mark.parametrize("n,max_len", [(0, 16), (70, 100), (2000, 2100)])
+def test_attention_scores_of_minus_infinity(dev, heads, n, max_len):
+    """Keys that give one head -inf everywhere: 0 there, as where a node sees
+    nothing; the other heads as in 64 bits, and so the first where it meets one
+    finite score."""
+    from maple_amd.kernels import tree_attention
+
+    nq, nkv, d = heads
+    parents = [[-1, 0, 0, 1]]
+    q = bf16(dev, 1, 4, nq, d)
+    q[..., 0] = 0
+    k, v = bf16(dev, 1, nkv, max_len, d, seed=1), bf16(dev, 1, nkv, max_len, d, seed=2)
+    q[:, :, 0, 0], q[:, :, 1:, 0] = 1.0, 2.0 ** -100
+    k[..., 0] = -3e38  # x 1 x scale: -inf in no float32, but alone in its sum
+    lone = k.clone()
+    k[..., 0] = float("-inf")
+    sl, p = torch.tensor([n], device=dev), as_parents(parents, dev)
+    out = tree_attention(q, k, v, sl, p, scale=d ** -0.5)
+    assert (out == 0).all()  # (-inf for every head: 2^-100 x -inf too)
+    lone[0, :, n + 1, 0] = 0  # node 1, which node 3 sees too
+    k[0, :, n + 1, 0] = 0
+    out = tree_attention(q, k, v, sl, p, scale=d ** -0.5)
+    assert (out[:, [0, 2]] == 0).all()
+    for node in (1, 3):
+        for h in range(nq):
+            assert torch.equal(out[0, node, h], v[0, h * nkv // nq, n + 1])
+    out = tree_attention(q, lone, v, sl, p, scale=d ** -0.5)
+    compare_attention(out[:, :, :1], q[:, :, :1], lone[:, :1], v[:, :1], parents, [n], d ** -0.5)
+    # The other heads' scores are 2^-100 x -3e38 = -2.4e8 and the other dims' few units: a step of
+    # float32 is 16 there, so those units are not held and the weights of equal keys say nothing; node 1's
+    # finite key takes all where it is seen, and any weights give values between the least and the largest V.
+    for node in (1, 3):
+        for h in range(1, nq):
+            assert torch.equal(out[0, node, h], v[0, h * nkv // nq, n + 1])
+    lo, hi = (f(v[:, :, :n + 4].float(), 2).view(1, 1, nkv, 1, d) for f in (torch.amin, torch.amax))
+    rest = out.float().view(1, 4, nkv, nq // nkv, d)
+    assert ((rest >= lo - 2.0 ** -7 * lo.abs()) & (rest <= hi + 2.0 ** -7 * hi.abs())).all()
 
 
 def test_attention_windows_past_every_distance(dev):
