@@ -700,8 +700,9 @@ int ma_fused_sample(const void* logits, int dtype, int64_t rows, int64_t vocab, 
  * whose slot falls behind the cache (max_len) is neither stored nor attended, so
  * the parents given to ma_verify_tree, which does not see the cache, have to mark
  * it as absent (ma_tree_fit);
- * mapped rows are clamped to [0, cache_rows), seqlen to [0, max_len].  batch x
- * nodes, batch x n_kv_heads and n_heads at most 65535.
+ * mapped rows are clamped to [0, cache_rows), seqlen to [0, max_len]; no two
+ * rows may be mapped to one (they would write each other's K/V).  batch x nodes,
+ * batch x n_kv_heads and n_heads at most 65535.
  *
  * QK RMSNorm + rotary positions + K/V store of the nodes: qkv bf16 [batch,
  * nodes, (n_heads + 2 n_kv_heads) * head_dim] (strides ldb, ldt, 1); per head
@@ -730,8 +731,9 @@ int ma_tree_qkv(const void* qkv, int64_t ldb, int64_t ldt, int64_t batch, int64_
  * only what is less than window steps above the node.  q / out bf16 [batch,
  * nodes, n_heads, head_dim]; float32 statistics and sums, P rounded to bf16
  * before P.V as in ma_decode_gqa_attn, whose results a tree of one node
- * repeats up to rounding.  Absent nodes, and nodes that see nothing, give 0; a
- * K or V that a node does not see does not reach it, finite or not.
+ * repeats up to rounding.  Absent nodes, and nodes that see nothing (or whose
+ * scores are all -inf), give 0; a K or V that a node does not see does not reach
+ * it, finite or not.  The splits are planned for max_len, or the window.
  * workspace: ma_tree_attn_workspace_bytes(...) bytes (may be 0), 16-byte
  * aligned, its content of no matter before and after; calls that share one
  * must not overlap.  scale x log2 e finite; q, out and the cache 16-byte aligned;

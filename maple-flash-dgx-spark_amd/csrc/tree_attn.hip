@@ -109,10 +109,11 @@ constexpr int kQkvThreads = 256;
 //   interleaved  y_2i     -> y_2i c_i - y_{2i+1} s_i, y_{2i+1} -> y_{2i+1} c_{i+h} + y_2i s_{i+h}
 // (the half layout's partners meet in LDS, whatever h is).  float32 inside; c
 // and s are rounded to bf16 first and y to bf16 at the end, as the one-token
-// path does, so a token's K is the same whichever wrote it.  Latency: two rounds
-// of loads (x, weights, tree and length; then the table's row): 4.3 us for 8
-// nodes of 32 + 8 heads of 64, 7.3 for 1024 (a wave a head with a tree of its
-// own: 15.2), 5.6 for 488 of 16 + 8 heads of 128.
+// path does; its squares are summed in another order, so a token's K is the same
+// whichever wrote it up to one bf16 step, in fewer than 1 of 100 values.  Latency:
+// two rounds of loads (x, weights, tree and length; then the table's row): 4.3 us
+// for 8 nodes of 32 + 8 heads of 64, 7.3 for 1024 (a wave a head with a tree of
+// its own: 15.2), 5.6 for 488 of 16 + 8 heads of 128.
 // VEC: all rows are 16-byte aligned.
 template <int HD, bool VEC>
 __global__ __launch_bounds__(kQkvThreads) void k_tree_qkv(
@@ -287,10 +288,12 @@ struct TreeRow {
 //     when the weights' sum shows that it has become too low (any m that keeps
 //     them in range gives the same quotient, and bf16 and float32 share one
 //     range; a running maximum costs 9 of 100 cycles of a tile and a wait for
-//     it: 54.5 us without, 57.9 with, at 32 rows of 32 nodes over 4096
-//     positions of 32 / 4 heads of 64), P rounded to bf16 as the matrix
-//     instruction takes it (half a step, 2^-8 of each weight at most),
-//     masked places exactly 0;
+//     it: of the 57.9 us that 32 rows of 32 nodes over 4096 positions of 32 / 4
+//     heads of 64 took with it, before the copies and tiles were as they are now,
+//     54.5 were left without it), P rounded to bf16 as the matrix instruction
+//     takes it (half a step, 2^-8 of each weight at most; it is the output's error
+//     beside its own rounding, 2.3e-3 against 1.7e-3 with P in float32), masked
+//     places exactly 0;
 //   the sum of P from the same rounded values, so that a weight's rounding
 //     enters the quotient on both sides;
 //   O += P V: A = the lane's own P values in the order they are in, B = V in the
@@ -828,6 +831,12 @@ static TreePlan tree_plan(int64_t batch, int64_t nodes, int nq, int nkv, int hea
   //   4 x 16 of 64 over 2048: 18 + 4 in two, 12 + 4 in four, 9 + 4 in eight, 11 + 5 in 16
   //   1 x 8 of 64 over 370: 11 in one, 6 + 4 in six; over 4096 13 + 4 in 4, 10 + 4 in 8,
   //     8 + 4 in 12, 7 + 5 in 24 to 32
+  // `over` is the cache's length here: the host does not know the rows'.  A cache much
+  // longer than what its rows hold gets splits that find nothing, which leave at
+  // once but are merged (caches of a little over the rows' length / 4224 / 32896):
+  //   32 x 32 of 64, rows of 1024: 21.5 / 21 + 6.5 / 21 + 7; 8 x 32: 12 + 4 / 12 + 4 / 14.5 + 8
+  //   1 x 8 of 64, rows of 500: 6 + 4 / 6 + 5 / 6 + 6; 8 x 16 of 128, rows of 600: 12 + 4 /
+  //     11 + 4 / 12 + 6
   const int64_t n = cdiv(span, head_dim == 64 ? TreeTile<64>::kStep : TreeTile<128>::kStep);
   const int64_t per_cu = head_dim == 64 ? TreeTile<64>::kWaves : TreeTile<128>::kWaves;
   const int64_t at_once = p.pairs * p.tiles > 0 ? p.pairs * p.tiles : 1;

@@ -16,7 +16,8 @@ below it, is padding; a row whose entry 0 is not -1 has no sequence.  Node ``i``
 is cached at ``seqlen[b] + i`` and stands at position ``seqlen[b] + depth``.
 Nodes past the cache's end are neither stored nor attended, so they must not be
 accepted either: where ``seqlen[b] + T`` may exceed ``max_len``, all four get the
-tree from ``fit_tree``, in which such nodes are padding.
+tree from ``fit_tree``, in which such nodes are padding.  ``row_map`` (slot ->
+cache row) names each cache row once.
 """
 
 from __future__ import annotations
