@@ -793,10 +793,10 @@ int ma_tree_fit(const void* parents, int wide, int64_t batch, int64_t nodes, con
  * row_map[b] (b when NULL) goes to seqlen[b] + j; new_seqlen[b] = seqlen[b] +
  * accepted[b] + 1 (accepted and path as ma_verify_tree writes them: path
  * ascending, of nodes that were stored; one that was not, its slot behind max_len,
- * moves nothing and is counted all the same; new_seqlen is not seqlen).  k_caches / v_caches: host arrays of
- * `layers` device pointers to bf16 caches [cache_rows, n_kv_heads, max_len,
- * head_dim], 16-byte aligned, distinct from one another; one launch per 64
- * layers.  head_dim 64 or 128.
+ * moves nothing and is counted all the same; new_seqlen is not seqlen).
+ * k_caches / v_caches: host arrays of `layers` device pointers to bf16 caches
+ * [cache_rows, n_kv_heads, max_len, head_dim], 16-byte aligned, distinct from one
+ * another; one launch per 64 layers.  head_dim 64 or 128.
  */
 int ma_tree_commit(void* const* k_caches, void* const* v_caches, int64_t layers, int64_t batch,
                    int64_t nodes, int n_kv_heads, int head_dim, int64_t cache_rows,

@@ -119,7 +119,8 @@ def decoder_config(config: dict) -> DecoderConfig:
                                   "for head_dim 64 and 128")
     meta = config.get("maple_run") or {}
     entry = config.get("rope_scaling") or {}
-    if entry and not meta.get("rope_scaling") and entry.get("rope_type", entry.get("type")) != "default":
+    kind = entry.get("rope_type", entry.get("type")) if isinstance(entry, dict) else entry
+    if entry and not meta.get("rope_scaling") and kind != "default":
         warnings.warn(f"the config's rope_scaling {entry} is not applied: positions past the trained context get the "
                       "plain rotary tables (this loader reads maple_run.rope_scaling, as save_decoder writes it)",
                       stacklevel=2)

@@ -860,12 +860,12 @@ static size_t tree_ws_bytes(const TreePlan& p, int head_dim) {
 // ---------------------------------------------------------------------------
 // Trees that fit the cache
 // ---------------------------------------------------------------------------
-// A thread per node.  Latency: a captured step of one row takes 5 us longer with
+// A thread per node (out may be parents: each reads its entry before it writes
+// it).  Latency: a captured step of one row takes 5 us longer with
 // it, 13 with the five torch launches of the same.
 template <typename P>
-__global__ __launch_bounds__(256) void k_tree_fit(const P* __restrict__ parents, int total, int nodes,
-                                                  const int64_t* __restrict__ seqlen, int64_t max_len,
-                                                  int32_t* __restrict__ out) {
+__global__ __launch_bounds__(256) void k_tree_fit(const P* parents, int total, int nodes, const int64_t* __restrict__ seqlen,
+                                                  int64_t max_len, int32_t* out) {
   const int at = static_cast<int>(blockIdx.x) * 256 + static_cast<int>(threadIdx.x);
   if (at >= total) return;
   const int b = at / nodes, i = at - b * nodes;

@@ -152,7 +152,7 @@ def _config(**kw):
 
 
 @pytest.mark.parametrize("entry", [{"type": "linear", "factor": 2.0}, {"rope_type": "yarn", "factor": 4.0},
-                                   {"factor": 2.0}])
+                                   {"factor": 2.0}, "linear"])
 def test_a_rope_scaling_entry_that_is_not_applied_is_named(entry):
     """A config's own rope_scaling entry is not read: the tables are the plain ones, and the user is told."""
     with pytest.warns(UserWarning, match="rope_scaling"):

@@ -705,6 +705,12 @@ def test_fit_tree_leaves_out_nodes_past_the_caches_end(dev, dtype):
         far = torch.tensor([2 ** 63 - 1, -2 ** 63], device=dev)
         assert fit_tree(parents[:2], far, 8).tolist() == [[-2] * 4, [-1, 0, 0, 1]]
     rng = np.random.default_rng(1)
+    if dtype == torch.int32:  # in place, through the library
+        from maple_amd import _lib
+
+        same = parents.clone()
+        _lib.call("ma_tree_fit", same.data_ptr(), 0, 6, 4, seqlen.data_ptr(), 8, same.data_ptr(), _lib.stream_of(same))
+        assert same.tolist() == want
     for b, t in ((1, 64), (1023, 64), (300, 7), (65535, 1)):
         p = torch.tensor(random_parents(rng, min(b, 40), t), dtype=dtype, device=dev).repeat(-(-b // min(b, 40)), 1)[:b]
         sl = torch.tensor(rng.integers(0, 200, b), device=dev)
