@@ -804,6 +804,81 @@ int ma_tree_commit(void* const* k_caches, void* const* v_caches, int64_t layers,
                    const int32_t* accepted, const int64_t* row_map, int64_t* new_seqlen,
                    void* stream);
 
+/*
+ * A quantised KV cache, the next three entries and ma_cache_attn: per (row, KV
+ * head, position) and for K and V each, head_dim e4m3 codes ([cache_rows,
+ * n_kv_heads, max_len, head_dim], 16-byte aligned) and one scale byte e + 127
+ * ([cache_rows, n_kv_heads, max_len]; e8m0): e is the least integer with which
+ * the largest finite value is at most 448 x 2^e, in [-126, 119]; a code is the
+ * e4m3 value nearest (even) to x 2^-e, at most 448 in size, NaN for what is not
+ * finite.  Positions outside the cache are not written, mapped rows (row_map, b
+ * when NULL) are clamped to it; no two rows that are written may be mapped to
+ * one.  head_dim 64 or 128.
+ *
+ * QK RMSNorm + rotary positions + quantising store of one token a row: qkv bf16
+ * [batch, (n_heads + 2 n_kv_heads) * head_dim] (row stride ldb); the norm as in
+ * ma_tree_qkv, rotary positions in the half layout (rotary_dim 0: none) at
+ * positions[b] (seqlen[b] when NULL; clamped to the table); K rounded to bf16 and
+ * V as it is, quantised at position seqlen[b].  q_out bf16 [batch, n_heads,
+ * head_dim], 16-byte aligned; seqlen[b] < 0: no token (q 0, nothing stored).
+ * The bf16 cache's form of it is ma_qk_norm_rope_store.
+ */
+int ma_quant_qkv(const void* qkv, int64_t ldb, int64_t batch, int n_heads, int n_kv_heads,
+                 int head_dim, const void* q_norm_w, const void* k_norm_w, int w_dtype,
+                 const void* cos, const void* sin, int cs_dtype, int64_t ld_cs, int64_t n_pos,
+                 int rotary_dim, float eps, const int64_t* seqlen, const int64_t* positions,
+                 const int64_t* row_map, void* k_codes, void* v_codes, void* k_scale,
+                 void* v_scale, int64_t cache_rows, int64_t max_len, void* q_out, void* stream);
+
+/*
+ * K and V of whole prompts into a quantised cache: bf16 [batch, n_kv_heads, T,
+ * head_dim] each (strides sb, sh, st, 1, in elements); row b's positions t <
+ * lengths[b] (all T when NULL) go to start[b] + t (t when NULL).
+ */
+int ma_quant_kv(const void* k, int64_t k_sb, int64_t k_sh, int64_t k_st, const void* v,
+                int64_t v_sb, int64_t v_sh, int64_t v_st, int64_t batch, int64_t T,
+                int n_kv_heads, int head_dim, const int64_t* start, const int64_t* lengths,
+                const int64_t* row_map, void* k_codes, void* v_codes, void* k_scale,
+                void* v_scale, int64_t cache_rows, int64_t max_len, void* stream);
+
+/*
+ * The first `length` positions of a quantised cache's rows (row_map[b], b when
+ * NULL) as bf16 [batch, n_kv_heads, length, head_dim], 16-byte aligned.
+ */
+int ma_dequant_kv(const void* k_codes, const void* v_codes, const void* k_scale,
+                  const void* v_scale, int64_t cache_rows, int64_t max_len, int64_t batch,
+                  int64_t length, int n_kv_heads, int head_dim, const int64_t* row_map,
+                  void* k_out, void* v_out, void* stream);
+
+/*
+ * Attention of one query token a row: out[b, h] = softmax(q[b, h] . K^T * scale) V
+ * over prefix p = prefix_of[b] (positions 0 .. prefix_len[p] - 1 of the prefix
+ * cache's row p; p outside [0, prefixes): none), then positions 0 .. seqlen[b] of
+ * cache row row_map[b] (b when NULL; none for a negative seqlen[b]); with window >
+ * 0 the last `window` of both together.  The caches [rows, n_kv_heads, max_len,
+ * head_dim], 16-byte aligned, are quantised with scales, bf16 where k_scale is
+ * NULL, the prefixes' of the same kind; prefixes = 0: none (pk .. prefix_of not
+ * read).  Lengths are clamped to the caches.  q / out bf16 [batch, n_heads,
+ * head_dim]; float32 statistics and sums, P rounded to bf16 before P.V; a row
+ * that sees nothing (or whose scores are all -inf) gives 0, and what lies behind
+ * its positions does not reach it, finite or not.  Without a window a prefix is
+ * read once for all of its rows.  At most 16 query heads to a KV head; batch x
+ * n_kv_heads and prefixes at most 65535; scale x log2 e finite.  workspace:
+ * ma_cache_attn_workspace_bytes(...) bytes (may be 0), 16-byte aligned, its
+ * content of no matter; calls that share one must not overlap.  The bf16 form
+ * without prefixes is ma_decode_gqa_attn.
+ */
+size_t ma_cache_attn_workspace_bytes(int64_t batch, int n_heads, int n_kv_heads, int head_dim,
+                                     int64_t max_len, int64_t prefixes, int64_t prefix_max_len,
+                                     int64_t window);
+int ma_cache_attn(const void* q, int64_t batch, int n_heads, int n_kv_heads, int head_dim,
+                  const void* k, const void* v, const void* k_scale, const void* v_scale,
+                  int64_t cache_rows, int64_t max_len, const int64_t* seqlen,
+                  const int64_t* row_map, const void* pk, const void* pv, const void* pk_scale,
+                  const void* pv_scale, int64_t prefixes, int64_t prefix_max_len,
+                  const int64_t* prefix_len, const int64_t* prefix_of, int64_t window,
+                  float scale, void* out, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

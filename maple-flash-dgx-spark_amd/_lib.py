@@ -103,6 +103,13 @@ _SIGNATURES = {
     "ma_verify_tree_workspace_bytes": [_L, _L, _L, _I],
     "ma_verify_tree": [_P, _I, _L, _L, _L, _L, _L, _P, _P, _P, _P, _I, _L, _L, _I, _D, _D, _P, _Z, _P, _P, _P,
                        _P],
+    "ma_quant_qkv": [_P, _L, _L, _I, _I, _I, _P, _P, _I, _P, _P, _I, _L, _L, _I, _F, _P, _P, _P, _P, _P, _P, _P, _L, _L,
+                     _P, _P],
+    "ma_quant_kv": [_P, _L, _L, _L, _P, _L, _L, _L, _L, _L, _I, _I, _P, _P, _P, _P, _P, _P, _P, _L, _L, _P],
+    "ma_dequant_kv": [_P, _P, _P, _P, _L, _L, _L, _L, _I, _I, _P, _P, _P, _P],
+    "ma_cache_attn_workspace_bytes": [_L, _I, _I, _I, _L, _L, _L, _L],
+    "ma_cache_attn": [_P, _L, _I, _I, _I, _P, _P, _P, _P, _L, _L, _P, _P, _P, _P, _P, _P, _L, _L, _P, _P, _L, _F, _P,
+                      _P, _Z, _P],
     "ma_tree_fit": [_P, _I, _L, _L, _P, _L, _P, _P],
     "ma_tree_commit": [_P, _P, _L, _L, _L, _I, _I, _L, _L, _P, _P, _P, _P, _P, _P],
 }
@@ -113,7 +120,8 @@ _RESTYPES = {"ma_last_error": ctypes.c_char_p, "ma_router_workspace_bytes": _Z,
              "ma_moe_grouped_noalloc_max_bytes": _Z, "ma_sampler_workspace_bytes": _Z,
              "ma_flash_head_workspace_bytes": _Z, "ma_rtn4_gemv_workspace_bytes": _Z,
              "ma_rtn4_gemv_mx_workspace_bytes": _Z, "ma_ternary_gemv_call_workspace_bytes": _Z,
-             "ma_tree_attn_workspace_bytes": _Z, "ma_verify_tree_workspace_bytes": _Z}
+             "ma_tree_attn_workspace_bytes": _Z, "ma_verify_tree_workspace_bytes": _Z,
+             "ma_cache_attn_workspace_bytes": _Z}
 
 _lib = None
 

@@ -1,0 +1,335 @@
+// Writing and reading a quantised KV cache (quant.h; gfx950): one token a row
+// from its QKV projection (ma_quant_qkv), prompts' K and V (ma_quant_kv) and
+// cached positions back as bf16 (ma_dequant_kv).  A position outside the cache is
+// not written, a mapped row outside it is clamped.
+
+#include "qkv_rows.h"
+#include "quant.h"
+
+namespace ma {
+
+struct QuantCache {
+  uint8_t* k;
+  uint8_t* v;
+  uint8_t* ks;
+  uint8_t* vs;
+  int64_t rows;
+  int64_t max_len;
+};
+
+constexpr int kQuantThreads = 256;
+
+// ---------------------------------------------------------------------------
+// QK RMSNorm + rotary positions + quantising store of one token a row
+// ---------------------------------------------------------------------------
+// A thread per 8 dims of a (row, head), as in k_tree_qkv (norm_turn): q heads go
+// out as bf16, k heads are rounded to bf16 (what a bf16 cache would hold, so both
+// ways of filling a cache give one set of codes) and quantised with their largest
+// value over the HD / 8 lanes of the head, v heads quantised as they are.
+// VEC: all rows are 16-byte aligned.
+template <int HD, bool VEC>
+__global__ __launch_bounds__(kQuantThreads) void k_quant_qkv(
+    const uint16_t* __restrict__ qkv, int64_t ldb, int64_t batch, const void* __restrict__ q_w,
+    const void* __restrict__ k_w, int w_dt, RopeTab rope, float eps, const int64_t* __restrict__ seqlen,
+    const int64_t* __restrict__ positions, const int64_t* __restrict__ row_map, QuantCache cache, int nq, int nkv,
+    uint16_t* __restrict__ q_out) {
+  constexpr int LPH = HD / 8;
+  __shared__ __align__(16) float ys[kQuantThreads * 8];
+  const int tid = threadIdx.x;
+  const int heads = nq + 2 * nkv;
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * kQuantThreads + tid;
+  const bool on = item < batch * heads * LPH;
+  const int l = tid % LPH, d0 = 8 * l;
+  const int64_t hd = on ? item / LPH : 0;
+  const int64_t b = hd / heads;
+  const int hs = static_cast<int>(hd - b * heads);
+  const bool is_q = hs < nq, is_v = hs >= nq + nkv;
+  const uint16_t* const x_row = qkv + b * ldb + static_cast<int64_t>(hs) * HD + d0;
+  uint4 xv = make_uint4(0u, 0u, 0u, 0u);
+  if constexpr (VEC) {
+    xv = *reinterpret_cast<const uint4*>(x_row);
+  } else {
+    uint16_t xs[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) xs[e] = x_row[e];
+    xv = make_uint4(xs[0] | static_cast<uint32_t>(xs[1]) << 16, xs[2] | static_cast<uint32_t>(xs[3]) << 16,
+                    xs[4] | static_cast<uint32_t>(xs[5]) << 16, xs[6] | static_cast<uint32_t>(xs[7]) << 16);
+  }
+  Eight wr{};
+  if (q_w) ld_eight<VEC>(wr, is_q ? q_w : k_w, w_dt, d0);
+  const int64_t slot = seqlen[b];
+  const int64_t at = positions ? positions[b] : slot;
+  const int64_t crow = row_map ? clamp_pos(row_map[b], 0, cache.rows - 1) : b;
+  MA_ISSUE_FENCE();
+  const bool turn = rope.mode && rope.rot > 0;
+  Eight cr{}, sr{};
+  if (turn) {
+    const int64_t row = clamp_pos(at, 0, rope.n_pos - 1) * rope.ld;
+    ld_turns<VEC>(cr, rope.cos, rope.dt, row, d0, rope.rot, rope.mode);
+    ld_turns<VEC>(sr, rope.sin, rope.dt, row, d0, rope.rot, rope.mode);
+  }
+  float y[8];
+  of_bf16x8(y, xv);
+  norm_turn<HD, VEC>(y, q_w != nullptr, !is_v, wr, w_dt, turn, cr, sr, rope, eps, ys, tid);
+  uint4 r = make_uint4(pack_bf16x2_rn(y[0], y[1]), pack_bf16x2_rn(y[2], y[3]), pack_bf16x2_rn(y[4], y[5]),
+                       pack_bf16x2_rn(y[6], y[7]));
+  if (is_v) r = xv;  // (the bits as they are)
+  int top = finite_top(finite_top(finite_top(finite_top(0, r.x), r.y), r.z), r.w);
+  top = group_top<LPH>(top);
+  if (!on) return;
+  if (is_q) {
+    if (slot < 0) r = make_uint4(0u, 0u, 0u, 0u);  // no sequence in the row
+    *reinterpret_cast<uint4*>(q_out + (b * nq + hs) * HD + d0) = r;
+    return;
+  }
+  if (slot < 0 || slot >= cache.max_len) return;
+  const int byte = quant_byte(top);
+  const float inv = quant_inverse(byte);
+  const int64_t to = (crow * nkv + (hs - nq) % nkv) * cache.max_len + slot;
+  *reinterpret_cast<uint2*>((is_v ? cache.v : cache.k) + to * HD + d0) =
+      make_uint2(quant_four(r.x, r.y, inv), quant_four(r.z, r.w, inv));
+  if (l == 0) (is_v ? cache.vs : cache.ks)[to] = static_cast<uint8_t>(byte);
+}
+
+// ---------------------------------------------------------------------------
+// Prompts in
+// ---------------------------------------------------------------------------
+struct KvRows {  // bf16 [batch, n_kv, T, HD], the last dim contiguous
+  const uint16_t* p;
+  int64_t sb, sh, st;
+};
+
+constexpr int kQuantRows = 4;  // rows a thread has in flight
+
+// HD / 16 lanes a row of 16 dims each, kQuantRows rows a thread; blockIdx.y: K or
+// V.  HEADS_IN: a batch row's heads lie next to each other (positions before heads,
+// as a projection leaves them), so they are walked first; else positions are.
+template <int HD, bool HEADS_IN, bool VEC>
+__global__ __launch_bounds__(kQuantThreads) void k_quant_kv(KvRows kr, KvRows vr, int64_t total, int64_t T, int nkv,
+                                                            const int64_t* __restrict__ start,
+                                                            const int64_t* __restrict__ lengths,
+                                                            const int64_t* __restrict__ row_map, QuantCache cache) {
+  constexpr int LPR = HD / 16, RPB = kQuantThreads / LPR;
+  const int tid = threadIdx.x, l = tid % LPR;
+  const bool is_v = blockIdx.y != 0;
+  const KvRows src = is_v ? vr : kr;
+  uint4 x[kQuantRows][2];
+  int64_t to[kQuantRows];
+#pragma unroll
+  for (int i = 0; i < kQuantRows; ++i) {
+    const int64_t r = (static_cast<int64_t>(blockIdx.x) * kQuantRows + i) * RPB + tid / LPR;
+    to[i] = -1;
+    x[i][0] = x[i][1] = make_uint4(0u, 0u, 0u, 0u);
+    if (r >= total) continue;
+    const int64_t per = T * nkv, b = r / per, rest = r - b * per;
+    const int64_t h = HEADS_IN ? rest % nkv : rest / T, t = HEADS_IN ? rest / nkv : rest % T;
+    const int64_t p = (start ? start[b] : 0) + t;
+    if ((lengths && t >= lengths[b]) || p < 0 || p >= cache.max_len) continue;
+    to[i] = ((row_map ? clamp_pos(row_map[b], 0, cache.rows - 1) : b) * nkv + h) * cache.max_len + p;
+    const uint16_t* const s = src.p + b * src.sb + h * src.sh + t * src.st + 16 * l;
+    if constexpr (VEC) {
+      x[i][0] = reinterpret_cast<const uint4*>(s)[0];
+      x[i][1] = reinterpret_cast<const uint4*>(s)[1];
+    } else {
+      uint32_t w[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w[e] = s[2 * e] | static_cast<uint32_t>(s[2 * e + 1]) << 16;
+      x[i][0] = make_uint4(w[0], w[1], w[2], w[3]);
+      x[i][1] = make_uint4(w[4], w[5], w[6], w[7]);
+    }
+  }
+  uint8_t* const codes = is_v ? cache.v : cache.k;
+  uint8_t* const scales = is_v ? cache.vs : cache.ks;
+#pragma unroll
+  for (int i = 0; i < kQuantRows; ++i) {
+    int top = 0;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      top = finite_top(finite_top(finite_top(finite_top(top, x[i][j].x), x[i][j].y), x[i][j].z), x[i][j].w);
+    top = group_top<LPR>(top);
+    if (to[i] < 0) continue;
+    const int byte = quant_byte(top);
+    const float inv = quant_inverse(byte);
+    *reinterpret_cast<uint4*>(codes + to[i] * HD + 16 * l) =
+        make_uint4(quant_four(x[i][0].x, x[i][0].y, inv), quant_four(x[i][0].z, x[i][0].w, inv),
+                   quant_four(x[i][1].x, x[i][1].y, inv), quant_four(x[i][1].z, x[i][1].w, inv));
+    if (l == 0) scales[to[i]] = static_cast<uint8_t>(byte);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Cached positions back
+// ---------------------------------------------------------------------------
+// HD / 16 lanes a row of 16 codes each.  A value is exact in bf16 (e4m3 has four
+// significant bits) unless 2^e takes it below bf16's least normal.
+template <int HD>
+__global__ __launch_bounds__(kQuantThreads) void k_dequant_kv(QuantCache cache, int64_t total, int64_t length, int nkv,
+                                                              const int64_t* __restrict__ row_map,
+                                                              uint16_t* __restrict__ k_out,
+                                                              uint16_t* __restrict__ v_out) {
+  constexpr int LPR = HD / 16, RPB = kQuantThreads / LPR;
+  const int tid = threadIdx.x, l = tid % LPR;
+  const bool is_v = blockIdx.y != 0;
+  const uint8_t* const codes = is_v ? cache.v : cache.k;
+  const uint8_t* const scales = is_v ? cache.vs : cache.ks;
+  uint16_t* const out = is_v ? v_out : k_out;
+  uint4 c[kQuantRows];
+  int byte[kQuantRows];
+  int64_t row[kQuantRows];
+#pragma unroll
+  for (int i = 0; i < kQuantRows; ++i) {
+    const int64_t r = (static_cast<int64_t>(blockIdx.x) * kQuantRows + i) * RPB + tid / LPR;
+    row[i] = r < total ? r : -1;
+    const int64_t q = r < total ? r : 0;
+    const int64_t pair = q / length, b = pair / nkv, h = pair - b * nkv;
+    const int64_t at = ((row_map ? clamp_pos(row_map[b], 0, cache.rows - 1) : b) * nkv + h) * cache.max_len +
+                       (q - pair * length);
+    c[i] = *reinterpret_cast<const uint4*>(codes + at * HD + 16 * l);
+    byte[i] = scales[at];
+  }
+  MA_ISSUE_FENCE();
+  typedef float f32x2q_t __attribute__((ext_vector_type(2)));
+#pragma unroll
+  for (int i = 0; i < kQuantRows; ++i) {
+    if (row[i] < 0) continue;
+    const float s = quant_scale(byte[i]);
+    const uint32_t w[4] = {c[i].x, c[i].y, c[i].z, c[i].w};
+    uint32_t o[8];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const f32x2q_t a = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(w[j]), false);
+      const f32x2q_t b = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(w[j]), true);
+      o[2 * j] = pack_bf16x2_rn(a.x * s, a.y * s);
+      o[2 * j + 1] = pack_bf16x2_rn(b.x * s, b.y * s);
+    }
+    uint4* const to = reinterpret_cast<uint4*>(out + row[i] * HD + 16 * l);
+    to[0] = make_uint4(o[0], o[1], o[2], o[3]);
+    to[1] = make_uint4(o[4], o[5], o[6], o[7]);
+  }
+}
+
+}  // namespace ma
+
+using namespace ma;
+
+namespace {
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+int check_quant(const char* what, int64_t batch, int n_kv_heads, int head_dim, const void* k, const void* v,
+                const void* ks, const void* vs, int64_t cache_rows, int64_t max_len, const void* row_map) {
+  if (head_dim != 64 && head_dim != 128) return fail(MA_EVALUE, "%s: head_dim %d unsupported (64 or 128)", what, head_dim);
+  if (batch < 0 || n_kv_heads < 1 || n_kv_heads > 65535) return fail(MA_EVALUE, "%s: bad sizes", what);
+  if (batch == 0) return MA_OK;
+  if (max_len < 1 || cache_rows < 1 || (!row_map && batch > cache_rows)) return fail(MA_EVALUE, "%s: bad cache sizes", what);
+  if (!k || !v || !ks || !vs) return fail(MA_EVALUE, "%s: null pointer", what);
+  if (!aligned16(k) || !aligned16(v)) return fail(MA_EVALUE, "%s: the codes must be 16-byte aligned", what);
+  return MA_OK;
+}
+
+}  // namespace
+
+extern "C" int ma_quant_qkv(const void* qkv, int64_t ldb, int64_t batch, int n_heads, int n_kv_heads, int head_dim,
+                            const void* q_norm_w, const void* k_norm_w, int w_dtype, const void* cos, const void* sin,
+                            int cs_dtype, int64_t ld_cs, int64_t n_pos, int rotary_dim, float eps,
+                            const int64_t* seqlen, const int64_t* positions, const int64_t* row_map, void* k_codes,
+                            void* v_codes, void* k_scale, void* v_scale, int64_t cache_rows, int64_t max_len,
+                            void* q_out, void* stream) {
+  const char* what = "quant_qkv";
+  if (int rc = check_quant(what, batch, n_kv_heads, head_dim, k_codes, v_codes, k_scale, v_scale, cache_rows, max_len, row_map))
+    return rc;
+  if (n_heads < n_kv_heads || n_heads % n_kv_heads != 0 || n_heads > 65535)
+    return fail(MA_EVALUE, "%s: %d query heads over %d KV heads", what, n_heads, n_kv_heads);
+  if (ldb < static_cast<int64_t>(n_heads + 2 * n_kv_heads) * head_dim) return fail(MA_EVALUE, "%s: qkv row stride too small", what);
+  if (rotary_dim < 0 || rotary_dim > head_dim || rotary_dim % 2 != 0)
+    return fail(MA_EVALUE, "%s: rotary_dim %d must be even and at most head_dim", what, rotary_dim);
+  if (rotary_dim > 0 && (!cos || !sin || n_pos < 1 || ld_cs < rotary_dim))
+    return fail(MA_EVALUE, "%s: the cos / sin tables need %d columns and a row", what, rotary_dim);
+  for (const int dt : {w_dtype, cs_dtype})
+    if (dt != MA_F32 && dt != MA_BF16 && dt != MA_F16) return fail(MA_ETYPE, "%s: dtype %d unsupported", what, dt);
+  if ((q_norm_w == nullptr) != (k_norm_w == nullptr)) return fail(MA_EVALUE, "%s: one norm weight without the other", what);
+  if (batch == 0) return MA_OK;
+  if (!qkv || !seqlen || !q_out) return fail(MA_EVALUE, "%s: null pointer", what);
+  if (!aligned16(q_out)) return fail(MA_EVALUE, "%s: q_out must be 16-byte aligned", what);
+  const int64_t blocks = cdiv(batch * (n_heads + 2 * n_kv_heads) * (head_dim / 8), kQuantThreads);
+  if (batch > (1 << 24) || blocks > INT32_MAX) return fail(MA_EVALUE, "%s: batch too large for one launch", what);
+  const RopeTab rope{cos, sin, cs_dtype, ld_cs, n_pos, rotary_dim, rotary_dim > 0 ? 1 : 0};
+  const QuantCache cache{static_cast<uint8_t*>(k_codes), static_cast<uint8_t*>(v_codes), static_cast<uint8_t*>(k_scale),
+                         static_cast<uint8_t*>(v_scale), cache_rows, max_len};
+  // 16-byte loads throughout: rows aligned, and the rotary part ends with a lane's dims
+  const bool rope_vec = rotary_dim == 0 || (aligned16(cos) && aligned16(sin) && rotary_dim % 8 == 0 &&
+                                            ld_cs * (cs_dtype == MA_F32 ? 4 : 2) % 16 == 0);
+  const bool vec = aligned16(qkv) && ldb % 8 == 0 && rope_vec && aligned16(q_norm_w) && aligned16(k_norm_w);
+  auto go = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kQuantThreads), 0, static_cast<hipStream_t>(stream),
+                       static_cast<const uint16_t*>(qkv), ldb, batch, q_norm_w, k_norm_w, w_dtype, rope, eps, seqlen,
+                       positions, row_map, cache, n_heads, n_kv_heads, static_cast<uint16_t*>(q_out));
+  };
+  if (head_dim == 64) vec ? go(k_quant_qkv<64, true>) : go(k_quant_qkv<64, false>);
+  else vec ? go(k_quant_qkv<128, true>) : go(k_quant_qkv<128, false>);
+  return check_launch(what);
+}
+
+extern "C" int ma_quant_kv(const void* k, int64_t k_sb, int64_t k_sh, int64_t k_st, const void* v, int64_t v_sb,
+                           int64_t v_sh, int64_t v_st, int64_t batch, int64_t T, int n_kv_heads, int head_dim,
+                           const int64_t* start, const int64_t* lengths, const int64_t* row_map, void* k_codes,
+                           void* v_codes, void* k_scale, void* v_scale, int64_t cache_rows, int64_t max_len,
+                           void* stream) {
+  const char* what = "quant_kv";
+  if (int rc = check_quant(what, batch, n_kv_heads, head_dim, k_codes, v_codes, k_scale, v_scale, cache_rows, max_len, row_map))
+    return rc;
+  if (T < 0) return fail(MA_EVALUE, "%s: bad sizes", what);
+  if (batch == 0 || T == 0) return MA_OK;
+  if (!k || !v) return fail(MA_EVALUE, "%s: null pointer", what);
+  const int64_t rpb = kQuantThreads / (head_dim / 16) * kQuantRows;
+  if (batch > (int64_t{1} << 31) || T > (int64_t{1} << 31) / batch || cdiv(batch * T * n_kv_heads, rpb) > INT32_MAX)
+    return fail(MA_EVALUE, "%s: batch x positions too large for one launch", what);
+  const int64_t total = batch * T * n_kv_heads;
+  const QuantCache cache{static_cast<uint8_t*>(k_codes), static_cast<uint8_t*>(v_codes), static_cast<uint8_t*>(k_scale),
+                         static_cast<uint8_t*>(v_scale), cache_rows, max_len};
+  const KvRows kr{static_cast<const uint16_t*>(k), k_sb, k_sh, k_st}, vr{static_cast<const uint16_t*>(v), v_sb, v_sh, v_st};
+  const bool vec = aligned16(k) && aligned16(v) && (k_sb | k_sh | k_st | v_sb | v_sh | v_st) % 8 == 0;
+  const bool heads_in = k_sh < k_st;
+  const dim3 grid(static_cast<unsigned>(cdiv(total, rpb)), 2);
+  auto go = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, grid, dim3(kQuantThreads), 0, static_cast<hipStream_t>(stream), kr, vr, total, T,
+                       n_kv_heads, start, lengths, row_map, cache);
+  };
+  if (head_dim == 64) {
+    if (vec) heads_in ? go(k_quant_kv<64, true, true>) : go(k_quant_kv<64, false, true>);
+    else go(k_quant_kv<64, false, false>);
+  } else {
+    if (vec) heads_in ? go(k_quant_kv<128, true, true>) : go(k_quant_kv<128, false, true>);
+    else go(k_quant_kv<128, false, false>);
+  }
+  return check_launch(what);
+}
+
+extern "C" int ma_dequant_kv(const void* k_codes, const void* v_codes, const void* k_scale, const void* v_scale,
+                             int64_t cache_rows, int64_t max_len, int64_t batch, int64_t length, int n_kv_heads,
+                             int head_dim, const int64_t* row_map, void* k_out, void* v_out, void* stream) {
+  const char* what = "dequant_kv";
+  if (int rc = check_quant(what, batch, n_kv_heads, head_dim, k_codes, v_codes, k_scale, v_scale, cache_rows, max_len, row_map))
+    return rc;
+  if (length < 0 || (batch > 0 && length > max_len))
+    return fail(MA_EVALUE, "%s: %lld positions of a cache of %lld", what, static_cast<long long>(length),
+                static_cast<long long>(max_len));
+  if (batch == 0 || length == 0) return MA_OK;
+  if (!k_out || !v_out || !aligned16(k_out) || !aligned16(v_out))
+    return fail(MA_EVALUE, "%s: the outputs must be there and 16-byte aligned", what);
+  const int64_t rpb = kQuantThreads / (head_dim / 16) * kQuantRows;
+  if (batch > (int64_t{1} << 31) || length > (int64_t{1} << 31) / batch ||
+      cdiv(batch * length * n_kv_heads, rpb) > INT32_MAX)
+    return fail(MA_EVALUE, "%s: batch x positions too large for one launch", what);
+  const int64_t total = batch * length * n_kv_heads;
+  auto u8 = [](const void* p) { return const_cast<uint8_t*>(static_cast<const uint8_t*>(p)); };
+  const QuantCache cache{u8(k_codes), u8(v_codes), u8(k_scale), u8(v_scale), cache_rows, max_len};
+  const dim3 grid(static_cast<unsigned>(cdiv(total, rpb)), 2);
+  auto go = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, grid, dim3(kQuantThreads), 0, static_cast<hipStream_t>(stream), cache, total, length,
+                       n_kv_heads, row_map, static_cast<uint16_t*>(k_out), static_cast<uint16_t*>(v_out));
+  };
+  if (head_dim == 64) go(k_dequant_kv<64>);
+  else go(k_dequant_kv<128>);
+  return check_launch(what);
+}

@@ -7,6 +7,7 @@
 
 #include <math.h>
 
+#include "qkv_rows.h"
 #include "tree.h"
 
 namespace ma {
@@ -15,91 +16,9 @@ typedef __bf16 bf16x8t_t __attribute__((ext_vector_type(8)));
 typedef float f32x16t_t __attribute__((ext_vector_type(16)));
 typedef short s16x4t_t __attribute__((ext_vector_type(4)));
 
-__device__ __forceinline__ int64_t clamp_pos(int64_t v, int64_t lo, int64_t hi) { return v < lo ? lo : (v > hi ? hi : v); }
-
 // ---------------------------------------------------------------------------
 // QK RMSNorm + rotary positions + K/V store
 // ---------------------------------------------------------------------------
-struct TreeRope {
-  const void* cos;
-  const void* sin;
-  int dt;
-  int64_t ld;
-  int64_t n_pos;
-  int rot;
-  int mode;  // 0 none, 1 half layout, 2 interleaved
-};
-
-// Eight consecutive elements of a float32, bf16 or f16 array from element i, as
-// loads without a dtype branch around them (a branch would put the wait for a
-// load right behind it) and their conversion.  VEC: i's bytes are 16-byte
-// aligned; else element by element.
-struct Eight {
-  uint4 lo, hi;  // VEC: the bytes (hi: the upper four float32)
-  AnyWord w[8];  // else
-};
-template <bool VEC>
-__device__ __forceinline__ void ld_eight(Eight& r, const void* p, int dt, int64_t i) {
-  if constexpr (VEC) {
-    const uint4* const a = reinterpret_cast<const uint4*>(static_cast<const char*>(p) + i * (dt == MA_F32 ? 4 : 2));
-    r.lo = a[0];
-    if (dt == MA_F32) r.hi = a[1];
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) r.w[e] = ld_any_word(p, dt, i + e);
-  }
-}
-template <bool VEC>
-__device__ __forceinline__ void of_eight(float (&f)[8], const Eight& r, int dt) {
-  if constexpr (VEC) {
-    const uint32_t u[8] = {r.lo.x, r.lo.y, r.lo.z, r.lo.w, r.hi.x, r.hi.y, r.hi.z, r.hi.w};
-    if (dt == MA_F32) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(u[e]);
-    } else if (dt == MA_BF16) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(e & 1 ? u[e / 2] & 0xffff0000u : u[e / 2] << 16);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] = from_raw<MA_F16>((u[e / 2] >> (16 * (e & 1))) & 0xffffu);
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = any_word_f(r.w[e], dt);
-  }
-}
-// The table columns that dims d0 .. +7 turn by, d0 < rot counted (others read
-// column 0 and are not used): half layout columns d0 .. +7; interleaved columns
-// d0 / 2 .. +3, then the same + rot / 2.
-template <bool VEC>
-__device__ __forceinline__ void ld_turns(Eight& r, const void* p, int dt, int64_t row, int d0, int rot, int mode) {
-  const int half = rot / 2;
-  if constexpr (VEC) {  // (rot is a multiple of 8: a lane's dims all turn or none does)
-    const int d = d0 < rot ? d0 : 0;
-    if (mode == 1) {
-      ld_eight<true>(r, p, dt, row + d);
-      return;
-    }
-    const int es = dt == MA_F32 ? 4 : 2;
-    const char* const a = static_cast<const char*>(p) + (row + d / 2) * es;
-    const char* const b = a + half * es;
-    if (dt == MA_F32) {
-      r.lo = *reinterpret_cast<const uint4*>(a);
-      r.hi = *reinterpret_cast<const uint4*>(b);
-    } else {
-      const uint2 a0 = *reinterpret_cast<const uint2*>(a), b0 = *reinterpret_cast<const uint2*>(b);
-      r.lo = make_uint4(a0.x, a0.y, b0.x, b0.y);
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int pair = d0 / 2 + (e & 3);
-      const int col = mode == 1 ? (d0 + e < rot ? d0 + e : 0) : (pair < half ? pair + (e < 4 ? 0 : half) : 0);
-      r.w[e] = ld_any_word(p, dt, row + col);
-    }
-  }
-}
-
 constexpr int kQkvThreads = 256;
 
 // A thread per 8 dims of a (node, head): q heads, then k heads, then v heads of
@@ -118,7 +37,7 @@ constexpr int kQkvThreads = 256;
 template <int HD, bool VEC>
 __global__ __launch_bounds__(kQkvThreads) void k_tree_qkv(
     const uint16_t* __restrict__ qkv, int64_t ldb, int64_t ldt, int nodes, const void* __restrict__ q_w,
-    const void* __restrict__ k_w, int w_dt, TreeRope rope, float eps, const int64_t* __restrict__ seqlen,
+    const void* __restrict__ k_w, int w_dt, RopeTab rope, float eps, const int64_t* __restrict__ seqlen,
     const int32_t* __restrict__ parents, const int64_t* __restrict__ row_map, uint16_t* __restrict__ k_cache,
     uint16_t* __restrict__ v_cache, int64_t cache_rows, int64_t max_len, int nq, int nkv,
     uint16_t* __restrict__ q_out) {
@@ -152,7 +71,6 @@ __global__ __launch_bounds__(kQkvThreads) void k_tree_qkv(
   const int depth = __shfl(tree_depth(par, nodes), node, 64);
   // the table's row
   const bool turn = rope.mode && rope.rot > 0;
-  const int half = rope.rot / 2;
   Eight cr{}, sr{};
   if (turn) {
     const int64_t pos = n0 + (depth > 0 ? depth : 0);
@@ -161,53 +79,11 @@ __global__ __launch_bounds__(kQkvThreads) void k_tree_qkv(
     ld_turns<VEC>(sr, rope.sin, rope.dt, row, d0, rope.rot, rope.mode);
   }
   float y[8];
-  {
-    const uint32_t u[4] = {xv.x, xv.y, xv.z, xv.w};
-    float sq = 0.f;
+  if constexpr (VEC) of_bf16x8(y, xv);
+  else
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      y[e] = VEC ? __uint_as_float(e & 1 ? u[e / 2] & 0xffff0000u : u[e / 2] << 16) : bf16_to_f32(xs[e]);
-      sq += y[e] * y[e];
-    }
-    if (q_w) {
-      const float inv = rsqrtf(group_sum<LPH>(sq) / HD + eps);
-      float w[8];
-      of_eight<VEC>(w, wr, w_dt);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = is_v ? y[e] : y[e] * inv * w[e];
-    }
-  }
-  if (turn) {
-    float other[8];
-    if (rope.mode == 1) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) ys[tid * 8 + e] = y[e];
-      __syncthreads();
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int d = d0 + e;
-        const int pd = d < half ? d + half : d - half;
-        other[e] = ys[(tid - l) * 8 + (d < rope.rot ? pd : d)];
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) other[e] = y[e ^ 1];
-    }
-    float c[8], s[8];
-    of_eight<VEC>(c, cr, rope.dt);
-    of_eight<VEC>(s, sr, rope.dt);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int d = d0 + e;
-      const bool lo = rope.mode == 2 ? !(e & 1) : d < half;
-      const float ce = bf16_to_f32(f32_to_bf16(rope.mode == 2 ? c[(e >> 1) + 4 * (e & 1)] : c[e]));
-      const float se = bf16_to_f32(f32_to_bf16(rope.mode == 2 ? s[(e >> 1) + 4 * (e & 1)] : s[e]));
-      const float r = lo ? y[e] * ce - other[e] * se : y[e] * ce + other[e] * se;
-      other[e] = d < rope.rot && !is_v ? r : y[e];
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) y[e] = other[e];
-  }
+    for (int e = 0; e < 8; ++e) y[e] = bf16_to_f32(xs[e]);
+  norm_turn<HD, VEC>(y, q_w != nullptr, !is_v, wr, w_dt, turn, cr, sr, rope, eps, ys, tid);
   if (!on) return;
   const int64_t slot = n0 + node;
   if (!is_q && (depth < 0 || slot >= max_len)) return;
@@ -975,7 +851,7 @@ extern "C" int ma_tree_qkv(const void* qkv, int64_t ldb, int64_t ldt, int64_t ba
   if (!qkv || !seqlen || !parents || !k_cache || !v_cache || !q_out) return fail(MA_EVALUE, "tree_qkv: null pointer");
   if (!aligned16(k_cache) || !aligned16(v_cache) || !aligned16(q_out))
     return fail(MA_EVALUE, "tree_qkv: the cache and q_out must be 16-byte aligned");
-  const TreeRope rope{cos, sin, cs_dtype, ld_cs, n_pos, rotary_dim, rope_mode};
+  const RopeTab rope{cos, sin, cs_dtype, ld_cs, n_pos, rotary_dim, rope_mode};
   // 16-byte loads throughout: rows aligned, and the rotary part ends with a lane's dims
   const int es = cs_dtype == MA_F32 ? 4 : 2;
   const bool rope_vec = !rope_mode || rotary_dim == 0 ||
