@@ -17,10 +17,18 @@ typedef __bf16 bf16x2c_t __attribute__((ext_vector_type(2)));
 typedef float f32x4c_t __attribute__((ext_vector_type(4)));
 typedef float f32x16c_t __attribute__((ext_vector_type(16)));
 typedef short s16x4c_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4c_t __attribute__((ext_vector_type(4)));  // (uint4, a class, keeps arrays of it in scratch memory)
 
 constexpr int kCacheThreads = 256;
+constexpr int kCacheWaves = kCacheThreads / 64;
+constexpr int kPrefixRows = 32;     // query rows of a workgroup on a shared prefix
+constexpr int kMaxShared = 64;      // prefixes that are read once for all of their rows: a lane each
 constexpr int kCacheGroup = 16;     // query heads per KV head at most
 constexpr float kCacheGrow = 8.0f;  // a row's reference moves when a score passes it by 2^8
+constexpr float kCacheSum = 65536.f;  // or, in a shared prefix, when a lane's sum passes this
+// References of this size are no longer close to the unrounded products (half a
+// step is 2^3 here): from here on products are rounded too.
+constexpr float kCacheFar = 134217728.f;  // 2^27
 
 struct CacheIn {
   const uint8_t* k;   // e4m3 codes or bf16
@@ -90,11 +98,31 @@ __device__ __forceinline__ f32x16c_t mfma32(uint4 a, uint4 b, f32x16c_t c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8c_t, a), __builtin_bit_cast(bf16x8c_t, b), c, 0, 0, 0);
 }
 
+// 16 bytes of a tile's 32 V rows a lane, into the wave's LDS rows as bf16.  s_of(row):
+// the row's scale (quantised).
+template <int HD, bool Q8, int VL, typename S>
+__device__ __forceinline__ void lay_v(char* vb, const u32x4c_t (&v)[VL], S&& s_of) {
+  constexpr int PPR = Q8 ? HD / 16 : HD / 8;  // such pieces of a row
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int i = 0; i < VL; ++i) {
+    const int at = i * 64 + lane, row = at / PPR, c = at % PPR;
+    char* const to = vb + row * 2 * HD;
+    if constexpr (Q8) {
+      const float s = s_of(row);
+      *reinterpret_cast<uint4*>(to + (((2 * c) ^ cache_key(row)) << 4)) = codes_bf16(v[i].x, v[i].y, s);
+      *reinterpret_cast<uint4*>(to + (((2 * c + 1) ^ cache_key(row)) << 4)) = codes_bf16(v[i].z, v[i].w, s);
+    } else {
+      *reinterpret_cast<u32x4c_t*>(to + ((c ^ cache_key(row)) << 4)) = v[i];
+    }
+  }
+}
+
 // ---------------------------------------------------------------------------
 // A row's own positions
 // ---------------------------------------------------------------------------
-// Workgroup: a split of the positions of (row b, KV head); its four waves take
-// every fourth tile of 32 positions, each on its own, and join at the end.  On
+// Workgroup: a split of the positions of (row b, KV head); its waves
+// take tiles of 32 positions in turn, each on its own, and join at the end.  On
 // v_mfma_f32_16x16x32_bf16 (A lane l: row l % 16, k 8 (l / 16)..+8; B: col l % 16,
 // the same k; C: col l % 16, rows 4 (l / 16)..+4):
 //   S^T = K Q^T, K from the cache into registers (a quantised lane's 16 codes are
@@ -105,21 +133,28 @@ __device__ __forceinline__ f32x16c_t mfma32(uint4 a, uint4 b, f32x16c_t c) {
 //   O += P V: A = the lane's own eight P (positions 4g.. of both halves), B = V in
 //     the same order from LDS, where a wave lays its tile as bf16 rows, by the
 //     transposing read.
+template <int HD>
+struct OwnLds {
+  char v[kCacheWaves][32 * 2 * HD];  // a wave's tile of V; at the end the waves' sums
+  float m[kCacheWaves][kCacheGroup], l[kCacheWaves][kCacheGroup];
+};
 template <int HD, bool Q8>
-__global__ __launch_bounds__(kCacheThreads) void k_cache_own(CacheAttn a) {
+__device__ __forceinline__ void cache_own(const CacheAttn& a, int wg, OwnLds<HD>& lds) {
+  constexpr int NW = kCacheWaves;
   constexpr int RB = Q8 ? HD : 2 * HD;      // bytes of a cached position
   constexpr int KL = RB / 64;               // 16-byte loads of K a lane and 16 positions
   constexpr int VL = 32 * RB / 1024;        // of V a lane and tile
   constexpr int KS = HD / 32;               // k slices of a score
   constexpr int NB = HD / 16;               // 16-dim blocks of the output
   constexpr int VB = 2 * HD;                // bytes of an LDS row
-  __shared__ __align__(16) char vt[4][32 * VB];
-  __shared__ float wm[4][kCacheGroup], wl[4][kCacheGroup];
+  auto& vt = lds.v;
+  auto& wm = lds.m;
+  auto& wl = lds.l;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r16 = lane & 15, g = lane >> 4;
-  const int sp = blockIdx.x % a.s_own;
-  const int64_t pair = blockIdx.x / a.s_own, b = pair / a.nkv;
+  const int sp = wg % a.s_own;
+  const int64_t pair = wg / a.s_own, b = pair / a.nkv;
   const int kvh = static_cast<int>(pair - b * a.nkv);
   const int group = a.nq / a.nkv;
   const CacheSpan span = cache_span(a, b);
@@ -130,9 +165,9 @@ __global__ __launch_bounds__(kCacheThreads) void k_cache_own(CacheAttn a) {
   const int64_t a1 = a.s_pre > 0 ? 0 : span.pre_n;
   const int64_t b0 = span.lo > span.pre_n ? span.lo - span.pre_n : 0, b1 = span.own_n;
   const int na = static_cast<int>(cdiv(a1 - a0, 32)), nt = na + static_cast<int>(cdiv(b1 - b0, 32));
-  const int fours = (nt + 3) / 4, per = (fours + a.s_own - 1) / a.s_own;
-  const int t_beg = sp * per * 4 < nt ? sp * per * 4 : nt;
-  const int t_end = t_beg + per * 4 < nt ? t_beg + per * 4 : nt;
+  const int rounds = (nt + NW - 1) / NW, per = (rounds + a.s_own - 1) / a.s_own * NW;
+  const int t_beg = sp * per < nt ? sp * per : nt;
+  const int t_end = t_beg + per < nt ? t_beg + per : nt;
 
   uint4 qf[KS];
   {
@@ -146,7 +181,7 @@ __global__ __launch_bounds__(kCacheThreads) void k_cache_own(CacheAttn a) {
     }
   }
   struct Tile {
-    uint4 k[2][KL], v[VL];
+    u32x4c_t k[2][KL], v[VL];
     int scale;  // of position lane % 32: K's, in the upper lanes V's
     int n;
   };
@@ -165,12 +200,12 @@ __global__ __launch_bounds__(kCacheThreads) void k_cache_own(CacheAttn a) {
     for (int h = 0; h < 2; ++h) {
       const int row = 16 * h + r16 < x.n ? 16 * h + r16 : x.n - 1;
 #pragma unroll
-      for (int j = 0; j < KL; ++j) x.k[h][j] = *reinterpret_cast<const uint4*>(kp + row * RB + 64 * j + 16 * g);
+      for (int j = 0; j < KL; ++j) x.k[h][j] = *reinterpret_cast<const u32x4c_t*>(kp + row * RB + 64 * j + 16 * g);
     }
 #pragma unroll
     for (int i = 0; i < VL; ++i) {
       const int at16 = i * 64 + lane, row = at16 / (RB / 16);
-      x.v[i] = *reinterpret_cast<const uint4*>(vp + (row < x.n ? row : x.n - 1) * RB + 16 * (at16 % (RB / 16)));
+      x.v[i] = *reinterpret_cast<const u32x4c_t*>(vp + (row < x.n ? row : x.n - 1) * RB + 16 * (at16 % (RB / 16)));
     }
     if constexpr (Q8) {
       const int row = (lane & 31) < x.n ? lane & 31 : x.n - 1;
@@ -197,19 +232,7 @@ __global__ __launch_bounds__(kCacheThreads) void k_cache_own(CacheAttn a) {
     auto scale_of = [&](int from) {
       return __int_as_float(__builtin_amdgcn_ds_bpermute(4 * from, __float_as_int(s_of)));
     };
-    // V into the wave's rows
-#pragma unroll
-    for (int i = 0; i < VL; ++i) {
-      const int at16 = i * 64 + lane, row = at16 / (RB / 16), c = at16 % (RB / 16);
-      char* const to = vb + row * VB;
-      if constexpr (Q8) {
-        const float s = scale_of(32 + row);
-        *reinterpret_cast<uint4*>(to + (((2 * c) ^ cache_key(row)) << 4)) = codes_bf16(x.v[i].x, x.v[i].y, s);
-        *reinterpret_cast<uint4*>(to + (((2 * c + 1) ^ cache_key(row)) << 4)) = codes_bf16(x.v[i].z, x.v[i].w, s);
-      } else {
-        *reinterpret_cast<uint4*>(to + ((c ^ cache_key(row)) << 4)) = x.v[i];
-      }
-    }
+    lay_v<HD, Q8>(vb, x.v, [&](int row) { return scale_of(32 + row); });
     f32x4c_t sc[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -223,7 +246,7 @@ __global__ __launch_bounds__(kCacheThreads) void k_cache_own(CacheAttn a) {
         }
       } else {
 #pragma unroll
-        for (int j = 0; j < KL; ++j) sc[h] = mfma16(x.k[h][j], qf[j], sc[h]);
+        for (int j = 0; j < KL; ++j) sc[h] = mfma16(__builtin_bit_cast(uint4, x.k[h][j]), qf[j], sc[h]);
       }
     }
     float t[8];
@@ -233,9 +256,11 @@ __global__ __launch_bounds__(kCacheThreads) void k_cache_own(CacheAttn a) {
       asm("" : "+v"(t[i]));  // (rounded, as the reference is, so that the largest weight is 1 at any size: no fused t - m)
     }
     if (x.n < 32) {
+      int mine = x.n - 4 * g;
+      asm volatile("" : "+v"(mine));  // (compared here, not with eight numbers kept in registers)
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        if (16 * (i / 4) + 4 * g + i % 4 >= x.n) t[i] = -INFINITY;
+        if (16 * (i / 4) + i % 4 >= mine) t[i] = -INFINITY;
     }
     float cm = t[0];
 #pragma unroll
@@ -273,17 +298,20 @@ __global__ __launch_bounds__(kCacheThreads) void k_cache_own(CacheAttn a) {
   };
 
   {
-    Tile x[2];
-    int t = t_beg + wv;
-    if (t < t_end) load(x[0], t);
-    for (; t < t_end; t += 8) {
-      if (t + 4 < t_end) load(x[1], t + 4);
-      MA_ISSUE_FENCE();
-      attend(x[0]);
-      if (t + 4 >= t_end) break;
-      if (t + 8 < t_end) load(x[0], t + 8);
-      MA_ISSUE_FENCE();
-      attend(x[1]);
+    // (Loads run past the wave's last tile, on it again: after one that a branch may
+    // have skipped every wait would be for all of them.)
+    const int t0 = t_beg + wv, last = t0 + (t_end - 1 - t0) / NW * NW;
+    if (t0 < t_end) {
+      Tile x0, x1;
+      load(x0, t0);
+      for (int t = t0; t < t_end; t += 2 * NW) {
+        load(x1, t + NW < t_end ? t + NW : last);
+        MA_ISSUE_FENCE();
+        attend(x0);
+        load(x0, t + 2 * NW < t_end ? t + 2 * NW : last);
+        MA_ISSUE_FENCE();
+        if (t + NW < t_end) attend(x1);
+      }
     }
   }
 
@@ -291,7 +319,7 @@ __global__ __launch_bounds__(kCacheThreads) void k_cache_own(CacheAttn a) {
   lsum += MA_SWZ_XOR(lsum, 16);
   lsum += __shfl_xor(lsum, 32, 64);
   float (*ow)[kCacheGroup][HD] = reinterpret_cast<float (*)[kCacheGroup][HD]>(&vt[0][0]);
-  static_assert(sizeof(vt) >= 4 * kCacheGroup * HD * sizeof(float), "the waves' sums");
+  static_assert(sizeof(vt) >= NW * kCacheGroup * HD * sizeof(float), "the waves' sums");
   __syncthreads();
   if (g == 0) {
     wm[wv][r16] = mref;
@@ -306,11 +334,13 @@ __global__ __launch_bounds__(kCacheThreads) void k_cache_own(CacheAttn a) {
   const int st = a.s_own + a.s_pre;
   for (int item = tid; item < group * (HD / 4); item += kCacheThreads) {
     const int hh = item / (HD / 4), d = item % (HD / 4) * 4;
-    const float M = fmaxf(fmaxf(wm[0][hh], wm[1][hh]), fmaxf(wm[2][hh], wm[3][hh]));
+    float M = wm[0][hh];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) M = fmaxf(M, wm[w][hh]);
     float L = 0.f;
     float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < NW; ++w) {
       const float f = wl[w][hh] == 0.f ? 0.f : __builtin_amdgcn_exp2f(wm[w][hh] - M);
       const float4 v = *reinterpret_cast<const float4*>(&ow[w][hh][d]);
       L += f * wl[w][hh];
@@ -322,7 +352,7 @@ __global__ __launch_bounds__(kCacheThreads) void k_cache_own(CacheAttn a) {
     const int64_t row = b * a.nq + kvh * group + hh;
     if (st > 1) {
       const int64_t p = row * st + sp;
-      *reinterpret_cast<float4*>(a.acc + p * HD + d) = s;
+      if (t_beg < t_end) *reinterpret_cast<float4*>(a.acc + p * HD + d) = s;
       if (d == 0) a.ml[p] = make_float2(M, L);
     } else {
       const float inv = L != 0.f ? 1.0f / L : 0.f;
@@ -336,119 +366,149 @@ __global__ __launch_bounds__(kCacheThreads) void k_cache_own(CacheAttn a) {
 // A prefix, for all of its rows
 // ---------------------------------------------------------------------------
 template <int HD>
-struct PrefixTile {
-  static constexpr int kRows = 128;                  // query rows of a workgroup, 32 a wave
-  static constexpr int kStep = HD == 64 ? 64 : 32;   // positions a step
-  static constexpr int kRowBytes = 2 * HD;
-  static constexpr int kRegion = kStep * kRowBytes;  // K or V of a step in LDS, as bf16
+struct PrefixLds {
+  union {
+    char kv[kCacheWaves][2][32 * 2 * HD];      // a wave's tile, K (bf16) and V
+    float sums[kCacheWaves][kPrefixRows][HD];  // at the end
+  };
+  float m[kCacheWaves][kPrefixRows], l[kCacheWaves][kPrefixRows];
+  int mem[kPrefixRows + 1];
+  int count[kCacheWaves];
+  int hist[kMaxShared];
 };
 
-// Workgroup: 128 query rows of (prefix, KV head), row r = (its r / group-th member,
-// query head r % group), and a split of the prefix's positions.  K and V of a step
-// come through registers (converted there) into two LDS buffers that the four
-// waves share.  On v_mfma_f32_32x32x16_bf16 (A lane l: row l % 32, k 8 (l / 32)..+8;
-// B: col l % 32, the same k; C: col l % 32, rows 8 (i / 4) + 4 (l / 32) + i % 4), as
-// k_cache_own otherwise: S^T = K Q^T, P from a reference per row, O += P V.
+// Workgroup: 32 query rows of (prefix, KV head), row r = (its r / group-th member,
+// query head r % group), and a split of the prefix's positions, of which its waves
+// take tiles of 32 in turn, each on its own, and join at the end.  On
+// v_mfma_f32_32x32x16_bf16 (A lane l: row l % 32, k 8 (l / 32)..+8; B: col l % 32,
+// the same k; C: col l % 32, rows 8 (i / 4) + 4 (l / 32) + i % 4), otherwise as
+// cache_own: S^T = K Q^T with K from the cache into registers, P from a reference
+// per row, O += P V with V through the wave's LDS rows.  The reference moves when
+// the weights' sum shows that it has become too low (any that keeps them in range
+// gives the same quotient).
 template <int HD, bool Q8>
-__global__ __launch_bounds__(kCacheThreads, 2) void k_cache_prefix(CacheAttn a, int tiles, int n_units) {
-  using T = PrefixTile<HD>;
-  constexpr int RB = Q8 ? HD : 2 * HD;
-  constexpr int XL = T::kStep * RB / 4096;  // 16-byte loads a thread and step, K and V each
-  constexpr int KS = HD / 16, DB = HD / 32, NT = T::kStep / 32;
-  __shared__ __align__(16) char buf[2][2 * T::kRegion];
-  __shared__ int mem[T::kRows + 1];
-  __shared__ int wcount[4];
+__device__ __forceinline__ void cache_prefix(const CacheAttn& a, int slot, int unit, PrefixLds<HD>& lds) {
+  constexpr int NW = kCacheWaves;
+  constexpr int RB = Q8 ? HD : 2 * HD;   // bytes of a cached position
+  constexpr int XL = 32 * RB / 1024;     // 16-byte loads a lane and tile, K and V each
+  constexpr int KS = HD / 16;            // k slices of a score
+  constexpr int DB = HD / 32;            // 32-dim blocks of the output
+  constexpr int VB = 2 * HD;             // bytes of an LDS row
+  constexpr bool TWO = Q8 || HD == 64;   // two tiles in registers (else they would not fit)
   const int tid = threadIdx.x, lane = tid & 63;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r32 = lane & 31, h = lane >> 5;
-  // tiles of the same positions follow each other on one XCD
-  const int xcd = blockIdx.x % kXcds, turn = blockIdx.x / kXcds;
-  const int tile = turn % tiles, unit = turn / tiles * kXcds + xcd;
-  if (unit >= n_units) return;
-  const int sp = unit % a.s_pre;
-  const int pk = unit / a.s_pre;
-  const int64_t pre = pk / a.nkv;
-  const int kvh = static_cast<int>(pk - pre * a.nkv);
+  const int sp = unit % a.s_pre, kvh = unit / a.s_pre;
   const int group = a.nq / a.nkv;
 
-  // the members that this tile's rows belong to
-  const int first = tile * T::kRows / group, last = (tile * T::kRows + T::kRows - 1) / group;
+  // Which prefix and tile the slot is: the prefixes' tiles follow each other.
+  const int np = static_cast<int>(a.pre.rows);  // (at most 64)
+  const int64_t of0 = a.of[tid < a.batch ? tid : 0];
+  int64_t length = a.length[lane < np ? lane : 0];
+  int pre = 0, tile = slot;
+  if (np > 1) {
+    if (tid < 64) lds.hist[tid] = 0;
+    __syncthreads();
+    for (int b0 = tid; b0 < a.batch; b0 += kCacheThreads) {
+      const int64_t p = b0 == tid ? of0 : a.of[b0];
+      if (p >= 0 && p < np) atomicAdd(&lds.hist[p], 1);
+    }
+    __syncthreads();
+    const int mine = (lds.hist[lane] * group + kPrefixRows - 1) / kPrefixRows;
+    int upto = mine;
+#pragma unroll
+    for (int off = 1; off < 64; off *= 2) {
+      const int below = __shfl_up(upto, off, 64);
+      upto += lane >= off ? below : 0;
+    }
+    const uint64_t past = __ballot(upto > slot);
+    if (past == 0) return;
+    pre = __builtin_ctzll(past);
+    tile = slot - __builtin_amdgcn_readlane(upto - mine, pre);
+    length = __shfl(length, pre, 64);
+  }
+  const int64_t end = clamp_pos(length, 0, a.pre.max_len);
+  const int nt = static_cast<int>(cdiv(end, 32)), rounds = (nt + NW - 1) / NW;
+  const int per = (rounds + a.s_pre - 1) / a.s_pre * NW;
+  const int t_beg = sp * per < nt ? sp * per : nt;
+  const int t_end = t_beg + per < nt ? t_beg + per : nt;
+  const int t0 = t_beg + wv, last = t0 + (t_end - 1 - t0) / NW * NW;
+  const int64_t base = (static_cast<int64_t>(pre) * a.nkv + kvh) * a.pre.max_len;
+
+  struct Tile {
+    u32x4c_t k[XL], v[XL];
+    int scale;  // of position lane % 32: K's, in the upper lanes V's
+    int n;
+  };
+  auto load = [&](Tile& x, int t) {
+    const int64_t at = base + 32 * static_cast<int64_t>(t), left = end - 32 * static_cast<int64_t>(t);
+    x.n = left < 32 ? static_cast<int>(left) : 32;
+    const uint8_t* const kp = a.pre.k + at * RB;
+    const uint8_t* const vp = a.pre.v + at * RB;
+    // (positions past the end read the last one again: their scores are masked)
+    uint32_t off[XL];
+#pragma unroll
+    for (int i = 0; i < XL; ++i) {
+      const int at16 = i * 64 + lane, row = at16 / (RB / 16);
+      off[i] = (row < x.n ? row : x.n - 1) * RB + 16 * (at16 % (RB / 16));
+    }
+    // (K codes as the products take them: 32 bytes of each row at a time)
+    const int mine = r32 < x.n ? r32 : x.n - 1;
+#pragma unroll
+    for (int i = 0; i < XL; ++i)
+      x.k[i] = *reinterpret_cast<const u32x4c_t*>(kp + (Q8 ? static_cast<uint32_t>(mine * RB + 32 * i + 16 * h) : off[i]));
+#pragma unroll
+    for (int i = 0; i < XL; ++i) x.v[i] = *reinterpret_cast<const u32x4c_t*>(vp + off[i]);
+    if constexpr (Q8) x.scale = (lane < 32 ? a.pre.ks : a.pre.vs)[at + mine];
+  };
+  // (Loads run past the wave's last tile, on it again: after one that a branch may
+  // have skipped every wait would be for all of them.)
+  auto at_most = [&](int t) { return t < t_end ? t : last; };
+  Tile x0, x1;
+  if (t0 < t_end) {
+    load(x0, t0);
+    if constexpr (TWO) load(x1, at_most(t0 + NW));
+  }
+  MA_ISSUE_FENCE();
+
+  // the members that this tile's rows belong to, while the first tiles come
+  auto& mem = lds.mem;
+  const int first = tile * kPrefixRows / group, final = (tile * kPrefixRows + kPrefixRows - 1) / group;
   int members = 0;
   for (int b0 = 0; b0 < a.batch; b0 += kCacheThreads) {
-    const bool is = b0 + tid < a.batch && a.of[b0 + tid] == pre;
+    const bool is = b0 + tid < a.batch && (b0 == 0 ? of0 : a.of[b0 + tid]) == pre;
     const uint64_t m = __ballot(is);
-    if (lane == 0) wcount[wv] = static_cast<int>(__popcll(m));
+    if (lane == 0) lds.count[wv] = static_cast<int>(__popcll(m));
     __syncthreads();
     int at = members + static_cast<int>(__popcll(m & ((1ull << lane) - 1)));
-    for (int w = 0; w < wv; ++w) at += wcount[w];
-    if (is && at >= first && at <= last) mem[at - first] = b0 + tid;
-    members += wcount[0] + wcount[1] + wcount[2] + wcount[3];
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      const int n = lds.count[w];
+      at += w < wv ? n : 0;
+      members += n;
+    }
+    if (is && at >= first && at <= final) mem[at - first] = b0 + tid;
     __syncthreads();
   }
   const int M = members * group;
-  if (tile * T::kRows >= M) return;
+  if (tile * kPrefixRows >= M) return;
 
-  const int64_t end = clamp_pos(a.length[pre], 0, a.pre.max_len);
-  const int n_steps = static_cast<int>(cdiv(end, T::kStep)), sps = (n_steps + a.s_pre - 1) / a.s_pre;
-  const int s_beg = sp * sps < n_steps ? sp * sps : n_steps;
-  const int s_end = s_beg + sps < n_steps ? s_beg + sps : n_steps;
-  const int64_t base = (pre * a.nkv + kvh) * a.pre.max_len;
-
-  uint4 xk[XL], xv[XL];
-  int bk = 0, bv = 0;
-  auto load = [&](int s) {
-    const int64_t at = static_cast<int64_t>(s) * T::kStep, left = end - 1 - at;
-    const int most = left < T::kStep ? static_cast<int>(left) : T::kStep - 1;
-#pragma unroll
-    for (int i = 0; i < XL; ++i) {
-      const int p16 = i * kCacheThreads + tid, row = p16 / (RB / 16);
-      const int64_t off = (base + at + (row < most ? row : most)) * RB + 16 * (p16 % (RB / 16));
-      xk[i] = *reinterpret_cast<const uint4*>(a.pre.k + off);
-      xv[i] = *reinterpret_cast<const uint4*>(a.pre.v + off);
-    }
-    if constexpr (Q8) {
-      static_assert(!Q8 || XL == 1, "one position a thread");
-      const int row = tid / (RB / 16);
-      bk = a.pre.ks[base + at + (row < most ? row : most)];
-      bv = a.pre.vs[base + at + (row < most ? row : most)];
-    }
-  };
-  auto store = [&](char* to) {
-#pragma unroll
-    for (int i = 0; i < XL; ++i) {
-      const int p16 = i * kCacheThreads + tid, row = p16 / (RB / 16), c = p16 % (RB / 16);
-      char* const k = to + row * T::kRowBytes;
-      char* const v = k + T::kRegion;
-      if constexpr (Q8) {
-        const float sk = quant_scale(bk), sv = quant_scale(bv);
-        const int c0 = ((2 * c) ^ cache_key(row)) << 4, c1 = ((2 * c + 1) ^ cache_key(row)) << 4;
-        *reinterpret_cast<uint4*>(k + c0) = codes_bf16(xk[i].x, xk[i].y, sk);
-        *reinterpret_cast<uint4*>(k + c1) = codes_bf16(xk[i].z, xk[i].w, sk);
-        *reinterpret_cast<uint4*>(v + c0) = codes_bf16(xv[i].x, xv[i].y, sv);
-        *reinterpret_cast<uint4*>(v + c1) = codes_bf16(xv[i].z, xv[i].w, sv);
-      } else {
-        *reinterpret_cast<uint4*>(k + ((c ^ cache_key(row)) << 4)) = xk[i];
-        *reinterpret_cast<uint4*>(v + ((c ^ cache_key(row)) << 4)) = xv[i];
-      }
-    }
-  };
-  if (s_beg < s_end) load(s_beg);
-
-  const int r = tile * T::kRows + wv * 32 + r32;
-  const bool on = r < M;
-  const int head = on ? r % group : 0;
-  const int64_t b = mem[(on ? r / group : first) - first];
+  const int r = tile * kPrefixRows + r32;
+  // a negative scale is taken with -q, a zero one with q = 0 (both exact)
+  const float scale2 = a.scale == 0.f ? 1.f : fabsf(a.scale) * kLog2e;
   uint4 qf[KS];
   {
-    const uint16_t* const src = a.q + (b * a.nq + kvh * group + head) * HD + 8 * h;
+    const bool on = r < M;
+    const int64_t b = mem[(on ? r / group : first) - first];
+    const uint16_t* const src = a.q + (b * a.nq + kvh * group + (on ? r % group : 0)) * HD;
+    const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u, keep = on && a.scale != 0.f ? 0xffffffffu : 0u;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
-      const uint4 v = *reinterpret_cast<const uint4*>(src + 16 * ks);
-      qf[ks] = on ? v : make_uint4(0u, 0u, 0u, 0u);
+      const int d = Q8 ? 32 * (ks / 2) + 16 * h + 8 * (ks % 2) : 16 * ks + 8 * h;
+      const uint4 v = *reinterpret_cast<const uint4*>(src + d);
+      qf[ks] = make_uint4((v.x ^ flip) & keep, (v.y ^ flip) & keep, (v.z ^ flip) & keep, (v.w ^ flip) & keep);
     }
   }
-  const bool busy = tile * T::kRows + wv * 32 < M;
-  const float scale2 = a.scale * kLog2e;
 
   f32x16c_t o[DB];
 #pragma unroll
@@ -456,175 +516,295 @@ __global__ __launch_bounds__(kCacheThreads, 2) void k_cache_prefix(CacheAttn a, 
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[db][i] = 0.f;
   float mref = -INFINITY, lsum = 0.f;
+  bool far = false;  // a row of this wave has a reference past kCacheFar
 
+  char* const kb = lds.kv[wv][0];
+  char* const vb = lds.kv[wv][1];
   const int g2 = (lane >> 4) & 1, i16 = lane & 15;
   int koff[4], voff[2];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) koff[i] = r32 * T::kRowBytes + (((2 * i + h) ^ cache_key(r32)) << 4);
+  for (int i = 0; i < 4; ++i) koff[i] = r32 * VB + (((2 * i + h) ^ cache_key(r32)) << 4);
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int vr = 4 * h + (i16 >> 2);
-    voff[i] = vr * T::kRowBytes + (((4 * i + 2 * g2 + ((i16 & 3) >> 1)) ^ cache_key(vr)) << 4) + (i16 & 1) * 8;
+    voff[i] = vr * VB + (((4 * i + 2 * g2 + ((i16 & 3) >> 1)) ^ cache_key(vr)) << 4) + (i16 & 1) * 8;
   }
-  auto of_row = [&](int v, int i) { return __builtin_amdgcn_ds_bpermute(4 * (8 * (i >> 2) + 4 * h + (i & 3)), v); };
-
-  auto attend = [&](const char* kb, int n) {  // 32 positions, n of them there
-    const char* const vb = kb + T::kRegion;
-    f32x16c_t sc;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) sc[i] = 0.f;
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks)
-      sc = mfma32(*reinterpret_cast<const uint4*>(kb + koff[ks & 3] + 128 * (ks >> 2)), qf[ks], sc);
+  auto of_row = [&](float v, int i) {
+    int at = 16 * h;
+    asm volatile("" : "+v"(at));  // (made anew where it is used, not kept in 16 registers)
+    return __int_as_float(__builtin_amdgcn_ds_bpermute(at + 4 * (8 * (i >> 2) + (i & 3)), __float_as_int(v)));
+  };
+  auto rescale = [&](float cm) {
+    cm = fmaxf(cm, __shfl_xor(cm, 32, 64));
+    const float mn = fmaxf(mref, cm);
+    const float f = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mref - mn);
+    mref = mn;
+    far = __any(fabsf(mn) >= kCacheFar && mn != -INFINITY);
+    lsum *= f;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      float t = sc[i] * scale2;
-      asm("" : "+v"(t));  // (rounded, as in k_cache_own)
-      sc[i] = t;
-    }
-    if (n < 32) {
+      const float fi = of_row(f, i);
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (8 * (i >> 2) + 4 * h + (i & 3) >= n) sc[i] = -INFINITY;
-    }
-    float cm = sc[0];
-#pragma unroll
-    for (int i = 1; i < 16; ++i) cm = fmaxf(cm, sc[i]);
-    if (__any(!(cm <= mref + kCacheGrow))) {
-      cm = fmaxf(cm, __shfl_xor(cm, 32, 64));
-      const float mn = fmaxf(mref, cm);
-      const float f = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mref - mn);
-      mref = mn;
-      lsum *= f;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float fi = __int_as_float(of_row(__float_as_int(f), i));
-#pragma unroll
-        for (int db = 0; db < DB; ++db) o[db][i] *= fi;
-      }
-    }
-    const float m = mref == -INFINITY ? 0.f : mref;
-#pragma unroll
-    for (int k2 = 0; k2 < 2; ++k2) {
-      uint32_t p[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        p[e] = pack_bf16x2_rn(__builtin_amdgcn_exp2f(sc[8 * k2 + 2 * e] - m),
-                              __builtin_amdgcn_exp2f(sc[8 * k2 + 2 * e + 1] - m));
-        lsum = dot2(p[e], kOneBf16x2, lsum);
-      }
-      const uint4 pa = make_uint4(p[0], p[1], p[2], p[3]);
-#pragma unroll
-      for (int db = 0; db < DB; ++db) {
-        const char* const at = vb + voff[db & 1] + 16 * k2 * T::kRowBytes + 128 * (db >> 1);
-        const uint2 v0 = lds_turned(at), v1 = lds_turned(at + 8 * T::kRowBytes);
-        o[db] = mfma32(pa, make_uint4(v0.x, v0.y, v1.x, v1.y), o[db]);
-      }
+      for (int db = 0; db < DB; ++db) o[db][i] *= fi;
     }
   };
 
-  if (s_beg < s_end) {
-    store(buf[0]);
-    if (s_beg + 1 < s_end) load(s_beg + 1);
-    __syncthreads();
-  }
-  for (int s = s_beg; s < s_end; ++s) {
-    const char* const cur = buf[(s - s_beg) & 1];
-    if (busy) {
-      const int64_t at = static_cast<int64_t>(s) * T::kStep;
+  // A tile; its registers take tile `next` as soon as they are free (unless next < 0).
+  auto attend = [&](Tile& x, int next) {
+    float s_of = 0.f;
+    if constexpr (Q8) s_of = quant_scale(x.scale);
+    auto scale_of = [&](int from) {
+      return __int_as_float(__builtin_amdgcn_ds_bpermute(4 * from, __float_as_int(s_of)));
+    };
+    if constexpr (!Q8) lay_v<HD, Q8>(kb, x.k, scale_of);
+    lay_v<HD, Q8>(vb, x.v, [&](int row) { return scale_of(32 + row); });
+    asm volatile("" ::: "memory");  // (the rows below are other lanes')
+    f32x16c_t sc;
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const int64_t left = end - at - 32 * t;
-        if (left > 0) attend(cur + 32 * t * T::kRowBytes, left < 32 ? static_cast<int>(left) : 32);
+    for (int i = 0; i < 16; ++i) sc[i] = 0.f;
+    if constexpr (Q8) {
+      const float s = scale_of(r32);
+#pragma unroll
+      for (int j = 0; j < XL; ++j) {
+        sc = mfma32(codes_bf16(x.k[j].x, x.k[j].y, s), qf[2 * j], sc);
+        sc = mfma32(codes_bf16(x.k[j].z, x.k[j].w, s), qf[2 * j + 1], sc);
+      }
+    } else {
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+        sc = mfma32(*reinterpret_cast<const uint4*>(kb + koff[ks & 3] + 128 * (ks >> 2)), qf[ks], sc);
+    }
+    const int n = x.n;
+    if (!TWO) {
+      MA_ISSUE_FENCE();
+      load(x, next);
+    }
+    uint4 vf[2][DB];
+#pragma unroll
+    for (int k2 = 0; k2 < 2; ++k2)
+#pragma unroll
+      for (int db = 0; db < DB; ++db) {
+        const char* const at = vb + voff[db & 1] + 16 * k2 * VB + 128 * (db >> 1);
+        const uint2 v0 = lds_turned(at), v1 = lds_turned(at + 8 * VB);
+        vf[k2][db] = make_uint4(v0.x, v0.y, v1.x, v1.y);
+      }
+    asm volatile("" ::: "memory");
+    MA_ISSUE_FENCE();
+    if (n < 32) {
+      int mine = n - 4 * h;
+      asm volatile("" : "+v"(mine));  // (compared here, not with 16 numbers kept in registers)
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (8 * (i >> 2) + (i & 3) >= mine) sc[i] = -INFINITY;
+    }
+    const float before = lsum;
+    float m = mref, factor = scale2;
+    uint4 pa[2];
+    for (bool again = false;;) {
+#pragma unroll
+      for (int k2 = 0; k2 < 2; ++k2) {
+        uint32_t p[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          p[e] = pack_bf16x2_rn(__builtin_amdgcn_exp2f(__builtin_fmaf(sc[8 * k2 + 2 * e], factor, -m)),
+                                __builtin_amdgcn_exp2f(__builtin_fmaf(sc[8 * k2 + 2 * e + 1], factor, -m)));
+          lsum = dot2(p[e], kOneBf16x2, lsum);
+        }
+        pa[k2] = make_uint4(p[0], p[1], p[2], p[3]);
+      }
+      if (again || !(far || __any(!(lsum <= kCacheSum)))) break;
+      // out of range, or the first scores: once more, from a new reference
+      again = true;
+      lsum = before;
+      float cm = sc[0];
+#pragma unroll
+      for (int i = 1; i < 16; ++i) cm = fmaxf(cm, sc[i]);
+      rescale(fmaxf(cm * scale2, before > 1.0f ? mref + __builtin_amdgcn_logf(before) : -INFINITY));
+      m = mref == -INFINITY ? 0.f : mref;
+      if (far) {  // (rounded products, as the reference is one, so that the largest weight is 1 at any size)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          float y = sc[i] * scale2;
+          asm volatile("" : "+v"(y));
+          sc[i] = y - m;
+        }
+        factor = 1.f;
+        m = 0.f;
       }
     }
-    if (s + 1 < s_end) {
-      store(buf[(s + 1 - s_beg) & 1]);
-      if (s + 2 < s_end) load(s + 2);
-      __syncthreads();
+#pragma unroll
+    for (int k2 = 0; k2 < 2; ++k2)
+#pragma unroll
+      for (int db = 0; db < DB; ++db) o[db] = mfma32(pa[k2], vf[k2][db], o[db]);
+  };
+
+  if constexpr (TWO) {
+    for (int t = t0; t < t_end; t += 2 * NW) {
+      attend(x0, -1);
+      load(x0, at_most(t + 2 * NW));
+      MA_ISSUE_FENCE();
+      if (t + NW < t_end) attend(x1, -1);
+      load(x1, at_most(t + 3 * NW));
+      MA_ISSUE_FENCE();
     }
+  } else {
+    for (int t = t0; t < t_end; t += NW) attend(x0, at_most(t + NW));
   }
 
+  // The waves' states in order, through LDS that V no longer needs.
   lsum += __shfl_xor(lsum, 32, 64);
-  const int st = a.s_own + a.s_pre;
-  const int row = static_cast<int>((b * a.nq + kvh * group + head) * st) + a.s_own + sp;
-  if (on && h == 0) a.ml[row] = make_float2(mref, lsum);
-  const int place = on ? row : -1;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int at = of_row(place, i);
-    if (at >= 0)
-#pragma unroll
-      for (int db = 0; db < DB; ++db) a.acc[static_cast<int64_t>(at) * HD + 32 * db + r32] = o[db][i];
+  __syncthreads();
+  if (h == 0) {
+    lds.m[wv][r32] = mref;
+    lds.l[wv][r32] = lsum;
   }
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+#pragma unroll
+    for (int db = 0; db < DB; ++db) lds.sums[wv][8 * (i >> 2) + 4 * h + (i & 3)][32 * db + r32] = o[db][i];
+  __syncthreads();
+  const int st = a.s_own + a.s_pre;
+#pragma unroll
+  for (int item = tid; item < kPrefixRows * (HD / 4); item += kCacheThreads) {
+    const int row = item / (HD / 4), d = item % (HD / 4) * 4, q = tile * kPrefixRows + row;
+    if (q >= M) break;
+    float m = lds.m[0][row];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) m = fmaxf(m, lds.m[w][row]);
+    float l = 0.f;
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      const float lw = lds.l[w][row];
+      const float f = lw == 0.f ? 0.f : __builtin_amdgcn_exp2f(lds.m[w][row] - m);
+      const float4 v = *reinterpret_cast<const float4*>(&lds.sums[w][row][d]);
+      l += f * lw;
+      s.x += f * v.x;
+      s.y += f * v.y;
+      s.z += f * v.z;
+      s.w += f * v.w;
+    }
+    const int64_t p = (static_cast<int64_t>(mem[q / group - first]) * a.nq + kvh * group + q % group) * st + a.s_own + sp;
+    if (t_beg < t_end) *reinterpret_cast<float4*>(a.acc + p * HD + d) = s;
+    if (d == 0) a.ml[p] = make_float2(m, l);
+  }
+}
+
+template <int HD, bool Q8>
+__global__ __launch_bounds__(kCacheThreads, (HD == 64 ? 4 : (Q8 ? 3 : 2))) void k_cache_own(CacheAttn a) {
+  __shared__ __align__(16) OwnLds<HD> lds;
+  cache_own<HD, Q8>(a, blockIdx.x, lds);
+}
+
+// The first `tiles` x units (rounded up to the XCDs) workgroups the prefixes, where
+// the tiles of the same positions fall to one XCD, the others the rows' own parts.
+template <int HD, bool Q8>
+__global__ __launch_bounds__(kCacheThreads, 2) void k_cache_both(CacheAttn a, int tiles, int n_units) {
+  __shared__ __align__(16) union Lds {
+    OwnLds<HD> own;
+    PrefixLds<HD> prefix;
+  } lds;
+  const int padded = (n_units + kXcds - 1) / kXcds * kXcds;
+  const int wg = blockIdx.x;
+  if (wg >= padded * tiles) {
+    cache_own<HD, Q8>(a, wg - padded * tiles, lds.own);
+    return;
+  }
+  const int tile = wg / padded, unit = wg - tile * padded;
+  if (unit < n_units) cache_prefix<HD, Q8>(a, tile, unit, lds.prefix);
 }
 
 // ---------------------------------------------------------------------------
 // The parts together
 // ---------------------------------------------------------------------------
 // out = sum_s 2^(m_s - m) acc_s / sum_s 2^(m_s - m) l_s over a row's own splits and,
-// where it has a prefix, that one's; 0 where nothing was seen.  HD / 4 lanes of 4 dims
-// times G groups of splits a row: a thread takes the splits g, g + G, .., four loads
-// at a time, then the groups meet in LDS, in order.
-template <int HD>
-__global__ __launch_bounds__(256) void k_cache_merge(CacheAttn a, int G) {
-  constexpr int LPR = HD / 4;
-  __shared__ float4 sa[256];
-  __shared__ float2 sml[256];
-  const int tid = threadIdx.x, d4 = tid % LPR, g = tid / LPR % G;
-  const int64_t total = static_cast<int64_t>(a.batch) * a.nq;
-  const int64_t r0 = static_cast<int64_t>(blockIdx.x) * (256 / (LPR * G)) + tid / (LPR * G);
-  const int64_t r = r0 < total ? r0 : total - 1;
-  int S = a.s_own;
-  if (a.s_pre > 0) {
-    const int64_t p = a.of[r / a.nq];
-    if (p >= 0 && p < a.pre.rows) S += a.s_pre;
-  }
-  const int64_t p0 = r * (a.s_own + a.s_pre);
+// where it has a prefix, that one's; 0 where nothing was seen.  W waves a row: HD / 4
+// lanes of 4 dims, G groups of them that take the splits g, g + G, .., eight loads at
+// a time, and meet through lane exchanges and LDS, in order.
+template <int HD, int W>
+__global__ __launch_bounds__(256) void k_cache_merge(const float* __restrict__ acc, const float2* __restrict__ ml,
+                                                     const int64_t* __restrict__ of, int64_t prefixes, int total, int nq,
+                                                     int s_own, int s_pre, uint16_t* __restrict__ out) {
+  constexpr int LPR = HD / 4, G = 64 / LPR * W, U = 8;
+  __shared__ float4 sv[4][LPR];
+  __shared__ float2 sml[4];
+  const int lane = threadIdx.x & 63, d4 = lane % LPR, wv = threadIdx.x >> 6;
+  const int g = wv % W * (64 / LPR) + lane / LPR;
+  const int r = __builtin_amdgcn_readfirstlane(blockIdx.x * (4 / W) + wv / W);
+  if (r >= total) return;  // (W = 4: the whole workgroup)
+  const int64_t p0 = static_cast<int64_t>(r) * (s_own + s_pre);
+  int S = s_own + s_pre;
   float m = -INFINITY, l = 0.f;
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-  auto add = [&](float2 ml, float4 x) {  // (ml.x <= m)
-    if (ml.y == 0.f) return;  // (nothing seen)
-    const float f = __builtin_amdgcn_exp2f(ml.x - m);
-    l += f * ml.y;
-    v.x += f * x.x;
-    v.y += f * x.y;
-    v.z += f * x.z;
-    v.w += f * x.w;
-  };
   auto raise = [&](float to) {
     const float f = l != 0.f ? __builtin_amdgcn_exp2f(m - to) : 0.f;
     m = to;
     l *= f;
     v = make_float4(v.x * f, v.y * f, v.z * f, v.w * f);
   };
-  for (int s0 = g; s0 < S; s0 += 4 * G) {
-    float2 ml[4];
-    float4 x[4];
+  for (int s0 = g; s0 - g < S; s0 += U * G) {
+    float2 w[U];
+    float4 x[U];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int s = s0 + e * G < S ? s0 + e * G : g;
-      ml[e] = a.ml[p0 + s];
-      x[e] = *reinterpret_cast<const float4*>(a.acc + (p0 + s) * HD + 4 * d4);
-      if (s0 + e * G >= S) ml[e] = make_float2(-INFINITY, 0.f);
+    for (int e = 0; e < U; ++e) {
+      const int64_t p = p0 + (s0 + e * G < S ? s0 + e * G : 0);
+      w[e] = ml[p];
+      x[e] = *reinterpret_cast<const float4*>(acc + p * HD + 4 * d4);
     }
-    raise(fmaxf(fmaxf(m, fmaxf(ml[0].x, ml[1].x)), fmaxf(ml[2].x, ml[3].x)));
-#pragma unroll
-    for (int e = 0; e < 4; ++e) add(ml[e], x[e]);
-  }
-  if (G > 1) {
-    sa[tid] = v;
-    sml[tid] = make_float2(m, l);
-    __syncthreads();
-    if (g > 0) return;
+    if (s0 == g && s_pre > 0) {  // (known while the first loads are in flight)
+      const int64_t p = of[r / nq];
+      if (p < 0 || p >= prefixes) S = s_own;
+    }
     float to = m;
-    for (int e = 1; e < G; ++e) to = fmaxf(to, sml[tid + e * LPR].x);
+#pragma unroll
+    for (int e = 0; e < U; ++e) {
+      if (s0 + e * G >= S || w[e].y == 0.f) w[e] = make_float2(-INFINITY, 0.f);  // (nothing seen: sums not written)
+      to = fmaxf(to, w[e].x);
+    }
     raise(to);
-    for (int e = 1; e < G; ++e) add(sml[tid + e * LPR], sa[tid + e * LPR]);
+#pragma unroll
+    for (int e = 0; e < U; ++e) {
+      if (w[e].y == 0.f) continue;
+      const float f = __builtin_amdgcn_exp2f(w[e].x - m);
+      l += f * w[e].y;
+      v.x += f * x[e].x;
+      v.y += f * x[e].y;
+      v.z += f * x[e].z;
+      v.w += f * x[e].w;
+    }
   }
-  if (r0 >= total) return;
+#pragma unroll
+  for (int off = LPR; off < 64; off *= 2) {  // (both sides of an exchange add the same two numbers)
+    raise(fmaxf(m, __shfl_xor(m, off, 64)));
+    l += __shfl_xor(l, off, 64);
+    v.x += __shfl_xor(v.x, off, 64);
+    v.y += __shfl_xor(v.y, off, 64);
+    v.z += __shfl_xor(v.z, off, 64);
+    v.w += __shfl_xor(v.w, off, 64);
+  }
+  if constexpr (W > 1) {
+    if (lane < LPR) sv[wv][d4] = v;
+    if (lane == 0) sml[wv] = make_float2(m, l);
+    __syncthreads();
+    if (wv > 0) return;
+    float to = m;
+    for (int e = 1; e < W; ++e) to = fmaxf(to, sml[e].x);
+    raise(to);
+    for (int e = 1; e < W; ++e) {
+      const float2 ml = sml[e];
+      if (ml.y == 0.f) continue;
+      const float f = __builtin_amdgcn_exp2f(ml.x - m);
+      const float4 x = sv[e][d4];
+      l += f * ml.y;
+      v.x += f * x.x;
+      v.y += f * x.y;
+      v.z += f * x.z;
+      v.w += f * x.w;
+    }
+  }
+  if (lane >= LPR) return;
   const float inv = l != 0.f ? 1.0f / l : 0.f;
-  *reinterpret_cast<uint2*>(a.out + r * HD + 4 * d4) =
+  *reinterpret_cast<uint2*>(out + static_cast<int64_t>(r) * HD + 4 * d4) =
       make_uint2(pack_bf16x2_rn(v.x * inv, v.y * inv), pack_bf16x2_rn(v.z * inv, v.w * inv));
 }
 
@@ -639,22 +819,41 @@ static int64_t cache_window(int64_t window, int64_t max_len, int64_t pre_len) {
 
 // prefixes: 0 where there are none.  A prefix is read once for all of its rows
 // except under a window, of which it holds at most that many positions a row and
-// each row others: there each row reads them with its own.
+// each row others, and among more than kMaxShared: there each row reads them with
+// its own.
+//
+// Splits, planned for the caches' lengths (the host does not know the rows').  A
+// workgroup a compute unit; two where a split would still hold more than 1024 of a
+// row's positions, or 2048 of a prefix; none of a row's where that saves less than the
+// launch that joins them (about 4 us, six rounds of 128 positions).  Measured (us,
+// for this many workgroups):
+//   1 x 4096 of 64: 7.2 for 128, 7.5 for 256 (the most there are);  32 x 1024: 9.3
+//     unsplit, 9.6 for 256;  32 x 4096: 25.6, 18.0 for 256, 15.8 for 512, 16.5 for 768;
+//     2 x 32768: 17.9, 12.8, 12.2, 13.0
+//   4 x 4096 of 128: 11.6, 10.2, 11.9 for 512;  8 x 32768: 83, 54, 51, 53
+//   prefixes, 32 rows behind 8192 of 64: 18.4, 14.5, 17.1;  behind 32768: 44, 28, 26;
+//     64 behind four of 8192: 49, 24, 20;  64 behind 8192 of 128: 29, 22, 28
 static CachePlan cache_plan(int64_t batch, int nq, int nkv, int64_t max_len, int64_t prefixes, int64_t pre_len, int64_t window) {
   CachePlan p{1, 0, 0};
   const int64_t pairs = batch * nkv;
-  int64_t span = max_len;
-  if (window > 0) span = window < max_len + (prefixes ? pre_len : 0) ? window : max_len + (prefixes ? pre_len : 0);
-  const int64_t n = cdiv(span, 128) + (window > 0 && prefixes ? 1 : 0);
-  int64_t s = cdiv(1024, pairs);
-  p.s_own = static_cast<int>(s < n ? s : n);
-  if (prefixes > 0 && window == 0) {
-    const int64_t rows = batch * (nq / nkv);
-    p.tiles = static_cast<int>(cdiv(rows, 128));
-    const int64_t busy = prefixes + rows / 128 < batch ? prefixes + rows / 128 : batch;  // about how many hold rows
-    const int64_t steps = cdiv(pre_len, 64);
-    s = cdiv(512, nkv * (busy > 0 ? busy : 1));
-    p.s_pre = static_cast<int>(s < steps ? s : steps);
+  const bool shared = prefixes > 0 && prefixes <= kMaxShared && window == 0;
+  int64_t span = max_len + (prefixes > 0 && !shared ? pre_len : 0);
+  if (window > 0 && window < span) span = window;
+  const int64_t n = cdiv(span, 128) + (prefixes > 0 && !shared ? 1 : 0);  // (either part ends in a round of its own)
+  int64_t s = 256 / pairs;
+  if (n > 8 * (s < 1 ? 1 : s)) s = cdiv(512, pairs);
+  s = s < 1 ? 1 : (s > n ? n : s);
+  if (n - n / s < 6) s = 1;
+  p.s_own = static_cast<int>(s);
+  if (shared) {
+    // tiles in all, each prefix's last one part empty
+    const int64_t some = prefixes < batch ? prefixes : batch;
+    p.tiles = static_cast<int>((batch * (nq / nkv) + (kPrefixRows - 1) * some) / kPrefixRows);
+    const int64_t rounds = cdiv(pre_len, 128), units = nkv * p.tiles;
+    s = 256 / units;
+    if (rounds > 16 * (s < 1 ? 1 : s)) s = cdiv(512, units);
+    s = s < 1 ? 1 : s;
+    p.s_pre = static_cast<int>(s < rounds ? s : rounds);
   }
   return p;
 }
@@ -668,6 +867,7 @@ static size_t cache_ws_bytes(const CachePlan& p, int64_t batch, int nq, int head
 
 using namespace ma;
 
+constexpr int64_t kMaxGroups = (1 << 24) - 1;  // (a launch counts its threads in 32 bits)
 static bool cache_aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 static int check_cache_sizes(const char* what, int64_t batch, int nq, int nkv, int hd, int64_t rows, int64_t max_len,
@@ -718,9 +918,9 @@ extern "C" int ma_cache_attn(const void* q, int64_t batch, int n_heads, int n_kv
   const size_t need = cache_ws_bytes(p, batch, n_heads, head_dim);
   if (need && (!workspace || workspace_bytes < need))
     return fail(MA_EVALUE, "%s: workspace of %zu bytes, need %zu", what, workspace ? workspace_bytes : 0, need);
-  const int64_t units = prefixes * n_kv_heads * p.s_pre, own_wgs = batch * n_kv_heads * p.s_own;
+  const int64_t units = static_cast<int64_t>(n_kv_heads) * p.s_pre, own_wgs = batch * n_kv_heads * p.s_own;
   const int64_t pre_wgs = cdiv(units, kXcds) * kXcds * p.tiles;
-  if (parts > INT32_MAX || own_wgs > INT32_MAX || pre_wgs > INT32_MAX) return fail(MA_EVALUE, "%s: batch too large for one launch", what);
+  if (parts > INT32_MAX || own_wgs + pre_wgs > kMaxGroups) return fail(MA_EVALUE, "%s: batch too large for one launch", what);
   auto u8 = [](const void* x) { return static_cast<const uint8_t*>(x); };
   float* const acc = static_cast<float*>(workspace);
   const CacheAttn a{seqlen, row_map, prefixes > 0 ? prefix_of : nullptr, prefix_len, static_cast<const uint16_t*>(q),
@@ -731,26 +931,26 @@ extern "C" int ma_cache_attn(const void* q, int64_t batch, int n_heads, int n_kv
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (p.s_pre > 0) {
     auto go = [&](auto kernel) {
-      hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(pre_wgs)), dim3(kCacheThreads), 0, s, a, p.tiles, static_cast<int>(units));
+      hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(pre_wgs + own_wgs)), dim3(kCacheThreads), 0, s, a, p.tiles, static_cast<int>(units));
     };
-    if (head_dim == 64) q8 ? go(k_cache_prefix<64, true>) : go(k_cache_prefix<64, false>);
-    else q8 ? go(k_cache_prefix<128, true>) : go(k_cache_prefix<128, false>);
-    if (int rc = check_launch("cache_attn prefix")) return rc;
-  }
-  {
+    if (head_dim == 64) q8 ? go(k_cache_both<64, true>) : go(k_cache_both<64, false>);
+    else q8 ? go(k_cache_both<128, true>) : go(k_cache_both<128, false>);
+  } else {
     auto go = [&](auto kernel) {
       hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(own_wgs)), dim3(kCacheThreads), 0, s, a);
     };
     if (head_dim == 64) q8 ? go(k_cache_own<64, true>) : go(k_cache_own<64, false>);
     else q8 ? go(k_cache_own<128, true>) : go(k_cache_own<128, false>);
-    if (int rc = check_launch(what)) return rc;
   }
+  if (int rc = check_launch(what)) return rc;
   if (!need) return MA_OK;
-  int G = 1;  // split groups of the merge: one for each four splits
-  while (G < 1024 / head_dim && 4 * G < p.s_own + p.s_pre) G *= 2;
-  const dim3 mg(static_cast<unsigned>(cdiv(batch * n_heads * (head_dim / 4) * G, 256)));
-  auto merge = [&](auto kernel) { hipLaunchKernelGGL(kernel, mg, dim3(256), 0, s, a, G); };
-  if (head_dim == 64) merge(k_cache_merge<64>);
-  else merge(k_cache_merge<128>);
+  const int rows = static_cast<int>(batch * n_heads);
+  const bool wide = p.s_own + p.s_pre > 8 * 256 / head_dim;  // more than one round of a wave's loads
+  auto merge = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(cdiv(rows, wide ? 1 : 4))), dim3(256), 0, s, a.acc, a.ml, a.of,
+                       prefixes, rows, n_heads, p.s_own, p.s_pre, a.out);
+  };
+  if (head_dim == 64) wide ? merge(k_cache_merge<64, 4>) : merge(k_cache_merge<64, 1>);
+  else wide ? merge(k_cache_merge<128, 4>) : merge(k_cache_merge<128, 1>);
   return check_launch("cache_attn merge");
 }

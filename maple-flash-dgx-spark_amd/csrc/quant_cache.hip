@@ -94,6 +94,8 @@ __global__ __launch_bounds__(kQuantThreads) void k_quant_qkv(
 // ---------------------------------------------------------------------------
 // Prompts in
 // ---------------------------------------------------------------------------
+typedef uint32_t u32x4q_t __attribute__((ext_vector_type(4)));
+
 struct KvRows {  // bf16 [batch, n_kv, T, HD], the last dim contiguous
   const uint16_t* p;
   int64_t sb, sh, st;
@@ -101,43 +103,44 @@ struct KvRows {  // bf16 [batch, n_kv, T, HD], the last dim contiguous
 
 constexpr int kQuantRows = 4;  // rows a thread has in flight
 
-// HD / 16 lanes a row of 16 dims each, kQuantRows rows a thread; blockIdx.y: K or
-// V.  HEADS_IN: a batch row's heads lie next to each other (positions before heads,
-// as a projection leaves them), so they are walked first; else positions are.
+// HD / 16 lanes a row of 16 dims each, kQuantRows rows a thread; blockIdx.x: `chunks`
+// of a batch row's n_kv x T rows, blockIdx.y: K or V.  HEADS_IN: a batch row's heads
+// lie next to each other (positions before heads, as a projection leaves them), so
+// they are walked first; else positions are.
 template <int HD, bool HEADS_IN, bool VEC>
-__global__ __launch_bounds__(kQuantThreads) void k_quant_kv(KvRows kr, KvRows vr, int64_t total, int64_t T, int nkv,
-                                                            const int64_t* __restrict__ start,
+__global__ __launch_bounds__(kQuantThreads) void k_quant_kv(KvRows kr, KvRows vr, int chunks, uint32_t per, uint32_t T,
+                                                            uint32_t nkv, const int64_t* __restrict__ start,
                                                             const int64_t* __restrict__ lengths,
                                                             const int64_t* __restrict__ row_map, QuantCache cache) {
   constexpr int LPR = HD / 16, RPB = kQuantThreads / LPR;
   const int tid = threadIdx.x, l = tid % LPR;
   const bool is_v = blockIdx.y != 0;
   const KvRows src = is_v ? vr : kr;
-  uint4 x[kQuantRows][2];
+  const int64_t b = blockIdx.x / chunks;
+  const uint32_t r0 = (blockIdx.x - static_cast<uint32_t>(b) * chunks) * (kQuantRows * RPB) + tid / LPR;
+  const int64_t p0 = start ? start[b] : 0, most = lengths ? lengths[b] : T;
+  const int64_t crow = row_map ? clamp_pos(row_map[b], 0, cache.rows - 1) : b;
+  u32x4q_t x[kQuantRows][2];
   int64_t to[kQuantRows];
 #pragma unroll
   for (int i = 0; i < kQuantRows; ++i) {
-    const int64_t r = (static_cast<int64_t>(blockIdx.x) * kQuantRows + i) * RPB + tid / LPR;
-    to[i] = -1;
-    x[i][0] = x[i][1] = make_uint4(0u, 0u, 0u, 0u);
-    if (r >= total) continue;
-    const int64_t per = T * nkv, b = r / per, rest = r - b * per;
-    const int64_t h = HEADS_IN ? rest % nkv : rest / T, t = HEADS_IN ? rest / nkv : rest % T;
-    const int64_t p = (start ? start[b] : 0) + t;
-    if ((lengths && t >= lengths[b]) || p < 0 || p >= cache.max_len) continue;
-    to[i] = ((row_map ? clamp_pos(row_map[b], 0, cache.rows - 1) : b) * nkv + h) * cache.max_len + p;
+    const uint32_t r = r0 + i * RPB;
+    const uint32_t h = HEADS_IN ? r % nkv : r / T, t = HEADS_IN ? r / nkv : r % T;
+    const int64_t p = p0 + t;
+    const bool in = r < per && t < most && p >= 0 && p < cache.max_len;
+    to[i] = in ? (crow * nkv + h) * cache.max_len + p : -1;
+    x[i][0] = x[i][1] = u32x4q_t{0u, 0u, 0u, 0u};
+    if (!in) continue;
     const uint16_t* const s = src.p + b * src.sb + h * src.sh + t * src.st + 16 * l;
     if constexpr (VEC) {
-      x[i][0] = reinterpret_cast<const uint4*>(s)[0];
-      x[i][1] = reinterpret_cast<const uint4*>(s)[1];
+      x[i][0] = reinterpret_cast<const u32x4q_t*>(s)[0];
+      x[i][1] = reinterpret_cast<const u32x4q_t*>(s)[1];
     } else {
-      uint32_t w[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) w[e] = s[2 * e] | static_cast<uint32_t>(s[2 * e + 1]) << 16;
-      x[i][0] = make_uint4(w[0], w[1], w[2], w[3]);
-      x[i][1] = make_uint4(w[4], w[5], w[6], w[7]);
+      for (int e = 0; e < 8; ++e) x[i][e / 4][e % 4] = s[2 * e] | static_cast<uint32_t>(s[2 * e + 1]) << 16;
     }
   }
+  MA_ISSUE_FENCE();
   uint8_t* const codes = is_v ? cache.v : cache.k;
   uint8_t* const scales = is_v ? cache.vs : cache.ks;
 #pragma unroll
@@ -160,10 +163,11 @@ __global__ __launch_bounds__(kQuantThreads) void k_quant_kv(KvRows kr, KvRows vr
 // ---------------------------------------------------------------------------
 // Cached positions back
 // ---------------------------------------------------------------------------
-// HD / 16 lanes a row of 16 codes each.  A value is exact in bf16 (e4m3 has four
+// HD / 16 lanes a row of 16 codes each; blockIdx.x: `chunks` of a (batch row, head)'s
+// positions, blockIdx.y: K or V.  A value is exact in bf16 (e4m3 has four
 // significant bits) unless 2^e takes it below bf16's least normal.
 template <int HD>
-__global__ __launch_bounds__(kQuantThreads) void k_dequant_kv(QuantCache cache, int64_t total, int64_t length, int nkv,
+__global__ __launch_bounds__(kQuantThreads) void k_dequant_kv(QuantCache cache, int chunks, uint32_t length, int nkv,
                                                               const int64_t* __restrict__ row_map,
                                                               uint16_t* __restrict__ k_out,
                                                               uint16_t* __restrict__ v_out) {
@@ -173,25 +177,24 @@ __global__ __launch_bounds__(kQuantThreads) void k_dequant_kv(QuantCache cache, 
   const uint8_t* const codes = is_v ? cache.v : cache.k;
   const uint8_t* const scales = is_v ? cache.vs : cache.ks;
   uint16_t* const out = is_v ? v_out : k_out;
-  uint4 c[kQuantRows];
+  const int64_t pair = blockIdx.x / chunks, b = pair / nkv, h = pair - b * nkv;
+  const uint32_t r0 = (blockIdx.x - static_cast<uint32_t>(pair) * chunks) * (kQuantRows * RPB) + tid / LPR;
+  const int64_t from = ((row_map ? clamp_pos(row_map[b], 0, cache.rows - 1) : b) * nkv + h) * cache.max_len;
+  u32x4q_t c[kQuantRows];
   int byte[kQuantRows];
-  int64_t row[kQuantRows];
 #pragma unroll
   for (int i = 0; i < kQuantRows; ++i) {
-    const int64_t r = (static_cast<int64_t>(blockIdx.x) * kQuantRows + i) * RPB + tid / LPR;
-    row[i] = r < total ? r : -1;
-    const int64_t q = r < total ? r : 0;
-    const int64_t pair = q / length, b = pair / nkv, h = pair - b * nkv;
-    const int64_t at = ((row_map ? clamp_pos(row_map[b], 0, cache.rows - 1) : b) * nkv + h) * cache.max_len +
-                       (q - pair * length);
-    c[i] = *reinterpret_cast<const uint4*>(codes + at * HD + 16 * l);
+    const uint32_t t = r0 + i * RPB;
+    const int64_t at = from + (t < length ? t : 0);
+    c[i] = *reinterpret_cast<const u32x4q_t*>(codes + at * HD + 16 * l);
     byte[i] = scales[at];
   }
   MA_ISSUE_FENCE();
   typedef float f32x2q_t __attribute__((ext_vector_type(2)));
 #pragma unroll
   for (int i = 0; i < kQuantRows; ++i) {
-    if (row[i] < 0) continue;
+    const uint32_t t = r0 + i * RPB;
+    if (t >= length) continue;
     const float s = quant_scale(byte[i]);
     const uint32_t w[4] = {c[i].x, c[i].y, c[i].z, c[i].w};
     uint32_t o[8];
@@ -202,7 +205,7 @@ __global__ __launch_bounds__(kQuantThreads) void k_dequant_kv(QuantCache cache, 
       o[2 * j] = pack_bf16x2_rn(a.x * s, a.y * s);
       o[2 * j + 1] = pack_bf16x2_rn(b.x * s, b.y * s);
     }
-    uint4* const to = reinterpret_cast<uint4*>(out + row[i] * HD + 16 * l);
+    uint4* const to = reinterpret_cast<uint4*>(out + (pair * length + t) * HD + 16 * l);
     to[0] = make_uint4(o[0], o[1], o[2], o[3]);
     to[1] = make_uint4(o[4], o[5], o[6], o[7]);
   }
@@ -213,6 +216,8 @@ __global__ __launch_bounds__(kQuantThreads) void k_dequant_kv(QuantCache cache, 
 using namespace ma;
 
 namespace {
+
+constexpr int64_t kMaxGroups = (1 << 24) - 1;  // (a launch counts its threads in 32 bits)
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
@@ -252,7 +257,7 @@ extern "C" int ma_quant_qkv(const void* qkv, int64_t ldb, int64_t batch, int n_h
   if (!qkv || !seqlen || !q_out) return fail(MA_EVALUE, "%s: null pointer", what);
   if (!aligned16(q_out)) return fail(MA_EVALUE, "%s: q_out must be 16-byte aligned", what);
   const int64_t blocks = cdiv(batch * (n_heads + 2 * n_kv_heads) * (head_dim / 8), kQuantThreads);
-  if (batch > (1 << 24) || blocks > INT32_MAX) return fail(MA_EVALUE, "%s: batch too large for one launch", what);
+  if (batch > (1 << 24) || blocks > kMaxGroups) return fail(MA_EVALUE, "%s: batch too large for one launch", what);
   const RopeTab rope{cos, sin, cs_dtype, ld_cs, n_pos, rotary_dim, rotary_dim > 0 ? 1 : 0};
   const QuantCache cache{static_cast<uint8_t*>(k_codes), static_cast<uint8_t*>(v_codes), static_cast<uint8_t*>(k_scale),
                          static_cast<uint8_t*>(v_scale), cache_rows, max_len};
@@ -282,18 +287,19 @@ extern "C" int ma_quant_kv(const void* k, int64_t k_sb, int64_t k_sh, int64_t k_
   if (batch == 0 || T == 0) return MA_OK;
   if (!k || !v) return fail(MA_EVALUE, "%s: null pointer", what);
   const int64_t rpb = kQuantThreads / (head_dim / 16) * kQuantRows;
-  if (batch > (int64_t{1} << 31) || T > (int64_t{1} << 31) / batch || cdiv(batch * T * n_kv_heads, rpb) > INT32_MAX)
+  if (T > INT32_MAX / n_kv_heads || batch > kMaxGroups / cdiv(T * n_kv_heads, rpb))
     return fail(MA_EVALUE, "%s: batch x positions too large for one launch", what);
-  const int64_t total = batch * T * n_kv_heads;
+  const int64_t per = T * n_kv_heads, chunks = cdiv(per, rpb);
   const QuantCache cache{static_cast<uint8_t*>(k_codes), static_cast<uint8_t*>(v_codes), static_cast<uint8_t*>(k_scale),
                          static_cast<uint8_t*>(v_scale), cache_rows, max_len};
   const KvRows kr{static_cast<const uint16_t*>(k), k_sb, k_sh, k_st}, vr{static_cast<const uint16_t*>(v), v_sb, v_sh, v_st};
   const bool vec = aligned16(k) && aligned16(v) && (k_sb | k_sh | k_st | v_sb | v_sh | v_st) % 8 == 0;
   const bool heads_in = k_sh < k_st;
-  const dim3 grid(static_cast<unsigned>(cdiv(total, rpb)), 2);
+  const dim3 grid(static_cast<unsigned>(batch * chunks), 2);
   auto go = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, grid, dim3(kQuantThreads), 0, static_cast<hipStream_t>(stream), kr, vr, total, T,
-                       n_kv_heads, start, lengths, row_map, cache);
+    hipLaunchKernelGGL(kernel, grid, dim3(kQuantThreads), 0, static_cast<hipStream_t>(stream), kr, vr,
+                       static_cast<int>(chunks), static_cast<uint32_t>(per), static_cast<uint32_t>(T),
+                       static_cast<uint32_t>(n_kv_heads), start, lengths, row_map, cache);
   };
   if (head_dim == 64) {
     if (vec) heads_in ? go(k_quant_kv<64, true, true>) : go(k_quant_kv<64, false, true>);
@@ -318,16 +324,15 @@ extern "C" int ma_dequant_kv(const void* k_codes, const void* v_codes, const voi
   if (!k_out || !v_out || !aligned16(k_out) || !aligned16(v_out))
     return fail(MA_EVALUE, "%s: the outputs must be there and 16-byte aligned", what);
   const int64_t rpb = kQuantThreads / (head_dim / 16) * kQuantRows;
-  if (batch > (int64_t{1} << 31) || length > (int64_t{1} << 31) / batch ||
-      cdiv(batch * length * n_kv_heads, rpb) > INT32_MAX)
+  if (length > INT32_MAX || batch > kMaxGroups / n_kv_heads / cdiv(length, rpb))
     return fail(MA_EVALUE, "%s: batch x positions too large for one launch", what);
-  const int64_t total = batch * length * n_kv_heads;
+  const int64_t chunks = cdiv(length, rpb);
   auto u8 = [](const void* p) { return const_cast<uint8_t*>(static_cast<const uint8_t*>(p)); };
   const QuantCache cache{u8(k_codes), u8(v_codes), u8(k_scale), u8(v_scale), cache_rows, max_len};
-  const dim3 grid(static_cast<unsigned>(cdiv(total, rpb)), 2);
+  const dim3 grid(static_cast<unsigned>(batch * n_kv_heads * chunks), 2);
   auto go = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, grid, dim3(kQuantThreads), 0, static_cast<hipStream_t>(stream), cache, total, length,
-                       n_kv_heads, row_map, static_cast<uint16_t*>(k_out), static_cast<uint16_t*>(v_out));
+    hipLaunchKernelGGL(kernel, grid, dim3(kQuantThreads), 0, static_cast<hipStream_t>(stream), cache,
+                       static_cast<int>(chunks), static_cast<uint32_t>(length), n_kv_heads, row_map, static_cast<uint16_t*>(k_out), static_cast<uint16_t*>(v_out));
   };
   if (head_dim == 64) go(k_dequant_kv<64>);
   else go(k_dequant_kv<128>);
