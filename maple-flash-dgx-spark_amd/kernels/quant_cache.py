@@ -25,6 +25,7 @@ is written once.  All of these can be captured into a graph.
 
 from __future__ import annotations
 
+import functools
 from typing import NamedTuple
 
 import torch
@@ -34,6 +35,13 @@ from .tree import _FAR, _call, _device, _positions
 
 CODE = torch.float8_e4m3fn
 SCALE = torch.float8_e8m0fnu
+
+_contiguous, _ptr = torch.Tensor.is_contiguous, torch.Tensor.data_ptr
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(*sizes: int) -> int:
+    return int(_lib.load().ma_cache_attn_workspace_bytes(*sizes))
 
 
 class KV(NamedTuple):
@@ -69,27 +77,25 @@ def make_quant_kv(rows: int, num_kv_heads: int, max_len: int, head_dim: int, dev
                    *(torch.full(shape, 1, device=device, dtype=torch.uint8).view(SCALE) for _ in range(2)))
 
 
-def _check_cache(what: str, cache, bsz: int | None, row_map) -> tuple:
+def _check_cache(what: str, cache, bsz: int | None, row_map):
     """The caches' shape ``[rows, n_kv, max_len, head_dim]``."""
-    quant = len(cache) == 4
     k, v = cache[0], cache[1]
     shape = k.shape
     if len(shape) != 4 or v.shape != shape:
         raise ValueError(f"{what}: K {tuple(shape)} and V {tuple(v.shape)} caches, "
                          "expected [rows, n_kv, max_len, head_dim] twice.")
-    want = CODE if quant else torch.bfloat16
+    want = torch.bfloat16
+    if len(cache) == 4:
+        want, k_scale, v_scale = CODE, cache[2], cache[3]
+        if k_scale.dtype != SCALE or v_scale.dtype != SCALE:
+            raise TypeError(f"{what}: scales must be {SCALE}; got {k_scale.dtype} and {v_scale.dtype}.")
+        if k_scale.shape != v_scale.shape or k_scale.shape != shape[:3]:
+            raise ValueError(f"{what}: scales {tuple(k_scale.shape)} and {tuple(v_scale.shape)} for a cache {tuple(shape)}.")
     if k.dtype != want or v.dtype != want:
         raise TypeError(f"{what}: K and V caches of {k.dtype} and {v.dtype}, expected {want}.")
-    if quant:
-        for s in cache[2:]:
-            if s.dtype != SCALE:
-                raise TypeError(f"{what}: scales must be {SCALE}; got {s.dtype}.")
-            if s.shape != shape[:3]:
-                raise ValueError(f"{what}: scales {tuple(s.shape)} for a cache {tuple(shape)}.")
-    for t in cache:
-        if not t.is_contiguous():
-            raise ValueError(f"{what}: the cache must be contiguous.")
-    if bsz is not None and row_map is None and shape[0] != bsz:
+    if not all(map(_contiguous, cache)):
+        raise ValueError(f"{what}: the cache must be contiguous.")
+    if row_map is None and bsz is not None and shape[0] != bsz:
         raise ValueError(f"KV cache batch {shape[0]} != {what} batch {bsz}.")
     return shape
 
@@ -181,7 +187,7 @@ def apply_qkv_quant(
     _call(
         idx, "ma_quant_qkv",
         qkv.data_ptr(), ldb if bsz > 1 else width, bsz, num_heads, num_kv_heads, head_dim, qw, kw, w_dt, c, s, dt, ld,
-        n_pos, rot, eps, sl.data_ptr(), at, rm, *(t.data_ptr() for t in cache), rows, max_len, out.data_ptr(),
+        n_pos, rot, eps, sl.data_ptr(), at, rm, *map(_ptr, cache), rows, max_len, out.data_ptr(),
     )
     return out
 
@@ -208,15 +214,19 @@ def quantize_kv(
     rows, c_kv, max_len, c_d = _check_cache("quantize_kv", cache, bsz, row_map)
     if (c_kv, c_d) != (n_kv, d):
         raise ValueError(f"quantize_kv: cache {tuple(cache.k.shape)} for {n_kv} KV heads of {d}.")
-    if k.stride(3) != 1 or v.stride(3) != 1:
+    k_s, v_s = k.stride(), v.stride()
+    if k_s[3] != 1 or v_s[3] != 1:
         raise ValueError("quantize_kv needs contiguous rows of k and v.")
-    more = [_positions(n, x, bsz) if x is not None else None
-            for n, x in (("start", start), ("lengths", lengths), ("row_map", row_map))]
-    idx = _device("quantize_kv", k, v, *cache, *(x for x in more if x is not None))
+    more, at = [], []
+    for name, x in (("start", start), ("lengths", lengths), ("row_map", row_map)):
+        if x is not None:
+            more.append(_positions(name, x, bsz))
+        at.append(None if x is None else more[-1].data_ptr())
+    idx = _device("quantize_kv", k, v, *cache, *more)
     _call(
         idx, "ma_quant_kv",
-        k.data_ptr(), *k.stride()[:3], v.data_ptr(), *v.stride()[:3], bsz, t, n_kv, d, *map(_lib.ptr, more),
-        *(x.data_ptr() for x in cache), rows, max_len,
+        k.data_ptr(), *k_s[:3], v.data_ptr(), *v_s[:3], bsz, t, n_kv, d, *at,
+        *map(_ptr, cache), rows, max_len,
     )
     return cache
 
@@ -232,13 +242,16 @@ def dequantize_kv(cache: QuantKV, length: int | None = None, *, row_map: torch.T
     rm = None if row_map is None else _positions("row_map", row_map, row_map.numel())
     idx = _device("dequantize_kv", *cache, *(() if rm is None else (rm,)))
     shape = (rows if rm is None else rm.numel(), n_kv, length, d)
-    out = KV(*(cache.k.new_empty(shape, dtype=torch.bfloat16) for _ in range(2)))
+    out = KV(cache.k.new_empty(shape, dtype=torch.bfloat16), cache.k.new_empty(shape, dtype=torch.bfloat16))
     _call(
         idx, "ma_dequant_kv",
-        *(x.data_ptr() for x in cache), rows, max_len, shape[0], length, n_kv, d, _lib.ptr(rm), out.k.data_ptr(),
+        *map(_ptr, cache), rows, max_len, shape[0], length, n_kv, d, _lib.ptr(rm), out.k.data_ptr(),
         out.v.data_ptr(),
     )
     return out
+
+
+_NO_PREFIX = (None,) * 4
 
 
 def _attend(what: str, q: torch.Tensor, cache, seqlen: torch.Tensor, prefix: SharedPrefix | None, row_map, scale: float,
@@ -258,10 +271,8 @@ def _attend(what: str, q: torch.Tensor, cache, seqlen: torch.Tensor, prefix: Sha
     if row_map is not None:
         more.append(_positions("row_map", row_map, bsz))
         rm = more[-1].data_ptr()
-    own = [t.data_ptr() for t in cache]
-    if len(own) == 2:
-        own += [None, None]
-    shared, n_pre, pre_max, p_len, p_of = [None] * 4, 0, 0, None, None
+    quant = len(cache) == 4
+    shared, n_pre, pre_max, p_len, p_of = _NO_PREFIX, 0, 0, None, None
     if prefix is not None:
         if type(prefix.cache) is not type(cache):
             raise TypeError(f"{what}: a {type(cache).__name__} cache behind a {type(prefix.cache).__name__} prefix.")
@@ -270,22 +281,21 @@ def _attend(what: str, q: torch.Tensor, cache, seqlen: torch.Tensor, prefix: Sha
             raise ValueError(f"{what}: prefixes {tuple(prefix.cache.k.shape)} for {n_kv} KV heads of {d}.")
         length, of = _positions("length", prefix.length, n_pre), _positions("of", prefix.of, bsz)
         more += [*prefix.cache, length, of]
-        shared = [t.data_ptr() for t in prefix.cache]
-        if len(shared) == 2:
-            shared += [None, None]
+        shared = (*map(_ptr, prefix.cache), *(() if quant else (None, None)))
         p_len, p_of = length.data_ptr(), of.data_ptr()
         if pre_max == 0:
             n_pre = 0
     idx = _device(what, q, *cache, sl, *more)
-    q = q.contiguous()
+    if not q.is_contiguous():
+        q = q.contiguous()
     out = torch.empty_like(q)
-    nbytes = _lib.load().ma_cache_attn_workspace_bytes(bsz, n_q, n_kv, head_dim, max_len, n_pre, pre_max, window)
+    nbytes = _workspace_bytes(bsz, n_q, n_kv, head_dim, max_len, n_pre, pre_max, window)
     # scratch of this call alone: the allocator keeps it to this stream, a
     # captured graph to its own pool
     ws = q.new_empty(nbytes // 2) if nbytes else None
     _call(
         idx, "ma_cache_attn",
-        q.data_ptr(), bsz, n_q, n_kv, head_dim, *own, rows, max_len, sl.data_ptr(), rm, *shared, n_pre, pre_max,
+        q.data_ptr(), bsz, n_q, n_kv, head_dim, *map(_ptr, cache), *(() if quant else (None, None)), rows, max_len, sl.data_ptr(), rm, *shared, n_pre, pre_max,
         p_len, p_of, window, scale, out.data_ptr(), _lib.ptr(ws), nbytes,
     )
     return out
