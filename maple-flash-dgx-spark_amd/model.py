@@ -23,6 +23,11 @@ layers over all nodes at once, with ``apply_qkv_tree`` and ``tree_attention`` in
 the place of ``decode_attention``; ``KVCache.commit`` then keeps an accepted
 branch.
 
+Over a quantised cache (``make_cache(quantized=True)``, ``KVCache.quantized``) the
+attention of a step is ``apply_qkv_quant`` and ``quant_gqa_attn``, and over rows
+behind shared prefixes (``KVCache.share``) ``prefix_gqa_attn``, in the place of
+``decode_attention``.
+
 Weights are random with the synthetic distributions (``synthetic.py``): every
 projection packed ternary, norm weights 1, the lm_head and embedding 4-bit RTN
 with group 128 and zero-centred dequantised values, RoPE on every layer over
@@ -38,9 +43,11 @@ from dataclasses import dataclass, field
 import torch
 
 from . import synthetic
-from .kernels.decode_attn import decode_attention, gqa_workspace, o_projection_supported
+from .kernels.decode_attn import apply_qkv_decode, decode_attention, gqa_workspace, o_projection_supported
 from .kernels.fused_norm import rms_norm
 from .kernels.greedy import greedy_argmax
+from .kernels.quant_cache import (KV, QuantKV, SharedPrefix, apply_qkv_quant, dequantize_kv, make_quant_kv,
+                                  prefix_gqa_attn, quant_gqa_attn, quantize_kv)
 from .kernels.rtn4 import rtn4_embedding, rtn4_gemv
 from .kernels.ternary_gemv import combine_gemv_supported, ternary_gemv, ternary_gemv_combine
 from .kernels.tree import apply_qkv_tree, check_tree, commit_tree, tree_attention
@@ -159,6 +166,40 @@ def rope_tables(max_len: int, rotary_dim: int, theta: float, device, scaling: Ro
     return emb.cos().contiguous(), emb.sin().contiguous()
 
 
+def _bytes(t: torch.Tensor) -> torch.Tensor:
+    """A float8 tensor as its bytes; any other as it is."""
+    return t.view(torch.uint8) if t.element_size() == 1 else t
+
+
+def _check_trees(cache) -> None:
+    if getattr(cache, "k_scale", None) is not None or getattr(cache, "prefix", None) is not None:
+        raise ValueError("drafted trees need a bf16 cache without shared prefixes.")
+
+
+@dataclass
+class SharedKV:
+    """Prefixes that rows of a ``KVCache`` share (``KVCache.share``): per layer K/V ``[P,
+    n_kv, longest, D]`` of the cache's kind, ``length [P]`` the prefixes' positions,
+    ``of [slots]`` each slot's prefix (-1: none).  Indexed by slot like ``seqlen``."""
+
+    k: list
+    v: list
+    length: torch.Tensor
+    of: torch.Tensor
+    k_scale: list | None = None
+    v_scale: list | None = None
+
+    @property
+    def max_len(self) -> int:
+        return int(self.k[0].shape[2])
+
+    def layer(self, i: int, width: int) -> SharedPrefix:
+        """Layer ``i``'s prefixes for a step over slots ``[0, width)``."""
+        kv = KV(self.k[i], self.v[i]) if self.k_scale is None else QuantKV(self.k[i], self.v[i], self.k_scale[i],
+                                                                           self.v_scale[i])
+        return SharedPrefix(kv, self.length, self.of[:width])
+
+
 @dataclass
 class KVCache:
     """Preallocated bf16 K/V per layer ``[rows, n_kv, max_len, D]``, one write
@@ -170,7 +211,12 @@ class KVCache:
     With ``remap`` off the map is the identity; a scheduler turns it on to
     keep live sequences in the low slots by swapping indices (never K/V), so
     a decode step can run at a narrow width.  A step of width ``w`` covers
-    slots ``[0, w)``."""
+    slots ``[0, w)``.
+
+    With ``k_scale`` / ``v_scale`` the K/V are e4m3 codes with a power of two per
+    position and head (``kernels.quant_cache``), half the bytes; with ``prefix``
+    slots' sequences may begin with shared prefixes, ``seqlen`` then counting a
+    slot's own positions.  Neither carries drafted trees."""
 
     k: list
     v: list
@@ -179,6 +225,9 @@ class KVCache:
     attn_ws: torch.Tensor = field(default=None)
     row_map: torch.Tensor = field(default=None)
     remap: bool = False
+    k_scale: list | None = None
+    v_scale: list | None = None
+    prefix: SharedKV | None = None
 
     def __post_init__(self):
         if self.row_map is None:
@@ -203,7 +252,7 @@ class KVCache:
         if not self.remap:
             raise RuntimeError("swap_slots needs cache.remap: without the map the kernels read "
                                "cache row == slot, and a swap would read another sequence's K/V.")
-        for t in (self.row_map, self.seqlen):
+        for t in (self.row_map, self.seqlen) + (() if self.prefix is None else (self.prefix.of,)):
             a = t[i].clone()
             t[i] = t[j]
             t[j] = a
@@ -211,6 +260,74 @@ class KVCache:
     def reset_slot(self, slot: int) -> None:
         """Forget a slot's history so a new sequence can take it."""
         self.seqlen[slot] = 0
+        if self.prefix is not None:
+            self.prefix.of[slot] = -1
+
+    @property
+    def is_quantized(self) -> bool:
+        return self.k_scale is not None
+
+    def layer(self, i: int):
+        """Layer ``i``'s ``KV`` or ``QuantKV``."""
+        if self.k_scale is None:
+            return KV(self.k[i], self.v[i])
+        return QuantKV(self.k[i], self.v[i], self.k_scale[i], self.v_scale[i])
+
+    def positions(self, width: int) -> torch.Tensor:
+        """Where the next token of slots ``[0, width)`` stands in its sequence: behind
+        its prefix and its own positions."""
+        seqlen, p = self.seqlen[:width], self.prefix
+        if p is None:
+            return seqlen
+        of = p.of[:width]
+        n = p.length.shape[0]
+        return seqlen + torch.where((of >= 0) & (of < n), p.length[of.clamp(0, n - 1)], 0)
+
+    def quantized(self) -> "KVCache":
+        """The same sequences in a quantised cache of their own (bf16 caches without
+        prefixes)."""
+        if self.is_quantized or self.prefix is not None:
+            raise ValueError("quantized takes a bf16 cache without shared prefixes.")
+        out = [quantize_kv(k, v, make_quant_kv(*k.shape, k.device)) for k, v in zip(self.k, self.v)]
+        return KVCache([c.k for c in out], [c.v for c in out], self.seqlen.clone(), self.max_len, self.attn_ws,
+                       self.row_map.clone(), self.remap, [c.k_scale for c in out], [c.v_scale for c in out])
+
+    def dequantized(self) -> "KVCache":
+        """The same sequences, as the codes stand for them, in a bf16 cache of their own."""
+        if not self.is_quantized or self.prefix is not None:
+            raise ValueError("dequantized takes a quantised cache without shared prefixes.")
+        out = [dequantize_kv(self.layer(i)) for i in range(len(self.k))]
+        rows, n_kv, max_len, d = self.k[0].shape
+        return KVCache([c.k for c in out], [c.v for c in out], self.seqlen.clone(), self.max_len,
+                       gqa_workspace(rows, n_kv, max_len, self.seqlen.device, d), self.row_map.clone(), self.remap)
+
+    def share(self, rows, lengths) -> SharedKV:
+        """Take the first ``lengths[p]`` positions of cache row ``rows[p]`` as prefix ``p``
+        (copied: the rows are free again), held once for all slots that begin with it.
+        Every slot begins with none; ``prefix.of[slot] = p`` with ``seqlen[slot]`` set to
+        the slot's own positions (0 for a new sequence) puts one behind prefix ``p``."""
+        rows, lengths = [int(r) for r in rows], [int(n) for n in lengths]
+        if self.prefix is not None:
+            raise ValueError("the cache has shared prefixes already.")
+        if len(rows) != len(lengths) or not rows:
+            raise ValueError(f"share expects a length for each row, got {len(rows)} rows and {len(lengths)} lengths.")
+        if any(not 0 <= r < self.rows for r in rows) or any(not 1 <= n <= self.max_len for n in lengths):
+            raise ValueError(f"share: rows {rows} and lengths {lengths} for a cache of {self.rows} rows of {self.max_len}.")
+        most = max(lengths)
+
+        def take(layers):
+            return None if layers is None else [t[rows, :, :most].contiguous() for t in layers]
+
+        def codes(layers):  # (float8 tensors are indexed as the bytes they are)
+            return None if layers is None else [t.view(torch.uint8)[rows, :, :most].contiguous().view(t.dtype)
+                                                for t in layers]
+
+        kv = codes if self.is_quantized else take
+        dev = self.seqlen.device
+        self.prefix = SharedKV(kv(self.k), kv(self.v), torch.tensor(lengths, device=dev, dtype=torch.int64),
+                               torch.full((self.rows,), -1, device=dev, dtype=torch.int64), codes(self.k_scale),
+                               codes(self.v_scale))
+        return self.prefix
 
     def commit(self, path: torch.Tensor, accepted: torch.Tensor) -> None:
         """Keep an accepted branch of the nodes that ``forward_tree`` wrote behind
@@ -218,6 +335,7 @@ class KVCache:
         returns them for a tree that fits the cache, ``kernels.tree.fit_tree``):
         their K/V move together, in every layer, and the write positions advance
         past them.  Graph-safe; no host synchronisation."""
+        _check_trees(self)
         seqlen, row_map = self.slot_rows(int(accepted.shape[0]))
         seqlen.copy_(commit_tree(self.k, self.v, seqlen, path, accepted, row_map=row_map))
 
@@ -231,18 +349,23 @@ class KVCache:
             lo = int(sl.min()) if sl.numel() else 0
             hi = min(self.max_len, int(sl.max()) + int(steps) + 1) if sl.numel() else 0
         return {"seqlen": self.seqlen.clone(), "row_map": self.row_map.clone(), "remap": self.remap,
-                "span": (lo, hi), "k": [t[:, :, lo:hi].clone() for t in self.k],
-                "v": [t[:, :, lo:hi].clone() for t in self.v]}
+                "of": None if self.prefix is None else self.prefix.of.clone(), "span": (lo, hi),
+                **{n: [_bytes(t)[:, :, lo:hi].clone() for t in ts] for n, ts in self._tensors().items()}}
+
+    def _tensors(self) -> dict:
+        names = ("k", "v", "k_scale", "v_scale") if self.is_quantized else ("k", "v")
+        return {n: getattr(self, n) for n in names}
 
     def restore(self, snap: dict) -> None:
         self.seqlen.copy_(snap["seqlen"])
         self.row_map.copy_(snap["row_map"])
         self.remap = snap["remap"]
+        if self.prefix is not None and snap["of"] is not None:
+            self.prefix.of.copy_(snap["of"])
         lo, hi = snap["span"]
-        for dst, src in zip(self.k, snap["k"]):
-            dst[:, :, lo:hi].copy_(src)
-        for dst, src in zip(self.v, snap["v"]):
-            dst[:, :, lo:hi].copy_(src)
+        for n, ts in self._tensors().items():
+            for dst, src in zip(ts, snap[n]):
+                _bytes(dst)[:, :, lo:hi].copy_(src)
 
 
 class SyntheticDecoder:
@@ -320,11 +443,14 @@ class SyntheticDecoder:
             self.layers[i] = dataclasses.replace(L, post_ln=views[0], q_norm=views[1], k_norm=views[2], moe=moe)
             self.read_ahead.append(buf)
 
-    def make_cache(self, batch: int, prefill_len: int, seed: int = 0) -> KVCache:
+    def make_cache(self, batch: int, prefill_len: int, seed: int = 0, *, quantized: bool = False,
+                   max_len: int | None = None) -> KVCache:
         """Cache rows filled with seeded N(0, 1) bf16 K/V for ``prefill_len``
-        positions; decoding then writes at ``prefill_len``."""
+        positions, of ``max_len`` (by default the model's); decoding then writes at
+        ``prefill_len``.  ``quantized``: the same values in a quantised cache."""
         c = self.cfg
-        shape = (batch, c.kv_heads, self.max_len, c.head_dim)
+        max_len = self.max_len if max_len is None else max_len
+        shape = (batch, c.kv_heads, max_len, c.head_dim)
         ks, vs = [], []
         for i in range(c.layers):
             k = synthetic.randn_bf16(shape, 50_000 + seed * 97 + 2 * i, self.device)
@@ -334,11 +460,45 @@ class SyntheticDecoder:
             ks.append(k)
             vs.append(v)
         seqlen = torch.full((batch,), prefill_len, device=self.device, dtype=torch.int64)
-        ws = gqa_workspace(batch, c.kv_heads, self.max_len, self.device, c.head_dim)
-        return KVCache(ks, vs, seqlen, self.max_len, ws)
+        ws = gqa_workspace(batch, c.kv_heads, max_len, self.device, c.head_dim)
+        cache = KVCache(ks, vs, seqlen, max_len, ws)
+        return cache.quantized() if quantized else cache
+
+    def _places(self, cache: KVCache, width: int):
+        """What a step over slots ``[0, width)`` of a quantised cache, or of one with
+        shared prefixes, needs in every layer: the new tokens' positions and, for a
+        bf16 cache, the RoPE rows there.  None for any other cache."""
+        if cache.prefix is None and not cache.is_quantized:
+            return None
+        if cache.prefix is not None and cache.prefix.max_len + cache.max_len > self.cos.shape[0]:
+            raise ValueError(f"rotary tables of {self.cos.shape[0]} positions for prefixes of {cache.prefix.max_len} and "
+                             f"rows of {cache.max_len}: give the model a larger max_len.")
+        pos = cache.positions(width)
+        if cache.is_quantized:
+            return pos, None, None
+        at = pos.clamp(0, self.cos.shape[0] - 1)
+        return pos, self.cos[at], self.sin[at]
+
+    def _cached_attention(self, i: int, qkv: torch.Tensor, cache: KVCache, seqlen: torch.Tensor, places, akw: dict):
+        """Layer ``i``'s store and attention over a quantised cache or behind shared
+        prefixes."""
+        c, L = self.cfg, self.layers[i]
+        pos, cos, sin = places
+        kw = dict(num_heads=c.heads, num_kv_heads=c.kv_heads, head_dim=c.head_dim, rotary_dim=c.rotary_dim,
+                  use_rope=akw["use_rope"], eps=c.eps, row_map=akw["row_map"])
+        kv = cache.layer(i)
+        if cache.is_quantized:
+            q = apply_qkv_quant(qkv, L.q_norm, L.k_norm, self.cos, self.sin, kv, seqlen, positions=pos, **kw)
+        else:
+            q = apply_qkv_decode(qkv, L.q_norm, L.k_norm, cos, sin, kv.k, kv.v, seqlen, use_qk_norm=True, **kw)
+        kw = dict(row_map=akw["row_map"], scale=akw["scale"], window=akw["window"])
+        if cache.prefix is None:
+            return quant_gqa_attn(q, kv, seqlen, **kw)
+        return prefix_gqa_attn(q, kv, seqlen, cache.prefix.layer(i, qkv.shape[0]), **kw)
 
     def _layer(self, i: int, hidden: torch.Tensor, cache: KVCache, routing=None,
-               qkv: torch.Tensor | None = None, fuse_next: bool = True, tree: torch.Tensor | None = None):
+               qkv: torch.Tensor | None = None, fuse_next: bool = True, tree: torch.Tensor | None = None,
+               places=None):
         """Layer ``i``; returns ``(y, next_qkv)``.  ``qkv``: this layer's input
         projection if an earlier launch already computed it.  ``next_qkv`` is
         layer ``i + 1``'s projection when the one-launch MoE kernel computed it
@@ -346,7 +506,7 @@ class SyntheticDecoder:
         ``PendingCombine`` where layer ``i + 1``'s QKV launch runs the MoE
         combine (``combine_next``, 17+ tokens); ``hidden`` may be one.
         ``tree [w, T]``: the parents of the ``w * T`` nodes that ``hidden``
-        holds, instead of one token per slot."""
+        holds, instead of one token per slot.  ``places``: ``_places`` of the step."""
         c, L = self.cfg, self.layers[i]
         if isinstance(hidden, PendingCombine):  # the previous layer's MoE combine runs here
             hidden, qkv = ternary_gemv_combine(hidden, L.qkv, L.qkv_alpha, rms_weight=L.input_ln,
@@ -360,7 +520,7 @@ class SyntheticDecoder:
                    use_rope=use_rope)
         seqlen, row_map = cache.slot_rows(bsz if tree is None else tree.shape[0])
         akw["row_map"] = row_map
-        if bsz == 1 and tree is None and self.fused_o and o_projection_supported(1, c.heads, c.kv_heads, c.head_dim,
+        if bsz == 1 and tree is None and places is None and self.fused_o and o_projection_supported(1, c.heads, c.kv_heads, c.head_dim,
                                                                 cache.max_len, window, c.hidden):
             # attention and its output projection in one launch (measured: no
             # faster than two launches at 4096 positions -- the grid barrier
@@ -368,7 +528,9 @@ class SyntheticDecoder:
             _, o = decode_attention(qkv, L.q_norm, L.k_norm, self.cos, self.sin, cache.k[i], cache.v[i],
                                     seqlen, cache.attn_ws, o_linear=(L.o, L.o_alpha), **akw)
         else:
-            if tree is None:
+            if places is not None:
+                attn = self._cached_attention(i, qkv, cache, seqlen, places, akw)
+            elif tree is None:
                 attn = decode_attention(qkv, L.q_norm, L.k_norm, self.cos, self.sin, cache.k[i], cache.v[i],
                                         seqlen, cache.attn_ws, **akw)
             else:
@@ -415,7 +577,7 @@ class SyntheticDecoder:
 
     def layer_step(self, i: int, hidden: torch.Tensor, cache: KVCache, routing=None) -> torch.Tensor:
         """Layer ``i`` on its own (its QKV projection computed here)."""
-        return self._layer(i, hidden, cache, routing, fuse_next=False)[0]
+        return self._layer(i, hidden, cache, routing, fuse_next=False, places=self._places(cache, hidden.shape[0]))[0]
 
     def forward(self, input_ids: torch.Tensor, cache: KVCache, routing: list | None = None) -> torch.Tensor:
         """One decode step for ``input_ids [w]`` over cache slots ``[0, w)``;
@@ -425,8 +587,9 @@ class SyntheticDecoder:
         cache.slot_rows(width)
         hidden = self.embed_tokens(input_ids.reshape(-1))
         qkv = None
+        places = self._places(cache, width)
         for i in range(self.cfg.layers):
-            hidden, qkv = self._layer(i, hidden, cache, routing, qkv)
+            hidden, qkv = self._layer(i, hidden, cache, routing, qkv, places=places)
         cache.seqlen[:width].add_(1)
         return self.head(hidden)
 
@@ -440,6 +603,7 @@ class SyntheticDecoder:
         rounding, from the head that such steps use: at one row the FlashHead, if
         one is attached, node by node.  Padding's logits say nothing."""
         w, t = tokens.shape
+        _check_trees(cache)
         cache.slot_rows(w)
         parents = check_tree("forward_tree", parents, w, t)  # (once, not in each layer)
         hidden = self.embed_tokens(tokens.reshape(-1))  # (padding's ids are clamped to the table)
