@@ -55,17 +55,27 @@ struct CacheAttn {
   uint16_t* out;
 };
 
+// What a workgroup's first loads need: arguments of their own ahead of the others,
+// which arrive in registers.
+struct CacheHot {
+  const int64_t* seqlen;
+  const int64_t* row_map;
+  const int64_t* of;
+  const int64_t* length;
+  int nq, nkv, s_own, s_pre, batch;
+};
+
 // Positions of row b: its prefix's, its own, and the first one seen.
 struct CacheSpan {
   int64_t pre_row, pre_n, own_n, lo;
 };
-__device__ __forceinline__ CacheSpan cache_span(const CacheAttn& a, int64_t b) {
-  CacheSpan s{0, 0, clamp_pos(a.seqlen[b], -1, a.own.max_len - 1) + 1, 0};
-  if (a.of) {
-    const int64_t p = a.of[b];
+__device__ __forceinline__ CacheSpan cache_span(const CacheAttn& a, const CacheHot& hot, int64_t b) {
+  CacheSpan s{0, 0, clamp_pos(hot.seqlen[b], -1, a.own.max_len - 1) + 1, 0};
+  if (hot.of) {
+    const int64_t p = hot.of[b];
     if (p >= 0 && p < a.pre.rows) {
       s.pre_row = p;
-      s.pre_n = clamp_pos(a.length[p], 0, a.pre.max_len);
+      s.pre_n = clamp_pos(hot.length[p], 0, a.pre.max_len);
     }
   }
   const int64_t n = s.pre_n + s.own_n;
@@ -139,7 +149,7 @@ struct OwnLds {
   float m[kCacheWaves][kCacheGroup], l[kCacheWaves][kCacheGroup];
 };
 template <int HD, bool Q8>
-__device__ __forceinline__ void cache_own(const CacheAttn& a, int wg, OwnLds<HD>& lds) {
+__device__ __forceinline__ void cache_own(const CacheAttn& a, const CacheHot& hot, int wg, OwnLds<HD>& lds) {
   constexpr int NW = kCacheWaves;
   constexpr int RB = Q8 ? HD : 2 * HD;      // bytes of a cached position
   constexpr int KL = RB / 64;               // 16-byte loads of K a lane and 16 positions
@@ -153,25 +163,25 @@ __device__ __forceinline__ void cache_own(const CacheAttn& a, int wg, OwnLds<HD>
   const int tid = threadIdx.x, lane = tid & 63;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r16 = lane & 15, g = lane >> 4;
-  const int sp = wg % a.s_own;
-  const int64_t pair = wg / a.s_own, b = pair / a.nkv;
-  const int kvh = static_cast<int>(pair - b * a.nkv);
-  const int group = a.nq / a.nkv;
-  const CacheSpan span = cache_span(a, b);
-  const int64_t crow = a.row_map ? clamp_pos(a.row_map[b], 0, a.own.rows - 1) : b;
+  const int sp = wg % hot.s_own;
+  const int64_t pair = wg / hot.s_own, b = pair / hot.nkv;
+  const int kvh = static_cast<int>(pair - b * hot.nkv);
+  const int group = hot.nq / hot.nkv;
+  const CacheSpan span = cache_span(a, hot, b);
+  const int64_t crow = hot.row_map ? clamp_pos(hot.row_map[b], 0, a.own.rows - 1) : b;
 
   // tiles: of the prefix where each row reads it itself, then of the row's own
-  const int64_t a0 = a.s_pre > 0 ? 0 : (span.lo < span.pre_n ? span.lo : span.pre_n);
-  const int64_t a1 = a.s_pre > 0 ? 0 : span.pre_n;
+  const int64_t a0 = hot.s_pre > 0 ? 0 : (span.lo < span.pre_n ? span.lo : span.pre_n);
+  const int64_t a1 = hot.s_pre > 0 ? 0 : span.pre_n;
   const int64_t b0 = span.lo > span.pre_n ? span.lo - span.pre_n : 0, b1 = span.own_n;
   const int na = static_cast<int>(cdiv(a1 - a0, 32)), nt = na + static_cast<int>(cdiv(b1 - b0, 32));
-  const int rounds = (nt + NW - 1) / NW, per = (rounds + a.s_own - 1) / a.s_own * NW;
+  const int rounds = (nt + NW - 1) / NW, per = (rounds + hot.s_own - 1) / hot.s_own * NW;
   const int t_beg = sp * per < nt ? sp * per : nt;
   const int t_end = t_beg + per < nt ? t_beg + per : nt;
 
   uint4 qf[KS];
   {
-    const uint16_t* const src = a.q + (b * a.nq + kvh * group + (r16 < group ? r16 : 0)) * HD;
+    const uint16_t* const src = a.q + (b * hot.nq + kvh * group + (r16 < group ? r16 : 0)) * HD;
     const uint32_t keep = r16 < group ? 0xffffffffu : 0u;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
@@ -192,7 +202,7 @@ __device__ __forceinline__ void cache_own(const CacheAttn& a, int wg, OwnLds<HD>
     const int64_t p = mine ? b0 + 32 * static_cast<int64_t>(t - na) : a0 + 32 * static_cast<int64_t>(t);
     const int64_t left = (mine ? b1 : a1) - p;
     x.n = left < 32 ? static_cast<int>(left) : 32;
-    const int64_t at = mine ? (crow * a.nkv + kvh) * own.max_len + p : (span.pre_row * a.nkv + kvh) * pre.max_len + p;
+    const int64_t at = mine ? (crow * hot.nkv + kvh) * own.max_len + p : (span.pre_row * hot.nkv + kvh) * pre.max_len + p;
     const uint8_t* const kp = (mine ? own.k : pre.k) + at * RB;
     const uint8_t* const vp = (mine ? own.v : pre.v) + at * RB;
     // (positions past the end read the last one again: their scores are masked)
@@ -331,7 +341,7 @@ __device__ __forceinline__ void cache_own(const CacheAttn& a, int wg, OwnLds<HD>
     for (int i = 0; i < 4; ++i)
       if (4 * g + i < group) ow[wv][4 * g + i][16 * nb + r16] = o[nb][i];
   __syncthreads();
-  const int st = a.s_own + a.s_pre;
+  const int st = hot.s_own + hot.s_pre;
   for (int item = tid; item < group * (HD / 4); item += kCacheThreads) {
     const int hh = item / (HD / 4), d = item % (HD / 4) * 4;
     float M = wm[0][hh];
@@ -349,7 +359,7 @@ __device__ __forceinline__ void cache_own(const CacheAttn& a, int wg, OwnLds<HD>
       s.z += f * v.z;
       s.w += f * v.w;
     }
-    const int64_t row = b * a.nq + kvh * group + hh;
+    const int64_t row = b * hot.nq + kvh * group + hh;
     if (st > 1) {
       const int64_t p = row * st + sp;
       if (t_beg < t_end) *reinterpret_cast<float4*>(a.acc + p * HD + d) = s;
@@ -387,7 +397,7 @@ struct PrefixLds {
 // the weights' sum shows that it has become too low (any that keeps them in range
 // gives the same quotient).
 template <int HD, bool Q8>
-__device__ __forceinline__ void cache_prefix(const CacheAttn& a, int slot, int unit, PrefixLds<HD>& lds) {
+__device__ __forceinline__ void cache_prefix(const CacheAttn& a, const CacheHot& hot, int slot, int unit, PrefixLds<HD>& lds) {
   constexpr int NW = kCacheWaves;
   constexpr int RB = Q8 ? HD : 2 * HD;   // bytes of a cached position
   constexpr int XL = 32 * RB / 1024;     // 16-byte loads a lane and tile, K and V each
@@ -398,19 +408,19 @@ __device__ __forceinline__ void cache_prefix(const CacheAttn& a, int slot, int u
   const int tid = threadIdx.x, lane = tid & 63;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r32 = lane & 31, h = lane >> 5;
-  const int sp = unit % a.s_pre, kvh = unit / a.s_pre;
-  const int group = a.nq / a.nkv;
+  const int sp = unit % hot.s_pre, kvh = unit / hot.s_pre;
+  const int group = hot.nq / hot.nkv;
 
   // Which prefix and tile the slot is: the prefixes' tiles follow each other.
   const int np = static_cast<int>(a.pre.rows);  // (at most 64)
-  const int64_t of0 = a.of[tid < a.batch ? tid : 0];
-  int64_t length = a.length[lane < np ? lane : 0];
+  const int64_t of0 = hot.of[tid < hot.batch ? tid : 0];
+  int64_t length = hot.length[lane < np ? lane : 0];
   int pre = 0, tile = slot;
   if (np > 1) {
     if (tid < 64) lds.hist[tid] = 0;
     __syncthreads();
-    for (int b0 = tid; b0 < a.batch; b0 += kCacheThreads) {
-      const int64_t p = b0 == tid ? of0 : a.of[b0];
+    for (int b0 = tid; b0 < hot.batch; b0 += kCacheThreads) {
+      const int64_t p = b0 == tid ? of0 : hot.of[b0];
       if (p >= 0 && p < np) atomicAdd(&lds.hist[p], 1);
     }
     __syncthreads();
@@ -429,11 +439,11 @@ __device__ __forceinline__ void cache_prefix(const CacheAttn& a, int slot, int u
   }
   const int64_t end = clamp_pos(length, 0, a.pre.max_len);
   const int nt = static_cast<int>(cdiv(end, 32)), rounds = (nt + NW - 1) / NW;
-  const int per = (rounds + a.s_pre - 1) / a.s_pre * NW;
+  const int per = (rounds + hot.s_pre - 1) / hot.s_pre * NW;
   const int t_beg = sp * per < nt ? sp * per : nt;
   const int t_end = t_beg + per < nt ? t_beg + per : nt;
   const int t0 = t_beg + wv, last = t0 + (t_end - 1 - t0) / NW * NW;
-  const int64_t base = (static_cast<int64_t>(pre) * a.nkv + kvh) * a.pre.max_len;
+  const int64_t base = (static_cast<int64_t>(pre) * hot.nkv + kvh) * a.pre.max_len;
 
   struct Tile {
     u32x4c_t k[XL], v[XL];
@@ -475,8 +485,8 @@ __device__ __forceinline__ void cache_prefix(const CacheAttn& a, int slot, int u
   auto& mem = lds.mem;
   const int first = tile * kPrefixRows / group, final = (tile * kPrefixRows + kPrefixRows - 1) / group;
   int members = 0;
-  for (int b0 = 0; b0 < a.batch; b0 += kCacheThreads) {
-    const bool is = b0 + tid < a.batch && (b0 == 0 ? of0 : a.of[b0 + tid]) == pre;
+  for (int b0 = 0; b0 < hot.batch; b0 += kCacheThreads) {
+    const bool is = b0 + tid < hot.batch && (b0 == 0 ? of0 : hot.of[b0 + tid]) == pre;
     const uint64_t m = __ballot(is);
     if (lane == 0) lds.count[wv] = static_cast<int>(__popcll(m));
     __syncthreads();
@@ -500,7 +510,7 @@ __device__ __forceinline__ void cache_prefix(const CacheAttn& a, int slot, int u
   {
     const bool on = r < M;
     const int64_t b = mem[(on ? r / group : first) - first];
-    const uint16_t* const src = a.q + (b * a.nq + kvh * group + (on ? r % group : 0)) * HD;
+    const uint16_t* const src = a.q + (b * hot.nq + kvh * group + (on ? r % group : 0)) * HD;
     const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u, keep = on && a.scale != 0.f ? 0xffffffffu : 0u;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
@@ -663,7 +673,7 @@ __device__ __forceinline__ void cache_prefix(const CacheAttn& a, int slot, int u
 #pragma unroll
     for (int db = 0; db < DB; ++db) lds.sums[wv][8 * (i >> 2) + 4 * h + (i & 3)][32 * db + r32] = o[db][i];
   __syncthreads();
-  const int st = a.s_own + a.s_pre;
+  const int st = hot.s_own + hot.s_pre;
 #pragma unroll
   for (int item = tid; item < kPrefixRows * (HD / 4); item += kCacheThreads) {
     const int row = item / (HD / 4), d = item % (HD / 4) * 4, q = tile * kPrefixRows + row;
@@ -684,34 +694,39 @@ __device__ __forceinline__ void cache_prefix(const CacheAttn& a, int slot, int u
       s.z += f * v.z;
       s.w += f * v.w;
     }
-    const int64_t p = (static_cast<int64_t>(mem[q / group - first]) * a.nq + kvh * group + q % group) * st + a.s_own + sp;
+    const int64_t p = (static_cast<int64_t>(mem[q / group - first]) * hot.nq + kvh * group + q % group) * st + hot.s_own + sp;
     if (t_beg < t_end) *reinterpret_cast<float4*>(a.acc + p * HD + d) = s;
     if (d == 0) a.ml[p] = make_float2(m, l);
   }
 }
 
 template <int HD, bool Q8>
-__global__ __launch_bounds__(kCacheThreads, (HD == 64 ? 4 : (Q8 ? 3 : 2))) void k_cache_own(CacheAttn a) {
+__global__ __launch_bounds__(kCacheThreads, (HD == 64 ? 4 : (Q8 ? 3 : 2))) void k_cache_own(
+    const int64_t* seqlen, const int64_t* row_map, const int64_t* of, const int64_t* length, int nq, int nkv, int s_own,
+    CacheAttn a) {
   __shared__ __align__(16) OwnLds<HD> lds;
-  cache_own<HD, Q8>(a, blockIdx.x, lds);
+  cache_own<HD, Q8>(a, CacheHot{seqlen, row_map, of, length, nq, nkv, s_own, 0, 0}, blockIdx.x, lds);
 }
 
 // The first `tiles` x units (rounded up to the XCDs) workgroups the prefixes, where
 // the tiles of the same positions fall to one XCD, the others the rows' own parts.
 template <int HD, bool Q8>
-__global__ __launch_bounds__(kCacheThreads, 2) void k_cache_both(CacheAttn a, int tiles, int n_units) {
+__global__ __launch_bounds__(kCacheThreads, 2) void k_cache_both(
+    const int64_t* seqlen, const int64_t* row_map, const int64_t* of, const int64_t* length, int n_units, int tiles,
+    int s_pre, int batch, int nq, int nkv, int s_own, CacheAttn a) {
   __shared__ __align__(16) union Lds {
     OwnLds<HD> own;
     PrefixLds<HD> prefix;
   } lds;
+  const CacheHot hot{seqlen, row_map, of, length, nq, nkv, s_own, s_pre, batch};
   const int padded = (n_units + kXcds - 1) / kXcds * kXcds;
   const int wg = blockIdx.x;
   if (wg >= padded * tiles) {
-    cache_own<HD, Q8>(a, wg - padded * tiles, lds.own);
+    cache_own<HD, Q8>(a, hot, wg - padded * tiles, lds.own);
     return;
   }
   const int tile = wg / padded, unit = wg - tile * padded;
-  if (unit < n_units) cache_prefix<HD, Q8>(a, tile, unit, lds.prefix);
+  if (unit < n_units) cache_prefix<HD, Q8>(a, hot, tile, unit, lds.prefix);
 }
 
 // ---------------------------------------------------------------------------
@@ -931,13 +946,15 @@ extern "C" int ma_cache_attn(const void* q, int64_t batch, int n_heads, int n_kv
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (p.s_pre > 0) {
     auto go = [&](auto kernel) {
-      hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(pre_wgs + own_wgs)), dim3(kCacheThreads), 0, s, a, p.tiles, static_cast<int>(units));
+      hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(pre_wgs + own_wgs)), dim3(kCacheThreads), 0, s, a.seqlen,
+                         a.row_map, a.of, a.length, static_cast<int>(units), p.tiles, a.s_pre, a.batch, a.nq, a.nkv, a.s_own, a);
     };
     if (head_dim == 64) q8 ? go(k_cache_both<64, true>) : go(k_cache_both<64, false>);
     else q8 ? go(k_cache_both<128, true>) : go(k_cache_both<128, false>);
   } else {
     auto go = [&](auto kernel) {
-      hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(own_wgs)), dim3(kCacheThreads), 0, s, a);
+      hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(own_wgs)), dim3(kCacheThreads), 0, s, a.seqlen, a.row_map,
+                         a.of, a.length, a.nq, a.nkv, a.s_own, a);
     };
     if (head_dim == 64) q8 ? go(k_cache_own<64, true>) : go(k_cache_own<64, false>);
     else q8 ? go(k_cache_own<128, true>) : go(k_cache_own<128, false>);
