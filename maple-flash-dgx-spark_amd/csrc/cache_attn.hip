@@ -847,7 +847,9 @@ static int64_t cache_window(int64_t window, int64_t max_len, int64_t pre_len) {
 //     2 x 32768: 17.9, 12.8, 12.2, 13.0
 //   4 x 4096 of 128: 11.6, 10.2, 11.9 for 512;  8 x 32768: 83, 54, 51, 53
 //   prefixes, 32 rows behind 8192 of 64: 18.4, 14.5, 17.1;  behind 32768: 44, 28, 26;
-//     64 behind four of 8192: 49, 24, 20;  64 behind 8192 of 128: 29, 22, 28
+//     64 behind two of 2000: 13.7 for 256, 17.6 for 512;  behind four of 4096: 15.9,
+//     16.0, 17.2 for 640;  of 8192: 20.7, 19.1, 20.2;  of 16384: 31.0, 23.6, 28.1;
+//     64 behind 8192 of 128: 29 for 128, 22, 28
 static CachePlan cache_plan(int64_t batch, int nq, int nkv, int64_t max_len, int64_t prefixes, int64_t pre_len, int64_t window) {
   CachePlan p{1, 0, 0};
   const int64_t pairs = batch * nkv;
@@ -864,8 +866,9 @@ static CachePlan cache_plan(int64_t batch, int nq, int nkv, int64_t max_len, int
     // tiles in all, each prefix's last one part empty
     const int64_t some = prefixes < batch ? prefixes : batch;
     p.tiles = static_cast<int>((batch * (nq / nkv) + (kPrefixRows - 1) * some) / kPrefixRows);
-    const int64_t rounds = cdiv(pre_len, 128), units = nkv * p.tiles;
-    s = 256 / units;
+    // (splits by the tiles to expect: of every prefix but one, half of the last one is empty)
+    const int64_t rounds = cdiv(pre_len, 128), units = nkv * cdiv(batch * (nq / nkv) + kPrefixRows / 2 * (some - 1), kPrefixRows);
+    s = (256 + units / 2) / units;
     if (rounds > 16 * (s < 1 ? 1 : s)) s = cdiv(512, units);
     s = s < 1 ? 1 : s;
     p.s_pre = static_cast<int>(s < rounds ? s : rounds);
