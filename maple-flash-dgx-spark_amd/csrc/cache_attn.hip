@@ -108,6 +108,18 @@ __device__ __forceinline__ f32x16c_t mfma32(uint4 a, uint4 b, f32x16c_t c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8c_t, a), __builtin_bit_cast(bf16x8c_t, b), c, 0, 0, 0);
 }
 
+// The bytes of a tile's positions; past them reads give 0, so that where a part ends
+// inside a tile the positions behind it are 0 under a weight of 0, whatever the cache
+// holds there.
+struct TileBytes {
+  __amdgpu_buffer_rsrc_t r;
+  __device__ __forceinline__ TileBytes(const uint8_t* p, int bytes)
+      : r(__builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p), 0, bytes, 0x00020000)) {}
+  __device__ __forceinline__ u32x4c_t at(int off) const {
+    return __builtin_bit_cast(u32x4c_t, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0));
+  }
+};
+
 // 16 bytes of a tile's 32 V rows a lane, into the wave's LDS rows as bf16.  s_of(row):
 // the row's scale (quantised).
 template <int HD, bool Q8, int VL, typename S>
@@ -203,20 +215,13 @@ __device__ __forceinline__ void cache_own(const CacheAttn& a, const CacheHot& ho
     const int64_t left = (mine ? b1 : a1) - p;
     x.n = left < 32 ? static_cast<int>(left) : 32;
     const int64_t at = mine ? (crow * hot.nkv + kvh) * own.max_len + p : (span.pre_row * hot.nkv + kvh) * pre.max_len + p;
-    const uint8_t* const kp = (mine ? own.k : pre.k) + at * RB;
-    const uint8_t* const vp = (mine ? own.v : pre.v) + at * RB;
-    // (positions past the end read the last one again: their scores are masked)
+    const TileBytes kt((mine ? own.k : pre.k) + at * RB, x.n * RB), vt((mine ? own.v : pre.v) + at * RB, x.n * RB);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int row = 16 * h + r16 < x.n ? 16 * h + r16 : x.n - 1;
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int j = 0; j < KL; ++j) x.k[h][j] = *reinterpret_cast<const u32x4c_t*>(kp + row * RB + 64 * j + 16 * g);
-    }
+      for (int j = 0; j < KL; ++j) x.k[h][j] = kt.at((16 * h + r16) * RB + 64 * j + 16 * g);
 #pragma unroll
-    for (int i = 0; i < VL; ++i) {
-      const int at16 = i * 64 + lane, row = at16 / (RB / 16);
-      x.v[i] = *reinterpret_cast<const u32x4c_t*>(vp + (row < x.n ? row : x.n - 1) * RB + 16 * (at16 % (RB / 16)));
-    }
+    for (int i = 0; i < VL; ++i) x.v[i] = vt.at(1024 * i + 16 * lane);
     if constexpr (Q8) {
       const int row = (lane & 31) < x.n ? lane & 31 : x.n - 1;
       const uint8_t* const s = lane < 32 ? (mine ? own.ks : pre.ks) : (mine ? own.vs : pre.vs);
@@ -414,7 +419,7 @@ __device__ __forceinline__ void cache_prefix(const CacheAttn& a, const CacheHot&
   // Which prefix and tile the slot is: the prefixes' tiles follow each other.
   const int np = static_cast<int>(a.pre.rows);  // (at most 64)
   const int64_t of0 = hot.of[tid < hot.batch ? tid : 0];
-  int64_t length = hot.length[lane < np ? lane : 0];
+  int64_t length = hot.length[lane < np ? lane : 0];  // (a lane each; below, the one prefix's)
   int pre = 0, tile = slot;
   if (np > 1) {
     if (tid < 64) lds.hist[tid] = 0;
@@ -435,8 +440,9 @@ __device__ __forceinline__ void cache_prefix(const CacheAttn& a, const CacheHot&
     if (past == 0) return;
     pre = __builtin_ctzll(past);
     tile = slot - __builtin_amdgcn_readlane(upto - mine, pre);
-    length = __shfl(length, pre, 64);
   }
+  length = static_cast<int64_t>(static_cast<uint64_t>(__builtin_amdgcn_readlane(static_cast<int>(length >> 32), pre)) << 32 |
+                                static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(length), pre)));
   const int64_t end = clamp_pos(length, 0, a.pre.max_len);
   const int nt = static_cast<int>(cdiv(end, 32)), rounds = (nt + NW - 1) / NW;
   const int per = (rounds + hot.s_pre - 1) / hot.s_pre * NW;
@@ -453,23 +459,13 @@ __device__ __forceinline__ void cache_prefix(const CacheAttn& a, const CacheHot&
   auto load = [&](Tile& x, int t) {
     const int64_t at = base + 32 * static_cast<int64_t>(t), left = end - 32 * static_cast<int64_t>(t);
     x.n = left < 32 ? static_cast<int>(left) : 32;
-    const uint8_t* const kp = a.pre.k + at * RB;
-    const uint8_t* const vp = a.pre.v + at * RB;
-    // (positions past the end read the last one again: their scores are masked)
-    uint32_t off[XL];
-#pragma unroll
-    for (int i = 0; i < XL; ++i) {
-      const int at16 = i * 64 + lane, row = at16 / (RB / 16);
-      off[i] = (row < x.n ? row : x.n - 1) * RB + 16 * (at16 % (RB / 16));
-    }
+    const TileBytes kt(a.pre.k + at * RB, x.n * RB), vt(a.pre.v + at * RB, x.n * RB);
     // (K codes as the products take them: 32 bytes of each row at a time)
-    const int mine = r32 < x.n ? r32 : x.n - 1;
 #pragma unroll
-    for (int i = 0; i < XL; ++i)
-      x.k[i] = *reinterpret_cast<const u32x4c_t*>(kp + (Q8 ? static_cast<uint32_t>(mine * RB + 32 * i + 16 * h) : off[i]));
+    for (int i = 0; i < XL; ++i) x.k[i] = kt.at(Q8 ? r32 * RB + 32 * i + 16 * h : 1024 * i + 16 * lane);
 #pragma unroll
-    for (int i = 0; i < XL; ++i) x.v[i] = *reinterpret_cast<const u32x4c_t*>(vp + off[i]);
-    if constexpr (Q8) x.scale = (lane < 32 ? a.pre.ks : a.pre.vs)[at + mine];
+    for (int i = 0; i < XL; ++i) x.v[i] = vt.at(1024 * i + 16 * lane);
+    if constexpr (Q8) x.scale = (lane < 32 ? a.pre.ks : a.pre.vs)[at + (r32 < x.n ? r32 : x.n - 1)];
   };
   // (Loads run past the wave's last tile, on it again: after one that a branch may
   // have skipped every wait would be for all of them.)

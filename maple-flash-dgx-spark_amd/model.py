@@ -360,8 +360,8 @@ class KVCache:
         self.seqlen.copy_(snap["seqlen"])
         self.row_map.copy_(snap["row_map"])
         self.remap = snap["remap"]
-        if self.prefix is not None and snap["of"] is not None:
-            self.prefix.of.copy_(snap["of"])
+        if self.prefix is not None:
+            self.prefix.of.fill_(-1) if snap["of"] is None else self.prefix.of.copy_(snap["of"])
         lo, hi = snap["span"]
         for n, ts in self._tensors().items():
             for dst, src in zip(ts, snap[n]):
@@ -449,7 +449,9 @@ class SyntheticDecoder:
         positions, of ``max_len`` (by default the model's); decoding then writes at
         ``prefill_len``.  ``quantized``: the same values in a quantised cache."""
         c = self.cfg
-        max_len = self.max_len if max_len is None else max_len
+        max_len = self.max_len if max_len is None else int(max_len)
+        if not 1 <= max_len <= self.max_len:
+            raise ValueError(f"make_cache: rows of {max_len} positions, the model has {self.max_len}.")
         shape = (batch, c.kv_heads, max_len, c.head_dim)
         ks, vs = [], []
         for i in range(c.layers):

@@ -393,6 +393,22 @@ def test_attn_what_is_not_finite_and_seen_does(dev):
     assert torch.isnan(out[0]).all() and torch.isfinite(out[1]).all()
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("at", ["own", "prefix"])
+def test_attn_infinite_values(dev, d, at):
+    """An infinite V, at the last position of a tile that is not full, is infinite in its dim and leaves the others."""
+    from maple_amd.kernels import KV, SharedPrefix, prefix_gqa_attn
+
+    own = KV(bf16(dev, 2, 2, 50, d, seed=30), bf16(dev, 2, 2, 50, d, seed=31))
+    pre = KV(bf16(dev, 1, 2, 75, d, seed=32), bf16(dev, 1, 2, 75, d, seed=33))
+    (own.v[0, :, 49] if at == "own" else pre.v[0, :, 74])[:, 5] = float("inf")
+    out = prefix_gqa_attn(bf16(dev, 2, 4, 1, d), own, i64(dev, [49, 20]),
+                          SharedPrefix(pre, i64(dev, [75]), i64(dev, [0, -1])), scale=d ** -0.5)
+    assert (out[0, :, 0, 5] == float("inf")).all()
+    out[0, :, 0, 5] = 0
+    assert torch.isfinite(out).all()
+
+
 @pytest.mark.parametrize("scale", [0.0, -0.125, 1e-30, 2.0])
 def test_attn_scales(dev, scale):
     # (at scale 2 scores reach 2^6.5 and their float32 errors 2^-15 of a weight: inside 2^-12)
@@ -491,6 +507,17 @@ def test_prefix_many_rows(dev, quant, nq, nkv):
     seqlen = [int(x) for x in g.integers(-1, 9, 333)]
     check_attn(dev, make(dev, quant, 333, nkv, 9, 64, 52), seqlen, nq,
                prefix=(make(dev, quant, 6, nkv, 90, 64, 54), [90, 1, 40, 7, 2 ** 40, -5], of))
+
+
+@pytest.mark.parametrize("quant", [False, True])
+@pytest.mark.parametrize("prefixes", [64, 65, 130])
+def test_prefix_many_prefixes(dev, quant, prefixes):
+    """As many as are read once for all of their rows, and more, which each row reads with its own positions."""
+    g = np.random.default_rng(prefixes)
+    of = [int(x) for x in g.integers(-1, prefixes + 1, 150)] + [prefixes - 1, 0]
+    seqlen = [int(x) for x in g.integers(-1, 40, 152)]
+    check_attn(dev, make(dev, quant, 152, 2, 40, 64, 55), seqlen, 4,
+               prefix=(make(dev, quant, prefixes, 2, 77, 64, 57), [int(x) for x in g.integers(0, 78, prefixes)], of))
 
 
 def test_prefix_long_and_split(dev):
