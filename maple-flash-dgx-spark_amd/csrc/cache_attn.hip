@@ -835,7 +835,7 @@ static int64_t cache_window(int64_t window, int64_t max_len, int64_t pre_len) {
 //
 // Splits, planned for the caches' lengths (the host does not know the rows').  A
 // workgroup a compute unit; two where a split would still hold more than 1024 of a
-// row's positions, or 2048 of a prefix; none of a row's where that saves less than the
+// row's positions, or 2048 and more of a prefix; none of a row's where that saves less than the
 // launch that joins them (about 4 us, six rounds of 128 positions).  Measured (us,
 // for this many workgroups):
 //   1 x 4096 of 64: 7.2 for 128, 7.5 for 256 (the most there are);  32 x 1024: 9.3
@@ -865,7 +865,7 @@ static CachePlan cache_plan(int64_t batch, int nq, int nkv, int64_t max_len, int
     // (splits by the tiles to expect: of every prefix but one, half of the last one is empty)
     const int64_t rounds = cdiv(pre_len, 128), units = nkv * cdiv(batch * (nq / nkv) + kPrefixRows / 2 * (some - 1), kPrefixRows);
     s = (256 + units / 2) / units;
-    if (rounds > 16 * (s < 1 ? 1 : s)) s = cdiv(512, units);
+    if (rounds >= 16 * (s < 1 ? 1 : s)) s = cdiv(512, units);
     s = s < 1 ? 1 : s;
     p.s_pre = static_cast<int>(s < rounds ? s : rounds);
   }
