@@ -805,7 +805,7 @@ int ma_tree_commit(void* const* k_caches, void* const* v_caches, int64_t layers,
                    void* stream);
 
 /*
- * A quantised KV cache, the next three entries and ma_cache_attn: per (row, KV
+ * A quantised KV cache, the next three entries, ma_cache_attn and ma_quant_attn: per (row, KV
  * head, position) and for K and V each, head_dim e4m3 codes ([cache_rows,
  * n_kv_heads, max_len, head_dim], 16-byte aligned) and one scale byte e + 127
  * ([cache_rows, n_kv_heads, max_len]; e8m0): e is the least integer with which
@@ -878,6 +878,22 @@ int ma_cache_attn(const void* q, int64_t batch, int n_heads, int n_kv_heads, int
                   const void* pv_scale, int64_t prefixes, int64_t prefix_max_len,
                   const int64_t* prefix_len, const int64_t* prefix_of, int64_t window,
                   float scale, void* out, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * ma_quant_qkv and ma_cache_attn over the cache (without prefixes) for a step's
+ * token, its query heads kept in the launch: the same codes and scales stored, out
+ * [batch, n_heads, head_dim] bf16 over positions 0 .. seqlen[b] (with window > 0 the
+ * last `window`).  Arguments and bounds as there; workspace:
+ * ma_cache_attn_workspace_bytes(batch, n_heads, n_kv_heads, head_dim, max_len, 0, 0,
+ * window) bytes (may be 0).  The bf16 cache's form of it is ma_decode_attn_fused.
+ */
+int ma_quant_attn(const void* qkv, int64_t ldb, int64_t batch, int n_heads, int n_kv_heads,
+                  int head_dim, const void* q_norm_w, const void* k_norm_w, int w_dtype,
+                  const void* cos, const void* sin, int cs_dtype, int64_t ld_cs, int64_t n_pos,
+                  int rotary_dim, float eps, const int64_t* seqlen, const int64_t* positions,
+                  const int64_t* row_map, void* k_codes, void* v_codes, void* k_scale,
+                  void* v_scale, int64_t cache_rows, int64_t max_len, int64_t window, float scale,
+                  void* out, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

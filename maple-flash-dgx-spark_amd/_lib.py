@@ -110,6 +110,8 @@ _SIGNATURES = {
     "ma_cache_attn_workspace_bytes": [_L, _I, _I, _I, _L, _L, _L, _L],
     "ma_cache_attn": [_P, _L, _I, _I, _I, _P, _P, _P, _P, _L, _L, _P, _P, _P, _P, _P, _P, _L, _L, _P, _P, _L, _F, _P,
                       _P, _Z, _P],
+    "ma_quant_attn": [_P, _L, _L, _I, _I, _I, _P, _P, _I, _P, _P, _I, _L, _L, _I, _F, _P, _P, _P, _P, _P, _P, _P, _L, _L,
+                      _L, _F, _P, _P, _Z, _P],
     "ma_tree_fit": [_P, _I, _L, _L, _P, _L, _P, _P],
     "ma_tree_commit": [_P, _P, _L, _L, _L, _I, _I, _L, _L, _P, _P, _P, _P, _P, _P],
 }

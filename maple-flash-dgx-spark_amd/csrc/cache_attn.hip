@@ -1,14 +1,13 @@
 // One query token a row over a quantised KV cache (quant.h) or a bf16 one, its
 // sequence the row's own positions behind a prefix that rows share, or without
-// one (ma_cache_attn; gfx950).  A row's sequence is prefix of[b] (length[of[b]]
+// one (ma_cache_attn; gfx950), or from its QKV projection on (ma_quant_attn).  A row's sequence is prefix of[b] (length[of[b]]
 // positions; any other value than 0 .. P-1: none), then its own positions 0 ..
 // seqlen[b].  Lengths are clamped to the caches and mapped rows too, so nothing
 // is read outside them.
 
 #include <math.h>
 
-#include "quant.h"
-#include "qkv_rows.h"
+#include "quant_qkv.h"
 
 namespace ma {
 
@@ -160,8 +159,25 @@ struct OwnLds {
   char v[kCacheWaves][32 * 2 * HD];  // a wave's tile of V; at the end the waves' sums
   float m[kCacheWaves][kCacheGroup], l[kCacheWaves][kCacheGroup];
 };
-template <int HD, bool Q8>
-__device__ __forceinline__ void cache_own(const CacheAttn& a, const CacheHot& hot, int wg, OwnLds<HD>& lds) {
+
+// NEW: q and the row's new token come from its QKV projection.  Every workgroup makes
+// its own query heads; the one of the last split also K and V, which it stores and
+// attends to as a tile of one position, so that nothing waits for the store.
+template <int HD>
+struct NewLds {
+  uint16_t q[kCacheGroup][HD];
+  uint8_t code[2][HD];  // K's and V's
+  int byte[2];
+};
+struct NewToken {
+  QkvIn in;
+  const int64_t* positions;
+};
+struct NoToken {};
+
+template <int HD, bool Q8, bool NEW = false, bool VEC = true, typename T = NoToken>
+__device__ __forceinline__ void cache_own(const CacheAttn& a, const CacheHot& hot, int wg, OwnLds<HD>& lds,
+                                          const T& token = T{}, NewLds<HD>* made = nullptr) {
   constexpr int NW = kCacheWaves;
   constexpr int RB = Q8 ? HD : 2 * HD;      // bytes of a cached position
   constexpr int KL = RB / 64;               // 16-byte loads of K a lane and 16 positions
@@ -185,15 +201,30 @@ __device__ __forceinline__ void cache_own(const CacheAttn& a, const CacheHot& ho
   // tiles: of the prefix where each row reads it itself, then of the row's own
   const int64_t a0 = hot.s_pre > 0 ? 0 : (span.lo < span.pre_n ? span.lo : span.pre_n);
   const int64_t a1 = hot.s_pre > 0 ? 0 : span.pre_n;
-  const int64_t b0 = span.lo > span.pre_n ? span.lo - span.pre_n : 0, b1 = span.own_n;
+  int64_t slot = -1;
+  if constexpr (NEW) slot = hot.seqlen[b];
+  const bool fresh = NEW && slot >= 0 && slot < a.own.max_len;  // the new token is the last position
+  const int64_t b0 = span.lo > span.pre_n ? span.lo - span.pre_n : 0, b1 = span.own_n - (fresh ? 1 : 0);
   const int na = static_cast<int>(cdiv(a1 - a0, 32)), nt = na + static_cast<int>(cdiv(b1 - b0, 32));
   const int rounds = (nt + NW - 1) / NW, per = (rounds + hot.s_own - 1) / hot.s_own * NW;
   const int t_beg = sp * per < nt ? sp * per : nt;
   const int t_end = t_beg + per < nt ? t_beg + per : nt;
 
+  // the split with the last tile, and the wave after that tile's
+  const bool mine = fresh && sp == (nt > 0 ? (nt - 1) / per : 0);
+  constexpr int LPH = HD / 8;
+  QkvEight<HD, VEC> e;
+  auto fetch = [&](int item) {
+    const int hh = item / LPH < group + 2 ? item / LPH : 0;
+    if constexpr (NEW) {
+      e.load(token.in, b, hh < group ? kvh * group + hh : hot.nq + kvh + (hh - group) * hot.nkv, 8 * (item % LPH), hh < group);
+      e.load_turns(token.in, token.positions ? token.positions[b] : slot, 8 * (item % LPH));
+    }
+  };
+  if constexpr (NEW) fetch(tid);
+
   uint4 qf[KS];
-  {
-    const uint16_t* const src = a.q + (b * hot.nq + kvh * group + (r16 < group ? r16 : 0)) * HD;
+  auto load_q = [&](const uint16_t* src) {
     const uint32_t keep = r16 < group ? 0xffffffffu : 0u;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
@@ -201,7 +232,8 @@ __device__ __forceinline__ void cache_own(const CacheAttn& a, const CacheHot& ho
       const uint4 v = *reinterpret_cast<const uint4*>(src + d);
       qf[ks] = make_uint4(v.x & keep, v.y & keep, v.z & keep, v.w & keep);
     }
-  }
+  };
+  if constexpr (!NEW) load_q(a.q + (b * hot.nq + kvh * group + (r16 < group ? r16 : 0)) * HD);
   struct Tile {
     u32x4c_t k[2][KL], v[VL];
     int scale;  // of position lane % 32: K's, in the upper lanes V's
@@ -210,12 +242,12 @@ __device__ __forceinline__ void cache_own(const CacheAttn& a, const CacheHot& ho
   const CacheIn& own = a.own;
   const CacheIn& pre = a.pre;
   auto load = [&](Tile& x, int t) {
-    const bool mine = t >= na;
-    const int64_t p = mine ? b0 + 32 * static_cast<int64_t>(t - na) : a0 + 32 * static_cast<int64_t>(t);
-    const int64_t left = (mine ? b1 : a1) - p;
+    const bool past = t >= na;  // (of the prefix)
+    const int64_t p = past ? b0 + 32 * static_cast<int64_t>(t - na) : a0 + 32 * static_cast<int64_t>(t);
+    const int64_t left = (past ? b1 : a1) - p;
     x.n = left < 32 ? static_cast<int>(left) : 32;
-    const int64_t at = mine ? (crow * hot.nkv + kvh) * own.max_len + p : (span.pre_row * hot.nkv + kvh) * pre.max_len + p;
-    const TileBytes kt((mine ? own.k : pre.k) + at * RB, x.n * RB), vt((mine ? own.v : pre.v) + at * RB, x.n * RB);
+    const int64_t at = past ? (crow * hot.nkv + kvh) * own.max_len + p : (span.pre_row * hot.nkv + kvh) * pre.max_len + p;
+    const TileBytes kt((past ? own.k : pre.k) + at * RB, x.n * RB), vt((past ? own.v : pre.v) + at * RB, x.n * RB);
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -223,8 +255,8 @@ __device__ __forceinline__ void cache_own(const CacheAttn& a, const CacheHot& ho
 #pragma unroll
     for (int i = 0; i < VL; ++i) x.v[i] = vt.at(1024 * i + 16 * lane);
     if constexpr (Q8) {
-      const int row = (lane & 31) < x.n ? lane & 31 : x.n - 1;
-      const uint8_t* const s = lane < 32 ? (mine ? own.ks : pre.ks) : (mine ? own.vs : pre.vs);
+      const int row = (lane & 31) < x.n ? lane & 31 : (NEW && x.n == 0 ? 0 : x.n - 1);
+      const uint8_t* const s = lane < 32 ? (past ? own.ks : pre.ks) : (past ? own.vs : pre.vs);
       x.scale = s[at + row];
     }
   };
@@ -316,9 +348,40 @@ __device__ __forceinline__ void cache_own(const CacheAttn& a, const CacheHot& ho
     // (Loads run past the wave's last tile, on it again: after one that a branch may
     // have skipped every wait would be for all of them.)
     const int t0 = t_beg + wv, last = t0 + (t_end - 1 - t0) / NW * NW;
+    Tile x0, x1;
+    if constexpr (NEW) {
+      load(x0, t0 < t_end ? t0 : 0);  // (tile 0 is there, if without positions)
+      MA_ISSUE_FENCE();
+      float* const ys = reinterpret_cast<float*>(&vt[0][0]);
+      static_assert(sizeof(vt) >= 8 * kCacheThreads * sizeof(float), "the partners' exchange");
+      for (int i0 = 0;;) {
+        const int item = i0 + tid, hh = item / LPH, d = 8 * (item % LPH);
+        uint4 r = e.made(token.in, hh > group, ys, tid);
+        const int byte = head_byte<HD>(r);
+        if (hh < group) {
+          if (slot < 0) r = make_uint4(0u, 0u, 0u, 0u);  // no sequence in the row
+          *reinterpret_cast<uint4*>(&made->q[hh][d]) = r;
+        } else if (mine && hh < group + 2) {
+          const bool is_v = hh > group;
+          const uint2 c = quant_eight(r, byte);
+          *reinterpret_cast<uint2*>(&made->code[is_v][d]) = c;
+          const int64_t to = (crow * hot.nkv + kvh) * own.max_len + slot;
+          *reinterpret_cast<uint2*>(const_cast<uint8_t*>(is_v ? own.v : own.k) + to * HD + d) = c;
+          if (d == 0) {
+            made->byte[is_v] = byte;
+            const_cast<uint8_t*>(is_v ? own.vs : own.ks)[to] = static_cast<uint8_t>(byte);
+          }
+        }
+        i0 += kCacheThreads;
+        if (i0 >= (group + 2) * LPH) break;
+        __syncthreads();
+        fetch(i0 + tid);
+      }
+      __syncthreads();
+      load_q(&made->q[r16 < group ? r16 : 0][0]);
+    }
     if (t0 < t_end) {
-      Tile x0, x1;
-      load(x0, t0);
+      if constexpr (!NEW) load(x0, t0);
       for (int t = t0; t < t_end; t += 2 * NW) {
         load(x1, t + NW < t_end ? t + NW : last);
         MA_ISSUE_FENCE();
@@ -326,6 +389,23 @@ __device__ __forceinline__ void cache_own(const CacheAttn& a, const CacheHot& ho
         load(x0, t + 2 * NW < t_end ? t + 2 * NW : last);
         MA_ISSUE_FENCE();
         if (t + NW < t_end) attend(x1);
+      }
+    }
+    if constexpr (NEW) {
+      if (mine && wv == (nt - t_beg) % NW) {
+        Tile& x = x0;
+        const u32x4c_t none = {0u, 0u, 0u, 0u};
+#pragma unroll
+        for (int j = 0; j < KL; ++j) {
+          x.k[0][j] = r16 == 0 ? *reinterpret_cast<const u32x4c_t*>(&made->code[0][64 * j + 16 * g]) : none;
+          x.k[1][j] = none;
+        }
+#pragma unroll
+        for (int i = 0; i < VL; ++i) x.v[i] = none;
+        if (lane < RB / 16) x.v[0] = *reinterpret_cast<const u32x4c_t*>(&made->code[1][16 * lane]);
+        x.scale = (lane & 31) == 0 ? made->byte[lane >> 5] : 1;
+        x.n = 1;
+        attend(x);
       }
     }
   }
@@ -367,7 +447,7 @@ __device__ __forceinline__ void cache_own(const CacheAttn& a, const CacheHot& ho
     const int64_t row = b * hot.nq + kvh * group + hh;
     if (st > 1) {
       const int64_t p = row * st + sp;
-      if (t_beg < t_end) *reinterpret_cast<float4*>(a.acc + p * HD + d) = s;
+      if (t_beg < t_end || mine) *reinterpret_cast<float4*>(a.acc + p * HD + d) = s;
       if (d == 0) a.ml[p] = make_float2(M, L);
     } else {
       const float inv = L != 0.f ? 1.0f / L : 0.f;
@@ -704,6 +784,17 @@ __global__ __launch_bounds__(kCacheThreads, (HD == 64 ? 4 : (Q8 ? 3 : 2))) void 
   cache_own<HD, Q8>(a, CacheHot{seqlen, row_map, of, length, nq, nkv, s_own, 0, 0}, blockIdx.x, lds);
 }
 
+// A step's token from its projection on: k_quant_qkv's work and the attention.
+template <int HD, bool VEC>
+__global__ __launch_bounds__(kCacheThreads, HD == 64 ? 4 : 3) void k_quant_attn(const int64_t* seqlen, const int64_t* row_map,
+                                                                                int nq, int nkv, int s_own, NewToken token,
+                                                                                CacheAttn a) {
+  __shared__ __align__(16) OwnLds<HD> lds;
+  __shared__ __align__(16) NewLds<HD> made;
+  cache_own<HD, true, true, VEC>(a, CacheHot{seqlen, row_map, nullptr, nullptr, nq, nkv, s_own, 0, 0}, blockIdx.x, lds, token,
+                                 &made);
+}
+
 // The first `tiles` x units (rounded up to the XCDs) workgroups the prefixes, where
 // the tiles of the same positions fall to one XCD, the others the rows' own parts.
 template <int HD, bool Q8>
@@ -881,9 +972,6 @@ static size_t cache_ws_bytes(const CachePlan& p, int64_t batch, int nq, int head
 
 using namespace ma;
 
-constexpr int64_t kMaxGroups = (1 << 24) - 1;  // (a launch counts its threads in 32 bits)
-static bool cache_aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-
 static int check_cache_sizes(const char* what, int64_t batch, int nq, int nkv, int hd, int64_t rows, int64_t max_len,
                              const void* row_map, int64_t prefixes, int64_t pre_len, int64_t window) {
   if (hd != 64 && hd != 128) return fail(MA_EVALUE, "%s: head_dim %d unsupported (64 or 128)", what, hd);
@@ -897,6 +985,20 @@ static int check_cache_sizes(const char* what, int64_t batch, int nq, int nkv, i
   if (prefixes < 0 || prefixes > 65535 || (prefixes > 0 && (pre_len < 1 || pre_len >= kMost)))
     return fail(MA_EVALUE, "%s: %lld prefixes of %lld positions", what, static_cast<long long>(prefixes), static_cast<long long>(pre_len));
   return MA_OK;
+}
+
+// The launch that joins the parts, where there are several.
+static int cache_merge(const CachePlan& p, const CacheAttn& a, int head_dim, int64_t prefixes, hipStream_t s) {
+  const int st = p.s_own + p.s_pre, rows = a.batch * a.nq;
+  if (st == 1) return MA_OK;
+  const bool wide = st > 8 * 256 / head_dim;  // more than one round of a wave's loads
+  auto merge = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(cdiv(rows, wide ? 1 : 4))), dim3(256), 0, s, a.acc, a.ml, a.of,
+                       prefixes, rows, a.nq, p.s_own, p.s_pre, a.out);
+  };
+  if (head_dim == 64) wide ? merge(k_cache_merge<64, 4>) : merge(k_cache_merge<64, 1>);
+  else wide ? merge(k_cache_merge<128, 4>) : merge(k_cache_merge<128, 1>);
+  return check_launch("cache_attn merge");
 }
 
 extern "C" size_t ma_cache_attn_workspace_bytes(int64_t batch, int n_heads, int n_kv_heads, int head_dim, int64_t max_len,
@@ -923,8 +1025,8 @@ extern "C" int ma_cache_attn(const void* q, int64_t batch, int n_heads, int n_kv
   if (!q || !k || !v || !seqlen || !out || (q8 && !v_scale) || (!q8 && v_scale)) return fail(MA_EVALUE, "%s: null pointer", what);
   if (prefixes > 0 && (!pk || !pv || !prefix_len || !prefix_of || (pk_scale != nullptr) != q8 || (pv_scale != nullptr) != q8))
     return fail(MA_EVALUE, "%s: null pointer, or a prefix of another kind than the cache", what);
-  if (!cache_aligned16(q) || !cache_aligned16(k) || !cache_aligned16(v) || !cache_aligned16(out) ||
-      !cache_aligned16(workspace) || (prefixes > 0 && (!cache_aligned16(pk) || !cache_aligned16(pv))))
+  if (!quant_aligned16(q) || !quant_aligned16(k) || !quant_aligned16(v) || !quant_aligned16(out) ||
+      !quant_aligned16(workspace) || (prefixes > 0 && (!quant_aligned16(pk) || !quant_aligned16(pv))))
     return fail(MA_EVALUE, "%s: q, the caches, out and the workspace must be 16-byte aligned", what);
   window = cache_window(window, max_len, prefixes > 0 ? prefix_max_len : 0);
   const CachePlan p = cache_plan(batch, n_heads, n_kv_heads, max_len, prefixes, prefix_max_len, window);
@@ -959,14 +1061,50 @@ extern "C" int ma_cache_attn(const void* q, int64_t batch, int n_heads, int n_kv
     else q8 ? go(k_cache_own<128, true>) : go(k_cache_own<128, false>);
   }
   if (int rc = check_launch(what)) return rc;
-  if (!need) return MA_OK;
-  const int rows = static_cast<int>(batch * n_heads);
-  const bool wide = p.s_own + p.s_pre > 8 * 256 / head_dim;  // more than one round of a wave's loads
-  auto merge = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(cdiv(rows, wide ? 1 : 4))), dim3(256), 0, s, a.acc, a.ml, a.of,
-                       prefixes, rows, n_heads, p.s_own, p.s_pre, a.out);
+  return cache_merge(p, a, head_dim, prefixes, s);
+}
+
+extern "C" int ma_quant_attn(const void* qkv, int64_t ldb, int64_t batch, int n_heads, int n_kv_heads, int head_dim,
+                             const void* q_norm_w, const void* k_norm_w, int w_dtype, const void* cos, const void* sin,
+                             int cs_dtype, int64_t ld_cs, int64_t n_pos, int rotary_dim, float eps, const int64_t* seqlen,
+                             const int64_t* positions, const int64_t* row_map, void* k_codes, void* v_codes, void* k_scale,
+                             void* v_scale, int64_t cache_rows, int64_t max_len, int64_t window, float scale, void* out,
+                             void* workspace, size_t workspace_bytes, void* stream) {
+  const char* what = "quant_attn";
+  if (int rc = check_cache_sizes(what, batch, n_heads, n_kv_heads, head_dim, cache_rows, max_len, row_map, 0, 0, window))
+    return rc;
+  if (int rc = check_quant(what, batch, n_kv_heads, head_dim, k_codes, v_codes, k_scale, v_scale, cache_rows, max_len, row_map))
+    return rc;
+  NewToken token;
+  bool vec;
+  if (int rc = check_qkv(what, qkv, ldb, n_heads, n_kv_heads, head_dim, q_norm_w, k_norm_w, w_dtype, cos, sin, cs_dtype,
+                         ld_cs, n_pos, rotary_dim, eps, token.in, vec))
+    return rc;
+  token.positions = positions;
+  if (!isfinite(scale * kLog2e)) return fail(MA_EVALUE, "%s: scale %g, or log2 e times it, is not finite", what, scale);
+  if (batch == 0) return MA_OK;
+  if (!qkv || !seqlen || !out) return fail(MA_EVALUE, "%s: null pointer", what);
+  if (!quant_aligned16(out) || !quant_aligned16(workspace))
+    return fail(MA_EVALUE, "%s: out and the workspace must be 16-byte aligned", what);
+  window = cache_window(window, max_len, 0);
+  const CachePlan p = cache_plan(batch, n_heads, n_kv_heads, max_len, 0, 0, window);
+  const int64_t parts = batch * n_heads * p.s_own, wgs = batch * n_kv_heads * p.s_own;
+  const size_t need = cache_ws_bytes(p, batch, n_heads, head_dim);
+  if (need && (!workspace || workspace_bytes < need))
+    return fail(MA_EVALUE, "%s: workspace of %zu bytes, need %zu", what, workspace ? workspace_bytes : 0, need);
+  if (parts > INT32_MAX || wgs > kMaxGroups) return fail(MA_EVALUE, "%s: batch too large for one launch", what);
+  auto u8 = [](const void* x) { return static_cast<const uint8_t*>(x); };
+  float* const acc = static_cast<float*>(workspace);
+  const CacheAttn a{seqlen, row_map, nullptr, nullptr, nullptr, static_cast<int>(batch), n_heads, n_kv_heads, p.s_own, 0,
+                    window, scale, {u8(k_codes), u8(v_codes), u8(k_scale), u8(v_scale), cache_rows, max_len}, {},
+                    acc, need ? reinterpret_cast<float2*>(acc + parts * head_dim) : nullptr, static_cast<uint16_t*>(out)};
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  auto go = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(wgs)), dim3(kCacheThreads), 0, s, seqlen, row_map, n_heads,
+                       n_kv_heads, p.s_own, token, a);
   };
-  if (head_dim == 64) wide ? merge(k_cache_merge<64, 4>) : merge(k_cache_merge<64, 1>);
-  else wide ? merge(k_cache_merge<128, 4>) : merge(k_cache_merge<128, 1>);
-  return check_launch("cache_attn merge");
+  if (head_dim == 64) vec ? go(k_quant_attn<64, true>) : go(k_quant_attn<64, false>);
+  else vec ? go(k_quant_attn<128, true>) : go(k_quant_attn<128, false>);
+  if (int rc = check_launch(what)) return rc;
+  return cache_merge(p, a, head_dim, 0, s);
 }

@@ -3,8 +3,7 @@
 // cached positions back as bf16 (ma_dequant_kv).  A position outside the cache is
 // not written, a mapped row outside it is clamped.
 
-#include "qkv_rows.h"
-#include "quant.h"
+#include "quant_qkv.h"
 
 namespace ma {
 
@@ -28,11 +27,10 @@ constexpr int kQuantThreads = 256;
 // value over the HD / 8 lanes of the head, v heads quantised as they are.
 // VEC: all rows are 16-byte aligned.
 template <int HD, bool VEC>
-__global__ __launch_bounds__(kQuantThreads) void k_quant_qkv(
-    const uint16_t* __restrict__ qkv, int64_t ldb, int64_t batch, const void* __restrict__ q_w,
-    const void* __restrict__ k_w, int w_dt, RopeTab rope, float eps, const int64_t* __restrict__ seqlen,
-    const int64_t* __restrict__ positions, const int64_t* __restrict__ row_map, QuantCache cache, int nq, int nkv,
-    uint16_t* __restrict__ q_out) {
+__global__ __launch_bounds__(kQuantThreads) void k_quant_qkv(QkvIn in, int64_t batch, const int64_t* __restrict__ seqlen,
+                                                             const int64_t* __restrict__ positions,
+                                                             const int64_t* __restrict__ row_map, QuantCache cache, int nq,
+                                                             int nkv, uint16_t* __restrict__ q_out) {
   constexpr int LPH = HD / 8;
   __shared__ __align__(16) float ys[kQuantThreads * 8];
   const int tid = threadIdx.x;
@@ -44,38 +42,15 @@ __global__ __launch_bounds__(kQuantThreads) void k_quant_qkv(
   const int64_t b = hd / heads;
   const int hs = static_cast<int>(hd - b * heads);
   const bool is_q = hs < nq, is_v = hs >= nq + nkv;
-  const uint16_t* const x_row = qkv + b * ldb + static_cast<int64_t>(hs) * HD + d0;
-  uint4 xv = make_uint4(0u, 0u, 0u, 0u);
-  if constexpr (VEC) {
-    xv = *reinterpret_cast<const uint4*>(x_row);
-  } else {
-    uint16_t xs[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) xs[e] = x_row[e];
-    xv = make_uint4(xs[0] | static_cast<uint32_t>(xs[1]) << 16, xs[2] | static_cast<uint32_t>(xs[3]) << 16,
-                    xs[4] | static_cast<uint32_t>(xs[5]) << 16, xs[6] | static_cast<uint32_t>(xs[7]) << 16);
-  }
-  Eight wr{};
-  if (q_w) ld_eight<VEC>(wr, is_q ? q_w : k_w, w_dt, d0);
+  QkvEight<HD, VEC> e;
+  e.load(in, b, hs, d0, is_q);
   const int64_t slot = seqlen[b];
   const int64_t at = positions ? positions[b] : slot;
   const int64_t crow = row_map ? clamp_pos(row_map[b], 0, cache.rows - 1) : b;
   MA_ISSUE_FENCE();
-  const bool turn = rope.mode && rope.rot > 0;
-  Eight cr{}, sr{};
-  if (turn) {
-    const int64_t row = clamp_pos(at, 0, rope.n_pos - 1) * rope.ld;
-    ld_turns<VEC>(cr, rope.cos, rope.dt, row, d0, rope.rot, rope.mode);
-    ld_turns<VEC>(sr, rope.sin, rope.dt, row, d0, rope.rot, rope.mode);
-  }
-  float y[8];
-  of_bf16x8(y, xv);
-  norm_turn<HD, VEC>(y, q_w != nullptr, !is_v, wr, w_dt, turn, cr, sr, rope, eps, ys, tid);
-  uint4 r = make_uint4(pack_bf16x2_rn(y[0], y[1]), pack_bf16x2_rn(y[2], y[3]), pack_bf16x2_rn(y[4], y[5]),
-                       pack_bf16x2_rn(y[6], y[7]));
-  if (is_v) r = xv;  // (the bits as they are)
-  int top = finite_top(finite_top(finite_top(finite_top(0, r.x), r.y), r.z), r.w);
-  top = group_top<LPH>(top);
+  e.load_turns(in, at, d0);
+  uint4 r = e.made(in, is_v, ys, tid);
+  const int byte = head_byte<HD>(r);
   if (!on) return;
   if (is_q) {
     if (slot < 0) r = make_uint4(0u, 0u, 0u, 0u);  // no sequence in the row
@@ -83,11 +58,8 @@ __global__ __launch_bounds__(kQuantThreads) void k_quant_qkv(
     return;
   }
   if (slot < 0 || slot >= cache.max_len) return;
-  const int byte = quant_byte(top);
-  const float inv = quant_inverse(byte);
   const int64_t to = (crow * nkv + (hs - nq) % nkv) * cache.max_len + slot;
-  *reinterpret_cast<uint2*>((is_v ? cache.v : cache.k) + to * HD + d0) =
-      make_uint2(quant_four(r.x, r.y, inv), quant_four(r.z, r.w, inv));
+  *reinterpret_cast<uint2*>((is_v ? cache.v : cache.k) + to * HD + d0) = quant_eight(r, byte);
   if (l == 0) (is_v ? cache.vs : cache.ks)[to] = static_cast<uint8_t>(byte);
 }
 
@@ -215,25 +187,6 @@ __global__ __launch_bounds__(kQuantThreads) void k_dequant_kv(QuantCache cache, 
 
 using namespace ma;
 
-namespace {
-
-constexpr int64_t kMaxGroups = (1 << 24) - 1;  // (a launch counts its threads in 32 bits)
-
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-
-int check_quant(const char* what, int64_t batch, int n_kv_heads, int head_dim, const void* k, const void* v,
-                const void* ks, const void* vs, int64_t cache_rows, int64_t max_len, const void* row_map) {
-  if (head_dim != 64 && head_dim != 128) return fail(MA_EVALUE, "%s: head_dim %d unsupported (64 or 128)", what, head_dim);
-  if (batch < 0 || n_kv_heads < 1 || n_kv_heads > 65535) return fail(MA_EVALUE, "%s: bad sizes", what);
-  if (batch == 0) return MA_OK;
-  if (max_len < 1 || cache_rows < 1 || (!row_map && batch > cache_rows)) return fail(MA_EVALUE, "%s: bad cache sizes", what);
-  if (!k || !v || !ks || !vs) return fail(MA_EVALUE, "%s: null pointer", what);
-  if (!aligned16(k) || !aligned16(v)) return fail(MA_EVALUE, "%s: the codes must be 16-byte aligned", what);
-  return MA_OK;
-}
-
-}  // namespace
-
 extern "C" int ma_quant_qkv(const void* qkv, int64_t ldb, int64_t batch, int n_heads, int n_kv_heads, int head_dim,
                             const void* q_norm_w, const void* k_norm_w, int w_dtype, const void* cos, const void* sin,
                             int cs_dtype, int64_t ld_cs, int64_t n_pos, int rotary_dim, float eps,
@@ -243,32 +196,21 @@ extern "C" int ma_quant_qkv(const void* qkv, int64_t ldb, int64_t batch, int n_h
   const char* what = "quant_qkv";
   if (int rc = check_quant(what, batch, n_kv_heads, head_dim, k_codes, v_codes, k_scale, v_scale, cache_rows, max_len, row_map))
     return rc;
-  if (n_heads < n_kv_heads || n_heads % n_kv_heads != 0 || n_heads > 65535)
-    return fail(MA_EVALUE, "%s: %d query heads over %d KV heads", what, n_heads, n_kv_heads);
-  if (ldb < static_cast<int64_t>(n_heads + 2 * n_kv_heads) * head_dim) return fail(MA_EVALUE, "%s: qkv row stride too small", what);
-  if (rotary_dim < 0 || rotary_dim > head_dim || rotary_dim % 2 != 0)
-    return fail(MA_EVALUE, "%s: rotary_dim %d must be even and at most head_dim", what, rotary_dim);
-  if (rotary_dim > 0 && (!cos || !sin || n_pos < 1 || ld_cs < rotary_dim))
-    return fail(MA_EVALUE, "%s: the cos / sin tables need %d columns and a row", what, rotary_dim);
-  for (const int dt : {w_dtype, cs_dtype})
-    if (dt != MA_F32 && dt != MA_BF16 && dt != MA_F16) return fail(MA_ETYPE, "%s: dtype %d unsupported", what, dt);
-  if ((q_norm_w == nullptr) != (k_norm_w == nullptr)) return fail(MA_EVALUE, "%s: one norm weight without the other", what);
+  QkvIn in;
+  bool vec;
+  if (int rc = check_qkv(what, qkv, ldb, n_heads, n_kv_heads, head_dim, q_norm_w, k_norm_w, w_dtype, cos, sin,
+                         cs_dtype, ld_cs, n_pos, rotary_dim, eps, in, vec))
+    return rc;
   if (batch == 0) return MA_OK;
   if (!qkv || !seqlen || !q_out) return fail(MA_EVALUE, "%s: null pointer", what);
-  if (!aligned16(q_out)) return fail(MA_EVALUE, "%s: q_out must be 16-byte aligned", what);
+  if (!quant_aligned16(q_out)) return fail(MA_EVALUE, "%s: q_out must be 16-byte aligned", what);
   const int64_t blocks = cdiv(batch * (n_heads + 2 * n_kv_heads) * (head_dim / 8), kQuantThreads);
   if (batch > (1 << 24) || blocks > kMaxGroups) return fail(MA_EVALUE, "%s: batch too large for one launch", what);
-  const RopeTab rope{cos, sin, cs_dtype, ld_cs, n_pos, rotary_dim, rotary_dim > 0 ? 1 : 0};
   const QuantCache cache{static_cast<uint8_t*>(k_codes), static_cast<uint8_t*>(v_codes), static_cast<uint8_t*>(k_scale),
                          static_cast<uint8_t*>(v_scale), cache_rows, max_len};
-  // 16-byte loads throughout: rows aligned, and the rotary part ends with a lane's dims
-  const bool rope_vec = rotary_dim == 0 || (aligned16(cos) && aligned16(sin) && rotary_dim % 8 == 0 &&
-                                            ld_cs * (cs_dtype == MA_F32 ? 4 : 2) % 16 == 0);
-  const bool vec = aligned16(qkv) && ldb % 8 == 0 && rope_vec && aligned16(q_norm_w) && aligned16(k_norm_w);
   auto go = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kQuantThreads), 0, static_cast<hipStream_t>(stream),
-                       static_cast<const uint16_t*>(qkv), ldb, batch, q_norm_w, k_norm_w, w_dtype, rope, eps, seqlen,
-                       positions, row_map, cache, n_heads, n_kv_heads, static_cast<uint16_t*>(q_out));
+                       in, batch, seqlen, positions, row_map, cache, n_heads, n_kv_heads, static_cast<uint16_t*>(q_out));
   };
   if (head_dim == 64) vec ? go(k_quant_qkv<64, true>) : go(k_quant_qkv<64, false>);
   else vec ? go(k_quant_qkv<128, true>) : go(k_quant_qkv<128, false>);
@@ -293,7 +235,7 @@ extern "C" int ma_quant_kv(const void* k, int64_t k_sb, int64_t k_sh, int64_t k_
   const QuantCache cache{static_cast<uint8_t*>(k_codes), static_cast<uint8_t*>(v_codes), static_cast<uint8_t*>(k_scale),
                          static_cast<uint8_t*>(v_scale), cache_rows, max_len};
   const KvRows kr{static_cast<const uint16_t*>(k), k_sb, k_sh, k_st}, vr{static_cast<const uint16_t*>(v), v_sb, v_sh, v_st};
-  const bool vec = aligned16(k) && aligned16(v) && (k_sb | k_sh | k_st | v_sb | v_sh | v_st) % 8 == 0;
+  const bool vec = quant_aligned16(k) && quant_aligned16(v) && (k_sb | k_sh | k_st | v_sb | v_sh | v_st) % 8 == 0;
   const bool heads_in = k_sh < k_st;
   const dim3 grid(static_cast<unsigned>(batch * chunks), 2);
   auto go = [&](auto kernel) {
@@ -321,7 +263,7 @@ extern "C" int ma_dequant_kv(const void* k_codes, const void* v_codes, const voi
     return fail(MA_EVALUE, "%s: %lld positions of a cache of %lld", what, static_cast<long long>(length),
                 static_cast<long long>(max_len));
   if (batch == 0 || length == 0) return MA_OK;
-  if (!k_out || !v_out || !aligned16(k_out) || !aligned16(v_out))
+  if (!k_out || !v_out || !quant_aligned16(k_out) || !quant_aligned16(v_out))
     return fail(MA_EVALUE, "%s: the outputs must be there and 16-byte aligned", what);
   const int64_t rpb = kQuantThreads / (head_dim / 16) * kQuantRows;
   if (length > INT32_MAX || batch > kMaxGroups / n_kv_heads / cdiv(length, rpb))

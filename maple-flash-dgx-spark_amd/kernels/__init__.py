@@ -23,6 +23,7 @@ from .quant_cache import (
     dequantize_kv,
     make_quant_kv,
     prefix_gqa_attn,
+    quant_attention,
     quant_gqa_attn,
     quantize_kv,
 )
@@ -62,6 +63,7 @@ __all__ = [
     "apply_qkv_quant",
     "quantize_kv",
     "dequantize_kv",
+    "quant_attention",
     "quant_gqa_attn",
     "prefix_gqa_attn",
 ]

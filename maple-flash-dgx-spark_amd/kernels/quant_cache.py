@@ -6,7 +6,8 @@ the largest finite value is at most ``448 * 2^e`` (``e`` in -126 .. 119), so
 ``head_dim + 1`` bytes where a bf16 cache holds ``2 * head_dim``.  A code is off by
 at most 2^-4 of its value (2^-10 of the scale for small ones); values that are not
 finite become NaN.  ``apply_qkv_quant`` writes a step's tokens, ``quantize_kv`` whole
-prompts, ``dequantize_kv`` reads positions back, ``quant_gqa_attn`` attends.
+prompts, ``dequantize_kv`` reads positions back, ``quant_gqa_attn`` attends;
+``quant_attention`` is a step's ``apply_qkv_quant`` and ``quant_gqa_attn`` together.
 
 A ``SharedPrefix`` holds the K/V with which several rows' sequences begin: row
 ``b``'s is the first ``length[of[b]]`` positions of prefix ``of[b]`` (any value that
@@ -113,43 +114,22 @@ def _window(window: int | None) -> int:
     return min(window, _FAR)  # (past every position; more would wrap in 64 bits)
 
 
-def apply_qkv_quant(
-    qkv: torch.Tensor,
-    q_weight: torch.Tensor | None,
-    k_weight: torch.Tensor | None,
-    cos_table: torch.Tensor,
-    sin_table: torch.Tensor,
-    cache: QuantKV,
-    seqlen: torch.Tensor,
-    *,
-    positions: torch.Tensor | None = None,
-    row_map: torch.Tensor | None = None,
-    num_heads: int,
-    num_kv_heads: int,
-    head_dim: int,
-    rotary_dim: int,
-    use_rope: bool = True,
-    eps: float = 1e-6,
-) -> torch.Tensor:
-    """QK RMSNorm + RoPE + quantising store of K/V at ``seqlen``; returns Q ``[B, H,
-    1, D]`` bf16.
-
-    ``qkv [B, (H + 2 Hkv) D]`` bf16; ``q_weight`` / ``k_weight`` both None: no norm.
-    The tables ``[n_pos, >= rotary_dim]`` are read at ``positions [B]``, by default
-    ``seqlen`` (behind a shared prefix a token's position is further on).  K is
-    rounded to bf16, as ``apply_qkv_decode`` stores it, and then quantised."""
-    _quant("apply_qkv_quant", cache)
+def _projection(what: str, qkv, q_weight, k_weight, cos_table, sin_table, cache, seqlen, positions, row_map, num_heads,
+                num_kv_heads, head_dim, rotary_dim, use_rope, eps):
+    """The checks of a token's projection and cache, the device, and the arguments from qkv to
+    the cache's sizes (the last item: the tensors that they point to)."""
+    _quant(what, cache)
     if qkv.ndim != 2 or qkv.dtype != torch.bfloat16:
-        raise ValueError(f"apply_qkv_quant expects bf16 qkv [B, qkv], got {qkv.dtype} {tuple(qkv.shape)}.")
+        raise ValueError(f"{what} expects bf16 qkv [B, qkv], got {qkv.dtype} {tuple(qkv.shape)}.")
     bsz, width = qkv.shape
     if width != (num_heads + 2 * num_kv_heads) * head_dim:
         raise ValueError(f"qkv rows of {width}, expected {(num_heads + 2 * num_kv_heads) * head_dim}.")
     ldb, one = qkv.stride()
     if one != 1:
-        raise ValueError("apply_qkv_quant needs a row-contiguous qkv.")
-    rows, n_kv, max_len, d = _check_cache("apply_qkv_quant", cache, bsz, row_map)
+        raise ValueError(f"{what} needs a row-contiguous qkv.")
+    rows, n_kv, max_len, d = _check_cache(what, cache, bsz, row_map)
     if n_kv != num_kv_heads or d != head_dim:
-        raise ValueError(f"apply_qkv_quant: cache {tuple(cache.k.shape)} for {num_kv_heads} KV heads of {head_dim}.")
+        raise ValueError(f"{what}: cache {tuple(cache.k.shape)} for {num_kv_heads} KV heads of {head_dim}.")
     more, qw, kw, c, s = [], None, None, None, None
     w_dt = dt = ld = n_pos = 0
     if q_weight is not None or k_weight is not None:
@@ -182,13 +162,41 @@ def apply_qkv_quant(
     if row_map is not None:
         more.append(_positions("row_map", row_map, bsz))
         rm = more[-1].data_ptr()
-    idx = _device("apply_qkv_quant", qkv, *cache, sl, *more)
-    out = qkv.new_empty((bsz, num_heads, 1, head_dim))
-    _call(
-        idx, "ma_quant_qkv",
-        qkv.data_ptr(), ldb if bsz > 1 else width, bsz, num_heads, num_kv_heads, head_dim, qw, kw, w_dt, c, s, dt, ld,
-        n_pos, rot, eps, sl.data_ptr(), at, rm, *map(_ptr, cache), rows, max_len, out.data_ptr(),
-    )
+    idx = _device(what, qkv, *cache, sl, *more)
+    more.append(sl)
+    return idx, (qkv.data_ptr(), ldb if bsz > 1 else width, bsz, num_heads, num_kv_heads, head_dim, qw, kw, w_dt, c, s, dt, ld,
+                 n_pos, rot, eps, sl.data_ptr(), at, rm, *map(_ptr, cache), rows, max_len), more
+
+
+def apply_qkv_quant(
+    qkv: torch.Tensor,
+    q_weight: torch.Tensor | None,
+    k_weight: torch.Tensor | None,
+    cos_table: torch.Tensor,
+    sin_table: torch.Tensor,
+    cache: QuantKV,
+    seqlen: torch.Tensor,
+    *,
+    positions: torch.Tensor | None = None,
+    row_map: torch.Tensor | None = None,
+    num_heads: int,
+    num_kv_heads: int,
+    head_dim: int,
+    rotary_dim: int,
+    use_rope: bool = True,
+    eps: float = 1e-6,
+) -> torch.Tensor:
+    """QK RMSNorm + RoPE + quantising store of K/V at ``seqlen``; returns Q ``[B, H,
+    1, D]`` bf16.
+
+    ``qkv [B, (H + 2 Hkv) D]`` bf16; ``q_weight`` / ``k_weight`` both None: no norm.
+    The tables ``[n_pos, >= rotary_dim]`` are read at ``positions [B]``, by default
+    ``seqlen`` (behind a shared prefix a token's position is further on).  K is
+    rounded to bf16, as ``apply_qkv_decode`` stores it, and then quantised."""
+    idx, args, _keep = _projection("apply_qkv_quant", qkv, q_weight, k_weight, cos_table, sin_table, cache, seqlen, positions,
+                                   row_map, num_heads, num_kv_heads, head_dim, rotary_dim, use_rope, eps)
+    out = qkv.new_empty((qkv.shape[0], num_heads, 1, head_dim))
+    _call(idx, "ma_quant_qkv", *args, out.data_ptr())
     return out
 
 
@@ -317,6 +325,39 @@ def quant_gqa_attn(
     heads to a KV head."""
     _quant("quant_gqa_attn", cache)
     return _attend("quant_gqa_attn", q, cache, seqlen, None, row_map, scale, window)
+
+
+def quant_attention(
+    qkv: torch.Tensor,
+    q_weight: torch.Tensor | None,
+    k_weight: torch.Tensor | None,
+    cos_table: torch.Tensor,
+    sin_table: torch.Tensor,
+    cache: QuantKV,
+    seqlen: torch.Tensor,
+    *,
+    positions: torch.Tensor | None = None,
+    row_map: torch.Tensor | None = None,
+    num_heads: int,
+    num_kv_heads: int,
+    head_dim: int,
+    rotary_dim: int,
+    use_rope: bool = True,
+    eps: float = 1e-6,
+    scale: float,
+    window: int | None = None,
+) -> torch.Tensor:
+    """``apply_qkv_quant`` and then ``quant_gqa_attn`` with one launch less, as
+    ``decode_attention`` is for a bf16 cache: the same codes stored, the attention output
+    ``[B, H, 1, D]`` (its sums in another order)."""
+    window = _window(window)
+    idx, args, _keep = _projection("quant_attention", qkv, q_weight, k_weight, cos_table, sin_table, cache, seqlen, positions,
+                                   row_map, num_heads, num_kv_heads, head_dim, rotary_dim, use_rope, eps)
+    out = qkv.new_empty((qkv.shape[0], num_heads, 1, head_dim))
+    nbytes = _workspace_bytes(qkv.shape[0], num_heads, num_kv_heads, head_dim, args[-1], 0, 0, window)
+    ws = qkv.new_empty(nbytes // 2) if nbytes else None  # (as in _attend)
+    _call(idx, "ma_quant_attn", *args, window, scale, out.data_ptr(), _lib.ptr(ws), nbytes)
+    return out
 
 
 def prefix_gqa_attn(

@@ -24,8 +24,8 @@ the place of ``decode_attention``; ``KVCache.commit`` then keeps an accepted
 branch.
 
 Over a quantised cache (``make_cache(quantized=True)``, ``KVCache.quantized``) the
-attention of a step is ``apply_qkv_quant`` and ``quant_gqa_attn``, and over rows
-behind shared prefixes (``KVCache.share``) ``prefix_gqa_attn``, in the place of
+attention of a step is ``quant_attention``, and over rows behind shared prefixes
+(``KVCache.share``) the store and ``prefix_gqa_attn``, in the place of
 ``decode_attention``.
 
 Weights are random with the synthetic distributions (``synthetic.py``): every
@@ -47,7 +47,7 @@ from .kernels.decode_attn import apply_qkv_decode, decode_attention, gqa_workspa
 from .kernels.fused_norm import rms_norm
 from .kernels.greedy import greedy_argmax
 from .kernels.quant_cache import (KV, QuantKV, SharedPrefix, apply_qkv_quant, dequantize_kv, make_quant_kv,
-                                  prefix_gqa_attn, quant_gqa_attn, quantize_kv)
+                                  prefix_gqa_attn, quant_attention, quantize_kv)
 from .kernels.rtn4 import rtn4_embedding, rtn4_gemv
 from .kernels.ternary_gemv import combine_gemv_supported, ternary_gemv, ternary_gemv_combine
 from .kernels.tree import apply_qkv_tree, check_tree, commit_tree, tree_attention
@@ -489,13 +489,14 @@ class SyntheticDecoder:
         kw = dict(num_heads=c.heads, num_kv_heads=c.kv_heads, head_dim=c.head_dim, rotary_dim=c.rotary_dim,
                   use_rope=akw["use_rope"], eps=c.eps, row_map=akw["row_map"])
         kv = cache.layer(i)
+        if cache.prefix is None:
+            return quant_attention(qkv, L.q_norm, L.k_norm, self.cos, self.sin, kv, seqlen, scale=akw["scale"],
+                                   window=akw["window"], **kw)
         if cache.is_quantized:
             q = apply_qkv_quant(qkv, L.q_norm, L.k_norm, self.cos, self.sin, kv, seqlen, positions=pos, **kw)
         else:
             q = apply_qkv_decode(qkv, L.q_norm, L.k_norm, cos, sin, kv.k, kv.v, seqlen, use_qk_norm=True, **kw)
         kw = dict(row_map=akw["row_map"], scale=akw["scale"], window=akw["window"])
-        if cache.prefix is None:
-            return quant_gqa_attn(q, kv, seqlen, **kw)
         return prefix_gqa_attn(q, kv, seqlen, cache.prefix.layer(i, qkv.shape[0]), **kw)
 
     def _layer(self, i: int, hidden: torch.Tensor, cache: KVCache, routing=None,

@@ -582,6 +582,95 @@ def test_prefix_same_as_a_joined_cache(dev):
 
 
 # ---------------------------------------------------------------------------
+# A step's token from its projection on
+# ---------------------------------------------------------------------------
+def check_fused(dev, seqlen, heads, rot=32, *, max_len=200, positions=None, norm=True, rows=None, row_map=None,
+                table=torch.float32, w_dtype=torch.float32, qkv=None, window=None, scale=None, seed=0):
+    """``quant_attention`` stores what ``apply_qkv_quant`` does, to the bit, and attends with its q."""
+    from maple_amd.kernels import QuantKV, apply_qkv_quant, quant_attention
+
+    nq, nkv, d = heads
+    b = len(seqlen)
+    qkv = bf16(dev, b, (nq + 2 * nkv) * d, seed=seed) if qkv is None else qkv
+    cache = filled(dev, rows or b, nkv, max_len, d, seed=seed + 1)
+    for r, n in enumerate(seqlen):  # what lies at the token's place and behind it does not matter
+        poison(cache, r if row_map is None else row_map[r], min(max(n, 0), max_len), max_len)
+    other = QuantKV(*(t.view(torch.uint8).clone().view(t.dtype) for t in cache))
+    qw = kw = None
+    if norm:
+        qw, kw = ((torch.rand(d, device=dev) + 0.5).to(w_dtype) for _ in range(2))
+    cos, sin = tables(max_len + 64, max(rot, 2), dev, table)
+    scale = d ** -0.5 if scale is None else scale
+    args = (qkv, qw, kw, cos, sin)
+    more = dict(positions=i64(dev, positions), row_map=i64(dev, row_map), num_heads=nq, num_kv_heads=nkv, head_dim=d,
+                rotary_dim=rot, use_rope=rot > 0, eps=EPS)
+    out = quant_attention(*args, cache, i64(dev, seqlen), scale=scale, window=window, **more)
+    q = apply_qkv_quant(*args, other, i64(dev, seqlen), **more)
+    assert all(torch.equal(x, y) for x, y in zip(bits(cache), bits(other)))
+    assert out.shape == q.shape and out.dtype == torch.bfloat16
+    k, v = values(cache)
+    for r in range(b):
+        cr = r if row_map is None else row_map[r]
+        ks, vs = oq.sequence((k[cr], v[cr]), min(seqlen[r] + 1, max_len), None, 0, window)
+        within(np64(out)[r, :, 0], *oq.attend(np64(q)[r, :, 0], ks, vs, scale))
+
+
+@pytest.mark.parametrize("heads", HEADS + [(16, 1, 128)])
+@pytest.mark.parametrize("rot", [0, 20, 64])
+def test_fused_layouts(dev, heads, rot):
+    check_fused(dev, [0, 1, 31, 32, 33, 127, 128, 199], heads, rot)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("window", [1, 2, 31, 64, 150, 2 ** 62])
+def test_fused_windows(dev, d, window):
+    check_fused(dev, [0, 1, 31, 63, 64, 65, 150, 199], (8, 2, d), window=window)
+
+
+@pytest.mark.parametrize("heads,n", [((8, 1, 64), 5000), ((16, 4, 128), 3001), ((32, 4, 64), 2048)])
+def test_fused_long_and_split(dev, heads, n):
+    check_fused(dev, [n - 1, n // 2, 0, 1023, 1024], heads, max_len=n)
+
+
+def test_fused_rows_positions_and_places(dev):
+    check_fused(dev, [-1, 3, 200, 2 ** 40, -2 ** 40, 199], (4, 2, 64), 64)  # no token; behind the cache's end
+    check_fused(dev, [-1, 1999, 2000], (16, 2, 128), 64, max_len=2000)
+    check_fused(dev, [3, 9], (4, 2, 64), positions=[100, -7])
+    check_fused(dev, [3, 9, 150], (4, 1, 128), 64, rows=5, row_map=[4, 0, 2])
+    check_fused(dev, [3, 70], (4, 1, 128), 64, norm=False)
+    check_fused(dev, [i % 70 for i in range(300)], (8, 1, 64), 64, max_len=70)
+
+
+@pytest.mark.parametrize("table", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("w_dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_fused_dtypes(dev, table, w_dtype):
+    check_fused(dev, [7, 101], (8, 2, 128), 128, table=table, w_dtype=w_dtype)
+
+
+def test_fused_odd_rows(dev):
+    w = (4 + 2 * 2) * 64
+    check_fused(dev, [1, 2, 130], (4, 2, 64), 64, qkv=bf16(dev, 3, w + 5, seed=12)[:, 5:])
+    check_fused(dev, [1, 2, 130], (16, 1, 128), 64, qkv=bf16(dev, 3, 18 * 128 + 1, seed=12)[:, 1:])
+
+
+def test_fused_not_finite_stays_in_its_row(dev):
+    from maple_amd.kernels import quant_attention
+
+    qkv = bf16(dev, 3, 8 * 64, seed=14)
+    qkv[0, 4 * 64 + 3] = float("nan")  # row 0, K head 0: query heads 0 and 1
+    qkv[1, 7 * 64 + 9] = float("inf")  # row 1, V head 1: dim 9 of query heads 2 and 3
+    c = filled(dev, 3, 2, 300, 64)
+    cos, sin = tables(300, 64, dev)
+    w = torch.ones(64, device=dev)
+    out = quant_attention(qkv, w, w, cos, sin, c, i64(dev, [200, 2, 77]), num_heads=4, num_kv_heads=2, head_dim=64,
+                          rotary_dim=64, scale=0.125)[:, :, 0]
+    odd = torch.isnan(out)
+    assert odd[0, :2].all() and odd[1, 2:, 9].all()
+    odd[0, :2], odd[1, 2:, 9] = False, False
+    assert not odd.any() and torch.isfinite(out[2]).all()
+
+
+# ---------------------------------------------------------------------------
 # Calls
 # ---------------------------------------------------------------------------
 def one_step(dev, cache, prefix, seqlen, qkv, w, cos, sin):
@@ -673,9 +762,47 @@ def test_two_captured_graphs(dev):
             assert torch.isfinite(other)
 
 
+def test_fused_captured_on_another_stream(dev):
+    """Two graphs of the fused step, replayed in turn on another stream, each against an eager step from the same cache."""
+    from maple_amd.kernels import QuantKV, quant_attention
+
+    states = [step_inputs(dev, seed=90), step_inputs(dev, seed=290)]
+
+    def step(s, cache):
+        _, _, seqlen, qkv, w, cos, sin = s
+        return quant_attention(qkv, w, w, cos, sin, cache, seqlen, num_heads=8, num_kv_heads=2, head_dim=64, rotary_dim=32,
+                               scale=0.125)
+
+    def copy(cache):
+        return QuantKV(*(t.view(torch.uint8).clone().view(t.dtype) for t in cache))
+
+    for s in states:
+        step(s, copy(s[0]))
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for s in states:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(step(s, s[0]))
+        graphs.append(g)
+    st = torch.cuda.Stream(dev)
+    for turn in range(4):
+        for i in (turn % 2, 1 - turn % 2):
+            states[i][3].copy_(bf16(dev, 5, 12 * 64, seed=2000 + 10 * turn + i))
+            states[i][2].add_(1 if turn else 0).clamp_(max=299)
+            fresh = copy(states[i][0])
+            want = step(states[i], fresh)
+            st.wait_stream(torch.cuda.current_stream(dev))
+            with torch.cuda.stream(st):
+                graphs[i].replay()
+            torch.cuda.synchronize()
+            assert torch.equal(want, outs[i])
+            assert all(torch.equal(x, y) for x, y in zip(bits(fresh), bits(states[i][0])))
+
+
 def test_empty_batches(dev):
     from maple_amd.kernels import (SharedPrefix, apply_qkv_quant, dequantize_kv, make_quant_kv, prefix_gqa_attn,
-                                   quant_gqa_attn, quantize_kv)
+                                   quant_attention, quant_gqa_attn, quantize_kv)
 
     c = make_quant_kv(2, 2, 16, 64, dev)
     none = i64(dev, [])
@@ -684,6 +811,8 @@ def test_empty_batches(dev):
                         head_dim=64, rotary_dim=32)
     assert q.shape == (0, 4, 1, 64)
     assert quant_gqa_attn(q, c, none, row_map=none, scale=1.0).shape == q.shape
+    assert quant_attention(bf16(dev, 0, 8 * 64), None, None, cos, sin, c, none, row_map=none, num_heads=4, num_kv_heads=2,
+                           head_dim=64, rotary_dim=32, scale=1.0).shape == q.shape
     assert prefix_gqa_attn(q, c, none, SharedPrefix(c, i64(dev, [3, 4]), none), row_map=none, scale=1.0).shape == q.shape
     assert dequantize_kv(c, 4, row_map=none).k.shape == (0, 2, 4, 64)
     x = bf16(dev, 2, 2, 0, 64)

@@ -8,7 +8,7 @@ import torch
 
 from maple_amd import _lib
 from maple_amd.kernels import (KV, QuantKV, SharedPrefix, apply_qkv_quant, dequantize_kv, make_quant_kv,
-                               prefix_gqa_attn, quant_gqa_attn, quantize_kv)
+                               prefix_gqa_attn, quant_attention, quant_gqa_attn, quantize_kv)
 
 BF = torch.bfloat16
 FAKE = 0x10000
@@ -36,14 +36,14 @@ def test_an_empty_cache_holds_zeros():
 QKV = dict(num_heads=4, num_kv_heads=2, head_dim=64, rotary_dim=32)
 
 
-def qkv_call(**kw):
+def qkv_call(of=apply_qkv_quant, **kw):
     a = dict(qkv=torch.zeros(2, 8 * 64, dtype=BF), q_weight=torch.ones(64), k_weight=torch.ones(64),
              cos_table=torch.zeros(16, 32), sin_table=torch.zeros(16, 32), cache=cache(), seqlen=n64(0, 1), **QKV)
     a.update(kw)
-    return apply_qkv_quant(**a)
+    return of(**a)
 
 
-@pytest.mark.parametrize("kw,error,match", [
+QKV_REFUSED = [
     (dict(), RuntimeError, "CUDA"),
     (dict(cache=plain()), TypeError, "QuantKV"),
     (dict(qkv=torch.zeros(2, 8 * 64)), ValueError, "bf16"),
@@ -68,10 +68,20 @@ def qkv_call(**kw):
     (dict(seqlen=torch.zeros(2)), TypeError, "whole"),
     (dict(positions=n64(0, 1, 2)), ValueError, "positions"),
     (dict(row_map=torch.ones(2)), TypeError, "row_map"),
-])
+]
+
+
+@pytest.mark.parametrize("kw,error,match", QKV_REFUSED)
 def test_qkv_refuses(kw, error, match):
     with pytest.raises(error, match=match):
         qkv_call(**kw)
+
+
+@pytest.mark.parametrize("kw,error,match", QKV_REFUSED + [(dict(window=0), ValueError, "window"),
+                                                         (dict(window=-1), ValueError, "window")])
+def test_fused_attention_refuses(kw, error, match):
+    with pytest.raises(error, match=match):
+        qkv_call(quant_attention, scale=0.125, **kw)
 
 
 @pytest.mark.parametrize("kw,error,match", [
@@ -201,17 +211,39 @@ def test_c_copies_refuse(entry, args, match):
                       a["out"], FAKE, None)
 
 
-@pytest.mark.parametrize("kw,error,match", [
+C_QKV_REFUSED = [
     (dict(d=32), ValueError, "head_dim"), (dict(nq=3), ValueError, "query heads"), (dict(ld=100), ValueError, "stride"),
     (dict(rot=66), ValueError, "rotary_dim"), (dict(rot=7), ValueError, "rotary_dim"), (dict(cos=None), ValueError, "tables"),
     (dict(n_pos=0), ValueError, "tables"), (dict(ld_cs=30), ValueError, "tables"), (dict(w_dt=9), TypeError, "dtype"),
     (dict(qw=None), ValueError, "norm weight"), (dict(qkv=None), ValueError, "null"), (dict(out=FAKE + 8), ValueError, "aligned"),
     (dict(batch=3), ValueError, "cache sizes"), (dict(batch=1 << 30, rm=FAKE), ValueError, "too large"),
-])
-def test_c_qkv_refuses(kw, error, match):
+]
+
+
+def c_qkv(**kw):
     a = dict(qkv=FAKE, ld=512, batch=2, nq=4, nkv=2, d=64, qw=FAKE, kw=FAKE, w_dt=0, cos=FAKE, sin=FAKE, dt=0, ld_cs=32,
              n_pos=16, rot=32, eps=1e-6, seqlen=FAKE, at=None, rm=None, kc=FAKE, vc=FAKE, ks=FAKE, vs=FAKE, rows=2, n=16,
              out=FAKE, stream=None)
     a.update(kw)
+    return a
+
+
+@pytest.mark.parametrize("kw,error,match", C_QKV_REFUSED)
+def test_c_qkv_refuses(kw, error, match):
     with pytest.raises(error, match=match):
-        _lib.call("ma_quant_qkv", *a.values())
+        _lib.call("ma_quant_qkv", *c_qkv(**kw).values())
+
+
+@pytest.mark.parametrize("kw,error,match", C_QKV_REFUSED + [
+    (dict(window=-1), ValueError, "window"), (dict(scale=float("inf")), ValueError, "scale"),
+    (dict(nq=34), ValueError, "query heads"), (dict(n=4096, ws=None), ValueError, "workspace"),
+    (dict(n=4096, nbytes=99), ValueError, "workspace"), (dict(ws=FAKE + 4), ValueError, "aligned"),
+    (dict(ks=None), ValueError, "null"), (dict(kc=FAKE + 8), ValueError, "aligned"), (dict(seqlen=None), ValueError, "null"),
+])
+def test_c_fused_attention_refuses(kw, error, match):
+    a = c_qkv()
+    out, stream = a.pop("out"), a.pop("stream")
+    a.update(window=0, scale=1.0, out=out, ws=FAKE, nbytes=1 << 40, stream=stream)
+    a.update(kw)
+    with pytest.raises(error, match=match):
+        _lib.call("ma_quant_attn", *a.values())
