@@ -4,6 +4,11 @@
 // positions; any other value than 0 .. P-1: none), then its own positions 0 ..
 // seqlen[b].  Lengths are clamped to the caches and mapped rows too, so nothing
 // is read outside them.
+//
+// A launch of splits, each a softmax of its own (reference, sum, sums of V), and one
+// that joins them.  Joined in the first launch, by the workgroup that is last to
+// arrive (sums written past the XCDs' L2s), it took longer than both: 1 x 4096 of 64
+// 12.8 us against 7.5, 16 x 4096 of 128 38 against 17.
 
 #include <math.h>
 
@@ -154,6 +159,12 @@ __device__ __forceinline__ void lay_v(char* vb, const u32x4c_t (&v)[VL], S&& s_o
 //   O += P V: A = the lane's own eight P (positions 4g.. of both halves), B = V in
 //     the same order from LDS, where a wave lays its tile as bf16 rows, by the
 //     transposing read.
+// Bound by the cache's bytes where there are many (quantised: 32 x 4096 of 64 13 us, 8 x
+// 32768 of 128 44 us: 4.0 and 4.8 TB/s of the 5.2 that a copy of 1 GiB reaches), by its
+// chain of loads where there are few (1 x 4096 of 64: 4.6 us; a wave has a tile).  Workgroups
+// of 16 waves (8 for heads of 128) in the place of splits were faster in calls one after
+// another (32 x 1000: 7.8 us against 8.6) but slower in whole steps (24 layers 1630
+// against 1584).
 template <int HD>
 struct OwnLds {
   char v[kCacheWaves][32 * 2 * HD];  // a wave's tile of V; at the end the waves' sums
@@ -481,6 +492,12 @@ struct PrefixLds {
 // per row, O += P V with V through the wave's LDS rows.  The reference moves when
 // the weights' sum shows that it has become too low (any that keeps them in range
 // gives the same quotient).
+// Bound by a tile's chain (scores, exponentials, products; the vector unit is busy half of
+// the time, the matrix unit a fifth) with two or three waves a SIMD: 32 rows of 32 heads
+// of 64 behind 8192 bf16 positions 12.7 us, 64 behind four prefixes of 16384 quantised ones
+// 19.6 (0.38 PFLOP/s; 0.6 behind 131072).  Leaving out 12 of a tile's 16 conversions of K
+// changes nothing.  64 rows a wave halve the conversions but leave too few waves (28
+// against 24 with the join), 128 rows of four waves on one tile in LDS took 33.
 template <int HD, bool Q8>
 __device__ __forceinline__ void cache_prefix(const CacheAttn& a, const CacheHot& hot, int slot, int unit, PrefixLds<HD>& lds) {
   constexpr int NW = kCacheWaves;
@@ -784,7 +801,9 @@ __global__ __launch_bounds__(kCacheThreads, (HD == 64 ? 4 : (Q8 ? 3 : 2))) void 
   cache_own<HD, Q8>(a, CacheHot{seqlen, row_map, of, length, nq, nkv, s_own, 0, 0}, blockIdx.x, lds);
 }
 
-// A step's token from its projection on: k_quant_qkv's work and the attention.
+// A step's token from its projection on: k_quant_qkv's work and the attention (a captured
+// step of 24 layers at 4000 positions: 697 us at one row, 1425 at 8, 1794 at 32, with
+// two launches 737, 1483, 1849).
 template <int HD, bool VEC>
 __global__ __launch_bounds__(kCacheThreads, HD == 64 ? 4 : 3) void k_quant_attn(const int64_t* seqlen, const int64_t* row_map,
                                                                                 int nq, int nkv, int s_own, NewToken token,
@@ -929,14 +948,14 @@ static int64_t cache_window(int64_t window, int64_t max_len, int64_t pre_len) {
 // row's positions, or 2048 and more of a prefix; none of a row's where that saves less than the
 // launch that joins them (about 4 us, six rounds of 128 positions).  Measured (us,
 // for this many workgroups):
-//   1 x 4096 of 64: 7.2 for 128, 7.5 for 256 (the most there are);  32 x 1024: 9.3
-//     unsplit, 9.6 for 256;  32 x 4096: 25.6, 18.0 for 256, 15.8 for 512, 16.5 for 768;
-//     2 x 32768: 17.9, 12.8, 12.2, 13.0
-//   4 x 4096 of 128: 11.6, 10.2, 11.9 for 512;  8 x 32768: 83, 54, 51, 53
-//   prefixes, 32 rows behind 8192 of 64: 18.4, 14.5, 17.1;  behind 32768: 44, 28, 26;
-//     64 behind two of 2000: 13.7 for 256, 17.6 for 512;  behind four of 4096: 15.9,
-//     16.0, 17.2 for 640;  of 8192: 20.7, 19.1, 20.2;  of 16384: 31.0, 23.6, 28.1;
-//     64 behind 8192 of 128: 29 for 128, 22, 28
+//   1 x 4096 of 64: 7.0 for 128, 7.3 for 256 (the most there are);  32 x 1024: 9.1
+//     unsplit, 9.2 for 256;  32 x 4096: 25.0, 18.1 for 256, 15.2 for 512, 15.9 for 768;
+//     2 x 32768: 17.7 for 128, 12.4, 12.0, 12.4
+//   4 x 4096 of 128: 11.5, 9.9, 10.7 for 512;  8 x 32768: 82, 55, 51, 52
+//   prefixes, 32 rows behind 8192 of 64: 18.0, 14.7, 15.3;  behind 32768: 44, 28, 24, 25;
+//     64 behind two of 2000: 14.4, 13.4, 14.3;  behind four of 4096: 18.9, 15.4, 15.6,
+//     18.8;  of 8192: 28, 20.2, 18.5, 21.5;  of 16384: 47, 29, 23, 29;
+//     64 behind 8192 of 128: 28, 21.5, 27
 static CachePlan cache_plan(int64_t batch, int nq, int nkv, int64_t max_len, int64_t prefixes, int64_t pre_len, int64_t window) {
   CachePlan p{1, 0, 0};
   const int64_t pairs = batch * nkv;

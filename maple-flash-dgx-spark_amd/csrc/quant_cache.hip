@@ -25,7 +25,9 @@ constexpr int kQuantThreads = 256;
 // out as bf16, k heads are rounded to bf16 (what a bf16 cache would hold, so both
 // ways of filling a cache give one set of codes) and quantised with their largest
 // value over the HD / 8 lanes of the head, v heads quantised as they are.
-// VEC: all rows are 16-byte aligned.
+// VEC: all rows are 16-byte aligned.  Bound by latency, two rounds of loads (the
+// token's row and place, then the tables): 3.7 us for a row of 32 + 8 heads of 64, 4.8 for
+// 256 rows of 16 + 8 heads of 128 (3 MB).
 template <int HD, bool VEC>
 __global__ __launch_bounds__(kQuantThreads) void k_quant_qkv(QkvIn in, int64_t batch, const int64_t* __restrict__ seqlen,
                                                              const int64_t* __restrict__ positions,
@@ -78,7 +80,9 @@ constexpr int kQuantRows = 4;  // rows a thread has in flight
 // HD / 16 lanes a row of 16 dims each, kQuantRows rows a thread; blockIdx.x: `chunks`
 // of a batch row's n_kv x T rows, blockIdx.y: K or V.  HEADS_IN: a batch row's heads
 // lie next to each other (positions before heads, as a projection leaves them), so
-// they are walked first; else positions are.
+// they are walked first; else positions are.  Bound by HBM: 32 prompts of up to 4096
+// positions (154 MB read and written) in 35.5 us, 4.3 TB/s (41 with 64-bit indexes); 3.0
+// for 7 positions.
 template <int HD, bool HEADS_IN, bool VEC>
 __global__ __launch_bounds__(kQuantThreads) void k_quant_kv(KvRows kr, KvRows vr, int chunks, uint32_t per, uint32_t T,
                                                             uint32_t nkv, const int64_t* __restrict__ start,
@@ -137,7 +141,9 @@ __global__ __launch_bounds__(kQuantThreads) void k_quant_kv(KvRows kr, KvRows vr
 // ---------------------------------------------------------------------------
 // HD / 16 lanes a row of 16 codes each; blockIdx.x: `chunks` of a (batch row, head)'s
 // positions, blockIdx.y: K or V.  A value is exact in bf16 (e4m3 has four
-// significant bits) unless 2^e takes it below bf16's least normal.
+// significant bits) unless 2^e takes it below bf16's least normal.  Bound by HBM: 32 rows
+// of 4096 positions (203 MB) in 37 to 43 us, 4.7 to 5.4 TB/s (45 with 64-bit indexes); 3.2
+// for 1001 positions of one row.
 template <int HD>
 __global__ __launch_bounds__(kQuantThreads) void k_dequant_kv(QuantCache cache, int chunks, uint32_t length, int nkv,
                                                               const int64_t* __restrict__ row_map,
