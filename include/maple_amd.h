@@ -861,8 +861,10 @@ int ma_dequant_kv(const void* k_codes, const void* v_codes, const void* k_scale,
  * read).  Lengths are clamped to the caches.  q / out bf16 [batch, n_heads,
  * head_dim]; float32 statistics and sums, P rounded to bf16 before P.V; a row
  * that sees nothing (or whose scores are all -inf) gives 0, and what lies behind
- * its positions does not reach it, finite or not.  Without a window a prefix is
- * read once for all of its rows.  At most 16 query heads to a KV head; batch x
+ * its positions does not reach it, finite or not.  `once`: a
+ * prefix is read once for all of its rows (> 0; refused under a window and with more
+ * than 64 prefixes), by each row with its own positions (0), or as is faster for the
+ * caches' sizes (< 0).  At most 16 query heads to a KV head; batch x
  * n_kv_heads and prefixes at most 65535; scale x log2 e finite.  workspace:
  * ma_cache_attn_workspace_bytes(...) bytes (may be 0), 16-byte aligned, its
  * content of no matter; calls that share one must not overlap.  The bf16 form
@@ -870,13 +872,13 @@ int ma_dequant_kv(const void* k_codes, const void* v_codes, const void* k_scale,
  */
 size_t ma_cache_attn_workspace_bytes(int64_t batch, int n_heads, int n_kv_heads, int head_dim,
                                      int64_t max_len, int64_t prefixes, int64_t prefix_max_len,
-                                     int64_t window);
+                                     int64_t window, int quantized, int once);
 int ma_cache_attn(const void* q, int64_t batch, int n_heads, int n_kv_heads, int head_dim,
                   const void* k, const void* v, const void* k_scale, const void* v_scale,
                   int64_t cache_rows, int64_t max_len, const int64_t* seqlen,
                   const int64_t* row_map, const void* pk, const void* pv, const void* pk_scale,
                   const void* pv_scale, int64_t prefixes, int64_t prefix_max_len,
-                  const int64_t* prefix_len, const int64_t* prefix_of, int64_t window,
+                  const int64_t* prefix_len, const int64_t* prefix_of, int once, int64_t window,
                   float scale, void* out, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
@@ -885,7 +887,7 @@ int ma_cache_attn(const void* q, int64_t batch, int n_heads, int n_kv_heads, int
  * [batch, n_heads, head_dim] bf16 over positions 0 .. seqlen[b] (with window > 0 the
  * last `window`).  Arguments and bounds as there; workspace:
  * ma_cache_attn_workspace_bytes(batch, n_heads, n_kv_heads, head_dim, max_len, 0, 0,
- * window) bytes (may be 0).  The bf16 cache's form of it is ma_decode_attn_fused.
+ * window, 1, -1) bytes (may be 0).  The bf16 cache's form of it is ma_decode_attn_fused.
  */
 int ma_quant_attn(const void* qkv, int64_t ldb, int64_t batch, int n_heads, int n_kv_heads,
                   int head_dim, const void* q_norm_w, const void* k_norm_w, int w_dtype,

@@ -107,8 +107,8 @@ _SIGNATURES = {
                      _P, _P],
     "ma_quant_kv": [_P, _L, _L, _L, _P, _L, _L, _L, _L, _L, _I, _I, _P, _P, _P, _P, _P, _P, _P, _L, _L, _P],
     "ma_dequant_kv": [_P, _P, _P, _P, _L, _L, _L, _L, _I, _I, _P, _P, _P, _P],
-    "ma_cache_attn_workspace_bytes": [_L, _I, _I, _I, _L, _L, _L, _L],
-    "ma_cache_attn": [_P, _L, _I, _I, _I, _P, _P, _P, _P, _L, _L, _P, _P, _P, _P, _P, _P, _L, _L, _P, _P, _L, _F, _P,
+    "ma_cache_attn_workspace_bytes": [_L, _I, _I, _I, _L, _L, _L, _L, _I, _I],
+    "ma_cache_attn": [_P, _L, _I, _I, _I, _P, _P, _P, _P, _L, _L, _P, _P, _P, _P, _P, _P, _L, _L, _P, _P, _I, _L, _F, _P,
                       _P, _Z, _P],
     "ma_quant_attn": [_P, _L, _L, _I, _I, _I, _P, _P, _I, _P, _P, _I, _L, _L, _I, _F, _P, _P, _P, _P, _P, _P, _P, _L, _L,
                       _L, _F, _P, _P, _Z, _P],

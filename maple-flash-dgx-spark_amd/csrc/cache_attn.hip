@@ -938,10 +938,25 @@ static int64_t cache_window(int64_t window, int64_t max_len, int64_t pre_len) {
   return window - pre_len > max_len ? 0 : window;
 }
 
-// prefixes: 0 where there are none.  A prefix is read once for all of its rows
-// except under a window, of which it holds at most that many positions a row and
-// each row others, and among more than kMaxShared: there each row reads them with
-// its own.
+// prefixes: 0 where there are none.  A prefix is read once for all of its rows or by
+// each row with its own positions (`once`, < 0: by this rule).  The second under a
+// window, of which a prefix holds at most that many positions a row and each row
+// others, among more than kMaxShared prefixes, and where it is faster: reads of one
+// prefix by several rows meet in the L2s, and workgroups for prefixes begin later (whose
+// rows?) and need the join.  Measured (us, once / each; rows of 100 own positions, 4 KV
+// heads, 32 query heads of 64 or 16 of 128; in the table's order by the bytes of a
+// position's K):
+//   64 (e4m3, 64): 8 rows behind one of 2000 9.6 / 9.4, of 4000 10.6 / 10.7;  64 behind
+//     1000 11.5 / 10.6, behind 2000 12.5 / 15.7;  256 behind 16 of 1000 25 / 18, of 2000
+//     25.5 / 27.5;  128 behind 64 of 2000 22.3 / 21.5
+//   128 (bf16, 64): 8 behind 4000 10.9 / 10.5;  64 behind 500 11.3 / 7.4, 1000 11.8 / 9.7,
+//     2000 12.9 / 19.5;  128 behind 64 of 2000 30.5 / 40.5;  64 behind as many 32 / 27.5
+//   128 (e4m3, 128): 64 behind 1000 14.6 / 14.3, 2000 15.0 / 21.4;  128 behind 64 of 2000
+//     45 / 31, 256 43 / 69
+//   256 (bf16, 128): 8 behind 2000 11.9 / 11.9;  64 behind 500 13.2 / 11.4, 1000 14.4 /
+//     15.7, 2000 15.6 / 30.9;  128 behind 64 of 2000 63 / 81;  64 behind as many 49 / 49
+// So once where a head's K of a prefix takes 112 KB, all rows' copies of it 14 MB, and a
+// position's K for the query rows of a prefix (on average) 2 KB.
 //
 // Splits, planned for the caches' lengths (the host does not know the rows').  A
 // workgroup a compute unit; two where a split would still hold more than 1024 of a
@@ -956,10 +971,17 @@ static int64_t cache_window(int64_t window, int64_t max_len, int64_t pre_len) {
 //     64 behind two of 2000: 14.4, 13.4, 14.3;  behind four of 4096: 18.9, 15.4, 15.6,
 //     18.8;  of 8192: 28, 20.2, 18.5, 21.5;  of 16384: 47, 29, 23, 29;
 //     64 behind 8192 of 128: 28, 21.5, 27
-static CachePlan cache_plan(int64_t batch, int nq, int nkv, int64_t max_len, int64_t prefixes, int64_t pre_len, int64_t window) {
+static bool prefix_once(int64_t batch, int nq, int nkv, int64_t row_bytes, int64_t prefixes, int64_t pre_len, int64_t window, int once) {
+  if (prefixes < 1 || prefixes > kMaxShared || window > 0) return false;
+  if (once >= 0) return once > 0;
+  const int64_t k = pre_len * row_bytes;
+  return k >= 112 << 10 && batch * nkv >= cdiv(14 << 20, k) && batch * (nq / nkv) * row_bytes >= (prefixes < batch ? prefixes : batch) << 11;
+}
+
+static CachePlan cache_plan(int64_t batch, int nq, int nkv, int64_t max_len, int64_t prefixes, int64_t pre_len, int64_t window,
+                            bool shared) {
   CachePlan p{1, 0, 0};
   const int64_t pairs = batch * nkv;
-  const bool shared = prefixes > 0 && prefixes <= kMaxShared && window == 0;
   int64_t span = max_len + (prefixes > 0 && !shared ? pre_len : 0);
   if (window > 0 && window < span) span = window;
   const int64_t n = cdiv(span, 128) + (prefixes > 0 && !shared ? 1 : 0);  // (either part ends in a round of its own)
@@ -992,7 +1014,7 @@ static size_t cache_ws_bytes(const CachePlan& p, int64_t batch, int nq, int head
 using namespace ma;
 
 static int check_cache_sizes(const char* what, int64_t batch, int nq, int nkv, int hd, int64_t rows, int64_t max_len,
-                             const void* row_map, int64_t prefixes, int64_t pre_len, int64_t window) {
+                             const void* row_map, int64_t prefixes, int64_t pre_len, int64_t window, int once = -1) {
   if (hd != 64 && hd != 128) return fail(MA_EVALUE, "%s: head_dim %d unsupported (64 or 128)", what, hd);
   if (nkv < 1 || nq < nkv || nq % nkv != 0 || nq / nkv > kCacheGroup || nq > 65535)
     return fail(MA_EVALUE, "%s: %d query heads over %d KV heads (at most %d to one)", what, nq, nkv, kCacheGroup);
@@ -1003,6 +1025,8 @@ static int check_cache_sizes(const char* what, int64_t batch, int nq, int nkv, i
     return fail(MA_EVALUE, "%s: bad cache sizes", what);
   if (prefixes < 0 || prefixes > 65535 || (prefixes > 0 && (pre_len < 1 || pre_len >= kMost)))
     return fail(MA_EVALUE, "%s: %lld prefixes of %lld positions", what, static_cast<long long>(prefixes), static_cast<long long>(pre_len));
+  if (once > 0 && prefixes > 0 && (prefixes > kMaxShared || cache_window(window, max_len, pre_len) > 0))
+    return fail(MA_EVALUE, "%s: more than %d prefixes, or a window's, are read by each row", what, kMaxShared);
   return MA_OK;
 }
 
@@ -1021,22 +1045,25 @@ static int cache_merge(const CachePlan& p, const CacheAttn& a, int head_dim, int
 }
 
 extern "C" size_t ma_cache_attn_workspace_bytes(int64_t batch, int n_heads, int n_kv_heads, int head_dim, int64_t max_len,
-                                                int64_t prefixes, int64_t prefix_max_len, int64_t window) {
+                                                int64_t prefixes, int64_t prefix_max_len, int64_t window, int quantized,
+                                                int once) {
   if (batch < 1 || check_cache_sizes("cache_attn", batch, n_heads, n_kv_heads, head_dim, batch, max_len, nullptr, prefixes,
-                                     prefix_max_len, window) != MA_OK)
+                                     prefix_max_len, window, once) != MA_OK)
     return 0;
   window = cache_window(window, max_len, prefixes > 0 ? prefix_max_len : 0);
-  return cache_ws_bytes(cache_plan(batch, n_heads, n_kv_heads, max_len, prefixes, prefix_max_len, window), batch, n_heads, head_dim);
+  const bool shared = prefix_once(batch, n_heads, n_kv_heads, quantized ? head_dim : 2 * head_dim, prefixes, prefix_max_len, window, once);
+  return cache_ws_bytes(cache_plan(batch, n_heads, n_kv_heads, max_len, prefixes, prefix_max_len, window, shared), batch, n_heads,
+                        head_dim);
 }
 
 extern "C" int ma_cache_attn(const void* q, int64_t batch, int n_heads, int n_kv_heads, int head_dim, const void* k,
                              const void* v, const void* k_scale, const void* v_scale, int64_t cache_rows, int64_t max_len,
                              const int64_t* seqlen, const int64_t* row_map, const void* pk, const void* pv,
                              const void* pk_scale, const void* pv_scale, int64_t prefixes, int64_t prefix_max_len,
-                             const int64_t* prefix_len, const int64_t* prefix_of, int64_t window, float scale, void* out,
+                             const int64_t* prefix_len, const int64_t* prefix_of, int once, int64_t window, float scale, void* out,
                              void* workspace, size_t workspace_bytes, void* stream) {
   const char* what = "cache_attn";
-  if (int rc = check_cache_sizes(what, batch, n_heads, n_kv_heads, head_dim, cache_rows, max_len, row_map, prefixes, prefix_max_len, window))
+  if (int rc = check_cache_sizes(what, batch, n_heads, n_kv_heads, head_dim, cache_rows, max_len, row_map, prefixes, prefix_max_len, window, once))
     return rc;
   if (!isfinite(scale * kLog2e)) return fail(MA_EVALUE, "%s: scale %g, or log2 e times it, is not finite", what, scale);
   if (batch == 0) return MA_OK;
@@ -1048,7 +1075,8 @@ extern "C" int ma_cache_attn(const void* q, int64_t batch, int n_heads, int n_kv
       !quant_aligned16(workspace) || (prefixes > 0 && (!quant_aligned16(pk) || !quant_aligned16(pv))))
     return fail(MA_EVALUE, "%s: q, the caches, out and the workspace must be 16-byte aligned", what);
   window = cache_window(window, max_len, prefixes > 0 ? prefix_max_len : 0);
-  const CachePlan p = cache_plan(batch, n_heads, n_kv_heads, max_len, prefixes, prefix_max_len, window);
+  const bool shared = prefix_once(batch, n_heads, n_kv_heads, q8 ? head_dim : 2 * head_dim, prefixes, prefix_max_len, window, once);
+  const CachePlan p = cache_plan(batch, n_heads, n_kv_heads, max_len, prefixes, prefix_max_len, window, shared);
   const int64_t parts = batch * n_heads * (p.s_own + p.s_pre);
   const size_t need = cache_ws_bytes(p, batch, n_heads, head_dim);
   if (need && (!workspace || workspace_bytes < need))
@@ -1106,7 +1134,7 @@ extern "C" int ma_quant_attn(const void* qkv, int64_t ldb, int64_t batch, int n_
   if (!quant_aligned16(out) || !quant_aligned16(workspace))
     return fail(MA_EVALUE, "%s: out and the workspace must be 16-byte aligned", what);
   window = cache_window(window, max_len, 0);
-  const CachePlan p = cache_plan(batch, n_heads, n_kv_heads, max_len, 0, 0, window);
+  const CachePlan p = cache_plan(batch, n_heads, n_kv_heads, max_len, 0, 0, window, false);
   const int64_t parts = batch * n_heads * p.s_own, wgs = batch * n_kv_heads * p.s_own;
   const size_t need = cache_ws_bytes(p, batch, n_heads, head_dim);
   if (need && (!workspace || workspace_bytes < need))

@@ -12,7 +12,7 @@ prompts, ``dequantize_kv`` reads positions back, ``quant_gqa_attn`` attends;
 A ``SharedPrefix`` holds the K/V with which several rows' sequences begin: row
 ``b``'s is the first ``length[of[b]]`` positions of prefix ``of[b]`` (any value that
 is no prefix's index: none), then the row's own cached positions 0 .. ``seqlen[b]``.
-``prefix_gqa_attn`` reads each prefix once for all of its rows, in a bf16 (``KV``) or a
+``prefix_gqa_attn`` reads a long prefix once for all of its rows, in a bf16 (``KV``) or a
 quantised cache.
 
 No reference counterpart: its cache is bf16 with a row to a sequence
@@ -263,7 +263,7 @@ _NO_PREFIX = (None,) * 4
 
 
 def _attend(what: str, q: torch.Tensor, cache, seqlen: torch.Tensor, prefix: SharedPrefix | None, row_map, scale: float,
-            window: int | None) -> torch.Tensor:
+            window: int | None, once: bool | None = None) -> torch.Tensor:
     if q.ndim != 4 or q.shape[2] != 1 or q.dtype != torch.bfloat16:
         raise ValueError(f"{what} expects bf16 q [B, H, 1, D], got {q.dtype} {tuple(q.shape)}.")
     bsz, n_q, _, head_dim = q.shape
@@ -297,14 +297,15 @@ def _attend(what: str, q: torch.Tensor, cache, seqlen: torch.Tensor, prefix: Sha
     if not q.is_contiguous():
         q = q.contiguous()
     out = torch.empty_like(q)
-    nbytes = _workspace_bytes(bsz, n_q, n_kv, head_dim, max_len, n_pre, pre_max, window)
+    form = -1 if once is None else int(once)
+    nbytes = _workspace_bytes(bsz, n_q, n_kv, head_dim, max_len, n_pre, pre_max, window, quant, form)
     # scratch of this call alone: the allocator keeps it to this stream, a
     # captured graph to its own pool
     ws = q.new_empty(nbytes // 2) if nbytes else None
     _call(
         idx, "ma_cache_attn",
         q.data_ptr(), bsz, n_q, n_kv, head_dim, *map(_ptr, cache), *(() if quant else (None, None)), rows, max_len, sl.data_ptr(), rm, *shared, n_pre, pre_max,
-        p_len, p_of, window, scale, out.data_ptr(), _lib.ptr(ws), nbytes,
+        p_len, p_of, form, window, scale, out.data_ptr(), _lib.ptr(ws), nbytes,
     )
     return out
 
@@ -354,7 +355,7 @@ def quant_attention(
     idx, args, _keep = _projection("quant_attention", qkv, q_weight, k_weight, cos_table, sin_table, cache, seqlen, positions,
                                    row_map, num_heads, num_kv_heads, head_dim, rotary_dim, use_rope, eps)
     out = qkv.new_empty((qkv.shape[0], num_heads, 1, head_dim))
-    nbytes = _workspace_bytes(qkv.shape[0], num_heads, num_kv_heads, head_dim, args[-1], 0, 0, window)
+    nbytes = _workspace_bytes(qkv.shape[0], num_heads, num_kv_heads, head_dim, args[-1], 0, 0, window, True, -1)
     ws = qkv.new_empty(nbytes // 2) if nbytes else None  # (as in _attend)
     _call(idx, "ma_quant_attn", *args, window, scale, out.data_ptr(), _lib.ptr(ws), nbytes)
     return out
@@ -369,13 +370,18 @@ def prefix_gqa_attn(
     row_map: torch.Tensor | None = None,
     scale: float,
     window: int | None = None,
+    once: bool | None = None,
 ) -> torch.Tensor:
     """GQA attention for ``q_len=1`` over rows whose sequences begin with shared
     prefixes: ``q [B, H, 1, D]`` bf16 over prefix ``of[b]`` and then the row's own
     positions 0 .. ``seqlen[b]`` (none where that is negative), the last ``window`` of
-    both together.  Without a window each prefix is read once for all of its rows;
-    with one each row reads the positions that it sees.  The prefix is of the
-    cache's kind."""
+    both together.  The prefix is of the cache's kind.
+
+    ``once``: each prefix is read once for all of its rows (True; not under a window, nor
+    for more than 64 prefixes), or by each row with its own positions (False).  By
+    default as is faster for the caches' sizes, which the host knows: a caller whose
+    prefixes are much shorter than their cache, or on whose longest one most rows
+    stand, may know better."""
     if not isinstance(cache, (KV, QuantKV)):
         raise TypeError(f"prefix_gqa_attn takes a KV or a QuantKV, got {type(cache).__name__}.")
-    return _attend("prefix_gqa_attn", q, cache, seqlen, prefix, row_map, scale, window)
+    return _attend("prefix_gqa_attn", q, cache, seqlen, prefix, row_map, scale, window, once)

@@ -305,7 +305,8 @@ class KVCache:
         """Take the first ``lengths[p]`` positions of cache row ``rows[p]`` as prefix ``p``
         (copied: the rows are free again), held once for all slots that begin with it.
         Every slot begins with none; ``prefix.of[slot] = p`` with ``seqlen[slot]`` set to
-        the slot's own positions (0 for a new sequence) puts one behind prefix ``p``."""
+        the slot's own positions (0 for a new sequence) puts one behind prefix ``p``.
+        Share before capturing a step: a graph captured earlier knows of no prefixes."""
         rows, lengths = [int(r) for r in rows], [int(n) for n in lengths]
         if self.prefix is not None:
             raise ValueError("the cache has shared prefixes already.")

@@ -299,22 +299,26 @@ def check_attn(dev, cache, seqlen, nq, *, prefix=None, window=None, row_map=None
         q = bf16(dev, b, nq, 1, d, seed=seed)
     kw = dict(row_map=i64(dev, row_map), scale=scale, window=window)
     if prefix is None:
-        out = quant_gqa_attn(q, cache, i64(dev, seqlen), **kw)
+        outs = [quant_gqa_attn(q, cache, i64(dev, seqlen), **kw)]
         of, plen = [-1] * b, []
-    else:
+    else:  # (as the sizes decide, by each row, and once for all rows)
         shared, plen, of = prefix
-        out = prefix_gqa_attn(q, cache, i64(dev, seqlen), SharedPrefix(shared, i64(dev, plen), i64(dev, of)), **kw)
+        forms = (None, False, True) if len(plen) <= 64 and (window or 2 ** 60) >= 2 ** 60 else (None, False)
+        outs = [prefix_gqa_attn(q, cache, i64(dev, seqlen), SharedPrefix(shared, i64(dev, plen), i64(dev, of)), once=once, **kw)
+                for once in forms]
         sk, sv = values(shared)
-    assert out.shape == q.shape and out.dtype == torch.bfloat16
     k, v = values(cache)
-    got, qn = np64(out)[:, :, 0], np64(q)[:, :, 0]
+    qn = np64(q)[:, :, 0]
     for r in range(b):
         cr = r if row_map is None else row_map[r]
         has = 0 <= of[r] < len(plen)
         pre, n_pre = ((sk[of[r]], sv[of[r]]), min(max(plen[of[r]], 0), sk.shape[2])) if has else (None, 0)
         ks, vs = oq.sequence((k[cr], v[cr]), min(seqlen[r] + 1, max_len), pre, n_pre, window)
-        within(got[r], *oq.attend(qn[r], ks, vs, scale))
-    return out
+        ref = oq.attend(qn[r], ks, vs, scale)
+        for out in outs:
+            assert out.shape == q.shape and out.dtype == torch.bfloat16
+            within(np64(out[r])[:, 0], *ref)
+    return outs[-1]
 
 
 HEADS = [(32, 4, 64), (16, 4, 128), (16, 1, 64), (3, 1, 128), (2, 2, 64), (12, 4, 128)]
@@ -395,7 +399,8 @@ def test_attn_what_is_not_finite_and_seen_does(dev):
 
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("at", ["own", "prefix"])
-def test_attn_infinite_values(dev, d, at):
+@pytest.mark.parametrize("once", [False, True])
+def test_attn_infinite_values(dev, d, at, once):
     """An infinite V, at the last position of a tile that is not full, is infinite in its dim and leaves the others."""
     from maple_amd.kernels import KV, SharedPrefix, prefix_gqa_attn
 
@@ -403,7 +408,7 @@ def test_attn_infinite_values(dev, d, at):
     pre = KV(bf16(dev, 1, 2, 75, d, seed=32), bf16(dev, 1, 2, 75, d, seed=33))
     (own.v[0, :, 49] if at == "own" else pre.v[0, :, 74])[:, 5] = float("inf")
     out = prefix_gqa_attn(bf16(dev, 2, 4, 1, d), own, i64(dev, [49, 20]),
-                          SharedPrefix(pre, i64(dev, [75]), i64(dev, [0, -1])), scale=d ** -0.5)
+                          SharedPrefix(pre, i64(dev, [75]), i64(dev, [0, -1])), scale=d ** -0.5, once=once)
     assert (out[0, :, 0, 5] == float("inf")).all()
     out[0, :, 0, 5] = 0
     assert torch.isfinite(out).all()
@@ -520,11 +525,43 @@ def test_prefix_many_prefixes(dev, quant, prefixes):
                prefix=(make(dev, quant, prefixes, 2, 77, 64, 57), [int(x) for x in g.integers(0, 78, prefixes)], of))
 
 
+@pytest.mark.parametrize("quant", [False, True])
+@pytest.mark.parametrize("once", [False, True])
+@pytest.mark.parametrize("big", [2.0 ** 20, -2.0 ** 40, 2.0 ** 60, 2.0 ** 110])
+def test_prefix_scores_of_any_size(dev, quant, once, big):
+    """One key of the prefix far above the rest: its value is the output, at any size of the scores and for q of either sign."""
+    from maple_amd.kernels import KV, SharedPrefix, make_quant_kv, prefix_gqa_attn, quantize_kv
+
+    sign = 1.0 if big > 0 else -1.0
+    k = torch.full((1, 1, 400, 64), 0.0, device=dev, dtype=torch.bfloat16)
+    k[..., 0] = sign
+    k[0, 0, 217, 0] = 1.5 * sign
+    v = bf16(dev, 1, 1, 400, 64, seed=59)
+    pre = quantize_kv(k, v, make_quant_kv(1, 1, 400, 64, dev)) if quant else KV(k, v)
+    own = make(dev, quant, 3, 1, 30, 64, 60)
+    for t in (own.k,):  # (the rows' own keys are far below)
+        t.view(torch.uint8).zero_()
+    q = torch.zeros(3, 16, 1, 64, device=dev, dtype=torch.bfloat16)
+    q[..., 0] = big
+    out = prefix_gqa_attn(q, own, i64(dev, [29, -1, 4]), SharedPrefix(pre, i64(dev, [400]), i64(dev, [0, 0, 0])), scale=1.0,
+                          once=once)
+    want = values(pre)[1][0, 0, 217]
+    assert (np.abs(np64(out)[:, :, 0] - want) <= 2.0 ** -8 * np.abs(want)).all()
+
+
 def test_prefix_long_and_split(dev):
     check_attn(dev, make(dev, True, 9, 1, 50, 64, 56), [49, 3, 7, 0, 1, 2, 20, 30, 40], 8,
                prefix=(make(dev, True, 1, 1, 9000, 64, 58), [8999], [0] * 9))
     check_attn(dev, make(dev, False, 3, 2, 50, 128, 60), [49, 3, 7], 8,
                prefix=(make(dev, False, 1, 2, 5000, 128, 62), [4801], [0] * 3))
+
+
+def test_prefix_forms_by_size(dev):
+    """A prefix cache past the sizes from which it is read once (rows' and prefixes' splits, tiles and one merge)."""
+    check_attn(dev, make(dev, True, 32, 4, 40, 64, 61), [i % 41 - 1 for i in range(32)], 32,
+               prefix=(make(dev, True, 2, 4, 2100, 64, 62), [2100, 1777], [(i % 5) // 2 for i in range(32)]))
+    check_attn(dev, make(dev, False, 24, 4, 40, 128, 63), [i % 41 - 1 for i in range(24)], 16,
+               prefix=(make(dev, False, 1, 4, 1100, 128, 64), [1100], [0] * 23 + [-1]))
 
 
 def test_prefix_row_map(dev):
@@ -533,23 +570,26 @@ def test_prefix_row_map(dev):
 
 
 @pytest.mark.parametrize("quant", [False, True])
-def test_prefix_what_is_not_seen_does_not_matter(dev, quant):
+@pytest.mark.parametrize("once", [False, True])
+def test_prefix_what_is_not_seen_does_not_matter(dev, quant, once):
     from maple_amd.kernels import SharedPrefix, prefix_gqa_attn
 
     own, pre = make(dev, quant, 4, 2, 70, 64, 68), make(dev, quant, 3, 2, 200, 64, 70)
     seqlen, plen, of = [-1, 10, 69, 31], [100, 64, 200], [0, 1, 0, -1]
-    want = check_attn(dev, own, seqlen, 8, prefix=(pre, plen, of))
+    want = prefix_gqa_attn(bf16(dev, 4, 8, 1, 64, seed=20), own, i64(dev, seqlen),
+                           SharedPrefix(pre, i64(dev, plen), i64(dev, of)), scale=0.125, once=once)
     for r, n in enumerate(seqlen):
         poison(own, r, n + 1, 70)
     for p, n in enumerate(plen[:2]):
         poison(pre, p, n, 200)
     poison(pre, 2, 0, 200)
     got = prefix_gqa_attn(bf16(dev, 4, 8, 1, 64, seed=20), own, i64(dev, seqlen),
-                          SharedPrefix(pre, i64(dev, plen), i64(dev, of)), scale=0.125)
+                          SharedPrefix(pre, i64(dev, plen), i64(dev, of)), scale=0.125, once=once)
     assert torch.equal(got, want)
 
 
-def test_prefix_stays_with_its_rows(dev):
+@pytest.mark.parametrize("once", [False, True])
+def test_prefix_stays_with_its_rows(dev, once):
     """A NaN in a prefix reaches the rows that begin with it and no other."""
     from maple_amd.kernels import SharedPrefix, prefix_gqa_attn
 
@@ -557,7 +597,7 @@ def test_prefix_stays_with_its_rows(dev):
     poison(pre, 1, 3, 4)
     of = [i % 3 - 1 for i in range(40)]
     out = prefix_gqa_attn(bf16(dev, 40, 16, 1, 64), own, i64(dev, [19] * 40),
-                          SharedPrefix(pre, i64(dev, [100, 100]), i64(dev, of)), scale=0.125)
+                          SharedPrefix(pre, i64(dev, [100, 100]), i64(dev, of)), scale=0.125, once=once)
     for r in range(40):
         assert (torch.isnan(out[r]).all() if of[r] == 1 else torch.isfinite(out[r]).all())
 
@@ -566,12 +606,12 @@ def test_prefix_same_as_a_joined_cache(dev):
     """The prefix copied into every row: the same output up to rounding of the weights, bf16 and quantised."""
     from maple_amd.kernels import KV, QuantKV, SharedPrefix, decode_gqa_attn, prefix_gqa_attn, quant_gqa_attn
 
-    for quant in (False, True):
+    for quant, once in ((False, False), (False, True), (True, False), (True, True)):
         own, pre = make(dev, quant, 3, 2, 40, 64, 76), make(dev, quant, 1, 2, 128, 64, 78)
         both = [torch.cat([p.view(torch.uint8).expand(3, *p.view(torch.uint8).shape[1:]), o.view(torch.uint8)],
                           2).view(o.dtype) for p, o in zip(pre, own)]
         q, n = bf16(dev, 3, 8, 1, 64, seed=80), i64(dev, [39, 39, 39])
-        a = prefix_gqa_attn(q, own, n, SharedPrefix(pre, i64(dev, [128]), i64(dev, [0, 0, 0])), scale=0.125)
+        a = prefix_gqa_attn(q, own, n, SharedPrefix(pre, i64(dev, [128]), i64(dev, [0, 0, 0])), scale=0.125, once=once)
         b = (quant_gqa_attn(q, QuantKV(*both), n + 128, scale=0.125) if quant else
              decode_gqa_attn(q, *both, n + 128, scale=0.125, window=None))
         k, v = values(QuantKV(*both) if quant else KV(*both))
@@ -680,7 +720,7 @@ def one_step(dev, cache, prefix, seqlen, qkv, w, cos, sin):
     at = seqlen + prefix.length[prefix.of.clamp(min=0)] * (prefix.of >= 0)
     q = apply_qkv_quant(qkv, w, w, cos, sin, cache, seqlen, positions=at, num_heads=8, num_kv_heads=2, head_dim=64,
                         rotary_dim=32)
-    return quant_gqa_attn(q, cache, seqlen, scale=0.125), prefix_gqa_attn(q, cache, seqlen, prefix, scale=0.125)
+    return quant_gqa_attn(q, cache, seqlen, scale=0.125), prefix_gqa_attn(q, cache, seqlen, prefix, scale=0.125, once=True)
 
 
 def step_inputs(dev, seed=90):

@@ -155,7 +155,7 @@ def test_prefixes_refused(prefix, error, match):
 
 def c_attn(**kw):
     a = dict(q=FAKE, batch=2, nq=4, nkv=2, d=64, k=FAKE, v=FAKE, ks=FAKE, vs=FAKE, rows=2, n=128, seqlen=FAKE, rm=None,
-             pk=None, pv=None, pks=None, pvs=None, p=0, pn=0, plen=None, of=None, window=0, scale=1.0, out=FAKE,
+             pk=None, pv=None, pks=None, pvs=None, p=0, pn=0, plen=None, of=None, once=-1, window=0, scale=1.0, out=FAKE,
              ws=FAKE, nbytes=1 << 40, stream=None)
     a.update(kw)
     return _lib.call("ma_cache_attn", *a.values())
@@ -174,6 +174,7 @@ PRE = dict(pk=FAKE, pv=FAKE, pks=FAKE, pvs=FAKE, p=3, pn=100, plen=FAKE, of=FAKE
     (dict(PRE, of=None), "null"), (dict(PRE, pks=None), "kind"), (dict(PRE, ks=None, vs=None), "kind"),
     (dict(PRE, pn=0), "prefixes"), (dict(PRE, p=-1), "prefixes"), (dict(PRE, p=70000), "prefixes"),
     (dict(PRE, pk=FAKE + 8), "aligned"),
+    (dict(PRE, once=1, window=5), "each row"), (dict(PRE, once=1, p=65), "each row"),
 ])
 def test_c_attention_refuses(kw, match):
     with pytest.raises(ValueError, match=match):
@@ -182,13 +183,19 @@ def test_c_attention_refuses(kw, match):
 
 def test_c_attention_workspace():
     lib = _lib.load()
-    need = lambda *a: int(lib.ma_cache_attn_workspace_bytes(*a))  # noqa: E731
+    need = lambda *a: int(lib.ma_cache_attn_workspace_bytes(*a, *(() if len(a) == 10 else (1, -1))))  # noqa: E731
     assert need(1, 32, 4, 64, 4096, 0, 0, 0) > 0
     assert need(1, 32, 4, 64, 128, 0, 0, 0) == 0  # one split: nothing to join
     assert need(0, 32, 4, 64, 4096, 0, 0, 0) == 0
     assert need(1, 32, 4, 96, 4096, 0, 0, 0) == 0
     # a window past every distance is none
     assert need(4, 32, 4, 64, 4096, 2, 1000, 2 ** 62) == need(4, 32, 4, 64, 4096, 2, 1000, 0) > 0
+    # a prefix that is read once is a part of its own
+    once = lambda kind, form, b=64, n=2000, p=2: need(b, 32, 4, 64, 128, p, n, 0, kind, form)  # noqa: E731
+    assert once(1, -1) == once(1, 1) != once(1, 0)
+    assert once(0, -1, n=1000) == once(0, 1, n=1000) and once(1, -1, n=1000) == once(1, 0, n=1000)  # (by its bytes)
+    assert once(1, -1, b=4) == once(1, 0, b=4) and once(1, -1, p=64) == once(1, 0, p=64)  # (by the rows behind it)
+    assert once(1, 1, p=65) == 0  # (refused)
 
 
 @pytest.mark.parametrize("entry,args,match", [
