@@ -68,6 +68,7 @@ __global__ __launch_bounds__(kQuantThreads) void k_quant_qkv(QkvIn in, int64_t b
 // ---------------------------------------------------------------------------
 // Prompts in
 // ---------------------------------------------------------------------------
+typedef uint32_t u32x2q_t __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4q_t __attribute__((ext_vector_type(4)));
 
 struct KvRows {  // bf16 [batch, n_kv, T, HD], the last dim contiguous
@@ -77,18 +78,20 @@ struct KvRows {  // bf16 [batch, n_kv, T, HD], the last dim contiguous
 
 constexpr int kQuantRows = 4;  // rows a thread has in flight
 
-// HD / 16 lanes a row of 16 dims each, kQuantRows rows a thread; blockIdx.x: `chunks`
+// HD / 8 lanes a row of 8 dims each, so that a wave's loads and stores are whole lines
+// (16 dims a lane: 34 to 36 us), kQuantRows rows a thread (8: 37); blockIdx.x: `chunks`
 // of a batch row's n_kv x T rows, blockIdx.y: K or V.  HEADS_IN: a batch row's heads
 // lie next to each other (positions before heads, as a projection leaves them), so
-// they are walked first; else positions are.  Bound by HBM: 32 prompts of up to 4096
-// positions (154 MB read and written) in 35.5 us, 4.3 TB/s (41 with 64-bit indexes); 3.0
-// for 7 positions.
+// they are walked first; else positions are.  Stores pass the caches by, which the
+// next reader would not find them in (33 to 37 us else).  Bound by HBM: 32 prompts of
+// up to 4096 positions (154 MB read and written) in 31 to 33 us, 4.8 TB/s; 2.9 for 7
+// positions.
 template <int HD, bool HEADS_IN, bool VEC>
 __global__ __launch_bounds__(kQuantThreads) void k_quant_kv(KvRows kr, KvRows vr, int chunks, uint32_t per, uint32_t T,
                                                             uint32_t nkv, const int64_t* __restrict__ start,
                                                             const int64_t* __restrict__ lengths,
                                                             const int64_t* __restrict__ row_map, QuantCache cache) {
-  constexpr int LPR = HD / 16, RPB = kQuantThreads / LPR;
+  constexpr int LPR = HD / 8, RPB = kQuantThreads / LPR;
   const int tid = threadIdx.x, l = tid % LPR;
   const bool is_v = blockIdx.y != 0;
   const KvRows src = is_v ? vr : kr;
@@ -96,7 +99,7 @@ __global__ __launch_bounds__(kQuantThreads) void k_quant_kv(KvRows kr, KvRows vr
   const uint32_t r0 = (blockIdx.x - static_cast<uint32_t>(b) * chunks) * (kQuantRows * RPB) + tid / LPR;
   const int64_t p0 = start ? start[b] : 0, most = lengths ? lengths[b] : T;
   const int64_t crow = row_map ? clamp_pos(row_map[b], 0, cache.rows - 1) : b;
-  u32x4q_t x[kQuantRows][2];
+  u32x4q_t x[kQuantRows];
   int64_t to[kQuantRows];
 #pragma unroll
   for (int i = 0; i < kQuantRows; ++i) {
@@ -105,15 +108,14 @@ __global__ __launch_bounds__(kQuantThreads) void k_quant_kv(KvRows kr, KvRows vr
     const int64_t p = p0 + t;
     const bool in = r < per && t < most && p >= 0 && p < cache.max_len;
     to[i] = in ? (crow * nkv + h) * cache.max_len + p : -1;
-    x[i][0] = x[i][1] = u32x4q_t{0u, 0u, 0u, 0u};
+    x[i] = u32x4q_t{0u, 0u, 0u, 0u};
     if (!in) continue;
-    const uint16_t* const s = src.p + b * src.sb + h * src.sh + t * src.st + 16 * l;
+    const uint16_t* const s = src.p + b * src.sb + h * src.sh + t * src.st + 8 * l;
     if constexpr (VEC) {
-      x[i][0] = reinterpret_cast<const u32x4q_t*>(s)[0];
-      x[i][1] = reinterpret_cast<const u32x4q_t*>(s)[1];
+      x[i] = *reinterpret_cast<const u32x4q_t*>(s);
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[i][e / 4][e % 4] = s[2 * e] | static_cast<uint32_t>(s[2 * e + 1]) << 16;
+      for (int e = 0; e < 4; ++e) x[i][e] = s[2 * e] | static_cast<uint32_t>(s[2 * e + 1]) << 16;
     }
   }
   MA_ISSUE_FENCE();
@@ -121,17 +123,11 @@ __global__ __launch_bounds__(kQuantThreads) void k_quant_kv(KvRows kr, KvRows vr
   uint8_t* const scales = is_v ? cache.vs : cache.ks;
 #pragma unroll
   for (int i = 0; i < kQuantRows; ++i) {
-    int top = 0;
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-      top = finite_top(finite_top(finite_top(finite_top(top, x[i][j].x), x[i][j].y), x[i][j].z), x[i][j].w);
-    top = group_top<LPR>(top);
+    const uint4 r = make_uint4(x[i].x, x[i].y, x[i].z, x[i].w);
+    const int byte = head_byte<HD>(r);
     if (to[i] < 0) continue;
-    const int byte = quant_byte(top);
-    const float inv = quant_inverse(byte);
-    *reinterpret_cast<uint4*>(codes + to[i] * HD + 16 * l) =
-        make_uint4(quant_four(x[i][0].x, x[i][0].y, inv), quant_four(x[i][0].z, x[i][0].w, inv),
-                   quant_four(x[i][1].x, x[i][1].y, inv), quant_four(x[i][1].z, x[i][1].w, inv));
+    const uint2 c = quant_eight(r, byte);
+    __builtin_nontemporal_store(u32x2q_t{c.x, c.y}, reinterpret_cast<u32x2q_t*>(codes + to[i] * HD + 8 * l));
     if (l == 0) scales[to[i]] = static_cast<uint8_t>(byte);
   }
 }
@@ -139,17 +135,17 @@ __global__ __launch_bounds__(kQuantThreads) void k_quant_kv(KvRows kr, KvRows vr
 // ---------------------------------------------------------------------------
 // Cached positions back
 // ---------------------------------------------------------------------------
-// HD / 16 lanes a row of 16 codes each; blockIdx.x: `chunks` of a (batch row, head)'s
+// HD / 8 lanes a row of 8 codes each (16: 43 us for the case below); blockIdx.x: `chunks` of a (batch row, head)'s
 // positions, blockIdx.y: K or V.  A value is exact in bf16 (e4m3 has four
 // significant bits) unless 2^e takes it below bf16's least normal.  Bound by HBM: 32 rows
-// of 4096 positions (203 MB) in 37 to 43 us, 4.7 to 5.4 TB/s (45 with 64-bit indexes); 3.2
-// for 1001 positions of one row.
+// of 4096 positions (203 MB) in 30.4 us, 6.7 TB/s with what the last-level cache holds of
+// the codes (36.3 without nontemporal stores); 2.9 for 1001 positions of one row.
 template <int HD>
 __global__ __launch_bounds__(kQuantThreads) void k_dequant_kv(QuantCache cache, int chunks, uint32_t length, int nkv,
                                                               const int64_t* __restrict__ row_map,
                                                               uint16_t* __restrict__ k_out,
                                                               uint16_t* __restrict__ v_out) {
-  constexpr int LPR = HD / 16, RPB = kQuantThreads / LPR;
+  constexpr int LPR = HD / 8, RPB = kQuantThreads / LPR;
   const int tid = threadIdx.x, l = tid % LPR;
   const bool is_v = blockIdx.y != 0;
   const uint8_t* const codes = is_v ? cache.v : cache.k;
@@ -158,13 +154,13 @@ __global__ __launch_bounds__(kQuantThreads) void k_dequant_kv(QuantCache cache, 
   const int64_t pair = blockIdx.x / chunks, b = pair / nkv, h = pair - b * nkv;
   const uint32_t r0 = (blockIdx.x - static_cast<uint32_t>(pair) * chunks) * (kQuantRows * RPB) + tid / LPR;
   const int64_t from = ((row_map ? clamp_pos(row_map[b], 0, cache.rows - 1) : b) * nkv + h) * cache.max_len;
-  u32x4q_t c[kQuantRows];
+  u32x2q_t c[kQuantRows];
   int byte[kQuantRows];
 #pragma unroll
   for (int i = 0; i < kQuantRows; ++i) {
     const uint32_t t = r0 + i * RPB;
     const int64_t at = from + (t < length ? t : 0);
-    c[i] = *reinterpret_cast<const u32x4q_t*>(codes + at * HD + 16 * l);
+    c[i] = *reinterpret_cast<const u32x2q_t*>(codes + at * HD + 8 * l);
     byte[i] = scales[at];
   }
   MA_ISSUE_FENCE();
@@ -174,18 +170,17 @@ __global__ __launch_bounds__(kQuantThreads) void k_dequant_kv(QuantCache cache, 
     const uint32_t t = r0 + i * RPB;
     if (t >= length) continue;
     const float s = quant_scale(byte[i]);
-    const uint32_t w[4] = {c[i].x, c[i].y, c[i].z, c[i].w};
-    uint32_t o[8];
+    const uint32_t w[2] = {c[i].x, c[i].y};
+    uint32_t o[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < 2; ++j) {
       const f32x2q_t a = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(w[j]), false);
       const f32x2q_t b = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(w[j]), true);
       o[2 * j] = pack_bf16x2_rn(a.x * s, a.y * s);
       o[2 * j + 1] = pack_bf16x2_rn(b.x * s, b.y * s);
     }
-    uint4* const to = reinterpret_cast<uint4*>(out + (pair * length + t) * HD + 16 * l);
-    to[0] = make_uint4(o[0], o[1], o[2], o[3]);
-    to[1] = make_uint4(o[4], o[5], o[6], o[7]);
+    __builtin_nontemporal_store(u32x4q_t{o[0], o[1], o[2], o[3]},
+                                reinterpret_cast<u32x4q_t*>(out + (pair * length + t) * HD + 8 * l));
   }
 }
 
@@ -234,7 +229,7 @@ extern "C" int ma_quant_kv(const void* k, int64_t k_sb, int64_t k_sh, int64_t k_
   if (T < 0) return fail(MA_EVALUE, "%s: bad sizes", what);
   if (batch == 0 || T == 0) return MA_OK;
   if (!k || !v) return fail(MA_EVALUE, "%s: null pointer", what);
-  const int64_t rpb = kQuantThreads / (head_dim / 16) * kQuantRows;
+  const int64_t rpb = kQuantThreads / (head_dim / 8) * kQuantRows;
   if (T > INT32_MAX / n_kv_heads || batch > kMaxGroups / cdiv(T * n_kv_heads, rpb))
     return fail(MA_EVALUE, "%s: batch x positions too large for one launch", what);
   const int64_t per = T * n_kv_heads, chunks = cdiv(per, rpb);
@@ -271,7 +266,7 @@ extern "C" int ma_dequant_kv(const void* k_codes, const void* v_codes, const voi
   if (batch == 0 || length == 0) return MA_OK;
   if (!k_out || !v_out || !quant_aligned16(k_out) || !quant_aligned16(v_out))
     return fail(MA_EVALUE, "%s: the outputs must be there and 16-byte aligned", what);
-  const int64_t rpb = kQuantThreads / (head_dim / 16) * kQuantRows;
+  const int64_t rpb = kQuantThreads / (head_dim / 8) * kQuantRows;
   if (length > INT32_MAX || batch > kMaxGroups / n_kv_heads / cdiv(length, rpb))
     return fail(MA_EVALUE, "%s: batch x positions too large for one launch", what);
   const int64_t chunks = cdiv(length, rpb);
