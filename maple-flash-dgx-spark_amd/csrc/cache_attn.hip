@@ -938,17 +938,16 @@ static int64_t cache_window(int64_t window, int64_t max_len, int64_t pre_len) {
   return window - pre_len > max_len ? 0 : window;
 }
 
-// prefixes: 0 where there are none.  A prefix is read once for all of its rows or by
-// each row with its own positions (`once`, < 0: by this rule).  The second under a
-// window, of which a prefix holds at most that many positions a row and each row
-// others, among more than kMaxShared prefixes, and where it is faster: reads of one
-// prefix by several rows meet in the L2s, and workgroups for prefixes begin later (whose
-// rows?) and need the join.  Measured (us, once / each; rows of 100 own positions, 4 KV
-// heads, 32 query heads of 64 or 16 of 128; in the table's order by the bytes of a
-// position's K):
-//   64 (e4m3, 64): 8 rows behind one of 2000 9.6 / 9.4, of 4000 10.6 / 10.7;  64 behind
-//     1000 11.5 / 10.6, behind 2000 12.5 / 15.7;  256 behind 16 of 1000 25 / 18, of 2000
-//     25.5 / 27.5;  128 behind 64 of 2000 22.3 / 21.5
+// A prefix is read once for all of its rows, or by each row with its own positions
+// (`once`; < 0: by this rule).  The second under a window, of which a prefix holds at
+// most that many positions a row and each row others, among more than kMaxShared
+// prefixes, and where it is faster: several rows' reads of one prefix meet in the L2s,
+// while a prefix's workgroups first have to find its rows and always need the join.
+// Measured (us, once / by each; rows of 100 own positions, 4 KV heads, 32 query heads of
+// 64 or 16 of 128), by the bytes of a position's K:
+//   64 (e4m3, heads of 64): 8 rows behind one prefix of 2000 9.6 / 9.4, of 4000 10.6 / 10.7;
+//     64 behind 1000 11.5 / 10.6, behind 2000 12.5 / 15.7;  256 behind 16 of 1000 25 / 18,
+//     of 2000 25.5 / 27.5;  128 behind 64 of 2000 22.3 / 21.5
 //   128 (bf16, 64): 8 behind 4000 10.9 / 10.5;  64 behind 500 11.3 / 7.4, 1000 11.8 / 9.7,
 //     2000 12.9 / 19.5;  128 behind 64 of 2000 30.5 / 40.5;  64 behind as many 32 / 27.5
 //   128 (e4m3, 128): 64 behind 1000 14.6 / 14.3, 2000 15.0 / 21.4;  128 behind 64 of 2000
@@ -957,7 +956,14 @@ static int64_t cache_window(int64_t window, int64_t max_len, int64_t pre_len) {
 //     15.7, 2000 15.6 / 30.9;  128 behind 64 of 2000 63 / 81;  64 behind as many 49 / 49
 // So once where a head's K of a prefix takes 112 KB, all rows' copies of it 14 MB, and a
 // position's K for the query rows of a prefix (on average) 2 KB.
-//
+static bool prefix_once(int64_t batch, int nq, int nkv, int64_t row_bytes, int64_t prefixes, int64_t pre_len, int64_t window,
+                        int once) {
+  if (prefixes < 1 || prefixes > kMaxShared || window > 0) return false;
+  if (once >= 0) return once > 0;
+  const int64_t k = pre_len * row_bytes, behind = prefixes < batch ? prefixes : batch;
+  return k >= (112 << 10) && batch * nkv >= cdiv(14 << 20, k) && batch * (nq / nkv) * row_bytes >= behind << 11;
+}
+
 // Splits, planned for the caches' lengths (the host does not know the rows').  A
 // workgroup a compute unit; two where a split would still hold more than 1024 of a
 // row's positions, or 2048 and more of a prefix; none of a row's where that saves less than the
@@ -971,13 +977,6 @@ static int64_t cache_window(int64_t window, int64_t max_len, int64_t pre_len) {
 //     64 behind two of 2000: 14.4, 13.4, 14.3;  behind four of 4096: 18.9, 15.4, 15.6,
 //     18.8;  of 8192: 28, 20.2, 18.5, 21.5;  of 16384: 47, 29, 23, 29;
 //     64 behind 8192 of 128: 28, 21.5, 27
-static bool prefix_once(int64_t batch, int nq, int nkv, int64_t row_bytes, int64_t prefixes, int64_t pre_len, int64_t window, int once) {
-  if (prefixes < 1 || prefixes > kMaxShared || window > 0) return false;
-  if (once >= 0) return once > 0;
-  const int64_t k = pre_len * row_bytes;
-  return k >= 112 << 10 && batch * nkv >= cdiv(14 << 20, k) && batch * (nq / nkv) * row_bytes >= (prefixes < batch ? prefixes : batch) << 11;
-}
-
 static CachePlan cache_plan(int64_t batch, int nq, int nkv, int64_t max_len, int64_t prefixes, int64_t pre_len, int64_t window,
                             bool shared) {
   CachePlan p{1, 0, 0};
