@@ -354,6 +354,25 @@ def test_attn_rows_without_tokens_and_past_the_end(dev):
     assert (out[:2] == 0).all()
 
 
+def test_attn_the_most_rows(dev):
+    """As many (row, KV head) pairs as a launch takes, all over two cache rows: each as the two alone."""
+    from maple_amd.kernels import SharedPrefix, prefix_gqa_attn, quant_gqa_attn
+
+    c, n = filled(dev, 2, 4, 40, 64, seed=37), 16383
+    two = bf16(dev, 2, 8, 1, 64, seed=38)
+    q = two.repeat(n // 2 + 1, 1, 1, 1)[:n]
+    rm = torch.arange(n, device=dev) % 2
+    sl = torch.full((n,), 39, device=dev)
+    want = quant_gqa_attn(two, c, i64(dev, [39, 39]), scale=0.125)
+    got = quant_gqa_attn(q, c, sl, row_map=rm, scale=0.125)
+    assert torch.equal(got, want.repeat(n // 2 + 1, 1, 1, 1)[:n])
+    pre = filled(dev, 1, 4, 50, 64, seed=39)
+    for once in (False, True):
+        one = [prefix_gqa_attn(x, c, y, SharedPrefix(pre, i64(dev, [50]), torch.zeros_like(y)), row_map=z, scale=0.125, once=once)
+               for x, y, z in ((two, sl[:2], rm[:2]), (q, sl, rm))]
+        assert torch.equal(one[1], one[0].repeat(n // 2 + 1, 1, 1, 1)[:n])
+
+
 def test_attn_row_map(dev):
     c = filled(dev, 6, 2, 200, 64, seed=26)
     check_attn(dev, c, [10, 199, 64], 4, row_map=[5, 0, 5])
@@ -776,6 +795,31 @@ def test_on_another_stream(dev):
         got = one_step(dev, *s)
     torch.cuda.current_stream(dev).wait_stream(st)
     assert torch.equal(want[0], got[0]) and torch.equal(want[1], got[1])
+
+
+def test_two_streams_at_once(dev):
+    """The same calls on two streams with no order between them, over one cache."""
+    from maple_amd.kernels import prefix_gqa_attn, quant_gqa_attn
+
+    cache, prefix, seqlen, _, _, _, _ = step_inputs(dev)
+    qs = [bf16(dev, 5, 8, 1, 64, seed=97 + i) for i in range(2)]
+
+    def calls(q):
+        return [quant_gqa_attn(q, cache, seqlen, scale=0.125)] + [
+            prefix_gqa_attn(q, cache, seqlen, prefix, scale=0.125, once=once) for once in (False, True)]
+
+    want = [calls(q) for q in qs]
+    streams = [torch.cuda.Stream(dev) for _ in qs]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(calls(qs[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for outs in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(want[i], outs))
 
 
 def test_two_captured_graphs(dev):

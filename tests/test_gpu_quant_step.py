@@ -116,6 +116,20 @@ def test_steps_behind_prefixes(dev, cfg, quantized, batch):
     _steps(model, cache, _ids(dev, batch), list(range(batch)))
 
 
+@pytest.mark.parametrize("quantized,longest", [(False, 2048), (True, 4096)])
+def test_steps_behind_a_long_prefix(dev, quantized, longest):
+    """At these sizes a prefix is read once for all of its rows."""
+    batch = 32
+    model = SyntheticDecoder(SMALL, dev, seed=8, max_len=longest + 64)
+    source = model.make_cache(1, prefill_len=longest, seed=4, quantized=quantized, max_len=longest)
+    cache = model.make_cache(batch, prefill_len=20, seed=5, quantized=quantized, max_len=64)
+    cache.prefix = source.share([0], [longest - 3])
+    cache.prefix.of = torch.zeros(batch, device=dev, dtype=torch.int64)
+    cache.prefix.of[5] = -1
+    cache.seqlen.copy_(torch.arange(batch, device=dev) % 21)
+    _steps(model, cache, _ids(dev, batch), list(range(batch)), n=2)
+
+
 def test_steps_through_a_slot_map(dev):
     model = SyntheticDecoder(SMALL, dev, seed=7, max_len=256)
     cache = model.make_cache(4, prefill_len=50, seed=3, quantized=True, max_len=100)
