@@ -195,7 +195,7 @@ def apply_qkv_quant(
     rounded to bf16, as ``apply_qkv_decode`` stores it, and then quantised."""
     idx, args, _keep = _projection("apply_qkv_quant", qkv, q_weight, k_weight, cos_table, sin_table, cache, seqlen, positions,
                                    row_map, num_heads, num_kv_heads, head_dim, rotary_dim, use_rope, eps)
-    out = qkv.new_empty((qkv.shape[0], num_heads, 1, head_dim))
+    out = qkv.new_empty(qkv.shape[0], num_heads, 1, head_dim)
     _call(idx, "ma_quant_qkv", *args, out.data_ptr())
     return out
 
@@ -250,7 +250,8 @@ def dequantize_kv(cache: QuantKV, length: int | None = None, *, row_map: torch.T
     rm = None if row_map is None else _positions("row_map", row_map, row_map.numel())
     idx = _device("dequantize_kv", *cache, *(() if rm is None else (rm,)))
     shape = (rows if rm is None else rm.numel(), n_kv, length, d)
-    out = KV(cache.k.new_empty(shape, dtype=torch.bfloat16), cache.k.new_empty(shape, dtype=torch.bfloat16))
+    k = cache.k.new_empty(*shape, dtype=torch.bfloat16)
+    out = KV(k, torch.empty_like(k))
     _call(
         idx, "ma_dequant_kv",
         *map(_ptr, cache), rows, max_len, shape[0], length, n_kv, d, _lib.ptr(rm), out.k.data_ptr(),
@@ -354,7 +355,7 @@ def quant_attention(
     window = _window(window)
     idx, args, _keep = _projection("quant_attention", qkv, q_weight, k_weight, cos_table, sin_table, cache, seqlen, positions,
                                    row_map, num_heads, num_kv_heads, head_dim, rotary_dim, use_rope, eps)
-    out = qkv.new_empty((qkv.shape[0], num_heads, 1, head_dim))
+    out = qkv.new_empty(qkv.shape[0], num_heads, 1, head_dim)
     nbytes = _workspace_bytes(qkv.shape[0], num_heads, num_kv_heads, head_dim, args[-1], 0, 0, window, True, -1)
     ws = qkv.new_empty(nbytes // 2) if nbytes else None  # (as in _attend)
     _call(idx, "ma_quant_attn", *args, window, scale, out.data_ptr(), _lib.ptr(ws), nbytes)
