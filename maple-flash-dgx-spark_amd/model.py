@@ -448,24 +448,29 @@ class SyntheticDecoder:
                    max_len: int | None = None) -> KVCache:
         """Cache rows filled with seeded N(0, 1) bf16 K/V for ``prefill_len``
         positions, of ``max_len`` (by default the model's); decoding then writes at
-        ``prefill_len``.  ``quantized``: the same values in a quantised cache."""
+        ``prefill_len``.  ``quantized``: the same values in a quantised cache, never
+        all of them in bf16."""
         c = self.cfg
         max_len = self.max_len if max_len is None else int(max_len)
         if not 1 <= max_len <= self.max_len:
             raise ValueError(f"make_cache: rows of {max_len} positions, the model has {self.max_len}.")
         shape = (batch, c.kv_heads, max_len, c.head_dim)
-        ks, vs = [], []
-        for i in range(c.layers):
-            k = synthetic.randn_bf16(shape, 50_000 + seed * 97 + 2 * i, self.device)
-            v = synthetic.randn_bf16(shape, 50_001 + seed * 97 + 2 * i, self.device)
-            k[:, :, prefill_len:] = 0
-            v[:, :, prefill_len:] = 0
-            ks.append(k)
-            vs.append(v)
+
+        def layer(i: int) -> KV:
+            kv = KV(*(synthetic.randn_bf16(shape, 50_000 + j + seed * 97 + 2 * i, self.device) for j in range(2)))
+            for t in kv:
+                t[:, :, prefill_len:] = 0
+            return kv
+
+        if quantized:  # (one bf16 layer at a time beside the codes)
+            layers = [quantize_kv(*layer(i), make_quant_kv(*shape, self.device)) for i in range(c.layers)]
+        else:
+            layers = [layer(i) for i in range(c.layers)]
         seqlen = torch.full((batch,), prefill_len, device=self.device, dtype=torch.int64)
         ws = gqa_workspace(batch, c.kv_heads, max_len, self.device, c.head_dim)
-        cache = KVCache(ks, vs, seqlen, max_len, ws)
-        return cache.quantized() if quantized else cache
+        names = ("k", "v", "k_scale", "v_scale") if quantized else ("k", "v")
+        return KVCache(seqlen=seqlen, max_len=max_len, attn_ws=ws,
+                       **{n: [kv[j] for kv in layers] for j, n in enumerate(names)})
 
     def _places(self, cache: KVCache, width: int):
         """What a step over slots ``[0, width)`` of a quantised cache, or of one with

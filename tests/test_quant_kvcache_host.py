@@ -2,11 +2,15 @@
 
 from __future__ import annotations
 
+import weakref
+
 import pytest
 import torch
 
+from maple_amd import model as model_module
+from maple_amd import synthetic
 from maple_amd.kernels import KV, QuantKV, make_quant_kv
-from maple_amd.model import KVCache
+from maple_amd.model import DecoderConfig, KVCache, SyntheticDecoder
 
 LAYERS, ROWS, NKV, N, D = 2, 4, 2, 16, 64
 
@@ -141,3 +145,38 @@ def test_what_has_no_form_is_refused():
             make()
     with pytest.raises(ValueError, match="drafted trees"):
         c.commit(path, accepted)
+
+
+def _decoder(max_len=N):
+    """A decoder without weights: what ``make_cache`` reads of it."""
+    m = SyntheticDecoder.__new__(SyntheticDecoder)
+    m.cfg = DecoderConfig(layers=5, heads=4, kv_heads=NKV, head_dim=D)
+    m.device, m.max_len = torch.device("cpu"), max_len
+    return m
+
+
+def test_a_quantised_cache_is_made_layer_by_layer(monkeypatch):
+    """No layer's bf16 K and V outlive their quantisation: a cache that only fits quantised can be made."""
+    made, seen, randn = [], [], synthetic.randn_bf16
+
+    def make(*args):
+        t = randn(*args)
+        made.append(weakref.ref(t))
+        return t
+
+    def quantize(k, v, cache):
+        live = [t for t in (r() for r in made) if t is not None]
+        assert len(live) == 2 and live[0] is k and live[1] is v
+        assert k.shape == v.shape == (ROWS, NKV, N, D) and not k[:, :, 9:].any() and k[:, :, :9].any()
+        seen.append((_raw(k).clone(), _raw(v).clone(), cache))
+        return cache
+
+    monkeypatch.setattr(synthetic, "randn_bf16", make)
+    monkeypatch.setattr(model_module, "quantize_kv", quantize)
+    c = _decoder().make_cache(ROWS, 9, seed=3, quantized=True)
+    assert len(made) == 10 and all(r() is None for r in made)
+    assert c.is_quantized and c.max_len == N and c.seqlen.tolist() == [9] * ROWS and len(seen) == 5
+    plain = _decoder().make_cache(ROWS, 9, seed=3)  # the same values
+    for i, (k, v, kv) in enumerate(seen):
+        assert all(a is b for a, b in zip(c.layer(i), kv))
+        assert torch.equal(k, _raw(plain.k[i])) and torch.equal(v, _raw(plain.v[i]))
