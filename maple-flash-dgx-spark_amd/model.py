@@ -216,7 +216,8 @@ class KVCache:
     With ``k_scale`` / ``v_scale`` the K/V are e4m3 codes with a power of two per
     position and head (``kernels.quant_cache``), half the bytes; with ``prefix``
     slots' sequences may begin with shared prefixes, ``seqlen`` then counting a
-    slot's own positions.  Neither carries drafted trees."""
+    slot's own positions.  Neither carries drafted trees.  ``attn_ws``: the
+    workspace of a bf16 cache's steps (a quantised one's need none that is kept)."""
 
     k: list
     v: list
@@ -289,7 +290,7 @@ class KVCache:
         if self.is_quantized or self.prefix is not None:
             raise ValueError("quantized takes a bf16 cache without shared prefixes.")
         out = [quantize_kv(k, v, make_quant_kv(*k.shape, k.device)) for k, v in zip(self.k, self.v)]
-        return KVCache([c.k for c in out], [c.v for c in out], self.seqlen.clone(), self.max_len, self.attn_ws,
+        return KVCache([c.k for c in out], [c.v for c in out], self.seqlen.clone(), self.max_len, None,
                        self.row_map.clone(), self.remap, [c.k_scale for c in out], [c.v_scale for c in out])
 
     def dequantized(self) -> "KVCache":
@@ -467,7 +468,7 @@ class SyntheticDecoder:
         else:
             layers = [layer(i) for i in range(c.layers)]
         seqlen = torch.full((batch,), prefill_len, device=self.device, dtype=torch.int64)
-        ws = gqa_workspace(batch, c.kv_heads, max_len, self.device, c.head_dim)
+        ws = None if quantized else gqa_workspace(batch, c.kv_heads, max_len, self.device, c.head_dim)
         names = ("k", "v", "k_scale", "v_scale") if quantized else ("k", "v")
         return KVCache(seqlen=seqlen, max_len=max_len, attn_ws=ws,
                        **{n: [kv[j] for kv in layers] for j, n in enumerate(names)})

@@ -180,3 +180,12 @@ def test_a_quantised_cache_is_made_layer_by_layer(monkeypatch):
     for i, (k, v, kv) in enumerate(seen):
         assert all(a is b for a, b in zip(c.layer(i), kv))
         assert torch.equal(k, _raw(plain.k[i])) and torch.equal(v, _raw(plain.v[i]))
+
+
+def test_quantised_caches_hold_no_workspace_of_bf16_steps(monkeypatch):
+    monkeypatch.setattr(model_module, "quantize_kv", lambda k, v, cache: cache)
+    c = _plain()
+    c.attn_ws = torch.zeros(8)
+    assert c.quantized().attn_ws is None
+    assert _decoder().make_cache(ROWS, 9, quantized=True).attn_ws is None
+    assert _decoder().make_cache(ROWS, 9).attn_ws is not None
