@@ -20,7 +20,8 @@ import torch
 from oracle import decoder as od
 from oracle import quant_cache as oq
 from test_gpu_decoder import _check_logits, _to_np
-from maple_amd.decode_graph import BucketedDecodeGraphs, Sampling, generate, tree_step, try_decode_graph
+from maple_amd.decode_graph import (BucketedDecodeGraphs, Sampling, _choose, batched_sampler_workspace, capture_decode_graph,
+                                    generate, tree_step, try_decode_graph)
 from maple_amd.model import DecoderConfig, SyntheticDecoder
 
 pytestmark = pytest.mark.gpu
@@ -182,6 +183,65 @@ def test_captured_steps_equal_eager_ones(dev, quantized, prefix, sampling):
         assert all(torch.equal(x, y) for x, y in zip(before[n], after[n]))
     graph = generate(model, c, _ids(dev, 3), 6, Sampling())
     assert len(graph.token_ids) == 3 and all(len(t) == 6 for t in graph.token_ids)
+
+
+@pytest.mark.parametrize("quantized,prefix", [(True, 0), (False, 30), (True, 30), (False, 2045), (True, 4093)],
+                         ids=["quantised", "bf16, prefix", "quantised, prefix", "bf16, long prefix", "quantised, long prefix"])
+@pytest.mark.parametrize("sampling", [Sampling(), Sampling(temperature=0.8, top_p=0.9, top_k=20)], ids=["greedy", "drawn"])
+def test_captured_steps_repeat_eager_ones_to_the_bit(dev, quantized, prefix, sampling):
+    """Logits, ids, write positions and every byte of the cache after each of six steps, replayed with eager work between
+    them, against the same steps run eagerly; the long prefixes are read once for all of their rows."""
+    rows = 32 if prefix > 1000 else 3
+    model = SyntheticDecoder(SMALL, dev, seed=9, max_len=max(256, prefix + 64))
+    cache = model.make_cache(rows, prefill_len=30, seed=2, quantized=quantized, max_len=64)
+    if prefix:
+        source = model.make_cache(1, prefill_len=prefix, seed=3, quantized=quantized, max_len=prefix)
+        cache.prefix = source.share([0], [prefix])
+        cache.prefix.of = torch.zeros(rows, device=dev, dtype=torch.int64)
+        cache.prefix.of[1] = -1
+        cache.seqlen.copy_(torch.arange(rows, device=dev) % 31)
+    if not sampling.greedy:
+        sampling = dataclasses.replace(sampling, generator=torch.Generator(device=dev))
+    first, snap, n = _ids(dev, rows), cache.snapshot(), 6
+
+    def state():
+        raw = [t.view(torch.uint8 if t.element_size() == 1 else torch.int16) for i in range(SMALL.layers) for t in cache.layer(i)]
+        return [cache.seqlen.clone()] + [t.clone() for t in raw]
+
+    def start():
+        cache.restore(snap)
+        if sampling.generator is not None:
+            sampling.generator.manual_seed(5)
+
+    start()
+    before, eager, tok, out = state(), [], first.clone(), torch.empty_like(first)
+    ws = None if sampling.greedy else batched_sampler_workspace(SMALL.vocab, sampling.top_k, rows, dev)[0]
+    for _ in range(n):
+        u = None if sampling.greedy else sampling.draw(rows, dev)
+        logits = model.forward(tok, cache)
+        _choose(logits, sampling, out, u, ws)
+        tok.copy_(out)
+        eager.append([logits.clone(), out.clone()] + state())
+    start()
+    assert all(torch.equal(a, b) for a, b in zip(before, state()))
+    g = capture_decode_graph(model, cache, first.clone(), sampling)
+    start()
+    g.token_ids.copy_(first)
+    for step in range(n):
+        ids = g.step(sampling)
+        other = torch.randn(1 << 16, device=dev).sum()  # eager work on the same allocator
+        torch.cuda.synchronize()
+        got = [g.logits, ids] + state()
+        assert all(torch.equal(a, b) for a, b in zip(eager[step], got)), step
+        assert torch.isfinite(other)
+    # each step wrote each row's token into every layer, and nothing else
+    at, was, now = before[0], before[1:], state()[1:]
+    for a, b in zip(was, now):
+        new = (torch.arange(64, device=dev) >= at.view(-1, 1)) & (torch.arange(64, device=dev) < at.view(-1, 1) + n)
+        mask = new.unsqueeze(1).expand(-1, SMALL.kv_heads, -1)
+        assert torch.equal(a[~mask], b[~mask])
+        if a.ndim == 4:
+            assert (a[mask] != b[mask]).any(-1).all()
 
 
 def test_bucketed_graphs_over_a_quantised_cache(dev):
