@@ -87,7 +87,9 @@ __device__ __forceinline__ CacheSpan cache_span(const CacheAttn& a, const CacheH
   return s;
 }
 
-// Eight e4m3 codes times 2^e as bf16 (exact).
+// Eight e4m3 codes times 2^e as bf16: exact (four significant bits) unless 2^e takes
+// a value below bf16's least normal, where it may need more than its least step (2^-133;
+// the least code at 2^-126 is 2^-135).
 __device__ __forceinline__ uint4 codes_bf16(uint32_t lo, uint32_t hi, float s) {
   auto two = [&](uint32_t w, bool up) {
     return up ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, s, true))

@@ -4,10 +4,12 @@
 //   e = the least integer with max_d |x_d| <= 448 2^e, in [-126, 119]
 //   code_d = e4m3(x_d 2^-e), to the nearest (even), at most 448; value = code_d 2^e
 //
-// A power of two instead of a float scale: e4m3 keeps half a step of 2^-4 of a
-// value over 2^14 below the largest wherever the binade ends, so a finer scale
-// gains nothing; codes take no division (a bf16 row has one set of codes, to the
-// bit, whoever computes them), and the scaled conversions apply it for nothing.
+// A power of two instead of a float scale: the largest scaled value lies in (224,
+// 448] and e4m3's least normal is 2^-6, so half a step is 2^-4 of a value over at
+// least 2^13.8 below the largest wherever the binade ends; a finer scale would add at
+// most one power of two to that.  Codes take no division (a bf16 row has one set of
+// codes, to the bit, whoever computes them), and the scaled conversions apply it for
+// nothing.
 // Values that are not finite become NaN codes and do not enter the maximum.
 #pragma once
 
