@@ -161,9 +161,10 @@ __device__ __forceinline__ void lay_v(char* vb, const u32x4c_t (&v)[VL], S&& s_o
 //   O += P V: A = the lane's own eight P (positions 4g.. of both halves), B = V in
 //     the same order from LDS, where a wave lays its tile as bf16 rows, by the
 //     transposing read.
-// Bound by the cache's bytes where there are many (quantised: 32 x 4096 of 64 13 us, 8 x
-// 32768 of 128 44 us: 4.0 and 4.8 TB/s of the 5.2 that a copy of 1 GiB reaches), by its
-// chain of loads where there are few (1 x 4096 of 64: 4.6 us; a wave has a tile).  Workgroups
+// Bound by the cache's bytes where there are many (quantised: 8 x 32768 of 128, 210 MB, 43
+// us, 4.9 TB/s of the 5.2 that a copy of 1 GiB reaches; 32 x 4096 of 64, 52 MB that the
+// last-level cache holds, 13 us, 4.0 TB/s of the 8.5 of a copy of that size), by its
+// chain of loads where there are few (1 x 4096 of 64: 4.7 us; a wave has a tile).  Workgroups
 // of 16 waves (8 for heads of 128) in the place of splits were faster in calls one after
 // another (32 x 1000: 7.8 us against 8.6) but slower in whole steps (24 layers 1630
 // against 1584).
@@ -496,8 +497,8 @@ struct PrefixLds {
 // gives the same quotient).
 // Bound by a tile's chain (scores, exponentials, products; the vector unit is busy half of
 // the time, the matrix unit a fifth) with two or three waves a SIMD: 32 rows of 32 heads
-// of 64 behind 8192 bf16 positions 12.7 us, 64 behind four prefixes of 16384 quantised ones
-// 19.6 (0.38 PFLOP/s; 0.6 behind 131072).  Leaving out 12 of a tile's 16 conversions of K
+// of 64 behind 8192 bf16 positions 13 us, 64 behind four prefixes of 16384 quantised ones
+// 21 (0.35 PFLOP/s; 0.6 behind 131072).  Leaving out 12 of a tile's 16 conversions of K
 // changes nothing.  64 rows a wave halve the conversions but leave too few waves (28
 // against 24 with the join), 128 rows of four waves on one tile in LDS took 33.
 template <int HD, bool Q8>
@@ -805,7 +806,8 @@ __global__ __launch_bounds__(kCacheThreads, (HD == 64 ? 4 : (Q8 ? 3 : 2))) void 
 
 // A step's token from its projection on: k_quant_qkv's work and the attention (a captured
 // step of 24 layers at 4000 positions: 697 us at one row, 1425 at 8, 1794 at 32, with
-// two launches 737, 1483, 1849).
+// two launches 737, 1483, 1849).  Both parts together are tight in registers: 4 spilled a
+// thread for heads of 128, 5 and (64) 11 where rows are not aligned.
 template <int HD, bool VEC>
 __global__ __launch_bounds__(kCacheThreads, HD == 64 ? 4 : 3) void k_quant_attn(const int64_t* seqlen, const int64_t* row_map,
                                                                                 int nq, int nkv, int s_own, NewToken token,
@@ -975,10 +977,10 @@ static bool prefix_once(int64_t batch, int nq, int nkv, int64_t row_bytes, int64
 //     unsplit, 9.2 for 256;  32 x 4096: 25.0, 18.1 for 256, 15.2 for 512, 15.9 for 768;
 //     2 x 32768: 17.7 for 128, 12.4, 12.0, 12.4
 //   4 x 4096 of 128: 11.5, 9.9, 10.7 for 512;  8 x 32768: 82, 55, 51, 52
-//   prefixes, 32 rows behind 8192 of 64: 18.0, 14.7, 15.3;  behind 32768: 44, 28, 24, 25;
-//     64 behind two of 2000: 14.4, 13.4, 14.3;  behind four of 4096: 18.9, 15.4, 15.6,
-//     18.8;  of 8192: 28, 20.2, 18.5, 21.5;  of 16384: 47, 29, 23, 29;
-//     64 behind 8192 of 128: 28, 21.5, 27
+//   prefixes, for 128, 256, 512 and 768: 32 rows behind 8192 of 64: 18.0, 14.6, 15.4, 17.7;
+//     behind 32768: 43.8, 28.0, 24.3, 25.7;  64 behind two of 2000: 14.4, 13.5, 14.5, 15.7;
+//     behind four of 4096: 18.9, 15.7, 15.8, 18.6;  of 8192: 28.5, 20.1, 18.5, 21.7;
+//     of 16384: 46.9, 29.4, 22.7, 28.6;  64 behind 8192 of 128: 28.3, 21.6, 27.0, 29.2
 static CachePlan cache_plan(int64_t batch, int nq, int nkv, int64_t max_len, int64_t prefixes, int64_t pre_len, int64_t window,
                             bool shared) {
   CachePlan p{1, 0, 0};
@@ -1019,13 +1021,15 @@ static int check_cache_sizes(const char* what, int64_t batch, int nq, int nkv, i
   if (hd != 64 && hd != 128) return fail(MA_EVALUE, "%s: head_dim %d unsupported (64 or 128)", what, hd);
   if (nkv < 1 || nq < nkv || nq % nkv != 0 || nq / nkv > kCacheGroup || nq > 65535)
     return fail(MA_EVALUE, "%s: %d query heads over %d KV heads (at most %d to one)", what, nq, nkv, kCacheGroup);
-  if (batch < 0 || batch > 65535 || batch * nkv > 65535) return fail(MA_EVALUE, "%s: batch %lld too large for one launch", what, static_cast<long long>(batch));
+  if (batch < 0 || batch > 65535 || batch * nkv > 65535)
+    return fail(MA_EVALUE, "%s: batch %lld too large for one launch", what, static_cast<long long>(batch));
   if (window < 0) return fail(MA_EVALUE, "%s: window %lld", what, static_cast<long long>(window));
   constexpr int64_t kMost = int64_t{1} << 34;  // (tiles of 32 positions are counted in 32 bits)
   if (batch > 0 && (max_len < 1 || max_len >= kMost || rows < 1 || (!row_map && batch > rows)))
     return fail(MA_EVALUE, "%s: bad cache sizes", what);
   if (prefixes < 0 || prefixes > 65535 || (prefixes > 0 && (pre_len < 1 || pre_len >= kMost)))
-    return fail(MA_EVALUE, "%s: %lld prefixes of %lld positions", what, static_cast<long long>(prefixes), static_cast<long long>(pre_len));
+    return fail(MA_EVALUE, "%s: %lld prefixes of %lld positions", what, static_cast<long long>(prefixes),
+                static_cast<long long>(pre_len));
   if (once > 0 && prefixes > 0 && (prefixes > kMaxShared || cache_window(window, max_len, pre_len) > 0))
     return fail(MA_EVALUE, "%s: more than %d prefixes, or a window's, are read by each row", what, kMaxShared);
   return MA_OK;
@@ -1052,19 +1056,21 @@ extern "C" size_t ma_cache_attn_workspace_bytes(int64_t batch, int n_heads, int 
                                      prefix_max_len, window, once) != MA_OK)
     return 0;
   window = cache_window(window, max_len, prefixes > 0 ? prefix_max_len : 0);
-  const bool shared = prefix_once(batch, n_heads, n_kv_heads, quantized ? head_dim : 2 * head_dim, prefixes, prefix_max_len, window, once);
-  return cache_ws_bytes(cache_plan(batch, n_heads, n_kv_heads, max_len, prefixes, prefix_max_len, window, shared), batch, n_heads,
-                        head_dim);
+  const bool shared = prefix_once(batch, n_heads, n_kv_heads, quantized ? head_dim : 2 * head_dim, prefixes, prefix_max_len,
+                                  window, once);
+  const CachePlan p = cache_plan(batch, n_heads, n_kv_heads, max_len, prefixes, prefix_max_len, window, shared);
+  return cache_ws_bytes(p, batch, n_heads, head_dim);
 }
 
 extern "C" int ma_cache_attn(const void* q, int64_t batch, int n_heads, int n_kv_heads, int head_dim, const void* k,
                              const void* v, const void* k_scale, const void* v_scale, int64_t cache_rows, int64_t max_len,
                              const int64_t* seqlen, const int64_t* row_map, const void* pk, const void* pv,
                              const void* pk_scale, const void* pv_scale, int64_t prefixes, int64_t prefix_max_len,
-                             const int64_t* prefix_len, const int64_t* prefix_of, int once, int64_t window, float scale, void* out,
-                             void* workspace, size_t workspace_bytes, void* stream) {
+                             const int64_t* prefix_len, const int64_t* prefix_of, int once, int64_t window, float scale,
+                             void* out, void* workspace, size_t workspace_bytes, void* stream) {
   const char* what = "cache_attn";
-  if (int rc = check_cache_sizes(what, batch, n_heads, n_kv_heads, head_dim, cache_rows, max_len, row_map, prefixes, prefix_max_len, window, once))
+  if (int rc = check_cache_sizes(what, batch, n_heads, n_kv_heads, head_dim, cache_rows, max_len, row_map, prefixes,
+                                 prefix_max_len, window, once))
     return rc;
   if (!isfinite(scale * kLog2e)) return fail(MA_EVALUE, "%s: scale %g, or log2 e times it, is not finite", what, scale);
   if (batch == 0) return MA_OK;
@@ -1076,7 +1082,8 @@ extern "C" int ma_cache_attn(const void* q, int64_t batch, int n_heads, int n_kv
       !quant_aligned16(workspace) || (prefixes > 0 && (!quant_aligned16(pk) || !quant_aligned16(pv))))
     return fail(MA_EVALUE, "%s: q, the caches, out and the workspace must be 16-byte aligned", what);
   window = cache_window(window, max_len, prefixes > 0 ? prefix_max_len : 0);
-  const bool shared = prefix_once(batch, n_heads, n_kv_heads, q8 ? head_dim : 2 * head_dim, prefixes, prefix_max_len, window, once);
+  const bool shared = prefix_once(batch, n_heads, n_kv_heads, q8 ? head_dim : 2 * head_dim, prefixes, prefix_max_len, window,
+                                  once);
   const CachePlan p = cache_plan(batch, n_heads, n_kv_heads, max_len, prefixes, prefix_max_len, window, shared);
   const int64_t parts = batch * n_heads * (p.s_own + p.s_pre);
   const size_t need = cache_ws_bytes(p, batch, n_heads, head_dim);

@@ -26,7 +26,7 @@ constexpr int kQuantThreads = 256;
 // ways of filling a cache give one set of codes) and quantised with their largest
 // value over the HD / 8 lanes of the head, v heads quantised as they are.
 // VEC: all rows are 16-byte aligned.  Bound by latency, two rounds of loads (the
-// token's row and place, then the tables): 3.7 us for a row of 32 + 8 heads of 64, 4.8 for
+// token's row and place, then the tables): 3.8 us for a row of 32 + 8 heads of 64, 5.1 for
 // 256 rows of 16 + 8 heads of 128 (3 MB).
 template <int HD, bool VEC>
 __global__ __launch_bounds__(kQuantThreads) void k_quant_qkv(QkvIn in, int64_t batch, const int64_t* __restrict__ seqlen,
@@ -84,7 +84,7 @@ constexpr int kQuantRows = 4;  // rows a thread has in flight
 // lie next to each other (positions before heads, as a projection leaves them), so
 // they are walked first; else positions are.  Stores pass the caches by, which the
 // next reader would not find them in (33 to 37 us else).  Bound by HBM: 32 prompts of
-// up to 4096 positions (154 MB read and written) in 31 to 33 us, 4.8 TB/s; 2.9 for 7
+// up to 4096 positions (154 MB read and written) in 31 us, 5.0 TB/s; 2.6 for 7
 // positions.
 template <int HD, bool HEADS_IN, bool VEC>
 __global__ __launch_bounds__(kQuantThreads) void k_quant_kv(KvRows kr, KvRows vr, int chunks, uint32_t per, uint32_t T,
@@ -135,11 +135,11 @@ __global__ __launch_bounds__(kQuantThreads) void k_quant_kv(KvRows kr, KvRows vr
 // ---------------------------------------------------------------------------
 // Cached positions back
 // ---------------------------------------------------------------------------
-// HD / 8 lanes a row of 8 codes each (16: 43 us for the case below); blockIdx.x: `chunks` of a (batch row, head)'s
-// positions, blockIdx.y: K or V.  A value is exact in bf16 (e4m3 has four
-// significant bits) unless 2^e takes it below bf16's least normal.  Bound by HBM: 32 rows
-// of 4096 positions (203 MB) in 30.4 us, 6.7 TB/s with what the last-level cache holds of
-// the codes (36.3 without nontemporal stores); 2.9 for 1001 positions of one row.
+// HD / 8 lanes a row of 8 codes each (16: 43 us for the case below); blockIdx.x: `chunks`
+// of a (batch row, head)'s positions, blockIdx.y: K or V.  A value is exact in bf16 (e4m3
+// has four significant bits) unless 2^e takes it below bf16's least normal.  Bound by HBM:
+// 32 rows of 4096 positions (203 MB) in 29.8 us, 6.8 TB/s with what the last-level cache
+// holds of the codes (36.3 without nontemporal stores); 3.1 for 1001 positions of one row.
 template <int HD>
 __global__ __launch_bounds__(kQuantThreads) void k_dequant_kv(QuantCache cache, int chunks, uint32_t length, int nkv,
                                                               const int64_t* __restrict__ row_map,
@@ -275,7 +275,8 @@ extern "C" int ma_dequant_kv(const void* k_codes, const void* v_codes, const voi
   const dim3 grid(static_cast<unsigned>(batch * n_kv_heads * chunks), 2);
   auto go = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, grid, dim3(kQuantThreads), 0, static_cast<hipStream_t>(stream), cache,
-                       static_cast<int>(chunks), static_cast<uint32_t>(length), n_kv_heads, row_map, static_cast<uint16_t*>(k_out), static_cast<uint16_t*>(v_out));
+                       static_cast<int>(chunks), static_cast<uint32_t>(length), n_kv_heads, row_map,
+                       static_cast<uint16_t*>(k_out), static_cast<uint16_t*>(v_out));
   };
   if (head_dim == 64) go(k_dequant_kv<64>);
   else go(k_dequant_kv<128>);

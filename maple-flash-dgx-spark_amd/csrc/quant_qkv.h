@@ -84,11 +84,13 @@ inline int check_quant(const char* what, int64_t batch, int n_kv_heads, int head
 
 // The arguments of a token's projection; `in` and whether all of it can be read 16
 // bytes at a time (rows aligned, and the rotary part ending with a lane's dims).
-inline int check_qkv(const char* what, const void* qkv, int64_t ldb, int n_heads, int n_kv_heads, int head_dim, const void* q_w, const void* k_w, int w_dtype, const void* cos, const void* sin,
-                     int cs_dtype, int64_t ld_cs, int64_t n_pos, int rotary_dim, float eps, QkvIn& in, bool& vec) {
+inline int check_qkv(const char* what, const void* qkv, int64_t ldb, int n_heads, int n_kv_heads, int head_dim, const void* q_w,
+                     const void* k_w, int w_dtype, const void* cos, const void* sin, int cs_dtype, int64_t ld_cs, int64_t n_pos,
+                     int rotary_dim, float eps, QkvIn& in, bool& vec) {
   if (n_heads < n_kv_heads || n_heads % n_kv_heads != 0 || n_heads > 65535)
     return fail(MA_EVALUE, "%s: %d query heads over %d KV heads", what, n_heads, n_kv_heads);
-  if (ldb < static_cast<int64_t>(n_heads + 2 * n_kv_heads) * head_dim) return fail(MA_EVALUE, "%s: qkv row stride too small", what);
+  if (ldb < static_cast<int64_t>(n_heads + 2 * n_kv_heads) * head_dim)
+    return fail(MA_EVALUE, "%s: qkv row stride too small", what);
   if (rotary_dim < 0 || rotary_dim > head_dim || rotary_dim % 2 != 0)
     return fail(MA_EVALUE, "%s: rotary_dim %d must be even and at most head_dim", what, rotary_dim);
   if (rotary_dim > 0 && (!cos || !sin || n_pos < 1 || ld_cs < rotary_dim))

@@ -1,6 +1,6 @@
 """HIP kernels of the hot path, exported under the reference's names
-(``src/maple_run/kernels/__init__.py:5-39``), plus ``moe_dispatch`` those of
-decoding with drafted token trees (``tree``) and those of quantised caches and
+(``src/maple_run/kernels/__init__.py:5-39``), plus ``moe_dispatch``, those
+of decoding with drafted token trees (``tree``) and those of quantised caches and
 shared prefixes (``quant_cache``).
 
 Importing this package does not load the HIP library; the first kernel call

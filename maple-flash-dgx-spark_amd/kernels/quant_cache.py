@@ -305,8 +305,8 @@ def _attend(what: str, q: torch.Tensor, cache, seqlen: torch.Tensor, prefix: Sha
     ws = q.new_empty(nbytes // 2) if nbytes else None
     _call(
         idx, "ma_cache_attn",
-        q.data_ptr(), bsz, n_q, n_kv, head_dim, *map(_ptr, cache), *(() if quant else (None, None)), rows, max_len, sl.data_ptr(), rm, *shared, n_pre, pre_max,
-        p_len, p_of, form, window, scale, out.data_ptr(), _lib.ptr(ws), nbytes,
+        q.data_ptr(), bsz, n_q, n_kv, head_dim, *map(_ptr, cache), *(() if quant else (None, None)), rows, max_len,
+        sl.data_ptr(), rm, *shared, n_pre, pre_max, p_len, p_of, form, window, scale, out.data_ptr(), _lib.ptr(ws), nbytes,
     )
     return out
 

@@ -307,6 +307,8 @@ class KVCache:
         (copied: the rows are free again), held once for all slots that begin with it.
         Every slot begins with none; ``prefix.of[slot] = p`` with ``seqlen[slot]`` set to
         the slot's own positions (0 for a new sequence) puts one behind prefix ``p``.
+        The model's rotary tables have to reach the longest prefix and a whole row
+        (``max_len`` of both together): its steps refuse the cache else.
         Share before capturing a step: a graph captured earlier knows of no prefixes."""
         rows, lengths = [int(r) for r in rows], [int(n) for n in lengths]
         if self.prefix is not None:
@@ -530,8 +532,8 @@ class SyntheticDecoder:
                    use_rope=use_rope)
         seqlen, row_map = cache.slot_rows(bsz if tree is None else tree.shape[0])
         akw["row_map"] = row_map
-        if bsz == 1 and tree is None and places is None and self.fused_o and o_projection_supported(1, c.heads, c.kv_heads, c.head_dim,
-                                                                cache.max_len, window, c.hidden):
+        if (bsz == 1 and tree is None and places is None and self.fused_o
+                and o_projection_supported(1, c.heads, c.kv_heads, c.head_dim, cache.max_len, window, c.hidden)):
             # attention and its output projection in one launch (measured: no
             # faster than two launches at 4096 positions -- the grid barrier
             # and the tail cost what the second launch does -- so off by default)
