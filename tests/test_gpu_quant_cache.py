@@ -915,3 +915,70 @@ def test_no_prefixes_at_all(dev):
         q, n = bf16(dev, 2, 8, 1, 64, seed=96), i64(dev, [99, 20])
         a = prefix_gqa_attn(q, c, n, SharedPrefix(empty, i64(dev, [0] * shape[0]), i64(dev, [0, -1])), scale=0.125)
         assert torch.equal(a, quant_gqa_attn(q, c, n, scale=0.125))
+
+
+@pytest.mark.parametrize("quant", [False, True])
+@pytest.mark.parametrize("once", [False, True])
+def test_prefixes_may_be_rows_of_the_same_cache(dev, quant, once):
+    """Rows that begin with what another row of their own cache holds, none of it copied."""
+    from maple_amd.kernels import KV, QuantKV, SharedPrefix, prefix_gqa_attn
+
+    c = make(dev, quant, 4, 2, 300, 64, 150)
+    other = (QuantKV if quant else KV)(*(b.view(t.dtype) for b, t in zip(bits(c), c)))
+    q, n, of = bf16(dev, 4, 8, 1, 64, seed=151), i64(dev, [299, 20, -1, 130]), i64(dev, [-1, 0, 0, 3])
+    got, want = (prefix_gqa_attn(q, c, n, SharedPrefix(p, i64(dev, [300, 7, 0, 129]), of), scale=0.125, once=once)
+                 for p in (c, other))
+    assert torch.equal(got, want) and all(torch.equal(a, b) for a, b in zip(bits(c), bits(other)))
+
+
+def test_index_tensors_of_32_bits(dev):
+    """Write positions, lengths, places and maps in int32 and strided: as in int64."""
+    from maple_amd.kernels import SharedPrefix, apply_qkv_quant, prefix_gqa_attn, quant_attention, quantize_kv
+
+    cos, sin = tables(400, 32, dev)
+    k, v, qkv = bf16(dev, 3, 2, 40, 64, seed=160), bf16(dev, 3, 2, 40, 64, seed=161), bf16(dev, 3, 8 * 64, seed=162)
+    pre = filled(dev, 2, 2, 90, 64, seed=163)
+
+    def calls(at):
+        c = filled(dev, 5, 2, 60, 64, seed=164)
+        rm, n = at([4, 0, 2]), at([39, 17, -1])
+        kw = dict(positions=at([100, 20, 3]), row_map=rm, num_heads=4, num_kv_heads=2, head_dim=64, rotary_dim=32)
+        quantize_kv(k, v, c, start=at([0, 3, 7]), lengths=at([40, 12, 0]), row_map=rm)
+        q = apply_qkv_quant(qkv, None, None, cos, sin, c, n, **kw)
+        outs = [q, quant_attention(qkv, None, None, cos, sin, c, n, scale=0.125, **kw)]
+        outs += [prefix_gqa_attn(q, c, n, SharedPrefix(pre, at([90, 33]), at([1, 0, -1])), row_map=rm, scale=0.125, once=o)
+                 for o in (False, True)]
+        return outs + bits(c)
+
+    want = calls(lambda x: i64(dev, x))
+    for got in (calls(lambda x: i64(dev, x).int()), calls(lambda x: i64(dev, [x, x]).t()[:, 1])):
+        assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+@pytest.mark.parametrize("once", [False, True])
+def test_a_graph_follows_its_prefixes(dev, once):
+    """Prefixes, their lengths and their rows changed in place between replays."""
+    from maple_amd.kernels import SharedPrefix, prefix_gqa_attn
+
+    own, pre = filled(dev, 6, 2, 40, 64, seed=170), filled(dev, 3, 2, 500, 64, seed=172)
+    q, n = bf16(dev, 6, 8, 1, 64, seed=174), i64(dev, [39, 3, -1, 0, 17, 38])
+    prefix = SharedPrefix(pre, i64(dev, [500, 0, 1]), i64(dev, [0, 0, 1, 2, -1, 7]))
+
+    def call():
+        return prefix_gqa_attn(q, own, n, prefix, scale=0.125, once=once)
+
+    call()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = call()
+    for length, of in (([500, 0, 1], [0, 0, 1, 2, -1, 7]), ([1, 499, 33], [2] * 6), ([0, 0, 0], [0, 1, 2, 0, 1, 2]),
+                       ([64, 65, 500], [1, 2, 0, 1, -1, 1]), ([500, 500, 500], [-1] * 6)):
+        prefix.length.copy_(i64(dev, length))
+        prefix.of.copy_(i64(dev, of))
+        for _ in range(2):
+            g.replay()
+            other = torch.randn(1 << 16, device=dev).sum()  # eager work on the same allocator
+            torch.cuda.synchronize()
+            assert torch.equal(out, call()) and torch.isfinite(other)
+        check_attn(dev, own, n.tolist(), 8, prefix=(pre, length, of), q=q)
